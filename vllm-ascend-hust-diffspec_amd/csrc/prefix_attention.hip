@@ -1,0 +1,948 @@
+// Paged attention of a verified batch that shares a long prefix, computed once for all rows.
+//
+// The verifier's side of a step: ragged rows of query tokens (query_start, query_len) attend over
+// their paged keys and values (block_table, target_len), causally at the end, and the natural-log
+// LSE of every query head comes back with the output: the snapshot the chunk scoring takes
+// (diffspec/runtime.py:841-878 captures both from the target's fused attention).  All rows agree on
+// their first prefix_len tokens.
+//
+//   L(b, i) = target_len[b] - query_len[b] + i + 1         keys that query token i of row b sees
+//   out     = sum_{t < L} softmax_t(scale q . k_t) v_t,  lse = ln sum_{t < L} exp(scale q . k_t)
+//
+// The prefix is one problem for the whole batch: the query heads of all rows' tokens that share a
+// KV head are rows of one matrix, so every prefix key is read once per 128 (or 64) of them instead
+// of once per request.  Each row's own tokens (prefix_len .. target_len) are a problem of the row.
+// Softmax pieces over disjoint key ranges join exactly: with m the maximum, l the sum of
+// exp(x - m) and O the sum of exp(x - m) v of each piece, out = sum_i 2^(m_i - m) O_i / sum_i
+// 2^(m_i - m) l_i (base 2 here, the logits pre-scaled by log2 e).
+//
+// Work: a unit is (KV head, tile of query rows, key range); its key tiles are laid end to end with
+// all other units' and dealt to the workgroups in equal contiguous shares, whatever the rows'
+// lengths.  Every workgroup derives the same layout from the lengths on the device, so a captured
+// launch follows changed lengths.  Prefix ranges are cut into segments of one share with the row
+// tiles inside a segment next to each other, and consecutive shares are given to one XCD, so the
+// row tiles that read the same keys do it at about the same time behind one L2.  A share that ends
+// inside a unit leaves its piece (m, l, O in fp32) in the workspace; prefix_join_kernel joins them.
+#include "ds355_common.h"
+
+namespace ds355 {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr float kLog2eP = 1.44269504088896340736f;
+constexpr float kLn2P = 0.69314718055994530942f;
+constexpr int kWideRows = 128, kNarrowRows = 64;  // query rows of a unit's tile
+constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
+constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
+constexpr uint32_t kStatusPage = 4;    // a page id is out of range
+
+template <int D>
+struct Shape {
+  static constexpr int kWaves = D == 128 ? 8 : 4;
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kTile = D <= 128 ? 128 : 64;   // keys per tile
+  static constexpr int kLanes = D / 8;                // 16-byte pieces of a key
+  static constexpr int kPerPass = kThreads / kLanes;  // keys that one load of all threads covers
+  static constexpr int kPasses = kTile / kPerPass;
+  static constexpr int kBuffer = kTile * D;           // elements of a staged tile of keys (or values)
+  static constexpr int kSteps = D / 16;               // score MFMAs per 32 keys
+  static constexpr int kBlocks = D / 32;              // output blocks of 32 dimensions
+  static constexpr int kGroupsPerCu = D <= 64 ? 2 : 1;
+};
+
+struct PrefixArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  uint16_t* out;
+  int64_t o_row, o_head;
+  float* lse;
+  int64_t l_row, l_head;
+  const uint16_t* k;
+  int64_t k_block, k_token, k_head;
+  const uint16_t* v;
+  int64_t v_block, v_token, v_head;
+  const int32_t* table;
+  int64_t bt_stride;
+  int capacity;  // keys that a table row can address
+  int num_blocks, block_size;
+  float per_block;  // 1 / block_size
+  const int32_t* q_start;
+  const int32_t* q_len;
+  const int32_t* t_len;
+  const int32_t* prefix_len;
+  int rows, tokens, hkv, group;
+  float scale_log2;
+  float* pieces;
+  int slots;
+  int groups;  // workgroups of the attention kernel
+  int32_t* status;
+};
+
+// ---------------------------------------------------------------------------------------------
+// The layout of the work, derived by every workgroup from the lengths.
+// ---------------------------------------------------------------------------------------------
+struct Plan {
+  int prefix;      // shared keys
+  int prefix_row;  // row whose table the prefix is read through
+  int seen_by_all;  // keys that every query token sees
+  int query_tokens;
+  int prefix_tile;   // query rows of a prefix tile
+  int row_tiles;     // prefix tiles of query rows, per KV head
+  int key_tiles;     // tiles of prefix keys
+  int segments;
+  int share;         // key tiles per workgroup, and per prefix segment
+  int prefix_work;   // key tiles of all prefix units
+  int prefix_units;
+  int work;          // key tiles of all units
+};
+
+struct RowTables {
+  int token[kMaxRows + 1];  // query tokens of the rows before
+  int work[kMaxRows + 1];   // own key tiles of the rows before, per KV head
+  int unit[kMaxRows + 1];   // own units of the rows before, per KV head
+};
+
+struct Row {
+  int start, len, keys;
+};
+
+// Row b's query tokens and keys; len 0 for a row without query tokens or with tokens out of range.
+__device__ __forceinline__ Row row_of(const PrefixArgs& a, int b) {
+  Row r{a.q_start[b], a.q_len[b], a.t_len[b]};
+  if (r.len <= 0 || r.start < 0 || r.len > a.tokens || r.start > a.tokens - r.len) r.len = 0;
+  r.keys = min(max(r.keys, 0), a.capacity);
+  return r;
+}
+
+__device__ __forceinline__ int tile_rows(int rows) { return rows > kNarrowRows ? kWideRows : kNarrowRows; }
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+template <int THREADS>
+__device__ __forceinline__ int block_min(int v, int* scratch) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = scratch[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) v = min(v, scratch[w]);
+  return v;
+}
+
+template <int THREADS>
+__device__ __forceinline__ int block_scan(int v, int* scratch, int& total) {
+  const int inc = wave_inclusive_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = inc;
+  __syncthreads();
+  int base = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const int s = scratch[w];
+    if (w < static_cast<int>(threadIdx.x >> 6)) base += s;
+    total += s;
+  }
+  return base + inc - v;
+}
+
+template <int D, int THREADS>
+__device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, int* scratch, bool report) {
+  constexpr int kTile = Shape<D>::kTile;
+  Plan p;
+  // Query tokens before each row.  Rows that would bring the sum over the query's own tokens (rows
+  // that overlap) are left out, which also bounds the workspace.
+  int carry = 0, first = INT_MAX, least = INT_MAX, seen = INT_MAX, count = 0, cut = INT_MAX;
+  for (int base = 0; base < a.rows; base += THREADS) {
+    const int b = base + static_cast<int>(threadIdx.x);
+    Row r{0, 0, 0};
+    if (b < a.rows) r = row_of(a, b);
+    int total;
+    const int before = carry + block_scan<THREADS>(r.len, scratch, total);
+    const bool fits = before <= a.tokens - r.len;
+    if (b < a.rows) t.token[b] = before;
+    if (!fits) cut = min(cut, before);
+    if (report && b < a.rows && a.status) {
+      const uint32_t bits = ((a.q_len[b] > 0 && (r.len == 0 || !fits)) ? kStatusRow : 0u) |
+                            (a.t_len[b] > a.capacity ? kStatusLength : 0u);
+      if (bits) __hip_atomic_fetch_or(a.status, static_cast<int>(bits), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (r.len > 0 && fits && r.keys > 0) {
+      first = min(first, b);
+      least = min(least, r.keys);
+      ++count;
+    }
+    if (r.len > 0) seen = min(seen, r.keys - r.len + 1);
+    carry = min(carry + total, a.tokens + 1);
+  }
+  first = block_min<THREADS>(first, scratch);
+  least = block_min<THREADS>(least, scratch);
+  cut = min(block_min<THREADS>(cut, scratch), carry);
+  p.seen_by_all = block_min<THREADS>(seen, scratch);
+  int rows_with_keys;
+  block_scan<THREADS>(count, scratch, rows_with_keys);
+  for (int b = threadIdx.x; b <= a.rows; b += THREADS) t.token[b] = b < a.rows ? min(t.token[b], cut) : cut;
+  __syncthreads();
+  // A single row has nobody to share with: all its keys are its own.
+  p.prefix = rows_with_keys > 1 ? min(max(a.prefix_len[0], 0), least) : 0;
+  p.prefix_row = rows_with_keys > 0 ? first : 0;
+  p.query_tokens = t.token[a.rows];
+  const int m = p.query_tokens * a.group;
+  p.prefix_tile = tile_rows(m);
+  p.row_tiles = ceil_div(m, p.prefix_tile);
+  p.key_tiles = ceil_div(p.prefix, kTile);
+  p.prefix_work = a.hkv * p.row_tiles * p.key_tiles;
+  // Own units.
+  int work = 0, units = 0;
+  for (int base = 0; base < a.rows; base += THREADS) {
+    const int b = base + static_cast<int>(threadIdx.x);
+    int n = 0, w = 0;
+    if (b < a.rows) {
+      const Row r = row_of(a, b);
+      if (r.len > 0 && t.token[b + 1] - t.token[b] == r.len && r.keys > p.prefix) {
+        const int own = r.len * a.group;
+        n = ceil_div(own, tile_rows(own));
+        w = n * ceil_div(r.keys - p.prefix, kTile);
+      }
+    }
+    int total;
+    const int wb = work + block_scan<THREADS>(w, scratch, total);
+    work += total;
+    const int ub = units + block_scan<THREADS>(n, scratch, total);
+    units += total;
+    if (b < a.rows) {
+      t.work[b] = wb;
+      t.unit[b] = ub;
+    }
+  }
+  if (threadIdx.x == 0) {
+    t.work[a.rows] = work;
+    t.unit[a.rows] = units;
+  }
+  __syncthreads();
+  p.work = p.prefix_work + a.hkv * work;
+  p.share = max(1, ceil_div(p.work, a.groups));
+  p.segments = ceil_div(p.key_tiles, p.share);
+  p.prefix_units = a.hkv * p.segments * p.row_tiles;
+  return p;
+}
+
+// One unit and where its key tiles lie in the work.
+struct Unit {
+  int index;      // in the order of the work
+  int kv_head;
+  int row;        // own units: the row; prefix units: -1
+  int tile;       // tile of query rows
+  int rows;       // query rows in all (of the row, or of the batch)
+  int tile_rows;
+  int first_work; // place of its first key tile in the work
+  int key_tiles;
+  int key0;       // first key
+  int key_end;    // one past the last key of the unit's range
+};
+
+template <int D>
+__device__ __forceinline__ Unit prefix_unit(const PrefixArgs& a, const Plan& p, int h, int segment, int tile) {
+  constexpr int kTile = Shape<D>::kTile;
+  Unit u;
+  const int before = segment * p.share;
+  u.key_tiles = min(p.share, p.key_tiles - before);
+  u.index = (h * p.segments + segment) * p.row_tiles + tile;
+  u.kv_head = h;
+  u.row = -1;
+  u.tile = tile;
+  u.rows = p.query_tokens * a.group;
+  u.tile_rows = p.prefix_tile;
+  u.first_work = (h * p.key_tiles + before) * p.row_tiles + tile * u.key_tiles;
+  u.key0 = before * kTile;
+  u.key_end = min(p.prefix, u.key0 + u.key_tiles * kTile);
+  return u;
+}
+
+template <int D>
+__device__ __forceinline__ Unit own_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, int b, int h,
+                                         int tile) {
+  Unit u;
+  const int n = t.unit[b + 1] - t.unit[b], w = t.work[b + 1] - t.work[b];
+  u.index = p.prefix_units + a.hkv * t.unit[b] + h * n + tile;
+  u.kv_head = h;
+  u.row = b;
+  u.tile = tile;
+  u.rows = (t.token[b + 1] - t.token[b]) * a.group;
+  u.tile_rows = tile_rows(u.rows);
+  u.key_tiles = w / n;
+  u.first_work = p.prefix_work + a.hkv * t.work[b] + h * w + tile * u.key_tiles;
+  u.key0 = p.prefix;
+  u.key_end = min(max(a.t_len[b], 0), a.capacity);
+  return u;
+}
+
+// The unit that holds place `w` of the work.
+template <int D>
+__device__ __forceinline__ Unit unit_at(const PrefixArgs& a, const Plan& p, const RowTables& t, int w) {
+  if (w < p.prefix_work) {
+    const int per_head = p.row_tiles * p.key_tiles;
+    const int h = w / per_head, rest = w - h * per_head;
+    const int segment = rest / (p.share * p.row_tiles);
+    const int in_segment = rest - segment * p.share * p.row_tiles;
+    const int len = min(p.share, p.key_tiles - segment * p.share);
+    return prefix_unit<D>(a, p, h, segment, in_segment / len);
+  }
+  const int rest = w - p.prefix_work;
+  int lo = 0, hi = a.rows - 1;  // the last row whose work starts at or before `rest`
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.hkv * t.work[mid] <= rest) lo = mid; else hi = mid - 1;
+  }
+  const int mine = t.work[lo + 1] - t.work[lo], n = t.unit[lo + 1] - t.unit[lo];
+  const int in_row = rest - a.hkv * t.work[lo];
+  const int h = in_row / mine;
+  return own_unit<D>(a, p, t, lo, h, (in_row - h * mine) / (mine / n));
+}
+
+// Row of the batch that holds query token `token` of the packed order.
+__device__ __forceinline__ int row_at(const PrefixArgs& a, const RowTables& t, int token) {
+  int lo = 0, hi = a.rows - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.token[mid] <= token) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// A query row of a unit: its token in the query tensor, its head and the keys it sees.
+struct QueryRow {
+  int token, head, limit;
+  bool valid;
+};
+__device__ __forceinline__ QueryRow query_row(const PrefixArgs& a, const RowTables& t, const Unit& u, int r) {
+  QueryRow q{0, 0, INT_MAX, r < u.rows};
+  if (q.valid) {
+    const int token = r / a.group;
+    int b = u.row, i = token;
+    if (b < 0) {
+      b = row_at(a, t, token);
+      i = token - t.token[b];
+    }
+    const Row row = row_of(a, b);
+    q.token = row.start + i;
+    q.head = u.kv_head * a.group + (r - token * a.group);
+    q.limit = row.keys - row.len + i + 1;
+  }
+  return q;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Matrix products: 32x32x16, A rows and B columns of 32, k-slot (lane / 32, e) = 8 (lane / 32) + e;
+// result i of a lane is row 8 (i / 4) + 4 (lane / 32) + i % 4 of column lane % 32.
+// ---------------------------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(u32x4 x, u32x4 y, f32x16 c) {
+  if constexpr (DT == DS_BF16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0,
+                                                   0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0,
+                                                  0);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (DT == DS_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {static_cast<__bf16>(x), static_cast<__bf16>(y)};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 v = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+// Combines a lane's value with lane ^ 32's.
+__device__ __forceinline__ float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// Where 16-byte piece `c` of staged key `t` lies (in pieces): the pieces of eight neighbouring keys
+// are turned against each other by two, so that the score MFMAs' reads (one piece of 32 keys) and
+// the transposing reads of the values (two pieces of four keys) touch all banks.
+template <int D>
+__device__ __forceinline__ int piece_at(int t, int c) {
+  const int turn = D >= 128 ? 2 * (t & 7) : 2 * ((t >> 1) & 3);
+  return t * (D / 8) + (c ^ turn);
+}
+
+// A tile's keys and values in flight to shared memory.
+template <int D>
+struct Staged {
+  u32x4 k[Shape<D>::kPasses], v[Shape<D>::kPasses];
+  int page[Shape<D>::kPasses];  // of the next tile
+};
+
+// Where a tile begins: its first key, and that key's page (in the table) and place.  Tiles follow
+// each other, so a key's page comes from the place and the distance, both small: (n + 0.5) / size in
+// floating point gives the exact quotient for n < 2^22 (the half keeps it away from the integers by
+// 0.5 / size, more than the 2^-23 relative error of a product with a rounded reciprocal).
+struct Cursor {
+  int key, page, place;
+};
+__device__ __forceinline__ int pages_in(const PrefixArgs& a, int n) {
+  return static_cast<int>((static_cast<float>(n) + 0.5f) * a.per_block);
+}
+__device__ __forceinline__ void advance(const PrefixArgs& a, Cursor& c, int keys) {
+  const int n = __builtin_amdgcn_readfirstlane(pages_in(a, c.place + keys));
+  c.key += keys;
+  c.page += n;
+  c.place += keys - n * a.block_size;
+}
+
+// Keys past the range take the place of its last one, and are zeroed on their way to shared memory.
+template <int D>
+__device__ __forceinline__ int staged_key(const Cursor& c, int i, int key_end) {
+  using S = Shape<D>;
+  return min(i * S::kPerPass + static_cast<int>(threadIdx.x) / S::kLanes, key_end - 1 - c.key);
+}
+
+template <int D>
+__device__ __forceinline__ void find_pages(const PrefixArgs& a, const int32_t* table, const Cursor& c, int key_end,
+                                           Staged<D>& s) {
+  if (c.key >= key_end) return;
+#pragma unroll
+  for (int i = 0; i < Shape<D>::kPasses; ++i) {
+    s.page[i] = table[c.page + pages_in(a, c.place + staged_key<D>(c, i, key_end))];
+  }
+}
+
+template <int D, bool ONCE>
+__device__ __forceinline__ void load_tile(const PrefixArgs& a, const Cursor& c, int key_end, int h, Staged<D>& s) {
+  using S = Shape<D>;
+  if (c.key >= key_end) return;
+  const uint16_t* keys = a.k + h * a.k_head + 8 * (static_cast<int>(threadIdx.x) % S::kLanes);
+  const uint16_t* values = a.v + h * a.v_head + 8 * (static_cast<int>(threadIdx.x) % S::kLanes);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < S::kPasses; ++i) {
+    const int n = c.place + staged_key<D>(c, i, key_end);
+    const int64_t in = n - pages_in(a, n) * a.block_size;
+    const bool fine = static_cast<unsigned>(s.page[i]) < static_cast<unsigned>(a.num_blocks);
+    const int64_t page = fine ? s.page[i] : 0;
+    const u32x4* kp = reinterpret_cast<const u32x4*>(keys + page * a.k_block + in * a.k_token);
+    const u32x4* vp = reinterpret_cast<const u32x4*>(values + page * a.v_block + in * a.v_token);
+    s.k[i] = ONCE ? __builtin_nontemporal_load(kp) : *kp;
+    s.v[i] = ONCE ? __builtin_nontemporal_load(vp) : *vp;
+    bad |= !fine;
+  }
+  if (__any(bad)) {
+#pragma unroll
+    for (int i = 0; i < S::kPasses; ++i) {
+      if (static_cast<unsigned>(s.page[i]) >= static_cast<unsigned>(a.num_blocks)) {
+        s.k[i] = u32x4{0, 0, 0, 0};
+        s.v[i] = u32x4{0, 0, 0, 0};
+      }
+    }
+    if (bad && a.status) {
+      __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void store_tile(Staged<D>& s, u32x4* keys, u32x4* values, int key, int key_end) {
+  using S = Shape<D>;
+  const int piece = static_cast<int>(threadIdx.x) % S::kLanes;
+  if (key + S::kTile > key_end) {
+#pragma unroll
+    for (int i = 0; i < S::kPasses; ++i) {
+      if (key + i * S::kPerPass + static_cast<int>(threadIdx.x) / S::kLanes >= key_end) {
+        s.k[i] = u32x4{0, 0, 0, 0};
+        s.v[i] = u32x4{0, 0, 0, 0};
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < S::kPasses; ++i) {
+    const int t = i * S::kPerPass + static_cast<int>(threadIdx.x) / S::kLanes;
+    keys[piece_at<D>(t, piece)] = s.k[i];
+    values[piece_at<D>(t, piece)] = s.v[i];
+  }
+}
+
+// Four values of one dimension, keys t .. t + 3, for each lane: lane l of 16 names key t + l / 4 and
+// dimensions 4 (l % 4) .. + 3 of the 16 that the group of lanes covers, and gets dimension l.
+template <int D>
+__device__ __forceinline__ u32x2 read_values(const u32x4* values, int t, int dim) {
+  const int l = threadIdx.x & 15;
+  const int at = piece_at<D>(t + (l >> 2), (dim >> 3) + ((l & 3) >> 1));
+  const lds_s16x4* p =
+      (const lds_s16x4*)(reinterpret_cast<const char*>(values + at) + 8 * (l & 1));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>(p)));
+}
+
+__device__ __forceinline__ bool not_finite2(uint32_t w, uint32_t exponent) {
+  return (w & exponent) == exponent || (w & (exponent << 16)) == (exponent << 16);
+}
+
+// A wave's softmax state for its 32 query rows (one per lane column): running maximum, the lane's
+// part of the sum, and the unnormalised output of the lane's dimensions.
+template <int D>
+struct State {
+  f32x16 acc[Shape<D>::kBlocks];
+  float m, l;
+};
+
+// A masked key of a tile may hold infinities or NaN, which a probability of 0 does not cancel in the
+// product, while another column sees that key.  The product then takes such values as 0, and they
+// are added to the columns that see them (where the sum is no longer finite whatever the weight).
+// `seen` is how many of the 32 keys from t0 on the lane column's query row sees.
+template <int DT, int D>
+__device__ __forceinline__ void add_not_finite(const u32x4* values, State<D>& st, int t0, int seen) {
+  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll 1
+  for (int t = 0; t < 32; ++t) {
+#pragma unroll
+    for (int j = 0; j < Shape<D>::kBlocks; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x2 v = reinterpret_cast<const u32x2*>(values + piece_at<D>(t0 + t, 4 * j + i))[half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint16_t x = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
+          if (t < seen && (x & kExponent) == kExponent) st.acc[j][4 * i + e] += Elem<DT>::load(x);
+        }
+      }
+    }
+  }
+}
+
+// 32 keys of a staged tile for one wave, from key t0 of the tile on.  `seen` (MASKED): how many of
+// them the lane column's query row sees.
+template <int DT, int D, bool MASKED>
+__device__ __forceinline__ void attend_keys(const u32x4* keys, const u32x4* values, const u32x4 (&q)[Shape<D>::kSteps],
+                                            State<D>& st, int t0, int seen, float scale_log2) {
+  using S = Shape<D>;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  f32x16 sc;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) sc = mfma32<DT>(keys[piece_at<D>(t0 + (lane & 31), 2 * s + half)], q[s], sc);
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    sc[i] *= scale_log2;
+    if constexpr (MASKED) sc[i] = 8 * (i >> 2) + 4 * half + (i & 3) < seen ? sc[i] : -INFINITY;
+    top = fmaxf(top, sc[i]);
+  }
+  top = fmaxf(top, other_half(top));
+  if (__any(top > st.m)) {
+    const float m = fmaxf(st.m, top);
+    const float keep = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+    st.m = m;
+    st.l *= keep;
+#pragma unroll
+    for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.acc[j][i] *= keep;
+    }
+  }
+  const float m = st.m == -INFINITY ? 0.f : st.m;
+  u32x4 p[2];
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const float x = __builtin_amdgcn_exp2f(sc[i] - m), y = __builtin_amdgcn_exp2f(sc[i + 1] - m);
+    st.l += x + y;
+    p[i >> 3][(i & 7) >> 1] = pack2<DT>(x, y);
+  }
+  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
+  bool poison = false;
+  if constexpr (MASKED) {
+    bool bad = false;
+#pragma unroll 1
+    for (int c = half; c < D / 8; c += 2) {
+      const u32x4 v = values[piece_at<D>(t0 + (lane & 31), c)];
+      bad |= not_finite2(v[0], kExponent) || not_finite2(v[1], kExponent) || not_finite2(v[2], kExponent) ||
+             not_finite2(v[3], kExponent);
+    }
+    poison = __any(bad);
+  }
+  // The lane's own probabilities are the B operand: k-slot (half, e) of step s is key 16 s + 8 (e /
+  // 4) + 4 half + e % 4 of the 32, and the values are read in that order.
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int j = 0; j < S::kBlocks; ++j) {
+      const int dim = 32 * j + 16 * ((lane >> 4) & 1), t = t0 + 16 * s + 4 * half;
+      const u32x2 lo = read_values<D>(values, t, dim), hi = read_values<D>(values, t + 8, dim);
+      u32x4 v = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      if constexpr (MASKED) {
+        if (poison) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] &= ((v[e] & kExponent) == kExponent ? 0u : 0xffffu) |
+                    ((v[e] & (kExponent << 16)) == (kExponent << 16) ? 0u : 0xffff0000u);
+          }
+        }
+      }
+      st.acc[j] = mfma32<DT>(v, p[s], st.acc[j]);
+    }
+  }
+  if constexpr (MASKED) {
+    if (poison) add_not_finite<DT, D>(values, st, t0, seen);
+  }
+}
+
+// Pieces in the workspace: for each slot 128 maxima and 128 sums, then the outputs as the waves
+// hold them ([query block][4 x dimension group][lane] of 4 floats).
+template <int D>
+__device__ __forceinline__ float* piece_sums(const PrefixArgs& a, int slot) {
+  return a.pieces + static_cast<int64_t>(slot) * (kWideRows * (D + 2));
+}
+
+// The key tiles [from, to) of a unit, and the unit's piece.
+template <int DT, int D, bool WIDE, bool ONCE>
+__device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, const Unit& u,
+                                         int from, int to, int slot, u32x4* lds) {
+  using S = Shape<D>;
+  constexpr int kQ = WIDE ? 4 : 2;             // blocks of 32 query rows
+  constexpr int kT = S::kWaves / kQ;           // waves that share a block's keys
+  constexpr int kN = S::kTile / 32 / kT;       // blocks of 32 keys of a tile per wave
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int qb = wave / kT, tb = wave % kT;
+  const int r0 = u.tile * u.tile_rows + 32 * qb;
+  const QueryRow qr = query_row(a, t, u, r0 + (lane & 31));
+  u32x4 q[S::kSteps];
+  {
+    const uint16_t* src = a.q + qr.token * a.q_row + qr.head * a.q_head + 8 * (lane >> 5);
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s) {
+      q[s] = u32x4{0, 0, 0, 0};
+      if (qr.valid) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
+    }
+  }
+  // Keys past the last query row's limit (own units: the tile's last token sees most).
+  int key_end = u.key_end, seen_by_all = p.seen_by_all;
+  if (u.row >= 0) {
+    const Row row = row_of(a, u.row);
+    seen_by_all = row.keys - row.len + u.tile * u.tile_rows / a.group + 1;
+    const int last = (min((u.tile + 1) * u.tile_rows, u.rows) - 1) / a.group;
+    key_end = min(key_end, row.keys - row.len + last + 1);
+  }
+  to = min(to, ceil_div(key_end - u.key0, S::kTile));
+  const int32_t* table = a.table + static_cast<int64_t>(u.row < 0 ? p.prefix_row : u.row) * a.bt_stride;
+
+  State<D> st;
+#pragma unroll
+  for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) st.acc[j][i] = 0.f;
+  }
+  st.m = -INFINITY;
+  st.l = 0.f;
+
+  Staged<D> s;
+  if (from < to) {
+    int key = u.key0 + from * S::kTile;
+    Cursor c{key, key / a.block_size, 0};  // of the tile whose pages are looked up next
+    c.place = key - c.page * a.block_size;
+    find_pages<D>(a, table, c, key_end, s);
+    load_tile<D, ONCE>(a, c, key_end, u.kv_head, s);
+    advance(a, c, S::kTile);
+    find_pages<D>(a, table, c, key_end, s);
+    __syncthreads();  // the unit before has read its last tile
+    store_tile<D>(s, lds, lds + S::kBuffer / 8, key, key_end);
+    load_tile<D, ONCE>(a, c, key_end, u.kv_head, s);
+    advance(a, c, S::kTile);
+    find_pages<D>(a, table, c, key_end, s);
+    lds_barrier();
+    int cur = 0, i = from;
+    auto stage_next = [&]() {
+      key += S::kTile;
+      if (++i < to) {
+        u32x4* next = lds + (cur ^ 1) * (S::kBuffer / 4);
+        store_tile<D>(s, next, next + S::kBuffer / 8, key, key_end);
+        load_tile<D, ONCE>(a, c, key_end, u.kv_head, s);
+        advance(a, c, S::kTile);
+        find_pages<D>(a, table, c, key_end, s);
+      }
+      lds_barrier();
+      cur ^= 1;
+    };
+    // Tiles that all query rows see whole, then the ones with a mask.
+    while (i < to && key + S::kTile <= min(seen_by_all, key_end)) {
+      const u32x4* staged = lds + cur * (S::kBuffer / 4);
+      if (r0 < u.rows) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          attend_keys<DT, D, false>(staged, staged + S::kBuffer / 8, q, st, 32 * (tb * kN + n), 32, a.scale_log2);
+        }
+      }
+      stage_next();
+    }
+    while (i < to) {
+      const u32x4* staged = lds + cur * (S::kBuffer / 4);
+      if (r0 < u.rows) {
+        const int seen = min(qr.limit, key_end) - key;
+#pragma unroll 1
+        for (int t0 = 32 * tb * kN; t0 < 32 * (tb + 1) * kN; t0 += 32) {
+          attend_keys<DT, D, true>(staged, staged + S::kBuffer / 8, q, st, t0, seen - t0, a.scale_log2);
+        }
+      }
+      stage_next();
+    }
+  }
+  st.l += other_half(st.l);
+
+  // The waves that share query rows join in shared memory.
+  if constexpr (kT > 1) {
+    constexpr int kWords = 16 * S::kBlocks;
+    float* area = reinterpret_cast<float*>(lds);  // [query block][wave after the first][output words, m, l][lane]
+    static_assert(kQ * (kT - 1) * (kWords + 2) * 64 * 4 <= 4 * S::kBuffer * 2, "the waves' results fit the tiles");
+    __syncthreads();
+    if (tb > 0) {
+      float* to_area = area + ((qb * (kT - 1) + tb - 1) * (kWords + 2)) * 64 + lane;
+#pragma unroll
+      for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to_area[(16 * j + i) * 64] = st.acc[j][i];
+      }
+      to_area[kWords * 64] = st.m;
+      to_area[(kWords + 1) * 64] = st.l;
+    }
+    __syncthreads();
+    if (tb == 0) {
+      for (int w = 0; w < kT - 1; ++w) {
+        const float* from_area = area + ((qb * (kT - 1) + w) * (kWords + 2)) * 64 + lane;
+        const float om = from_area[kWords * 64], ol = from_area[(kWords + 1) * 64];
+        const float m = fmaxf(st.m, om);
+        const float mine = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+        const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - m);
+        st.m = m;
+        st.l = st.l * mine + ol * other;
+#pragma unroll
+        for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st.acc[j][i] = st.acc[j][i] * mine + from_area[(16 * j + i) * 64] * other;
+        }
+      }
+    }
+  }
+  if (tb == 0 && r0 < u.rows && slot < a.slots) {
+    float* sums = piece_sums<D>(a, slot);
+    if (lane < 32) {
+      sums[32 * qb + lane] = st.m;
+      sums[kWideRows + 32 * qb + lane] = st.l;
+    }
+    f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kWideRows) + qb * (S::kBlocks * 4 * 64) + lane;
+#pragma unroll
+    for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[(4 * j + i) * 64] = f32x4{st.acc[j][4 * i], st.acc[j][4 * i + 1], st.acc[j][4 * i + 2], st.acc[j][4 * i + 3]};
+      }
+    }
+  }
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_attention_kernel(
+    PrefixArgs a) {
+  using S = Shape<D>;
+  __shared__ u32x4 lds[4 * S::kBuffer / 8];
+  __shared__ RowTables tables;
+  __shared__ int scratch[S::kWaves];
+  const Plan p = make_plan<D, S::kThreads>(a, tables, scratch, blockIdx.x == 0);
+  // Consecutive shares on one XCD (workgroups are dealt to the eight in turn).
+  const int per_xcd = a.groups / 8;
+  const int group = a.groups % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + static_cast<int>(blockIdx.x / 8)
+                                      : static_cast<int>(blockIdx.x);
+  int w = min(group * p.share, p.work);
+  const int end = min(w + p.share, p.work);
+  while (w < end) {
+    Unit u = unit_at<D>(a, p, tables, w);
+    const int from = w - u.first_work, to = min(u.key_tiles, end - u.first_work);
+    const int slot = u.index + group;
+    if (u.tile_rows != kWideRows) run_unit<DT, D, false, true>(a, p, tables, u, from, to, slot, lds);
+    else if (u.row >= 0 || p.row_tiles == 1) run_unit<DT, D, true, true>(a, p, tables, u, from, to, slot, lds);
+    else run_unit<DT, D, true, false>(a, p, tables, u, from, to, slot, lds);
+    w = u.first_work + to;
+  }
+}
+
+// Joins the pieces of 32 query rows of one KV head (the batch's order): a wave per 32 dimensions.
+template <int DT, int D>
+__global__ __launch_bounds__(2 * D) void prefix_join_kernel(PrefixArgs a) {
+  using S = Shape<D>;
+  __shared__ RowTables tables;
+  __shared__ int scratch[S::kBlocks];
+  const Plan p = make_plan<D, 2 * D>(a, tables, scratch, false);
+  const int rows = p.query_tokens * a.group, blocks = ceil_div(rows, 32);
+  const int h = blockIdx.y, block = blockIdx.x;
+  if (block >= blocks) return;
+  const int j = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int r = 32 * block + (lane & 31);
+  const bool valid = r < rows;
+  const int token = (valid ? r : rows - 1) / a.group;
+  const int b = row_at(a, tables, token), i = token - tables.token[b];
+
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto join = [&](const Unit& u, int row_in_tile) {
+    const int first = u.first_work / p.share, last = (u.first_work + u.key_tiles - 1) / p.share;
+    const int qb = row_in_tile >> 5, at = (row_in_tile & 31) + (lane & 32);
+    for (int g = first; g <= last; ++g) {
+      const float* sums = piece_sums<D>(a, u.index + g);
+      const float om = sums[row_in_tile], ol = sums[kWideRows + row_in_tile];
+      const f32x4* o = reinterpret_cast<const f32x4*>(sums + 2 * kWideRows) + (qb * S::kBlocks + j) * 4 * 64 + at;
+      f32x4 part[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) part[k] = o[k * 64];
+      const float top = fmaxf(m, om);
+      const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+      const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - top);
+      m = top;
+      l = l * mine + ol * other;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] = acc[k] * mine + part[k] * other;
+    }
+  };
+  const int tile = 32 * block / p.prefix_tile;
+  for (int segment = 0; segment < p.segments; ++segment) {
+    join(prefix_unit<D>(a, p, h, segment, tile), 32 * block - tile * p.prefix_tile + (lane & 31));
+  }
+  if (tables.work[b + 1] > tables.work[b]) {
+    const int in_row = i * a.group + (valid ? r : rows - 1) % a.group;
+    const int n = tile_rows((tables.token[b + 1] - tables.token[b]) * a.group);
+    join(own_unit<D>(a, p, tables, b, h, in_row / n), in_row % n);
+  }
+  if (!valid) return;
+  const int head = h * a.group + r % a.group;
+  const int64_t q_token = static_cast<int64_t>(a.q_start[b]) + i;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // nothing seen: zeros; NaN stays NaN
+  uint16_t* out = a.out + q_token * a.o_row + head * a.o_head + 32 * j + 4 * (lane >> 5);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const f32x4 x = acc[k] * inv;
+    *reinterpret_cast<u32x2*>(out + 8 * k) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+  }
+  if (a.lse && j == 0 && lane < 32) {
+    a.lse[q_token * a.l_row + head * a.l_head] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2P;
+  }
+}
+
+int attention_groups(int head_dim) { return device_cu_count() * (head_dim <= 64 ? 2 : 1); }
+
+// Pieces of a launch: units of the prefix (at most a segment per workgroup and one per tile of query
+// rows), units of the rows, and one more per workgroup where a share ends inside a unit.
+int64_t piece_slots(int rows, int tokens, int num_q_heads, int num_kv_heads, int head_dim) {
+  const int64_t query_rows = static_cast<int64_t>(tokens) * (num_q_heads / num_kv_heads);
+  const int64_t tiles = query_rows / kNarrowRows + 1;
+  return 2 * static_cast<int64_t>(attention_groups(head_dim)) + num_kv_heads * (2 * tiles + rows);
+}
+
+template <int DT, int D>
+int launch(hipStream_t stream, const PrefixArgs& a) {
+  prefix_attention_kernel<DT, D><<<a.groups, Shape<D>::kThreads, 0, stream>>>(a);
+  const int blocks = static_cast<int>((static_cast<int64_t>(a.tokens) * a.group + 31) / 32);
+  prefix_join_kernel<DT, D><<<dim3(blocks, a.hkv), 2 * D, 0, stream>>>(a);
+  return check_launch("ds_prefix_attention");
+}
+
+template <int DT>
+int launch_dim(hipStream_t stream, int d, const PrefixArgs& a) {
+  if (d == 64) return launch<DT, 64>(stream, a);
+  if (d == 128) return launch<DT, 128>(stream, a);
+  return launch<DT, 256>(stream, a);
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+size_t workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads, int head_dim) {
+  if (rows <= 0 || tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return 0;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
+  return static_cast<size_t>(piece_slots(rows, tokens, num_q_heads, num_kv_heads, head_dim)) * kWideRows *
+         (head_dim + 2) * sizeof(float);
+}
+
+int prefix_attention_impl(hipStream_t stream, const ds_prefix_attention_desc* d) {
+  DS_REQUIRE(d != nullptr, "null descriptor");
+  DS_REQUIRE(d->dtype == DS_BF16 || d->dtype == DS_FP16, "queries and KV caches must use BF16 or FP16");
+  DS_REQUIRE(d->rows >= 0 && d->tokens >= 0, "row and token counts must be non-negative");
+  DS_REQUIRE(d->num_q_heads > 0 && d->num_kv_heads > 0 && d->num_q_heads % d->num_kv_heads == 0,
+             "query heads must be divisible by KV heads");
+  DS_SUPPORTED(d->head_dim == 64 || d->head_dim == 128 || d->head_dim == 256, "head_dim must be 64, 128 or 256");
+  DS_SUPPORTED(d->rows <= kMaxRows, "at most %d rows", kMaxRows);
+  DS_REQUIRE(d->block_size > 0 && d->num_blocks > 0 && d->max_blocks > 0, "block sizes and counts must be positive");
+  DS_SUPPORTED(d->block_size <= (1 << 20), "at most 2^20 tokens per page");
+  if (d->rows == 0 || d->tokens == 0) return clear_error();
+  DS_REQUIRE(d->query && d->output && d->key_cache && d->value_cache && d->block_table && d->query_start &&
+                 d->query_len && d->target_len && d->prefix_len,
+             "null tensor pointer");
+  const int64_t strides[] = {d->q_row_stride,   d->q_head_stride,  d->o_row_stride,   d->o_head_stride, d->k_block_stride,
+                             d->k_token_stride, d->k_head_stride,  d->v_block_stride, d->v_token_stride, d->v_head_stride};
+  for (int64_t s : strides) DS_REQUIRE(s % 8 == 0, "row, page and head strides must be multiples of 8 elements");
+  DS_REQUIRE(aligned(d->query) && aligned(d->output) && aligned(d->key_cache) && aligned(d->value_cache),
+             "query, output and KV caches must be 16-byte aligned");
+  const size_t need = workspace_bytes(d->rows, d->tokens, d->num_q_heads, d->num_kv_heads, d->head_dim);
+  DS_REQUIRE(d->workspace && d->workspace_bytes >= need && (reinterpret_cast<uintptr_t>(d->workspace) & 255u) == 0,
+             "workspace must be 256-byte aligned and hold ds_prefix_attention_workspace_bytes()");
+  const int group = d->num_q_heads / d->num_kv_heads;
+  const int64_t capacity = std::min<int64_t>(static_cast<int64_t>(d->max_blocks) * d->block_size, 1 << 30);
+  const int tile = d->head_dim <= 128 ? 128 : 64;
+  const int64_t tiles = static_cast<int64_t>(d->tokens) * group / kNarrowRows + 1 + d->rows;
+  DS_SUPPORTED(d->tokens <= (1 << 20), "at most 2^20 query tokens");
+  DS_SUPPORTED(d->num_kv_heads * tiles * ((capacity + tile - 1) / tile + 1) * 2 < INT_MAX &&
+                   static_cast<int64_t>(d->tokens) * group < INT_MAX / 2 && d->num_kv_heads <= 65535,
+               "too many query tokens, KV heads or keys for one launch");
+  PrefixArgs a{};
+  a.q = static_cast<const uint16_t*>(d->query);
+  a.q_row = d->q_row_stride, a.q_head = d->q_head_stride;
+  a.out = static_cast<uint16_t*>(d->output);
+  a.o_row = d->o_row_stride, a.o_head = d->o_head_stride;
+  a.lse = d->lse;
+  a.l_row = d->lse_token_stride, a.l_head = d->lse_head_stride;
+  a.k = static_cast<const uint16_t*>(d->key_cache);
+  a.k_block = d->k_block_stride, a.k_token = d->k_token_stride, a.k_head = d->k_head_stride;
+  a.v = static_cast<const uint16_t*>(d->value_cache);
+  a.v_block = d->v_block_stride, a.v_token = d->v_token_stride, a.v_head = d->v_head_stride;
+  a.table = d->block_table;
+  a.bt_stride = d->bt_stride;
+  a.capacity = static_cast<int>(capacity);
+  a.num_blocks = d->num_blocks;
+  a.block_size = d->block_size;
+  a.per_block = 1.f / static_cast<float>(d->block_size);
+  a.q_start = d->query_start, a.q_len = d->query_len, a.t_len = d->target_len, a.prefix_len = d->prefix_len;
+  a.rows = d->rows, a.tokens = d->tokens, a.hkv = d->num_kv_heads, a.group = group;
+  a.scale_log2 = d->scale * kLog2eP;
+  a.pieces = static_cast<float*>(d->workspace);
+  a.slots = static_cast<int>(piece_slots(d->rows, d->tokens, d->num_q_heads, d->num_kv_heads, d->head_dim));
+  a.groups = attention_groups(d->head_dim);
+  a.status = d->status;
+  return d->dtype == DS_BF16 ? launch_dim<DS_BF16>(stream, d->head_dim, a) : launch_dim<DS_FP16>(stream, d->head_dim, a);
+}
+
+}  // namespace
+}  // namespace ds355
+
+extern "C" size_t ds_prefix_attention_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads,
+                                                      int head_dim) {
+  return ds355::workspace_bytes(rows, tokens, num_q_heads, num_kv_heads, head_dim);
+}
+
+extern "C" int ds_prefix_attention(ds_stream_t stream, const ds_prefix_attention_desc* desc) {
+  return ds355::prefix_attention_impl(reinterpret_cast<hipStream_t>(stream), desc);
+}

@@ -7,6 +7,7 @@ live on a GPU.  There is no CPU fallback.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -22,7 +23,7 @@ DS_STAGE_SCORE, DS_STAGE_SELECT, DS_STAGE_PLAN, DS_STAGE_ALL, DS_STAGE_PREFIX = 
 DS_STEP_SELECTORS_GATHER, DS_STEP_EXPIRE_WAITS = 1, 2
 # Regions of the static scratch of ds_retrieval_step_static (include/ds355.h).
 DS_STATIC_FUSED_BYTES, DS_STATIC_PARTIALS_BYTES, DS_STATIC_PAIRS_BYTES = 8 << 20, 4 << 20, 12 << 20
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 EXPORTED_SYMBOLS = (
     "ds_last_error",
@@ -37,6 +38,8 @@ EXPORTED_SYMBOLS = (
     "ds_draft_attention",
     "ds_draft_attention_workspace_bytes",
     "ds_capture_raw_kv",
+    "ds_prefix_attention",
+    "ds_prefix_attention_workspace_bytes",
 )
 
 _DTYPES = {torch.bfloat16: DS_BF16, torch.float16: DS_FP16, torch.float32: DS_FP32}
@@ -92,6 +95,27 @@ class StepDesc(ctypes.Structure):
     ]
 
 
+class PrefixAttentionDesc(ctypes.Structure):
+    """Mirror of ``ds_prefix_attention_desc`` (include/ds355.h)."""
+
+    _fields_ = [
+        ("dtype", _i32),
+        ("query", _p), ("q_row_stride", _i64), ("q_head_stride", _i64),
+        ("output", _p), ("o_row_stride", _i64), ("o_head_stride", _i64),
+        ("lse", _p), ("lse_token_stride", _i64), ("lse_head_stride", _i64),
+        ("key_cache", _p), ("k_block_stride", _i64), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("value_cache", _p), ("v_block_stride", _i64), ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("block_table", _p), ("bt_stride", _i64), ("max_blocks", _i32),
+        ("num_blocks", _i32), ("block_size", _i32),
+        ("query_start", _p), ("query_len", _p), ("target_len", _p), ("prefix_len", _p),
+        ("rows", _i32), ("tokens", _i32),
+        ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("scale", _f32),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+        ("status", _p),
+    ]
+
+
 _SIGNATURES = {
     "ds_last_error": (ctypes.c_char_p, []),
     "ds_abi_version": (_i32, []),
@@ -117,6 +141,8 @@ _SIGNATURES = {
         _p, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i32, _p, _i32, _p, _p,
         _i32, _i32, _i32, _i32, _p, _p, _p, _i32, _i32, _p,
     ]),
+    "ds_prefix_attention": (_i32, [_p, ctypes.POINTER(PrefixAttentionDesc)]),
+    "ds_prefix_attention_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32, _i32]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -234,6 +260,16 @@ def stream_handle(device: torch.device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_same_device = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` current for a launch on one of its streams (nothing to do when it is)."""
+    if device.index is None or torch.cuda.current_device() == device.index:
+        return _same_device
+    return torch.cuda.device(device)
 
 
 def require_gpu(*tensors: torch.Tensor | None) -> torch.device:

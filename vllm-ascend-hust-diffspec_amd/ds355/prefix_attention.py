@@ -1,0 +1,166 @@
+"""Paged attention of a verified batch that shares a long prefix (two HIP launches).
+
+The reference leaves the target model's attention to its platform and
+captures query, softmax LSE and paged keys from it
+(diffspec/ascend_patch.py:191-240, diffspec/runtime.py:841-878).  This is that
+attention for a batch whose rows agree on their first ``prefix_len`` tokens
+(requests forked from one prompt): the prefix's keys and values are read once
+for all rows' query tokens, each row's own tokens row by row, and the pieces
+are joined by their softmax statistics.  The LSE it writes is what
+``step.VerifierSnapshot`` and ``kernels.paged_chunk_attention_scores`` take.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+__all__ = ["prefix_workspace_bytes", "new_prefix_workspace", "shared_prefix_attention"]
+
+STATUS_BAD_ROW = 1
+STATUS_LENGTH = 2
+STATUS_BAD_PAGE = 4
+
+
+def prefix_workspace_bytes(batch_rows: int, tokens: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of the workspace for up to ``batch_rows`` rows and ``tokens`` query tokens."""
+    return int(_lib.load().ds_prefix_attention_workspace_bytes(batch_rows, tokens, num_q_heads, num_kv_heads,
+                                                               head_dim))
+
+
+def new_prefix_workspace(batch_rows: int, tokens: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                         device: torch.device | str) -> torch.Tensor:
+    """A workspace (uint8); it keeps nothing between calls, and serves one launch at a time."""
+    size = prefix_workspace_bytes(batch_rows, tokens, num_q_heads, num_kv_heads, head_dim)
+    if size <= 0:
+        raise ValueError("workspace sizes must be positive, num_q_heads a multiple of num_kv_heads and head_dim "
+                         "64, 128 or 256")
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def _layout(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def shared_prefix_attention(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    output: torch.Tensor,
+    lse: torch.Tensor | None,
+    block_table: torch.Tensor,
+    query_start: torch.Tensor,
+    query_len: torch.Tensor,
+    target_len: torch.Tensor,
+    prefix_len: torch.Tensor,
+    *,
+    scale: float,
+    workspace: torch.Tensor,
+    batch_size: int | None = None,
+    status: torch.Tensor | None = None,
+    reuse: dict | None = None,
+) -> torch.Tensor:
+    """Attention of ragged query rows over paged keys and values, causal at each row's end.
+
+    ``query`` / ``output`` ``[tokens, Hq, D]`` (bf16 or fp16, rows contiguous
+    in D), ``key_cache`` / ``value_cache`` ``[blocks, block_size, Hkv, D]``,
+    ``block_table`` int32 ``[rows, *]``; ``query_start`` / ``query_len`` /
+    ``target_len`` int32 ``[rows]`` as in ``step.VerifierRows``: row b's
+    query tokens are the last ``query_len[b]`` of its ``target_len[b]``
+    tokens.  ``lse`` fp32 ``[tokens, Hq]`` (any strides) or None.
+    ``prefix_len`` is an int32 device word: every row's first
+    ``prefix_len`` keys are the same, and are read through one row's table;
+    0 when the rows share nothing.  A query token that sees no key gets a
+    zero output and an LSE of -infinity; output and LSE rows of tokens that
+    no row has (graph padding) are left as they were.  Rows at or beyond
+    ``batch_size`` are padding.  Rows must not share query tokens.
+
+    ``status`` (an int32 device word the caller clears) receives
+    ``STATUS_BAD_ROW``, ``STATUS_LENGTH`` and ``STATUS_BAD_PAGE``
+    (include/ds355.h).  ``reuse`` (a dict the caller keeps) holds the
+    validated descriptor of each layout (shapes, strides, types, devices): a
+    later call of the same layout skips the checks; every address is taken
+    from the call.  Returns ``output``.
+    """
+    key = None
+    if reuse is not None:
+        key = (_layout(query), _layout(key_cache), _layout(value_cache), _layout(output), _layout(lse),
+               _layout(block_table), _layout(query_start), _layout(query_len), _layout(target_len),
+               _layout(prefix_len), _layout(workspace), _layout(status), batch_size)
+        hit = reuse.get(key)
+        if hit is not None:
+            return _launch(hit[0], hit[1], query, key_cache, value_cache, output, lse, block_table, query_start,
+                           query_len, target_len, prefix_len, scale, workspace, status)
+    if query.ndim != 3 or output.shape != query.shape:
+        raise ValueError("query and output must both be [tokens, query_heads, head_dim]")
+    if key_cache.ndim != 4 or value_cache.shape != key_cache.shape:
+        raise ValueError("key and value caches must both be [blocks, block_size, kv_heads, head_dim]")
+    tokens, hq, head_dim = query.shape
+    blocks, block_size, hkv, key_dim = key_cache.shape
+    if key_dim != head_dim:
+        raise ValueError("query and key head dimensions must match")
+    if hkv == 0 or hq % hkv != 0:
+        raise ValueError("query heads must be divisible by KV heads")
+    for name, t in (("query", query), ("output", output), ("key cache", key_cache), ("value cache", value_cache)):
+        if t.dtype != query.dtype:
+            raise ValueError("query, output and KV caches must share a dtype")
+        if t.stride(-1) != 1:
+            raise ValueError(f"{name} must be contiguous in head_dim")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, hq)):
+        raise ValueError("lse must be fp32 [tokens, query_heads]")
+    rows = query_len.numel()
+    for name, t in (("query_start", query_start), ("query_len", query_len), ("target_len", target_len),
+                    ("prefix_len", prefix_len)):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor")
+    if query_start.numel() != rows or target_len.numel() != rows or prefix_len.numel() != 1:
+        raise ValueError("query_start, query_len and target_len need one entry per row, prefix_len one in all")
+    if batch_size is not None:
+        if not 0 <= batch_size <= rows:
+            raise ValueError("batch_size must be between zero and the number of rows")
+        rows = batch_size
+    if block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.stride(1) != 1 or \
+            block_table.shape[0] < rows:
+        raise ValueError("block_table must be int32 [rows, blocks] with unit last stride")
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor (see new_prefix_workspace)")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError("status must be an int32 device word")
+    device = _lib.require_gpu(query, key_cache, value_cache, output, lse, block_table, query_start, query_len,
+                              target_len, prefix_len, workspace, status)
+    desc = _lib.PrefixAttentionDesc()
+    desc.dtype = _lib.dtype_code(query.dtype)
+    desc.q_row_stride, desc.q_head_stride = query.stride(0), query.stride(1)
+    desc.o_row_stride, desc.o_head_stride = output.stride(0), output.stride(1)
+    if lse is not None:
+        desc.lse_token_stride, desc.lse_head_stride = lse.stride(0), lse.stride(1)
+    desc.k_block_stride, desc.k_token_stride, desc.k_head_stride = key_cache.stride()[:3]
+    desc.v_block_stride, desc.v_token_stride, desc.v_head_stride = value_cache.stride()[:3]
+    desc.bt_stride, desc.max_blocks = block_table.stride(0), block_table.shape[1]
+    desc.num_blocks, desc.block_size = blocks, block_size
+    desc.rows, desc.tokens = rows, tokens
+    desc.num_q_heads, desc.num_kv_heads, desc.head_dim = hq, hkv, head_dim
+    desc.workspace_bytes = workspace.numel()
+    _launch(desc, device, query, key_cache, value_cache, output, lse, block_table, query_start, query_len, target_len,
+            prefix_len, scale, workspace, status)
+    if key is not None:
+        if len(reuse) >= 64:
+            reuse.clear()
+        reuse[key] = (desc, device)
+    return output
+
+
+def _launch(desc, device, query, key_cache, value_cache, output, lse, block_table, query_start, query_len, target_len,
+            prefix_len, scale, workspace, status):
+    desc.query, desc.output, desc.lse = query.data_ptr(), output.data_ptr(), _lib.ptr(lse)
+    desc.key_cache, desc.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
+    desc.block_table, desc.query_start = block_table.data_ptr(), query_start.data_ptr()
+    desc.query_len, desc.target_len = query_len.data_ptr(), target_len.data_ptr()
+    desc.prefix_len, desc.workspace, desc.status = prefix_len.data_ptr(), workspace.data_ptr(), _lib.ptr(status)
+    desc.scale = float(scale)
+    with _lib.on_device(device):
+        _lib.check(_lib.load().ds_prefix_attention(_lib.stream_handle(device), ctypes.byref(desc)))
+    return output
