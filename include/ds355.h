@@ -505,6 +505,58 @@ int ds_prefix_attention(ds_stream_t stream, const ds_prefix_attention_desc* desc
  */
 size_t ds_prefix_attention_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads, int head_dim);
 
+/*
+ * RMS norm of each query and key head with the position rotation in the
+ * same pass, and the write of the keys and values into a paged cache.
+ * The reference's models leave these to their platform; the rotation's two
+ * pairings are those of diffspec/compact_kv.py:68-101.
+ *
+ *   n = x / sqrt(mean(x^2) + eps) * weight     per head, over head_dim
+ *   y = n rotated at positions[t]              over the first rotary_dim
+ *       (cos at cos_sin[p, i], sin at cos_sin[p, rotary_dim / 2 + i])
+ *   query_out[t, h] = y of query; key_out[t, h] = y of key (or NULL);
+ *   normed_key[t, h] = n of key, not rotated (or NULL): what a draft whose
+ *       keys are normed captures into its raw cache (ds_capture_raw_kv);
+ *   with slot_mapping: key_cache[s / block_size, s % block_size, h] = y of
+ *       key and value_cache[...] = value, s = slot_mapping[t]; s < 0 writes
+ *       nothing (graph padding).  Slots must be distinct.
+ * Computed in fp32 and rounded once.  An output may be its input (the same
+ * address and strides); other overlaps are not allowed.  key_cache,
+ * value_cache, slot_mapping and value come together, or none (then value is
+ * not read).
+ * *status (optional, the caller clears it) gets bit 0 for a position outside
+ * [0, cs_rows) (nothing of that token is written), bit 1 for a slot past the
+ * cache (nothing of it is written there).
+ *
+ * dtype: DS_BF16, DS_FP16 or DS_FP32 for all heads and caches; the weights
+ * ([head_dim] each, contiguous) and the cos/sin cache in it or in DS_FP32.
+ * head_dim even and at most 256, contiguous; strides in elements.  Heads,
+ * strides and addresses in whole 4-element vectors move as vectors, others
+ * element by element.  One launch.
+ */
+typedef struct ds_qk_norm_rope_desc {
+  int dtype, weight_dtype, cos_sin_dtype;
+  const void* query; int64_t q_row_stride, q_head_stride;
+  const void* key; int64_t k_row_stride, k_head_stride;
+  const void* value; int64_t v_row_stride, v_head_stride;
+  const void* q_weight;
+  const void* k_weight;
+  const void* positions; int positions_int64;
+  const void* cos_sin; int64_t cs_stride; int cs_rows;
+  void* query_out; int64_t qo_row_stride, qo_head_stride;
+  void* key_out; int64_t ko_row_stride, ko_head_stride;
+  void* normed_key; int64_t nk_row_stride, nk_head_stride;
+  void* key_cache; int64_t kc_block_stride, kc_token_stride, kc_head_stride;
+  void* value_cache; int64_t vc_block_stride, vc_token_stride, vc_head_stride;
+  const void* slot_mapping; int slots_int64;
+  int num_blocks, block_size;
+  int tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim, is_neox_style;
+  float eps;
+  int32_t* status;
+} ds_qk_norm_rope_desc;
+
+int ds_qk_norm_rope(ds_stream_t stream, const ds_qk_norm_rope_desc* desc);
+
 #ifdef __cplusplus
 }
 #endif

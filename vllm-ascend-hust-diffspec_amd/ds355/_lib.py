@@ -40,6 +40,7 @@ EXPORTED_SYMBOLS = (
     "ds_capture_raw_kv",
     "ds_prefix_attention",
     "ds_prefix_attention_workspace_bytes",
+    "ds_qk_norm_rope",
 )
 
 _DTYPES = {torch.bfloat16: DS_BF16, torch.float16: DS_FP16, torch.float32: DS_FP32}
@@ -116,6 +117,31 @@ class PrefixAttentionDesc(ctypes.Structure):
     ]
 
 
+class QkNormRopeDesc(ctypes.Structure):
+    """Mirror of ``ds_qk_norm_rope_desc`` (include/ds355.h)."""
+
+    _fields_ = [
+        ("dtype", _i32), ("weight_dtype", _i32), ("cos_sin_dtype", _i32),
+        ("query", _p), ("q_row_stride", _i64), ("q_head_stride", _i64),
+        ("key", _p), ("k_row_stride", _i64), ("k_head_stride", _i64),
+        ("value", _p), ("v_row_stride", _i64), ("v_head_stride", _i64),
+        ("q_weight", _p), ("k_weight", _p),
+        ("positions", _p), ("positions_int64", _i32),
+        ("cos_sin", _p), ("cs_stride", _i64), ("cs_rows", _i32),
+        ("query_out", _p), ("qo_row_stride", _i64), ("qo_head_stride", _i64),
+        ("key_out", _p), ("ko_row_stride", _i64), ("ko_head_stride", _i64),
+        ("normed_key", _p), ("nk_row_stride", _i64), ("nk_head_stride", _i64),
+        ("key_cache", _p), ("kc_block_stride", _i64), ("kc_token_stride", _i64), ("kc_head_stride", _i64),
+        ("value_cache", _p), ("vc_block_stride", _i64), ("vc_token_stride", _i64), ("vc_head_stride", _i64),
+        ("slot_mapping", _p), ("slots_int64", _i32),
+        ("num_blocks", _i32), ("block_size", _i32),
+        ("tokens", _i32), ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("rotary_dim", _i32),
+        ("is_neox_style", _i32),
+        ("eps", _f32),
+        ("status", _p),
+    ]
+
+
 _SIGNATURES = {
     "ds_last_error": (ctypes.c_char_p, []),
     "ds_abi_version": (_i32, []),
@@ -143,6 +169,7 @@ _SIGNATURES = {
     ]),
     "ds_prefix_attention": (_i32, [_p, ctypes.POINTER(PrefixAttentionDesc)]),
     "ds_prefix_attention_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32, _i32]),
+    "ds_qk_norm_rope": (_i32, [_p, ctypes.POINTER(QkNormRopeDesc)]),
 }
 
 _lib: ctypes.CDLL | None = None
