@@ -557,6 +557,69 @@ typedef struct ds_qk_norm_rope_desc {
 
 int ds_qk_norm_rope(ds_stream_t stream, const ds_qk_norm_rope_desc* desc);
 
+/*
+ * Pages of a paged cache: copying, forking, growing, freeing and compacting
+ * rows.  The reference takes pages and block tables from the serving
+ * engine's host allocator (diffspec/runtime.py:869-875); this keeps them on
+ * the device.
+ *
+ * ref_counts: int32 [num_pages], how many rows hold a page (0: free).
+ * block_table: int32 [table_rows, table_width], row stride bt_stride: a
+ *   row's pages in order, -1 behind its last one.
+ * caches: device array of 4 int64 per cache tensor whose pages move
+ *   together: address, bytes between pages, bytes of a page (contiguous),
+ *   and 1 when all three are multiples of 16.  max_page_bytes is the largest.
+ * Free pages are taken in ascending order, for the list's entries in turn, so
+ * results depend on the state alone.  Lists are int32 device arrays of
+ * `count` entries; at most 4096 entries and 4096 table rows.
+ * workspace: ds_pages_workspace_bytes(), zero-filled once, 16-byte aligned;
+ *   one call at a time.
+ * *status (optional, the caller clears it): bit 0 an entry was left out (a row
+ *   out of range or named again, a negative length, a length beyond the
+ *   table's width or the parent's pages); bit 1 the pool ran out of free pages
+ *   (entries that did not get all theirs got none); bit 2 a page id was
+ *   outside the pool, or already free when a row gave it back.
+ * No host synchronisation; calls can be captured.  Calls that change one
+ * pool's state must be ordered (one stream).
+ */
+size_t ds_pages_workspace_bytes(int num_pages);
+
+/* caches[dst[i]] = caches[src[i]] in every cache.  Destinations are distinct
+ * and no entry's source (src[i] == dst[i] copies nothing). */
+int ds_pages_copy(ds_stream_t stream, const int64_t* caches, int num_caches, int64_t max_page_bytes,
+                  int num_pages, const int32_t* src, const int32_t* dst, int count, int32_t* status);
+
+/* Row children[i] gives its pages back and becomes the first lens[i] tokens
+ * of row parents[i]: it shares the full pages, and a last partial page is
+ * copied to a page of its own.  A child that an earlier entry names, or that
+ * is a parent in the list, is left out; without a free page it stays empty. */
+int ds_pages_fork(ds_stream_t stream, const int64_t* caches, int num_caches, int64_t max_page_bytes,
+                  int num_pages, int32_t* ref_counts, int32_t* block_table, int64_t bt_stride,
+                  int table_rows, int table_width, const int32_t* parents, const int32_t* children,
+                  const int32_t* lens, int count, int block_size, void* workspace, size_t workspace_bytes,
+                  int32_t* status);
+
+/* Row rows[i] gets as many free pages as lens[i] tokens need more than it
+ * holds (it never loses any). */
+int ds_pages_extend(ds_stream_t stream, int num_pages, int32_t* ref_counts, int32_t* block_table,
+                    int64_t bt_stride, int table_rows, int table_width, const int32_t* rows,
+                    const int32_t* lens, int count, int block_size, int32_t* status);
+
+/* Row rows[i] gives back the pages that its first keep_lens[i] tokens do not
+ * need (keep_lens NULL: all).  A row named twice keeps the smaller length. */
+int ds_pages_free(ds_stream_t stream, int num_pages, int32_t* ref_counts, int32_t* block_table,
+                  int64_t bt_stride, int table_rows, int table_width, const int32_t* rows,
+                  const int32_t* keep_lens, int count, int block_size, int32_t* status);
+
+/* Held pages move to the front: with n held pages, the k-th held page at or
+ * past n (ascending) moves to the k-th free page below n in every cache, and
+ * the counts and the table follow.  page_map[num_pages] gets each page's new
+ * place, -1 for free ones. */
+int ds_pages_compact(ds_stream_t stream, const int64_t* caches, int num_caches, int64_t max_page_bytes,
+                     int num_pages, int32_t* ref_counts, int32_t* block_table, int64_t bt_stride,
+                     int table_rows, int table_width, int32_t* page_map, void* workspace,
+                     size_t workspace_bytes, int32_t* status);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,6 +41,12 @@ EXPORTED_SYMBOLS = (
     "ds_prefix_attention",
     "ds_prefix_attention_workspace_bytes",
     "ds_qk_norm_rope",
+    "ds_pages_workspace_bytes",
+    "ds_pages_copy",
+    "ds_pages_fork",
+    "ds_pages_extend",
+    "ds_pages_free",
+    "ds_pages_compact",
 )
 
 _DTYPES = {torch.bfloat16: DS_BF16, torch.float16: DS_FP16, torch.float32: DS_FP32}
@@ -170,6 +176,16 @@ _SIGNATURES = {
     "ds_prefix_attention": (_i32, [_p, ctypes.POINTER(PrefixAttentionDesc)]),
     "ds_prefix_attention_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32, _i32]),
     "ds_qk_norm_rope": (_i32, [_p, ctypes.POINTER(QkNormRopeDesc)]),
+    "ds_pages_workspace_bytes": (ctypes.c_size_t, [_i32]),
+    "ds_pages_copy": (_i32, [_p, _p, _i32, _i64, _i32, _p, _p, _i32, _p]),
+    "ds_pages_fork": (_i32, [
+        _p, _p, _i32, _i64, _i32, _p, _p, _i64, _i32, _i32, _p, _p, _p, _i32, _i32, _p, ctypes.c_size_t, _p,
+    ]),
+    "ds_pages_extend": (_i32, [_p, _i32, _p, _p, _i64, _i32, _i32, _p, _p, _i32, _i32, _p]),
+    "ds_pages_free": (_i32, [_p, _i32, _p, _p, _i64, _i32, _i32, _p, _p, _i32, _i32, _p]),
+    "ds_pages_compact": (_i32, [
+        _p, _p, _i32, _i64, _i32, _p, _p, _i64, _i32, _i32, _p, _p, ctypes.c_size_t, _p,
+    ]),
 }
 
 _lib: ctypes.CDLL | None = None
