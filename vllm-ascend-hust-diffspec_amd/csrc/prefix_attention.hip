@@ -23,6 +23,8 @@
 // tiles inside a segment next to each other, and consecutive shares are given to one XCD, so the
 // row tiles that read the same keys do it at about the same time behind one L2.  A share that ends
 // inside a unit leaves its piece (m, l, O in fp32) in the workspace; prefix_join_kernel joins them.
+#include <cmath>
+
 #include "ds355_common.h"
 
 namespace ds355 {
@@ -46,16 +48,20 @@ constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
 template <int D>
 struct Shape {
-  static constexpr int kWaves = D == 128 ? 8 : 4;
+  static constexpr int kWaves = D <= 128 ? 8 : 4;
   static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kTile = D <= 128 ? 128 : 64;   // keys per tile
+  static constexpr int kTile = 16384 / D;             // keys per tile: 32 KiB of keys and of values
   static constexpr int kLanes = D / 8;                // 16-byte pieces of a key
   static constexpr int kPerPass = kThreads / kLanes;  // keys that one load of all threads covers
+  static constexpr int kPerLoad = 64 / kLanes;        // keys that one load of a wave covers
   static constexpr int kPasses = kTile / kPerPass;
-  static constexpr int kBuffer = kTile * D;           // elements of a staged tile of keys (or values)
+  // A staged key takes 16 bytes more than its elements, so that the 16-byte reads of eight
+  // neighbouring keys touch different banks; values lie close, their pieces turned (piece_at).
+  static constexpr int kKeyBytes = 2 * D + 16;
+  static constexpr int kValuesAt = kTile * kKeyBytes;
+  static constexpr int kStage = kValuesAt + kTile * 2 * D;  // bytes of a staged tile
   static constexpr int kSteps = D / 16;               // score MFMAs per 32 keys
   static constexpr int kBlocks = D / 32;              // output blocks of 32 dimensions
-  static constexpr int kGroupsPerCu = D <= 64 ? 2 : 1;
 };
 
 struct PrefixArgs {
@@ -79,7 +85,8 @@ struct PrefixArgs {
   const int32_t* t_len;
   const int32_t* prefix_len;
   int rows, tokens, hkv, group;
-  float scale_log2;
+  float scale_log2;  // |scale| log2 e
+  uint32_t q_sign;   // sign bits that a negative scale turns in the queries
   float* pieces;
   int slots;
   int groups;  // workgroups of the attention kernel
@@ -107,7 +114,8 @@ struct Plan {
 struct RowTables {
   int token[kMaxRows + 1];  // query tokens of the rows before
   int work[kMaxRows + 1];   // own key tiles of the rows before, per KV head
-  int unit[kMaxRows + 1];   // own units of the rows before, per KV head
+  int start[kMaxRows];      // first query token
+  int seen[kMaxRows];       // keys that its first query token sees, less one
 };
 
 struct Row {
@@ -124,109 +132,134 @@ __device__ __forceinline__ Row row_of(const PrefixArgs& a, int b) {
 
 __device__ __forceinline__ int tile_rows(int rows) { return rows > kNarrowRows ? kWideRows : kNarrowRows; }
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__device__ __forceinline__ int query_tiles(int rows) { return ceil_div(rows, tile_rows(rows)); }
 
-template <int THREADS>
-__device__ __forceinline__ int block_min(int v, int* scratch) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = min(v, __shfl_xor(v, off, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = scratch[0];
-#pragma unroll
-  for (int w = 1; w < THREADS / 64; ++w) v = min(v, scratch[w]);
-  return v;
+__device__ __forceinline__ int wave_min(int v) {
+  return static_cast<int>(wave_pick<false>(static_cast<uint32_t>(v) ^ 0x80000000u) ^ 0x80000000u);
 }
 
-template <int THREADS>
-__device__ __forceinline__ int block_scan(int v, int* scratch, int& total) {
-  const int inc = wave_inclusive_scan(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) scratch[threadIdx.x >> 6] = inc;
-  __syncthreads();
-  int base = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    const int s = scratch[w];
-    if (w < static_cast<int>(threadIdx.x >> 6)) base += s;
-    total += s;
-  }
-  return base + inc - v;
-}
+// What one wave's rows add to the plan, and the sums over the waves before it.
+struct Part {
+  int tokens, first, least, seen, cut, count;
+};
 
+// Rows are held a lane each, round by round of THREADS rows, and every wave sums the parts of all
+// waves itself: one barrier for the query tokens, one for the own work, one before the tables are read.
 template <int D, int THREADS>
-__device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, int* scratch, bool report) {
-  constexpr int kTile = Shape<D>::kTile;
+__device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, bool report) {
+  constexpr int kTile = Shape<D>::kTile, kRounds = kMaxRows / THREADS, kParts = kMaxRows / 64;
+  __shared__ Part parts[kParts];
+  __shared__ int part_work[kParts];
   Plan p;
-  // Query tokens before each row.  Rows that would bring the sum over the query's own tokens (rows
-  // that overlap) are left out, which also bounds the workspace.
-  int carry = 0, first = INT_MAX, least = INT_MAX, seen = INT_MAX, count = 0, cut = INT_MAX;
-  for (int base = 0; base < a.rows; base += THREADS) {
-    const int b = base + static_cast<int>(threadIdx.x);
-    Row r{0, 0, 0};
-    if (b < a.rows) r = row_of(a, b);
-    int total;
-    const int before = carry + block_scan<THREADS>(r.len, scratch, total);
-    const bool fits = before <= a.tokens - r.len;
-    if (b < a.rows) t.token[b] = before;
-    if (!fits) cut = min(cut, before);
-    if (report && b < a.rows && a.status) {
-      const uint32_t bits = ((a.q_len[b] > 0 && (r.len == 0 || !fits)) ? kStatusRow : 0u) |
-                            (a.t_len[b] > a.capacity ? kStatusLength : 0u);
-      if (bits) __hip_atomic_fetch_or(a.status, static_cast<int>(bits), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (r.len > 0 && fits && r.keys > 0) {
-      first = min(first, b);
-      least = min(least, r.keys);
-      ++count;
-    }
-    if (r.len > 0) seen = min(seen, r.keys - r.len + 1);
-    carry = min(carry + total, a.tokens + 1);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int used = ceil_div(a.rows, 64);
+  Row row[kRounds];
+  int before[kRounds];  // query tokens before the row, of its part
+  const int asked = a.prefix_len[0];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int part = i * (THREADS / 64) + wave, b = 64 * part + lane;
+    row[i] = Row{0, 0, 0};
+    before[i] = 0;
+    if (part >= used) continue;
+    if (b < a.rows) row[i] = row_of(a, b);
+    const int sum = wave_inclusive_scan(row[i].len);
+    before[i] = sum - row[i].len;
+    const bool keys = row[i].len > 0 && row[i].keys > 0;
+    const int first = wave_min(keys ? b : INT_MAX), least = wave_min(keys ? row[i].keys : INT_MAX);
+    const int seen = wave_min(row[i].len > 0 ? row[i].keys - row[i].len + 1 : INT_MAX);
+    const int count = __builtin_popcountll(__ballot(keys));
+    if (lane == 63) parts[part] = Part{sum, first, least, seen, 0, count};
   }
-  first = block_min<THREADS>(first, scratch);
-  least = block_min<THREADS>(least, scratch);
-  cut = min(block_min<THREADS>(cut, scratch), carry);
-  p.seen_by_all = block_min<THREADS>(seen, scratch);
-  int rows_with_keys;
-  block_scan<THREADS>(count, scratch, rows_with_keys);
-  for (int b = threadIdx.x; b <= a.rows; b += THREADS) t.token[b] = b < a.rows ? min(t.token[b], cut) : cut;
   __syncthreads();
+  // Rows that would bring the sum over the query's own tokens (rows that overlap) are left out, which
+  // also bounds the workspace: `cut` is the sum before the first of them.
+  int sum = 0, least = INT_MAX, count = 0, mine[kRounds];
+  p.prefix_row = INT_MAX;
+  p.seen_by_all = INT_MAX;
+  for (int w = 0; w < used; ++w) {
+    const Part q = parts[w];
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      if (w == i * (THREADS / 64) + wave) mine[i] = sum;
+    }
+    sum = min(sum + q.tokens, a.tokens + 1);
+    p.prefix_row = min(p.prefix_row, q.first);
+    least = min(least, q.least);
+    p.seen_by_all = min(p.seen_by_all, q.seen);
+    count += q.count;
+  }
+  const bool overlap = sum > a.tokens;
+  int cut = sum;
+  if (overlap) {  // the parts again, now knowing where each begins
+    cut = INT_MAX;
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      const int part = i * (THREADS / 64) + wave;
+      if (part >= used) continue;
+      const int at = mine[i] + before[i];
+      const int c = wave_min(at > a.tokens - row[i].len ? at : INT_MAX);
+      if (lane == 63) parts[part].cut = c;
+    }
+    __syncthreads();
+    for (int w = 0; w < used; ++w) cut = min(cut, parts[w].cut);
+    cut = min(cut, a.tokens);
+    __syncthreads();
+  }
   // A single row has nobody to share with: all its keys are its own.
-  p.prefix = rows_with_keys > 1 ? min(max(a.prefix_len[0], 0), least) : 0;
-  p.prefix_row = rows_with_keys > 0 ? first : 0;
-  p.query_tokens = t.token[a.rows];
+  // Key ranges begin at multiples of 16: what is left of the prefix is read row by row.
+  p.prefix = count > 1 ? min(max(asked, 0), least) & ~15 : 0;
+  p.prefix_row = count > 0 ? p.prefix_row : 0;
+  p.query_tokens = cut;
   const int m = p.query_tokens * a.group;
   p.prefix_tile = tile_rows(m);
   p.row_tiles = ceil_div(m, p.prefix_tile);
   p.key_tiles = ceil_div(p.prefix, kTile);
   p.prefix_work = a.hkv * p.row_tiles * p.key_tiles;
   // Own units.
-  int work = 0, units = 0;
-  for (int base = 0; base < a.rows; base += THREADS) {
-    const int b = base + static_cast<int>(threadIdx.x);
-    int n = 0, w = 0;
-    if (b < a.rows) {
-      const Row r = row_of(a, b);
-      if (r.len > 0 && t.token[b + 1] - t.token[b] == r.len && r.keys > p.prefix) {
-        const int own = r.len * a.group;
-        n = ceil_div(own, tile_rows(own));
-        w = n * ceil_div(r.keys - p.prefix, kTile);
-      }
+  int own_work[kRounds];
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int part = i * (THREADS / 64) + wave, b = 64 * part + lane;
+    own_work[i] = 0;
+    if (part >= used) continue;
+    const int at = mine[i] + before[i];
+    const bool fits = at <= a.tokens - row[i].len && at + row[i].len <= cut;
+    if (report && b < a.rows && a.status) {
+      const uint32_t bits = ((a.q_len[b] > 0 && (row[i].len == 0 || !fits)) ? kStatusRow : 0u) |
+                            (a.t_len[b] > a.capacity ? kStatusLength : 0u);
+      if (bits) __hip_atomic_fetch_or(a.status, static_cast<int>(bits), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    int total;
-    const int wb = work + block_scan<THREADS>(w, scratch, total);
-    work += total;
-    const int ub = units + block_scan<THREADS>(n, scratch, total);
-    units += total;
+    int w = 0;
+    if (row[i].len > 0 && fits && row[i].keys > p.prefix) {
+      w = query_tiles(row[i].len * a.group) * ceil_div(row[i].keys - p.prefix, kTile);
+    }
+    const int work = wave_inclusive_scan(w);
+    own_work[i] = work - w;
+    if (lane == 63) part_work[part] = work;
     if (b < a.rows) {
-      t.work[b] = wb;
-      t.unit[b] = ub;
+      t.token[b] = min(at, cut);
+      t.start[b] = row[i].start;
+      t.seen[b] = row[i].keys - row[i].len;
     }
   }
+  __syncthreads();
+  int work = 0;
+  for (int w = 0; w < used; ++w) {
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+      if (w == i * (THREADS / 64) + wave) own_work[i] += work;
+    }
+    work += part_work[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int b = 64 * (i * (THREADS / 64) + wave) + lane;
+    if (b < a.rows) t.work[b] = own_work[i];
+  }
   if (threadIdx.x == 0) {
+    t.token[a.rows] = cut;
     t.work[a.rows] = work;
-    t.unit[a.rows] = units;
   }
   __syncthreads();
   p.work = p.prefix_work + a.hkv * work;
@@ -256,13 +289,13 @@ __device__ __forceinline__ Unit prefix_unit(const PrefixArgs& a, const Plan& p, 
   Unit u;
   const int before = segment * p.share;
   u.key_tiles = min(p.share, p.key_tiles - before);
-  u.index = (h * p.segments + segment) * p.row_tiles + tile;
+  u.index = (segment * a.hkv + h) * p.row_tiles + tile;
   u.kv_head = h;
   u.row = -1;
   u.tile = tile;
   u.rows = p.query_tokens * a.group;
   u.tile_rows = p.prefix_tile;
-  u.first_work = (h * p.key_tiles + before) * p.row_tiles + tile * u.key_tiles;
+  u.first_work = before * a.hkv * p.row_tiles + (h * p.row_tiles + tile) * u.key_tiles;
   u.key0 = before * kTile;
   u.key_end = min(p.prefix, u.key0 + u.key_tiles * kTile);
   return u;
@@ -272,17 +305,20 @@ template <int D>
 __device__ __forceinline__ Unit own_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, int b, int h,
                                          int tile) {
   Unit u;
-  const int n = t.unit[b + 1] - t.unit[b], w = t.work[b + 1] - t.work[b];
-  u.index = p.prefix_units + a.hkv * t.unit[b] + h * n + tile;
+  const int w = t.work[b + 1] - t.work[b];
+  u.rows = (t.token[b + 1] - t.token[b]) * a.group;
+  const int n = query_tiles(u.rows);
+  // Places for a row's units start past those of the rows before: they have at most one tile each
+  // more than whole tiles of kNarrowRows query rows.
+  u.index = p.prefix_units + a.hkv * (b + t.token[b] * a.group / kNarrowRows) + h * n + tile;
   u.kv_head = h;
   u.row = b;
   u.tile = tile;
-  u.rows = (t.token[b + 1] - t.token[b]) * a.group;
   u.tile_rows = tile_rows(u.rows);
   u.key_tiles = w / n;
   u.first_work = p.prefix_work + a.hkv * t.work[b] + h * w + tile * u.key_tiles;
   u.key0 = p.prefix;
-  u.key_end = min(max(a.t_len[b], 0), a.capacity);
+  u.key_end = t.seen[b] + t.token[b + 1] - t.token[b];
   return u;
 }
 
@@ -290,12 +326,10 @@ __device__ __forceinline__ Unit own_unit(const PrefixArgs& a, const Plan& p, con
 template <int D>
 __device__ __forceinline__ Unit unit_at(const PrefixArgs& a, const Plan& p, const RowTables& t, int w) {
   if (w < p.prefix_work) {
-    const int per_head = p.row_tiles * p.key_tiles;
-    const int h = w / per_head, rest = w - h * per_head;
-    const int segment = rest / (p.share * p.row_tiles);
-    const int in_segment = rest - segment * p.share * p.row_tiles;
-    const int len = min(p.share, p.key_tiles - segment * p.share);
-    return prefix_unit<D>(a, p, h, segment, in_segment / len);
+    const int per_segment = p.share * a.hkv * p.row_tiles;
+    const int segment = w / per_segment, len = min(p.share, p.key_tiles - segment * p.share);
+    const int i = (w - segment * per_segment) / len;
+    return prefix_unit<D>(a, p, i / p.row_tiles, segment, i % p.row_tiles);
   }
   const int rest = w - p.prefix_work;
   int lo = 0, hi = a.rows - 1;  // the last row whose work starts at or before `rest`
@@ -303,7 +337,7 @@ __device__ __forceinline__ Unit unit_at(const PrefixArgs& a, const Plan& p, cons
     const int mid = (lo + hi + 1) >> 1;
     if (a.hkv * t.work[mid] <= rest) lo = mid; else hi = mid - 1;
   }
-  const int mine = t.work[lo + 1] - t.work[lo], n = t.unit[lo + 1] - t.unit[lo];
+  const int mine = t.work[lo + 1] - t.work[lo], n = query_tiles((t.token[lo + 1] - t.token[lo]) * a.group);
   const int in_row = rest - a.hkv * t.work[lo];
   const int h = in_row / mine;
   return own_unit<D>(a, p, t, lo, h, (in_row - h * mine) / (mine / n));
@@ -333,10 +367,9 @@ __device__ __forceinline__ QueryRow query_row(const PrefixArgs& a, const RowTabl
       b = row_at(a, t, token);
       i = token - t.token[b];
     }
-    const Row row = row_of(a, b);
-    q.token = row.start + i;
+    q.token = t.start[b] + i;
     q.head = u.kv_head * a.group + (r - token * a.group);
-    q.limit = row.keys - row.len + i + 1;
+    q.limit = t.seen[b] + i + 1;
   }
   return q;
 }
@@ -375,21 +408,14 @@ __device__ __forceinline__ float other_half(float v) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// Where 16-byte piece `c` of staged key `t` lies (in pieces): the pieces of eight neighbouring keys
-// are turned against each other by two, so that the score MFMAs' reads (one piece of 32 keys) and
-// the transposing reads of the values (two pieces of four keys) touch all banks.
+// Where 16-byte piece `c` of staged value `t` lies (in pieces): the pieces of eight neighbouring keys
+// are turned against each other by two, so that a transposing read (two pieces of four keys) touches
+// different banks.
 template <int D>
 __device__ __forceinline__ int piece_at(int t, int c) {
   const int turn = D >= 128 ? 2 * (t & 7) : 2 * ((t >> 1) & 3);
   return t * (D / 8) + (c ^ turn);
 }
-
-// A tile's keys and values in flight to shared memory.
-template <int D>
-struct Staged {
-  u32x4 k[Shape<D>::kPasses], v[Shape<D>::kPasses];
-  int page[Shape<D>::kPasses];  // of the next tile
-};
 
 // Where a tile begins: its first key, and that key's page (in the table) and place.  Tiles follow
 // each other, so a key's page comes from the place and the distance, both small: (n + 0.5) / size in
@@ -408,86 +434,114 @@ __device__ __forceinline__ void advance(const PrefixArgs& a, Cursor& c, int keys
   c.place += keys - n * a.block_size;
 }
 
-// Keys past the range take the place of its last one, and are zeroed on their way to shared memory.
+// A tile's keys and values in flight to shared memory.  One load of a wave takes kPerLoad neighbouring
+// keys (whole 128-byte lines of one head); ranges begin at multiples of 16 keys, so where the page
+// size is a multiple of kPerLoad they lie in one page and the addresses are the wave's, computed on the
+// scalar unit (WHOLE).  Lane i of a wave looks up the page of its load i, a tile ahead.
 template <int D>
-__device__ __forceinline__ int staged_key(const Cursor& c, int i, int key_end) {
+struct Staged {
+  u32x4 k[Shape<D>::kPasses], v[Shape<D>::kPasses];
+  int page, in;  // of the next tile's loads
+  int bad;       // loads of a page out of range
+};
+
+// First key of the wave's load i, from the tile's first; loads past the range take its last keys (and
+// are zeroed on their way to shared memory).
+template <int D>
+__device__ __forceinline__ int load_key(const Cursor& c, int i, int wave, int key_end) {
   using S = Shape<D>;
-  return min(i * S::kPerPass + static_cast<int>(threadIdx.x) / S::kLanes, key_end - 1 - c.key);
+  return min(i * S::kPerPass + wave * S::kPerLoad, (key_end - 1 - c.key) & ~(S::kPerLoad - 1));
 }
 
-template <int D>
+template <int D, bool WHOLE>
 __device__ __forceinline__ void find_pages(const PrefixArgs& a, const int32_t* table, const Cursor& c, int key_end,
+                                           int wave, Staged<D>& s) {
+  if (c.key >= key_end || !WHOLE) return;
+  const int n = c.place + load_key<D>(c, threadIdx.x % Shape<D>::kPasses, wave, key_end);
+  const int j = pages_in(a, n);
+  s.in = n - j * a.block_size;
+  s.page = table[c.page + j];
+}
+
+template <bool ONCE>
+__device__ __forceinline__ u32x4 load_piece(const uint16_t* base, uint32_t bytes) {
+  const u32x4* p = reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + bytes);
+  return ONCE ? __builtin_nontemporal_load(p) : *p;
+}
+
+template <int D, bool WHOLE, bool ONCE>
+__device__ __forceinline__ void load_keys(const PrefixArgs& a, const int32_t* table, const Cursor& c, int key_end, int h,
+                                          int wave, int i, Staged<D>& s) {
+  using S = Shape<D>;
+  const int lane = threadIdx.x & 63, piece = lane % S::kLanes, mine = lane / S::kLanes;
+  if constexpr (WHOLE) {
+    const int found = __builtin_amdgcn_readlane(s.page, i);
+    const int64_t in = __builtin_amdgcn_readlane(s.in, i);
+    const bool fine = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
+    const int64_t page = fine ? found : 0;
+    s.bad = (s.bad & ~(1 << i)) | (fine ? 0 : 1 << i);
+    s.k[i] = load_piece<ONCE>(a.k + (page * a.k_block + in * a.k_token + h * a.k_head),
+                              2 * (mine * static_cast<uint32_t>(a.k_token) + 8 * piece));
+    s.v[i] = load_piece<ONCE>(a.v + (page * a.v_block + in * a.v_token + h * a.v_head),
+                              2 * (mine * static_cast<uint32_t>(a.v_token) + 8 * piece));
+  } else {  // a page a lane
+    const int n = c.place + min(i * S::kPerPass + wave * S::kPerLoad + mine, key_end - 1 - c.key);
+    const int j = pages_in(a, n);
+    const int found = table[c.page + j];
+    const int64_t in = n - j * a.block_size;
+    const bool fine = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
+    const int64_t page = fine ? found : 0;
+    s.bad = (s.bad & ~(1 << i)) | (fine ? 0 : 1 << i);
+    s.k[i] = load_piece<ONCE>(a.k + (page * a.k_block + in * a.k_token + h * a.k_head), 16 * piece);
+    s.v[i] = load_piece<ONCE>(a.v + (page * a.v_block + in * a.v_token + h * a.v_head), 16 * piece);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void store_keys(const PrefixArgs& a, char* stage, int key, int key_end, int wave, int i,
                                            Staged<D>& s) {
-  if (c.key >= key_end) return;
-#pragma unroll
-  for (int i = 0; i < Shape<D>::kPasses; ++i) {
-    s.page[i] = table[c.page + pages_in(a, c.place + staged_key<D>(c, i, key_end))];
-  }
-}
-
-template <int D, bool ONCE>
-__device__ __forceinline__ void load_tile(const PrefixArgs& a, const Cursor& c, int key_end, int h, Staged<D>& s) {
   using S = Shape<D>;
-  if (c.key >= key_end) return;
-  const uint16_t* keys = a.k + h * a.k_head + 8 * (static_cast<int>(threadIdx.x) % S::kLanes);
-  const uint16_t* values = a.v + h * a.v_head + 8 * (static_cast<int>(threadIdx.x) % S::kLanes);
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < S::kPasses; ++i) {
-    const int n = c.place + staged_key<D>(c, i, key_end);
-    const int64_t in = n - pages_in(a, n) * a.block_size;
-    const bool fine = static_cast<unsigned>(s.page[i]) < static_cast<unsigned>(a.num_blocks);
-    const int64_t page = fine ? s.page[i] : 0;
-    const u32x4* kp = reinterpret_cast<const u32x4*>(keys + page * a.k_block + in * a.k_token);
-    const u32x4* vp = reinterpret_cast<const u32x4*>(values + page * a.v_block + in * a.v_token);
-    s.k[i] = ONCE ? __builtin_nontemporal_load(kp) : *kp;
-    s.v[i] = ONCE ? __builtin_nontemporal_load(vp) : *vp;
-    bad |= !fine;
-  }
-  if (__any(bad)) {
-#pragma unroll
-    for (int i = 0; i < S::kPasses; ++i) {
-      if (static_cast<unsigned>(s.page[i]) >= static_cast<unsigned>(a.num_blocks)) {
-        s.k[i] = u32x4{0, 0, 0, 0};
-        s.v[i] = u32x4{0, 0, 0, 0};
-      }
-    }
-    if (bad && a.status) {
-      __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-  }
-}
-
-template <int D>
-__device__ __forceinline__ void store_tile(Staged<D>& s, u32x4* keys, u32x4* values, int key, int key_end) {
-  using S = Shape<D>;
-  const int piece = static_cast<int>(threadIdx.x) % S::kLanes;
-  if (key + S::kTile > key_end) {
-#pragma unroll
-    for (int i = 0; i < S::kPasses; ++i) {
-      if (key + i * S::kPerPass + static_cast<int>(threadIdx.x) / S::kLanes >= key_end) {
-        s.k[i] = u32x4{0, 0, 0, 0};
-        s.v[i] = u32x4{0, 0, 0, 0};
+  const int lane = threadIdx.x & 63, piece = lane % S::kLanes;
+  const int t = i * S::kPerPass + wave * S::kPerLoad + lane / S::kLanes;
+  if (key + S::kTile > key_end || __any(s.bad != 0)) {
+    if (key + t >= key_end || (s.bad >> i) & 1) {
+      s.k[i] = u32x4{0, 0, 0, 0};
+      s.v[i] = u32x4{0, 0, 0, 0};
+      if (key + t < key_end && a.status) {
+        __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < S::kPasses; ++i) {
-    const int t = i * S::kPerPass + static_cast<int>(threadIdx.x) / S::kLanes;
-    keys[piece_at<D>(t, piece)] = s.k[i];
-    values[piece_at<D>(t, piece)] = s.v[i];
-  }
+  *reinterpret_cast<u32x4*>(stage + t * S::kKeyBytes + 16 * piece) = s.k[i];
+  reinterpret_cast<u32x4*>(stage + S::kValuesAt)[piece_at<D>(t, piece)] = s.v[i];
 }
 
-// Four values of one dimension, keys t .. t + 3, for each lane: lane l of 16 names key t + l / 4 and
-// dimensions 4 (l % 4) .. + 3 of the 16 that the group of lanes covers, and gets dimension l.
+// Where a lane reads in a staged tile, in bytes: a key's piece 0 for the score product (key lane % 32
+// of 32, the first 16 bytes of its half of a step), and for the output product the values of four keys
+// of output block j.  A transposing read gives lane l of 16 four keys of dimension l, where lane l names
+// key l / 4 and dimensions 4 (l % 4) .. + 3; keys 8 (or 16, 32) further on are a constant away, since
+// the turn of the pieces repeats every eight.
 template <int D>
-__device__ __forceinline__ u32x2 read_values(const u32x4* values, int t, int dim) {
-  const int l = threadIdx.x & 15;
-  const int at = piece_at<D>(t + (l >> 2), (dim >> 3) + ((l & 3) >> 1));
-  const lds_s16x4* p =
-      (const lds_s16x4*)(reinterpret_cast<const char*>(values + at) + 8 * (l & 1));
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>(p)));
+struct Lane {
+  int key, value[Shape<D>::kBlocks];
+};
+template <int D>
+__device__ __forceinline__ Lane<D> lane_places() {
+  using S = Shape<D>;
+  const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 15;
+  Lane<D> p;
+  p.key = (lane & 31) * S::kKeyBytes + 16 * half;
+#pragma unroll
+  for (int j = 0; j < S::kBlocks; ++j) {
+    p.value[j] = S::kValuesAt + 16 * piece_at<D>(4 * half + (l >> 2), 4 * j + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) +
+                 8 * (l & 1);
+  }
+  return p;
+}
+
+__device__ __forceinline__ u32x2 read_values(const char* p) {
+  const lds_s16x4* q = (const lds_s16x4*)p;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>(q)));
 }
 
 __device__ __forceinline__ bool not_finite2(uint32_t w, uint32_t exponent) {
@@ -528,25 +582,45 @@ __device__ __forceinline__ void add_not_finite(const u32x4* values, State<D>& st
 }
 
 // 32 keys of a staged tile for one wave, from key t0 of the tile on.  `seen` (MASKED): how many of
-// them the lane column's query row sees.
+// them the lane column's query row sees.  Reads of a step are issued together, ahead of the products
+// that take them: the keys' before the first product, the values' before the softmax.
 template <int DT, int D, bool MASKED>
-__device__ __forceinline__ void attend_keys(const u32x4* keys, const u32x4* values, const u32x4 (&q)[Shape<D>::kSteps],
+__device__ __forceinline__ void attend_keys(const char* stage, const Lane<D>& at, const u32x4 (&q)[Shape<D>::kSteps],
                                             State<D>& st, int t0, int seen, float scale_log2) {
   using S = Shape<D>;
+  constexpr int kBatch = S::kSteps < 8 ? S::kSteps : 8;
   const int lane = threadIdx.x & 63, half = lane >> 5;
+  const char* keys = stage + at.key + t0 * S::kKeyBytes;
   f32x16 sc;
 #pragma unroll
   for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
-  for (int s = 0; s < S::kSteps; ++s) sc = mfma32<DT>(keys[piece_at<D>(t0 + (lane & 31), 2 * s + half)], q[s], sc);
+  for (int s0 = 0; s0 < S::kSteps; s0 += kBatch) {
+    u32x4 k[kBatch];
+#pragma unroll
+    for (int s = 0; s < kBatch; ++s) k[s] = *reinterpret_cast<const u32x4*>(keys + 32 * (s0 + s));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < kBatch; ++s) sc = mfma32<DT>(k[s], q[s0 + s], sc);
+  }
+  constexpr int kAhead = S::kBlocks <= 4 ? S::kBlocks : 4;  // blocks whose values are read before the softmax
+  u32x2 v[2][kAhead][2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v[s][j][e] = read_values(stage + at.value[j] + (t0 + 16 * s + 8 * e) * 2 * D);
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    sc[i] *= scale_log2;
     if constexpr (MASKED) sc[i] = 8 * (i >> 2) + 4 * half + (i & 3) < seen ? sc[i] : -INFINITY;
     top = fmaxf(top, sc[i]);
   }
-  top = fmaxf(top, other_half(top));
+  top = fmaxf(top, other_half(top)) * scale_log2;
   if (__any(top > st.m)) {
     const float m = fmaxf(st.m, top);
     const float keep = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
@@ -562,8 +636,9 @@ __device__ __forceinline__ void attend_keys(const u32x4* keys, const u32x4* valu
   u32x4 p[2];
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
-    const float x = __builtin_amdgcn_exp2f(sc[i] - m), y = __builtin_amdgcn_exp2f(sc[i + 1] - m);
-    st.l += x + y;
+    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], scale_log2, -m));
+    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i + 1], scale_log2, -m));
+    st.l += x + y;  // as computed, not as rounded for the product: the LSE is fp32
     p[i >> 3][(i & 7) >> 1] = pack2<DT>(x, y);
   }
   constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
@@ -572,35 +647,44 @@ __device__ __forceinline__ void attend_keys(const u32x4* keys, const u32x4* valu
     bool bad = false;
 #pragma unroll 1
     for (int c = half; c < D / 8; c += 2) {
-      const u32x4 v = values[piece_at<D>(t0 + (lane & 31), c)];
-      bad |= not_finite2(v[0], kExponent) || not_finite2(v[1], kExponent) || not_finite2(v[2], kExponent) ||
-             not_finite2(v[3], kExponent);
+      const u32x4 x = reinterpret_cast<const u32x4*>(stage + S::kValuesAt)[piece_at<D>(t0 + (lane & 31), c)];
+      bad |= not_finite2(x[0], kExponent) || not_finite2(x[1], kExponent) || not_finite2(x[2], kExponent) ||
+             not_finite2(x[3], kExponent);
     }
     poison = __any(bad);
   }
   // The lane's own probabilities are the B operand: k-slot (half, e) of step s is key 16 s + 8 (e /
   // 4) + 4 half + e % 4 of the 32, and the values are read in that order.
+  auto output = [&](int j, int s, u32x2 lo, u32x2 hi) {
+    u32x4 x = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    if constexpr (MASKED) {
+      if (poison) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] &= ((x[e] & kExponent) == kExponent ? 0u : 0xffffu) |
+                  ((x[e] & (kExponent << 16)) == (kExponent << 16) ? 0u : 0xffff0000u);
+        }
+      }
+    }
+    st.acc[j] = mfma32<DT>(x, p[s], st.acc[j]);
+  };
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
 #pragma unroll
-    for (int j = 0; j < S::kBlocks; ++j) {
-      const int dim = 32 * j + 16 * ((lane >> 4) & 1), t = t0 + 16 * s + 4 * half;
-      const u32x2 lo = read_values<D>(values, t, dim), hi = read_values<D>(values, t + 8, dim);
-      u32x4 v = u32x4{lo[0], lo[1], hi[0], hi[1]};
-      if constexpr (MASKED) {
-        if (poison) {
+    for (int j = 0; j < kAhead; ++j) output(j, s, v[s][j][0], v[s][j][1]);
+  }
+  if constexpr (S::kBlocks > kAhead) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] &= ((v[e] & kExponent) == kExponent ? 0u : 0xffffu) |
-                    ((v[e] & (kExponent << 16)) == (kExponent << 16) ? 0u : 0xffff0000u);
-          }
-        }
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int j = kAhead; j < S::kBlocks; ++j) {
+        const char* from = stage + at.value[j] + (t0 + 16 * s) * 2 * D;
+        output(j, s, read_values(from), read_values(from + 8 * 2 * D));
       }
-      st.acc[j] = mfma32<DT>(v, p[s], st.acc[j]);
     }
   }
   if constexpr (MASKED) {
-    if (poison) add_not_finite<DT, D>(values, st, t0, seen);
+    if (poison) add_not_finite<DT, D>(reinterpret_cast<const u32x4*>(stage + S::kValuesAt), st, t0, seen);
   }
 }
 
@@ -612,9 +696,9 @@ __device__ __forceinline__ float* piece_sums(const PrefixArgs& a, int slot) {
 }
 
 // The key tiles [from, to) of a unit, and the unit's piece.
-template <int DT, int D, bool WIDE, bool ONCE>
+template <int DT, int D, bool WHOLE, bool WIDE, bool ONCE>
 __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, const Unit& u,
-                                         int from, int to, int slot, u32x4* lds) {
+                                         int from, int to, int slot, char* lds) {
   using S = Shape<D>;
   constexpr int kQ = WIDE ? 4 : 2;             // blocks of 32 query rows
   constexpr int kT = S::kWaves / kQ;           // waves that share a block's keys
@@ -622,6 +706,22 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int qb = wave / kT, tb = wave % kT;
   const int r0 = u.tile * u.tile_rows + 32 * qb;
+  // Keys past the last query row's limit (own units: the tile's last token sees most).
+  int key_end = u.key_end, seen_by_all = p.seen_by_all;
+  if (u.row >= 0) {
+    seen_by_all = t.seen[u.row] + u.tile * u.tile_rows / a.group + 1;
+    const int last = (min((u.tile + 1) * u.tile_rows, u.rows) - 1) / a.group;
+    key_end = min(key_end, t.seen[u.row] + last + 1);
+  }
+  to = min(to, ceil_div(key_end - u.key0, S::kTile));
+  const int32_t* table = a.table + static_cast<int64_t>(u.row < 0 ? p.prefix_row : u.row) * a.bt_stride;
+  int key = u.key0 + from * S::kTile;
+  Cursor c{key, key / a.block_size, 0};  // of the tile whose pages are looked up next
+  c.place = key - c.page * a.block_size;
+  Staged<D> s;
+  s.page = s.in = s.bad = 0;
+  find_pages<D, WHOLE>(a, table, c, from < to ? key_end : 0, wave, s);
+
   const QueryRow qr = query_row(a, t, u, r0 + (lane & 31));
   u32x4 q[S::kSteps];
   {
@@ -629,20 +729,9 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s) {
       q[s] = u32x4{0, 0, 0, 0};
-      if (qr.valid) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
+      if (qr.valid) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s) ^ a.q_sign;
     }
   }
-  // Keys past the last query row's limit (own units: the tile's last token sees most).
-  int key_end = u.key_end, seen_by_all = p.seen_by_all;
-  if (u.row >= 0) {
-    const Row row = row_of(a, u.row);
-    seen_by_all = row.keys - row.len + u.tile * u.tile_rows / a.group + 1;
-    const int last = (min((u.tile + 1) * u.tile_rows, u.rows) - 1) / a.group;
-    key_end = min(key_end, row.keys - row.len + last + 1);
-  }
-  to = min(to, ceil_div(key_end - u.key0, S::kTile));
-  const int32_t* table = a.table + static_cast<int64_t>(u.row < 0 ? p.prefix_row : u.row) * a.bt_stride;
-
   State<D> st;
 #pragma unroll
   for (int j = 0; j < S::kBlocks; ++j) {
@@ -652,52 +741,49 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
   st.m = -INFINITY;
   st.l = 0.f;
 
-  Staged<D> s;
+  const Lane<D> at = lane_places<D>();
   if (from < to) {
-    int key = u.key0 + from * S::kTile;
-    Cursor c{key, key / a.block_size, 0};  // of the tile whose pages are looked up next
-    c.place = key - c.page * a.block_size;
-    find_pages<D>(a, table, c, key_end, s);
-    load_tile<D, ONCE>(a, c, key_end, u.kv_head, s);
+#pragma unroll
+    for (int i = 0; i < S::kPasses; ++i) load_keys<D, WHOLE, ONCE>(a, table, c, key_end, u.kv_head, wave, i, s);
     advance(a, c, S::kTile);
-    find_pages<D>(a, table, c, key_end, s);
+    find_pages<D, WHOLE>(a, table, c, key_end, wave, s);
     __syncthreads();  // the unit before has read its last tile
-    store_tile<D>(s, lds, lds + S::kBuffer / 8, key, key_end);
-    load_tile<D, ONCE>(a, c, key_end, u.kv_head, s);
-    advance(a, c, S::kTile);
-    find_pages<D>(a, table, c, key_end, s);
-    lds_barrier();
+    // A register is loaded again as soon as its keys are in shared memory.
+    auto stage = [&](char* to_stage) {
+#pragma unroll
+      for (int i = 0; i < S::kPasses; ++i) {
+        store_keys<D>(a, to_stage, key, key_end, wave, i, s);
+        if (c.key < key_end) load_keys<D, WHOLE, ONCE>(a, table, c, key_end, u.kv_head, wave, i, s);
+      }
+      advance(a, c, S::kTile);
+      find_pages<D, WHOLE>(a, table, c, key_end, wave, s);
+      lds_barrier();
+    };
+    stage(lds);
     int cur = 0, i = from;
     auto stage_next = [&]() {
       key += S::kTile;
-      if (++i < to) {
-        u32x4* next = lds + (cur ^ 1) * (S::kBuffer / 4);
-        store_tile<D>(s, next, next + S::kBuffer / 8, key, key_end);
-        load_tile<D, ONCE>(a, c, key_end, u.kv_head, s);
-        advance(a, c, S::kTile);
-        find_pages<D>(a, table, c, key_end, s);
-      }
-      lds_barrier();
+      if (++i < to) stage(lds + (cur ^ 1) * S::kStage);
+      else lds_barrier();
       cur ^= 1;
     };
     // Tiles that all query rows see whole, then the ones with a mask.
     while (i < to && key + S::kTile <= min(seen_by_all, key_end)) {
-      const u32x4* staged = lds + cur * (S::kBuffer / 4);
       if (r0 < u.rows) {
+        const char* stage = lds + cur * S::kStage;
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
-          attend_keys<DT, D, false>(staged, staged + S::kBuffer / 8, q, st, 32 * (tb * kN + n), 32, a.scale_log2);
+          attend_keys<DT, D, false>(stage, at, q, st, 32 * (tb * kN + n), 32, a.scale_log2);
         }
       }
       stage_next();
     }
     while (i < to) {
-      const u32x4* staged = lds + cur * (S::kBuffer / 4);
       if (r0 < u.rows) {
         const int seen = min(qr.limit, key_end) - key;
 #pragma unroll 1
-        for (int t0 = 32 * tb * kN; t0 < 32 * (tb + 1) * kN; t0 += 32) {
-          attend_keys<DT, D, true>(staged, staged + S::kBuffer / 8, q, st, t0, seen - t0, a.scale_log2);
+        for (int t0 = 32 * tb * kN; t0 < min(32 * (tb + 1) * kN, key_end - key); t0 += 32) {
+          attend_keys<DT, D, true>(lds + cur * S::kStage, at, q, st, t0, seen - t0, a.scale_log2);
         }
       }
       stage_next();
@@ -705,65 +791,79 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
   }
   st.l += other_half(st.l);
 
-  // The waves that share query rows join in shared memory.
-  if constexpr (kT > 1) {
-    constexpr int kWords = 16 * S::kBlocks;
-    float* area = reinterpret_cast<float*>(lds);  // [query block][wave after the first][output words, m, l][lane]
-    static_assert(kQ * (kT - 1) * (kWords + 2) * 64 * 4 <= 4 * S::kBuffer * 2, "the waves' results fit the tiles");
+  // The waves that share query rows join in shared memory, each for its part of the dimensions (in
+  // groups of four accumulators, as they are stored).
+  constexpr int kGroups = 4 * S::kBlocks, kMine = kGroups / kT, kOther = kGroups - kMine;
+  auto group = [&](int g) {
+    return f32x4{st.acc[g >> 2][4 * (g & 3)], st.acc[g >> 2][4 * (g & 3) + 1], st.acc[g >> 2][4 * (g & 3) + 2],
+                 st.acc[g >> 2][4 * (g & 3) + 3]};
+  };
+  f32x4 sum[kMine];
+  if constexpr (kT == 1) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) sum[g] = group(g);
+  } else {
+    // [wave][its groups for the other waves, in their order][lane], then each wave's m and l.
+    static_assert(S::kWaves * (4 * kOther + 2) * 64 * 4 <= 2 * S::kStage, "the waves' results fit the tiles");
+    f32x4* area = reinterpret_cast<f32x4*>(lds);
+    float* sums = reinterpret_cast<float*>(area + S::kWaves * kOther * 64);
     __syncthreads();
-    if (tb > 0) {
-      float* to_area = area + ((qb * (kT - 1) + tb - 1) * (kWords + 2)) * 64 + lane;
+    if (r0 < u.rows) {
 #pragma unroll
-      for (int j = 0; j < S::kBlocks; ++j) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) to_area[(16 * j + i) * 64] = st.acc[j][i];
+      for (int g = 0; g < kGroups; ++g) {
+        const int w = g / kMine;
+        if (w != tb) area[(wave * kOther + (w < tb ? g : g - kMine)) * 64 + lane] = group(g);
       }
-      to_area[kWords * 64] = st.m;
-      to_area[(kWords + 1) * 64] = st.l;
+      sums[2 * wave * 64 + lane] = st.m;
+      sums[(2 * wave + 1) * 64 + lane] = st.l;
     }
     __syncthreads();
-    if (tb == 0) {
-      for (int w = 0; w < kT - 1; ++w) {
-        const float* from_area = area + ((qb * (kT - 1) + w) * (kWords + 2)) * 64 + lane;
-        const float om = from_area[kWords * 64], ol = from_area[(kWords + 1) * 64];
-        const float m = fmaxf(st.m, om);
-        const float mine = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
-        const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - m);
-        st.m = m;
-        st.l = st.l * mine + ol * other;
+    if (r0 < u.rows) {
+      float m = st.m, l = 0.f, weight[kT];
 #pragma unroll
-        for (int j = 0; j < S::kBlocks; ++j) {
+      for (int w = 0; w < kT; ++w) m = fmaxf(m, sums[2 * (qb * kT + w) * 64 + lane]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) st.acc[j][i] = st.acc[j][i] * mine + from_area[(16 * j + i) * 64] * other;
+      for (int w = 0; w < kT; ++w) {
+        const float om = sums[2 * (qb * kT + w) * 64 + lane], ol = sums[(2 * (qb * kT + w) + 1) * 64 + lane];
+        weight[w] = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - m);
+        l += ol * weight[w];
+      }
+      const float own = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        if (g / kMine == tb) sum[g % kMine] = group(g) * own;
+      }
+#pragma unroll
+      for (int w = 0; w < kT; ++w) {
+        if (w == tb) continue;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) {  // group tb kMine + k, in wave w's list without its own groups
+          sum[k] += area[((qb * kT + w) * kOther + (tb < w ? tb : tb - 1) * kMine + k) * 64 + lane] * weight[w];
         }
       }
+      st.m = m;
+      st.l = l;
     }
   }
-  if (tb == 0 && r0 < u.rows && slot < a.slots) {
+  if (r0 < u.rows && slot < a.slots) {
     float* sums = piece_sums<D>(a, slot);
-    if (lane < 32) {
+    if (lane < 32 && tb == 0) {
       sums[32 * qb + lane] = st.m;
       sums[kWideRows + 32 * qb + lane] = st.l;
     }
-    f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kWideRows) + qb * (S::kBlocks * 4 * 64) + lane;
+    f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kWideRows) + (qb * kGroups + tb * kMine) * 64 + lane;
 #pragma unroll
-    for (int j = 0; j < S::kBlocks; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[(4 * j + i) * 64] = f32x4{st.acc[j][4 * i], st.acc[j][4 * i + 1], st.acc[j][4 * i + 2], st.acc[j][4 * i + 3]};
-      }
-    }
+    for (int k = 0; k < kMine; ++k) o[k * 64] = sum[k];
   }
 }
 
-template <int DT, int D>
+template <int DT, int D, bool WHOLE>
 __global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_attention_kernel(
     PrefixArgs a) {
   using S = Shape<D>;
-  __shared__ u32x4 lds[4 * S::kBuffer / 8];
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::kStage];
   __shared__ RowTables tables;
-  __shared__ int scratch[S::kWaves];
-  const Plan p = make_plan<D, S::kThreads>(a, tables, scratch, blockIdx.x == 0);
+  const Plan p = make_plan<D, S::kThreads>(a, tables, blockIdx.x == 0);
   // Consecutive shares on one XCD (workgroups are dealt to the eight in turn).
   const int per_xcd = a.groups / 8;
   const int group = a.groups % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + static_cast<int>(blockIdx.x / 8)
@@ -774,24 +874,26 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_a
     Unit u = unit_at<D>(a, p, tables, w);
     const int from = w - u.first_work, to = min(u.key_tiles, end - u.first_work);
     const int slot = u.index + group;
-    if (u.tile_rows != kWideRows) run_unit<DT, D, false, true>(a, p, tables, u, from, to, slot, lds);
-    else if (u.row >= 0 || p.row_tiles == 1) run_unit<DT, D, true, true>(a, p, tables, u, from, to, slot, lds);
-    else run_unit<DT, D, true, false>(a, p, tables, u, from, to, slot, lds);
+    if (u.tile_rows != kWideRows) run_unit<DT, D, WHOLE, false, true>(a, p, tables, u, from, to, slot, lds);
+    else if (u.row >= 0 || p.row_tiles == 1) run_unit<DT, D, WHOLE, true, true>(a, p, tables, u, from, to, slot, lds);
+    else run_unit<DT, D, WHOLE, true, false>(a, p, tables, u, from, to, slot, lds);
     w = u.first_work + to;
   }
 }
 
-// Joins the pieces of 32 query rows of one KV head (the batch's order): a wave per 32 dimensions.
+// Joins the pieces of 32 query rows of one KV head (the batch's order) for 32 dimensions: eight waves
+// take the pieces in turn, and the first four join the waves' sums, four dimensions of a lane each.
+constexpr int kJoinWaves = 8;
 template <int DT, int D>
-__global__ __launch_bounds__(2 * D) void prefix_join_kernel(PrefixArgs a) {
+__global__ __launch_bounds__(64 * kJoinWaves) void prefix_join_kernel(PrefixArgs a) {
   using S = Shape<D>;
   __shared__ RowTables tables;
-  __shared__ int scratch[S::kBlocks];
-  const Plan p = make_plan<D, 2 * D>(a, tables, scratch, false);
-  const int rows = p.query_tokens * a.group, blocks = ceil_div(rows, 32);
-  const int h = blockIdx.y, block = blockIdx.x;
-  if (block >= blocks) return;
-  const int j = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __shared__ float joined[kJoinWaves][18][64];
+  const Plan p = make_plan<D, 64 * kJoinWaves>(a, tables, false);
+  const int rows = p.query_tokens * a.group;
+  const int block = blockIdx.x, j = blockIdx.y, h = blockIdx.z;
+  if (32 * block >= rows) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = 32 * block + (lane & 31);
   const bool valid = r < rows;
   const int token = (valid ? r : rows - 1) / a.group;
@@ -801,64 +903,80 @@ __global__ __launch_bounds__(2 * D) void prefix_join_kernel(PrefixArgs a) {
   f32x4 acc[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto join = [&](const Unit& u, int row_in_tile) {
-    const int first = u.first_work / p.share, last = (u.first_work + u.key_tiles - 1) / p.share;
-    const int qb = row_in_tile >> 5, at = (row_in_tile & 31) + (lane & 32);
-    for (int g = first; g <= last; ++g) {
-      const float* sums = piece_sums<D>(a, u.index + g);
-      const float om = sums[row_in_tile], ol = sums[kWideRows + row_in_tile];
-      const f32x4* o = reinterpret_cast<const f32x4*>(sums + 2 * kWideRows) + (qb * S::kBlocks + j) * 4 * 64 + at;
-      f32x4 part[4];
+  auto join = [&](int slot, int row_in_tile) {
+    const float* sums = piece_sums<D>(a, slot);
+    const float om = sums[row_in_tile], ol = sums[kWideRows + row_in_tile];
+    const f32x4* o = reinterpret_cast<const f32x4*>(sums + 2 * kWideRows) +
+                     ((row_in_tile >> 5) * S::kBlocks + j) * 4 * 64 + (row_in_tile & 31) + (lane & 32);
+    f32x4 part[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) part[k] = o[k * 64];
-      const float top = fmaxf(m, om);
-      const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-      const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - top);
-      m = top;
-      l = l * mine + ol * other;
+    for (int k = 0; k < 4; ++k) part[k] = o[k * 64];
+    const float top = fmaxf(m, om);
+    const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - top);
+    m = top;
+    l = l * mine + ol * other;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] = acc[k] * mine + part[k] * other;
-    }
+    for (int k = 0; k < 4; ++k) acc[k] = acc[k] * mine + part[k] * other;
   };
-  const int tile = 32 * block / p.prefix_tile;
-  for (int segment = 0; segment < p.segments; ++segment) {
-    join(prefix_unit<D>(a, p, h, segment, tile), 32 * block - tile * p.prefix_tile + (lane & 31));
+  // A segment is at most a share long: its pieces are of one workgroup or of two.
+  const int tile = 32 * block / p.prefix_tile, in_tile = 32 * block - tile * p.prefix_tile + (lane & 31);
+  for (int k = wave; k < 2 * p.segments; k += kJoinWaves) {
+    const Unit u = prefix_unit<D>(a, p, h, k >> 1, tile);
+    const int group = u.first_work / p.share + (k & 1);
+    if (group <= (u.first_work + u.key_tiles - 1) / p.share) join(u.index + group, in_tile);
   }
   if (tables.work[b + 1] > tables.work[b]) {
     const int in_row = i * a.group + (valid ? r : rows - 1) % a.group;
     const int n = tile_rows((tables.token[b + 1] - tables.token[b]) * a.group);
-    join(own_unit<D>(a, p, tables, b, h, in_row / n), in_row % n);
+    const Unit u = own_unit<D>(a, p, tables, b, h, in_row / n);
+    const int last = (u.first_work + u.key_tiles - 1) / p.share;
+    for (int group = u.first_work / p.share + wave; group <= last; group += kJoinWaves) join(u.index + group, in_row % n);
   }
-  if (!valid) return;
-  const int head = h * a.group + r % a.group;
-  const int64_t q_token = static_cast<int64_t>(a.q_start[b]) + i;
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // nothing seen: zeros; NaN stays NaN
-  uint16_t* out = a.out + q_token * a.o_row + head * a.o_head + 32 * j + 4 * (lane >> 5);
+  joined[wave][16][lane] = m;
+  joined[wave][17][lane] = l;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const f32x4 x = acc[k] * inv;
-    *reinterpret_cast<u32x2*>(out + 8 * k) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+  for (int k = 0; k < 16; ++k) joined[wave][k][lane] = acc[k >> 2][k & 3];
+  __syncthreads();
+  if (wave >= 4 || !valid) return;
+  m = joined[0][16][lane];
+  for (int w = 1; w < kJoinWaves; ++w) m = fmaxf(m, joined[w][16][lane]);
+  l = 0.f;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int w = 0; w < kJoinWaves; ++w) {
+    const float om = joined[w][16][lane];
+    const float weight = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - m);
+    l += joined[w][17][lane] * weight;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] += joined[w][4 * wave + k][lane] * weight;
   }
-  if (a.lse && j == 0 && lane < 32) {
+  const int head = h * a.group + r % a.group;
+  const int64_t q_token = static_cast<int64_t>(tables.start[b]) + i;
+  x *= l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // nothing seen: zeros; NaN stays NaN
+  uint16_t* out = a.out + q_token * a.o_row + head * a.o_head + 32 * j + 8 * wave + 4 * (lane >> 5);
+  *reinterpret_cast<u32x2*>(out) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+  if (a.lse && j == 0 && wave == 0 && lane < 32) {
     a.lse[q_token * a.l_row + head * a.l_head] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2P;
   }
 }
 
-int attention_groups(int head_dim) { return device_cu_count() * (head_dim <= 64 ? 2 : 1); }
+int attention_groups() { return device_cu_count(); }
 
 // Pieces of a launch: units of the prefix (at most a segment per workgroup and one per tile of query
 // rows), units of the rows, and one more per workgroup where a share ends inside a unit.
-int64_t piece_slots(int rows, int tokens, int num_q_heads, int num_kv_heads, int head_dim) {
+int64_t piece_slots(int rows, int tokens, int num_q_heads, int num_kv_heads) {
   const int64_t query_rows = static_cast<int64_t>(tokens) * (num_q_heads / num_kv_heads);
   const int64_t tiles = query_rows / kNarrowRows + 1;
-  return 2 * static_cast<int64_t>(attention_groups(head_dim)) + num_kv_heads * (2 * tiles + rows);
+  return 2 * static_cast<int64_t>(attention_groups()) + num_kv_heads * (2 * tiles + rows);
 }
 
 template <int DT, int D>
 int launch(hipStream_t stream, const PrefixArgs& a) {
-  prefix_attention_kernel<DT, D><<<a.groups, Shape<D>::kThreads, 0, stream>>>(a);
+  const bool whole = a.block_size % Shape<D>::kPerLoad == 0;
+  if (whole) prefix_attention_kernel<DT, D, true><<<a.groups, Shape<D>::kThreads, 0, stream>>>(a);
+  else prefix_attention_kernel<DT, D, false><<<a.groups, Shape<D>::kThreads, 0, stream>>>(a);
   const int blocks = static_cast<int>((static_cast<int64_t>(a.tokens) * a.group + 31) / 32);
-  prefix_join_kernel<DT, D><<<dim3(blocks, a.hkv), 2 * D, 0, stream>>>(a);
+  prefix_join_kernel<DT, D><<<dim3(blocks, Shape<D>::kBlocks, a.hkv), 64 * kJoinWaves, 0, stream>>>(a);
   return check_launch("ds_prefix_attention");
 }
 
@@ -874,7 +992,7 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0
 size_t workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads, int head_dim) {
   if (rows <= 0 || tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return 0;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256) return 0;
-  return static_cast<size_t>(piece_slots(rows, tokens, num_q_heads, num_kv_heads, head_dim)) * kWideRows *
+  return static_cast<size_t>(piece_slots(rows, tokens, num_q_heads, num_kv_heads)) * kWideRows *
          (head_dim + 2) * sizeof(float);
 }
 
@@ -894,7 +1012,8 @@ int prefix_attention_impl(hipStream_t stream, const ds_prefix_attention_desc* d)
              "null tensor pointer");
   const int64_t strides[] = {d->q_row_stride,   d->q_head_stride,  d->o_row_stride,   d->o_head_stride, d->k_block_stride,
                              d->k_token_stride, d->k_head_stride,  d->v_block_stride, d->v_token_stride, d->v_head_stride};
-  for (int64_t s : strides) DS_REQUIRE(s % 8 == 0, "row, page and head strides must be multiples of 8 elements");
+  for (int64_t s : strides) DS_REQUIRE(s >= 0 && s % 8 == 0, "row, page and head strides must be multiples of 8 elements");
+  DS_SUPPORTED(d->k_token_stride < (1 << 28) && d->v_token_stride < (1 << 28), "token strides of at most 2^28 elements");
   DS_REQUIRE(aligned(d->query) && aligned(d->output) && aligned(d->key_cache) && aligned(d->value_cache),
              "query, output and KV caches must be 16-byte aligned");
   const size_t need = workspace_bytes(d->rows, d->tokens, d->num_q_heads, d->num_kv_heads, d->head_dim);
@@ -902,7 +1021,7 @@ int prefix_attention_impl(hipStream_t stream, const ds_prefix_attention_desc* d)
              "workspace must be 256-byte aligned and hold ds_prefix_attention_workspace_bytes()");
   const int group = d->num_q_heads / d->num_kv_heads;
   const int64_t capacity = std::min<int64_t>(static_cast<int64_t>(d->max_blocks) * d->block_size, 1 << 30);
-  const int tile = d->head_dim <= 128 ? 128 : 64;
+  const int tile = 16384 / d->head_dim;
   const int64_t tiles = static_cast<int64_t>(d->tokens) * group / kNarrowRows + 1 + d->rows;
   DS_SUPPORTED(d->tokens <= (1 << 20), "at most 2^20 query tokens");
   DS_SUPPORTED(d->num_kv_heads * tiles * ((capacity + tile - 1) / tile + 1) * 2 < INT_MAX &&
@@ -927,10 +1046,11 @@ int prefix_attention_impl(hipStream_t stream, const ds_prefix_attention_desc* d)
   a.per_block = 1.f / static_cast<float>(d->block_size);
   a.q_start = d->query_start, a.q_len = d->query_len, a.t_len = d->target_len, a.prefix_len = d->prefix_len;
   a.rows = d->rows, a.tokens = d->tokens, a.hkv = d->num_kv_heads, a.group = group;
-  a.scale_log2 = d->scale * kLog2eP;
+  a.scale_log2 = std::fabs(d->scale) * kLog2eP;
+  a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
   a.pieces = static_cast<float*>(d->workspace);
-  a.slots = static_cast<int>(piece_slots(d->rows, d->tokens, d->num_q_heads, d->num_kv_heads, d->head_dim));
-  a.groups = attention_groups(d->head_dim);
+  a.slots = static_cast<int>(piece_slots(d->rows, d->tokens, d->num_q_heads, d->num_kv_heads));
+  a.groups = attention_groups();
   a.status = d->status;
   return d->dtype == DS_BF16 ? launch_dim<DS_BF16>(stream, d->head_dim, a) : launch_dim<DS_FP16>(stream, d->head_dim, a);
 }
