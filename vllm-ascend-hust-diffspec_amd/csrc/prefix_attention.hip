@@ -18,7 +18,7 @@
 //
 // Work: a unit is (KV head, tile of query rows, key range); its key tiles are laid end to end with
 // all other units' and dealt to the workgroups in equal contiguous shares, whatever the rows'
-// lengths.  Every workgroup derives the same layout from the lengths on the device, so a captured
+// lengths (a unit also counts a few places for what it costs beside its tiles).  Every workgroup derives the same layout from the lengths on the device, so a captured
 // launch follows changed lengths.  Prefix ranges are cut into segments of one share with the row
 // tiles inside a segment next to each other, and consecutive shares are given to one XCD, so the
 // row tiles that read the same keys do it at about the same time behind one L2.  A share that ends
@@ -42,6 +42,9 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 constexpr float kLog2eP = 1.44269504088896340736f;
 constexpr float kLn2P = 0.69314718055994530942f;
 constexpr int kWideRows = 128, kNarrowRows = 64;  // query rows of a unit's tile
+// Places that a unit takes in the work beside its key tiles: what its queries' loads, its joins and its
+// piece cost, in tiles.
+constexpr int kUnitCost = 2;
 constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
@@ -104,16 +107,16 @@ struct Plan {
   int prefix_tile;   // query rows of a prefix tile
   int row_tiles;     // prefix tiles of query rows, per KV head
   int key_tiles;     // tiles of prefix keys
-  int segments;
-  int share;         // key tiles per workgroup, and per prefix segment
-  int prefix_work;   // key tiles of all prefix units
+  int segments, segment;  // pieces of the prefix, and the key tiles of one
+  int prefix_work;   // places of all prefix units
   int prefix_units;
-  int work;          // key tiles of all units
+  int work;          // places of all units
+  int share;         // places per workgroup
 };
 
 struct RowTables {
   int token[kMaxRows + 1];  // query tokens of the rows before
-  int work[kMaxRows + 1];   // own key tiles of the rows before, per KV head
+  int work[kMaxRows + 1];   // places of the own units of the rows before, per KV head
   int start[kMaxRows];      // first query token
   int seen[kMaxRows];       // keys that its first query token sees, less one
 };
@@ -133,6 +136,18 @@ __device__ __forceinline__ Row row_of(const PrefixArgs& a, int b) {
 __device__ __forceinline__ int tile_rows(int rows) { return rows > kNarrowRows ? kWideRows : kNarrowRows; }
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 __device__ __forceinline__ int query_tiles(int rows) { return ceil_div(rows, tile_rows(rows)); }
+
+// The thread's index, opaque to the compiler: what a part of the loop derives from it is derived there
+// again, instead of being kept in registers that the loop needs (spilled ones would be loaded in order
+// behind the keys in flight).
+__device__ __forceinline__ int fresh_thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// A value that is the same in all lanes, to the scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 __device__ __forceinline__ int wave_min(int v) {
   return static_cast<int>(wave_pick<false>(static_cast<uint32_t>(v) ^ 0x80000000u) ^ 0x80000000u);
@@ -209,13 +224,14 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
   // A single row has nobody to share with: all its keys are its own.
   // Key ranges begin at multiples of 16: what is left of the prefix is read row by row.
   p.prefix = count > 1 ? min(max(asked, 0), least) & ~15 : 0;
-  p.prefix_row = count > 0 ? p.prefix_row : 0;
-  p.query_tokens = cut;
+  p.prefix = uniform(p.prefix);
+  p.prefix_row = uniform(count > 0 ? p.prefix_row : 0);
+  p.seen_by_all = uniform(p.seen_by_all);
+  p.query_tokens = uniform(cut);
   const int m = p.query_tokens * a.group;
   p.prefix_tile = tile_rows(m);
   p.row_tiles = ceil_div(m, p.prefix_tile);
   p.key_tiles = ceil_div(p.prefix, kTile);
-  p.prefix_work = a.hkv * p.row_tiles * p.key_tiles;
   // Own units.
   int own_work[kRounds];
 #pragma unroll
@@ -232,7 +248,7 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
     }
     int w = 0;
     if (row[i].len > 0 && fits && row[i].keys > p.prefix) {
-      w = query_tiles(row[i].len * a.group) * ceil_div(row[i].keys - p.prefix, kTile);
+      w = query_tiles(row[i].len * a.group) * (kUnitCost + ceil_div(row[i].keys - p.prefix, kTile));
     }
     const int work = wave_inclusive_scan(w);
     own_work[i] = work - w;
@@ -250,7 +266,7 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
     for (int i = 0; i < kRounds; ++i) {
       if (w == i * (THREADS / 64) + wave) own_work[i] += work;
     }
-    work += part_work[w];
+    work += uniform(part_work[w]);
   }
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
@@ -262,42 +278,47 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
     t.work[a.rows] = work;
   }
   __syncthreads();
+  // A segment of the prefix is a share without the cost of a unit, so that a unit is about a share.
+  p.segment = max(1, ceil_div(a.hkv * p.row_tiles * p.key_tiles + a.hkv * work, a.groups));
+  p.segments = ceil_div(p.key_tiles, p.segment);
+  p.prefix_units = a.hkv * p.segments * p.row_tiles;
+  p.prefix_work = a.hkv * p.row_tiles * p.key_tiles + kUnitCost * p.prefix_units;
   p.work = p.prefix_work + a.hkv * work;
   p.share = max(1, ceil_div(p.work, a.groups));
-  p.segments = ceil_div(p.key_tiles, p.share);
-  p.prefix_units = a.hkv * p.segments * p.row_tiles;
   return p;
 }
 
-// One unit and where its key tiles lie in the work.
+// One unit and where it lies in the work: kUnitCost places, then one for each of its key tiles.
 struct Unit {
-  int index;      // in the order of the work
+  int index;       // in the order of the work
   int kv_head;
-  int row;        // own units: the row; prefix units: -1
-  int tile;       // tile of query rows
-  int rows;       // query rows in all (of the row, or of the batch)
+  int row;         // own units: the row; prefix units: -1
+  int tile;        // tile of query rows
+  int rows;        // query rows in all (of the row, or of the batch)
   int tile_rows;
-  int first_work; // place of its first key tile in the work
+  int first_tile;  // place of its first key tile
   int key_tiles;
-  int key0;       // first key
-  int key_end;    // one past the last key of the unit's range
+  int key0;        // first key
+  int key_end;     // one past the last key
+  int seen_by_all; // keys that all its query rows see
 };
 
 template <int D>
 __device__ __forceinline__ Unit prefix_unit(const PrefixArgs& a, const Plan& p, int h, int segment, int tile) {
   constexpr int kTile = Shape<D>::kTile;
   Unit u;
-  const int before = segment * p.share;
-  u.key_tiles = min(p.share, p.key_tiles - before);
+  const int before = segment * p.segment;
+  u.key_tiles = min(p.segment, p.key_tiles - before);
   u.index = (segment * a.hkv + h) * p.row_tiles + tile;
   u.kv_head = h;
   u.row = -1;
   u.tile = tile;
   u.rows = p.query_tokens * a.group;
   u.tile_rows = p.prefix_tile;
-  u.first_work = before * a.hkv * p.row_tiles + (h * p.row_tiles + tile) * u.key_tiles;
+  u.first_tile = before * a.hkv * p.row_tiles + (h * p.row_tiles + tile) * u.key_tiles + kUnitCost * (u.index + 1);
   u.key0 = before * kTile;
   u.key_end = min(p.prefix, u.key0 + u.key_tiles * kTile);
+  u.seen_by_all = min(p.seen_by_all, u.key_end);
   return u;
 }
 
@@ -308,39 +329,53 @@ __device__ __forceinline__ Unit own_unit(const PrefixArgs& a, const Plan& p, con
   const int w = t.work[b + 1] - t.work[b];
   u.rows = (t.token[b + 1] - t.token[b]) * a.group;
   const int n = query_tiles(u.rows);
-  // Places for a row's units start past those of the rows before: they have at most one tile each
+  // Indexes of a row's units start past those of the rows before: they have at most one tile each
   // more than whole tiles of kNarrowRows query rows.
   u.index = p.prefix_units + a.hkv * (b + t.token[b] * a.group / kNarrowRows) + h * n + tile;
   u.kv_head = h;
   u.row = b;
   u.tile = tile;
   u.tile_rows = tile_rows(u.rows);
-  u.key_tiles = w / n;
-  u.first_work = p.prefix_work + a.hkv * t.work[b] + h * w + tile * u.key_tiles;
+  u.key_tiles = w / n - kUnitCost;
+  u.first_tile = p.prefix_work + a.hkv * t.work[b] + h * w + tile * (w / n) + kUnitCost;
   u.key0 = p.prefix;
-  u.key_end = t.seen[b] + t.token[b + 1] - t.token[b];
+  // The tile's last query token sees most.
+  u.key_end = t.seen[b] + (min((tile + 1) * u.tile_rows, u.rows) - 1) / a.group + 1;
+  u.seen_by_all = min(t.seen[b] + tile * u.tile_rows / a.group + 1, u.key_end);
   return u;
 }
 
-// The unit that holds place `w` of the work.
+// The unit that holds place `w` of the work (the same for all lanes).
 template <int D>
-__device__ __forceinline__ Unit unit_at(const PrefixArgs& a, const Plan& p, const RowTables& t, int w) {
+__device__ __forceinline__ Unit unit_at(const PrefixArgs& a, const Plan& plan, const RowTables& t, int w) {
+  Plan p;
+  p.prefix = uniform(plan.prefix), p.seen_by_all = uniform(plan.seen_by_all);
+  p.query_tokens = uniform(plan.query_tokens), p.prefix_tile = uniform(plan.prefix_tile);
+  p.row_tiles = uniform(plan.row_tiles), p.key_tiles = uniform(plan.key_tiles), p.segment = uniform(plan.segment);
+  p.prefix_work = uniform(plan.prefix_work), p.prefix_units = uniform(plan.prefix_units);
+  Unit u;
   if (w < p.prefix_work) {
-    const int per_segment = p.share * a.hkv * p.row_tiles;
-    const int segment = w / per_segment, len = min(p.share, p.key_tiles - segment * p.share);
+    const int per_segment = (p.segment + kUnitCost) * a.hkv * p.row_tiles;
+    const int segment = w / per_segment, len = min(p.segment, p.key_tiles - segment * p.segment) + kUnitCost;
     const int i = (w - segment * per_segment) / len;
-    return prefix_unit<D>(a, p, i / p.row_tiles, segment, i % p.row_tiles);
+    u = prefix_unit<D>(a, p, i / p.row_tiles, segment, i % p.row_tiles);
+  } else {
+    const int rest = w - p.prefix_work;
+    int lo = 0, hi = a.rows - 1;  // the last row whose work starts at or before `rest`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.hkv * uniform(t.work[mid]) <= rest) lo = mid; else hi = mid - 1;
+    }
+    const int before = uniform(t.work[lo]), mine = uniform(t.work[lo + 1]) - before;
+    const int in_row = rest - a.hkv * before, h = in_row / mine;
+    const int n = query_tiles((uniform(t.token[lo + 1]) - uniform(t.token[lo])) * a.group);
+    u = own_unit<D>(a, p, t, lo, h, (in_row - h * mine) / (mine / n));
   }
-  const int rest = w - p.prefix_work;
-  int lo = 0, hi = a.rows - 1;  // the last row whose work starts at or before `rest`
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.hkv * t.work[mid] <= rest) lo = mid; else hi = mid - 1;
-  }
-  const int mine = t.work[lo + 1] - t.work[lo], n = query_tiles((t.token[lo + 1] - t.token[lo]) * a.group);
-  const int in_row = rest - a.hkv * t.work[lo];
-  const int h = in_row / mine;
-  return own_unit<D>(a, p, t, lo, h, (in_row - h * mine) / (mine / n));
+  u.index = uniform(u.index), u.kv_head = uniform(u.kv_head), u.row = uniform(u.row), u.tile = uniform(u.tile);
+  u.rows = uniform(u.rows), u.tile_rows = uniform(u.tile_rows), u.first_tile = uniform(u.first_tile);
+  u.key_tiles = uniform(u.key_tiles), u.key0 = uniform(u.key0), u.key_end = uniform(u.key_end);
+  u.seen_by_all = uniform(u.seen_by_all);
+  return u;
 }
 
 // Row of the batch that holds query token `token` of the packed order.
@@ -417,22 +452,57 @@ __device__ __forceinline__ int piece_at(int t, int c) {
   return t * (D / 8) + (c ^ turn);
 }
 
-// Where a tile begins: its first key, and that key's page (in the table) and place.  Tiles follow
-// each other, so a key's page comes from the place and the distance, both small: (n + 0.5) / size in
-// floating point gives the exact quotient for n < 2^22 (the half keeps it away from the integers by
-// 0.5 / size, more than the 2^-23 relative error of a product with a rounded reciprocal).
-struct Cursor {
-  int key, page, place;
-};
+// (n + 0.5) / size in floating point gives the exact quotient for n < 2^22: the half keeps it away from
+// the integers by 0.5 / size, more than the 2^-23 relative error of a product with a rounded reciprocal.
 __device__ __forceinline__ int pages_in(const PrefixArgs& a, int n) {
   return static_cast<int>((static_cast<float>(n) + 0.5f) * a.per_block);
 }
-__device__ __forceinline__ void advance(const PrefixArgs& a, Cursor& c, int keys) {
-  const int n = __builtin_amdgcn_readfirstlane(pages_in(a, c.place + keys));
-  c.key += keys;
-  c.page += n;
-  c.place += keys - n * a.block_size;
-}
+
+// A key tile of the share: its keys [key, key_end) and the page and place of the first one, which the
+// places of the others follow by small distances.
+struct Step {
+  int key, key_end, head;
+  bool once;             // no other workgroup reads the keys
+  const int32_t* pages;  // the table entry of the first key's page
+  int place;
+};
+
+// The share's key tiles in order, across its units.
+template <int D>
+struct Feed {
+  Unit unit;
+  int at, end;  // places: the next one, the share's end
+  Step step;    // of the next key tile of the unit
+
+  __device__ __forceinline__ void start(const PrefixArgs& a, const Plan& p, const RowTables& t) {
+    unit = unit_at<D>(a, p, t, at);
+    at = max(at, unit.first_tile);
+    step.key = unit.key0 + (at - unit.first_tile) * Shape<D>::kTile;
+    step.key_end = unit.key_end;
+    step.head = unit.kv_head;
+    step.once = unit.row >= 0 || uniform(p.row_tiles) == 1;
+    const int page = uniform(step.key / a.block_size);
+    step.place = step.key - page * a.block_size;
+    step.pages = a.table + static_cast<int64_t>(unit.row < 0 ? uniform(p.prefix_row) : unit.row) * a.bt_stride + page;
+  }
+  // The next key tile; one without keys behind the last.
+  __device__ __forceinline__ Step next(const PrefixArgs& a, const Plan& p, const RowTables& t) {
+    Step s = step;
+    if (at >= end) {
+      s.key = s.key_end = 0;
+      return s;
+    }
+    if (++at == unit.first_tile + unit.key_tiles) {
+      if (at < end) start(a, p, t);
+    } else {
+      const int n = uniform(pages_in(a, step.place + Shape<D>::kTile));
+      step.key += Shape<D>::kTile;
+      step.pages += n;
+      step.place += Shape<D>::kTile - n * a.block_size;
+    }
+    return s;
+  }
+};
 
 // A tile's keys and values in flight to shared memory.  One load of a wave takes kPerLoad neighbouring
 // keys (whole 128-byte lines of one head); ranges begin at multiples of 16 keys, so where the page
@@ -445,22 +515,16 @@ struct Staged {
   int bad;       // loads of a page out of range
 };
 
-// First key of the wave's load i, from the tile's first; loads past the range take its last keys (and
-// are zeroed on their way to shared memory).
-template <int D>
-__device__ __forceinline__ int load_key(const Cursor& c, int i, int wave, int key_end) {
-  using S = Shape<D>;
-  return min(i * S::kPerPass + wave * S::kPerLoad, (key_end - 1 - c.key) & ~(S::kPerLoad - 1));
-}
-
+// Loads past the range take its last keys (and are zeroed on their way to shared memory).
 template <int D, bool WHOLE>
-__device__ __forceinline__ void find_pages(const PrefixArgs& a, const int32_t* table, const Cursor& c, int key_end,
-                                           int wave, Staged<D>& s) {
-  if (c.key >= key_end || !WHOLE) return;
-  const int n = c.place + load_key<D>(c, threadIdx.x % Shape<D>::kPasses, wave, key_end);
+__device__ __forceinline__ void find_pages(const PrefixArgs& a, const Step& step, int wave, Staged<D>& s) {
+  using S = Shape<D>;
+  if (step.key >= step.key_end || !WHOLE) return;
+  const int i = fresh_thread() % S::kPasses;
+  const int n = step.place + min(i * S::kPerPass + wave * S::kPerLoad, (step.key_end - 1 - step.key) & ~(S::kPerLoad - 1));
   const int j = pages_in(a, n);
   s.in = n - j * a.block_size;
-  s.page = table[c.page + j];
+  s.page = step.pages[j];
 }
 
 template <bool ONCE>
@@ -470,44 +534,46 @@ __device__ __forceinline__ u32x4 load_piece(const uint16_t* base, uint32_t bytes
 }
 
 template <int D, bool WHOLE, bool ONCE>
-__device__ __forceinline__ void load_keys(const PrefixArgs& a, const int32_t* table, const Cursor& c, int key_end, int h,
-                                          int wave, int i, Staged<D>& s) {
+__device__ __forceinline__ void load_keys(const PrefixArgs& a, const Step& step, int thread, int wave, int i,
+                                          Staged<D>& s) {
   using S = Shape<D>;
-  const int lane = threadIdx.x & 63, piece = lane % S::kLanes, mine = lane / S::kLanes;
+  const int lane = thread & 63, piece = lane % S::kLanes, mine = lane / S::kLanes;
+  const uint16_t* keys = a.k + step.head * a.k_head;
+  const uint16_t* values = a.v + step.head * a.v_head;
   if constexpr (WHOLE) {
     const int found = __builtin_amdgcn_readlane(s.page, i);
     const int64_t in = __builtin_amdgcn_readlane(s.in, i);
     const bool fine = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
     const int64_t page = fine ? found : 0;
     s.bad = (s.bad & ~(1 << i)) | (fine ? 0 : 1 << i);
-    s.k[i] = load_piece<ONCE>(a.k + (page * a.k_block + in * a.k_token + h * a.k_head),
+    s.k[i] = load_piece<ONCE>(keys + (page * a.k_block + in * a.k_token),
                               2 * (mine * static_cast<uint32_t>(a.k_token) + 8 * piece));
-    s.v[i] = load_piece<ONCE>(a.v + (page * a.v_block + in * a.v_token + h * a.v_head),
+    s.v[i] = load_piece<ONCE>(values + (page * a.v_block + in * a.v_token),
                               2 * (mine * static_cast<uint32_t>(a.v_token) + 8 * piece));
   } else {  // a page a lane
-    const int n = c.place + min(i * S::kPerPass + wave * S::kPerLoad + mine, key_end - 1 - c.key);
+    const int n = step.place + min(i * S::kPerPass + wave * S::kPerLoad + mine, step.key_end - 1 - step.key);
     const int j = pages_in(a, n);
-    const int found = table[c.page + j];
+    const int found = step.pages[j];
     const int64_t in = n - j * a.block_size;
     const bool fine = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
     const int64_t page = fine ? found : 0;
     s.bad = (s.bad & ~(1 << i)) | (fine ? 0 : 1 << i);
-    s.k[i] = load_piece<ONCE>(a.k + (page * a.k_block + in * a.k_token + h * a.k_head), 16 * piece);
-    s.v[i] = load_piece<ONCE>(a.v + (page * a.v_block + in * a.v_token + h * a.v_head), 16 * piece);
+    s.k[i] = load_piece<ONCE>(keys + (page * a.k_block + in * a.k_token), 16 * piece);
+    s.v[i] = load_piece<ONCE>(values + (page * a.v_block + in * a.v_token), 16 * piece);
   }
 }
 
 template <int D>
-__device__ __forceinline__ void store_keys(const PrefixArgs& a, char* stage, int key, int key_end, int wave, int i,
-                                           Staged<D>& s) {
+__device__ __forceinline__ void store_keys(const PrefixArgs& a, char* stage, const Step& step, int thread, int wave,
+                                           int i, Staged<D>& s) {
   using S = Shape<D>;
-  const int lane = threadIdx.x & 63, piece = lane % S::kLanes;
+  const int lane = thread & 63, piece = lane % S::kLanes;
   const int t = i * S::kPerPass + wave * S::kPerLoad + lane / S::kLanes;
-  if (key + S::kTile > key_end || __any(s.bad != 0)) {
-    if (key + t >= key_end || (s.bad >> i) & 1) {
+  if (step.key + S::kTile > step.key_end || __any(s.bad != 0)) {
+    if (step.key + t >= step.key_end || (s.bad >> i) & 1) {
       s.k[i] = u32x4{0, 0, 0, 0};
       s.v[i] = u32x4{0, 0, 0, 0};
-      if (key + t < key_end && a.status) {
+      if (step.key + t < step.key_end && a.status) {
         __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
@@ -518,30 +584,25 @@ __device__ __forceinline__ void store_keys(const PrefixArgs& a, char* stage, int
 
 // Where a lane reads in a staged tile, in bytes: a key's piece 0 for the score product (key lane % 32
 // of 32, the first 16 bytes of its half of a step), and for the output product the values of four keys
-// of output block j.  A transposing read gives lane l of 16 four keys of dimension l, where lane l names
+// of output block 0.  A transposing read gives lane l of 16 four keys of dimension l, where lane l names
 // key l / 4 and dimensions 4 (l % 4) .. + 3; keys 8 (or 16, 32) further on are a constant away, since
-// the turn of the pieces repeats every eight.
-template <int D>
+// the turn of the pieces repeats every eight, and block j's address differs in bits 6 and up by j (a
+// value's pieces of a block are the low two bits of a piece's number, and stages begin at 512 bytes).
 struct Lane {
-  int key, value[Shape<D>::kBlocks];
+  int key, value;
 };
 template <int D>
-__device__ __forceinline__ Lane<D> lane_places() {
+__device__ __forceinline__ Lane lane_places() {
   using S = Shape<D>;
-  const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 15;
-  Lane<D> p;
-  p.key = (lane & 31) * S::kKeyBytes + 16 * half;
-#pragma unroll
-  for (int j = 0; j < S::kBlocks; ++j) {
-    p.value[j] = S::kValuesAt + 16 * piece_at<D>(4 * half + (l >> 2), 4 * j + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) +
-                 8 * (l & 1);
-  }
-  return p;
+  static_assert(S::kValuesAt % 512 == 0 && S::kStage % 512 == 0, "block numbers are address bits of their own");
+  const int lane = fresh_thread() & 63, half = lane >> 5, l = lane & 15;
+  return Lane{(lane & 31) * S::kKeyBytes + 16 * half,
+              S::kValuesAt + 16 * piece_at<D>(4 * half + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) + 8 * (l & 1)};
 }
 
-__device__ __forceinline__ u32x2 read_values(const char* p) {
-  const lds_s16x4* q = (const lds_s16x4*)p;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(const_cast<lds_s16x4*>(q)));
+typedef __attribute__((address_space(3))) char lds_char;
+__device__ __forceinline__ u32x2 read_values(uint32_t at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_char*)at));
 }
 
 __device__ __forceinline__ bool not_finite2(uint32_t w, uint32_t exponent) {
@@ -563,7 +624,7 @@ struct State {
 template <int DT, int D>
 __device__ __forceinline__ void add_not_finite(const u32x4* values, State<D>& st, int t0, int seen) {
   constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
-  const int half = (threadIdx.x >> 5) & 1;
+  const int half = (fresh_thread() >> 5) & 1;
 #pragma unroll 1
   for (int t = 0; t < 32; ++t) {
 #pragma unroll
@@ -585,7 +646,7 @@ __device__ __forceinline__ void add_not_finite(const u32x4* values, State<D>& st
 // them the lane column's query row sees.  Reads of a step are issued together, ahead of the products
 // that take them: the keys' before the first product, the values' before the softmax.
 template <int DT, int D, bool MASKED>
-__device__ __forceinline__ void attend_keys(const char* stage, const Lane<D>& at, const u32x4 (&q)[Shape<D>::kSteps],
+__device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, const u32x4 (&q)[Shape<D>::kSteps],
                                             State<D>& st, int t0, int seen, float scale_log2) {
   using S = Shape<D>;
   constexpr int kBatch = S::kSteps < 8 ? S::kSteps : 8;
@@ -605,23 +666,26 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane<D>& at
   }
   constexpr int kAhead = S::kBlocks <= 4 ? S::kBlocks : 4;  // blocks whose values are read before the softmax
   u32x2 v[2][kAhead][2];
+  const uint32_t values = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)stage)) + at.value;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) v[s][j][e] = read_values(stage + at.value[j] + (t0 + 16 * s + 8 * e) * 2 * D);
+      for (int e = 0; e < 2; ++e) v[s][j][e] = read_values((values ^ (64 * j)) + (t0 + 16 * s + 8 * e) * 2 * D);
     }
   }
   __builtin_amdgcn_sched_barrier(0);
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    if constexpr (MASKED) sc[i] = 8 * (i >> 2) + 4 * half + (i & 3) < seen ? sc[i] : -INFINITY;
+    if constexpr (MASKED) sc[i] = 8 * (i >> 2) + (i & 3) < seen - 4 * half ? sc[i] : -INFINITY;
     top = fmaxf(top, sc[i]);
   }
   top = fmaxf(top, other_half(top)) * scale_log2;
-  if (__any(top > st.m)) {
+  // The reference of the exponents follows the maximum only when it is 2^8 behind: weights of up to 2^8
+  // keep their relative precision, and most tiles leave the sums as they are.
+  if (__any(top > st.m + 8.f)) {
     const float m = fmaxf(st.m, top);
     const float keep = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
     st.m = m;
@@ -645,9 +709,10 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane<D>& at
   bool poison = false;
   if constexpr (MASKED) {
     bool bad = false;
+    const int thread = fresh_thread();
 #pragma unroll 1
-    for (int c = half; c < D / 8; c += 2) {
-      const u32x4 x = reinterpret_cast<const u32x4*>(stage + S::kValuesAt)[piece_at<D>(t0 + (lane & 31), c)];
+    for (int c = (thread >> 5) & 1; c < D / 8; c += 2) {
+      const u32x4 x = reinterpret_cast<const u32x4*>(stage + S::kValuesAt)[piece_at<D>(t0 + (thread & 31), c)];
       bad |= not_finite2(x[0], kExponent) || not_finite2(x[1], kExponent) || not_finite2(x[2], kExponent) ||
              not_finite2(x[3], kExponent);
     }
@@ -678,7 +743,7 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane<D>& at
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
       for (int j = kAhead; j < S::kBlocks; ++j) {
-        const char* from = stage + at.value[j] + (t0 + 16 * s) * 2 * D;
+        const uint32_t from = (values ^ (64 * j)) + (t0 + 16 * s) * 2 * D;
         output(j, s, read_values(from), read_values(from + 8 * 2 * D));
       }
     }
@@ -695,102 +760,48 @@ __device__ __forceinline__ float* piece_sums(const PrefixArgs& a, int slot) {
   return a.pieces + static_cast<int64_t>(slot) * (kWideRows * (D + 2));
 }
 
-// The key tiles [from, to) of a unit, and the unit's piece.
-template <int DT, int D, bool WHOLE, bool WIDE, bool ONCE>
-__device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, const Unit& u,
-                                         int from, int to, int slot, char* lds) {
+// How a unit's tile lies over the waves: kQ blocks of 32 query rows, kT waves to a block, which share the
+// keys of a tile, kN blocks of 32 each.
+template <int D, bool WIDE>
+struct Split {
+  static constexpr int kQ = WIDE ? 4 : 2;
+  static constexpr int kT = Shape<D>::kWaves / kQ;
+  static constexpr int kN = Shape<D>::kTile / 32 / kT;
+};
+
+// A wave's query rows of a unit.
+template <int D>
+struct Queries {
+  u32x4 q[Shape<D>::kSteps];
+  int limit;  // keys that the lane column's row sees
+  bool any;
+};
+
+template <int D, bool WIDE>
+__device__ __forceinline__ void load_queries(const PrefixArgs& a, const RowTables& t, const Unit& u, int wave,
+                                             Queries<D>& q) {
   using S = Shape<D>;
-  constexpr int kQ = WIDE ? 4 : 2;             // blocks of 32 query rows
-  constexpr int kT = S::kWaves / kQ;           // waves that share a block's keys
-  constexpr int kN = S::kTile / 32 / kT;       // blocks of 32 keys of a tile per wave
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int qb = wave / kT, tb = wave % kT;
+  const int lane = fresh_thread() & 63, r0 = u.tile * u.tile_rows + 32 * (wave / Split<D, WIDE>::kT);
+  const QueryRow row = query_row(a, t, u, r0 + (lane & 31));
+  q.any = r0 < u.rows;
+  q.limit = row.limit;
+  const uint16_t* src = a.q + row.token * a.q_row + row.head * a.q_head + 8 * (lane >> 5);
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) {
+    q.q[s] = u32x4{0, 0, 0, 0};
+    if (row.valid) q.q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s) ^ a.q_sign;
+  }
+}
+
+// The end of a unit (or of the share inside it): its piece.
+template <int D, bool WIDE>
+__device__ __forceinline__ void finish_unit(const PrefixArgs& a, const Unit& u, int slot, State<D>& st, int wave,
+                                            char* lds) {
+  using S = Shape<D>;
+  constexpr int kT = Split<D, WIDE>::kT;
+  const int lane = fresh_thread() & 63, qb = wave / kT, tb = wave % kT;
   const int r0 = u.tile * u.tile_rows + 32 * qb;
-  // Keys past the last query row's limit (own units: the tile's last token sees most).
-  int key_end = u.key_end, seen_by_all = p.seen_by_all;
-  if (u.row >= 0) {
-    seen_by_all = t.seen[u.row] + u.tile * u.tile_rows / a.group + 1;
-    const int last = (min((u.tile + 1) * u.tile_rows, u.rows) - 1) / a.group;
-    key_end = min(key_end, t.seen[u.row] + last + 1);
-  }
-  to = min(to, ceil_div(key_end - u.key0, S::kTile));
-  const int32_t* table = a.table + static_cast<int64_t>(u.row < 0 ? p.prefix_row : u.row) * a.bt_stride;
-  int key = u.key0 + from * S::kTile;
-  Cursor c{key, key / a.block_size, 0};  // of the tile whose pages are looked up next
-  c.place = key - c.page * a.block_size;
-  Staged<D> s;
-  s.page = s.in = s.bad = 0;
-  find_pages<D, WHOLE>(a, table, c, from < to ? key_end : 0, wave, s);
-
-  const QueryRow qr = query_row(a, t, u, r0 + (lane & 31));
-  u32x4 q[S::kSteps];
-  {
-    const uint16_t* src = a.q + qr.token * a.q_row + qr.head * a.q_head + 8 * (lane >> 5);
-#pragma unroll
-    for (int s = 0; s < S::kSteps; ++s) {
-      q[s] = u32x4{0, 0, 0, 0};
-      if (qr.valid) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s) ^ a.q_sign;
-    }
-  }
-  State<D> st;
-#pragma unroll
-  for (int j = 0; j < S::kBlocks; ++j) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) st.acc[j][i] = 0.f;
-  }
-  st.m = -INFINITY;
-  st.l = 0.f;
-
-  const Lane<D> at = lane_places<D>();
-  if (from < to) {
-#pragma unroll
-    for (int i = 0; i < S::kPasses; ++i) load_keys<D, WHOLE, ONCE>(a, table, c, key_end, u.kv_head, wave, i, s);
-    advance(a, c, S::kTile);
-    find_pages<D, WHOLE>(a, table, c, key_end, wave, s);
-    __syncthreads();  // the unit before has read its last tile
-    // A register is loaded again as soon as its keys are in shared memory.
-    auto stage = [&](char* to_stage) {
-#pragma unroll
-      for (int i = 0; i < S::kPasses; ++i) {
-        store_keys<D>(a, to_stage, key, key_end, wave, i, s);
-        if (c.key < key_end) load_keys<D, WHOLE, ONCE>(a, table, c, key_end, u.kv_head, wave, i, s);
-      }
-      advance(a, c, S::kTile);
-      find_pages<D, WHOLE>(a, table, c, key_end, wave, s);
-      lds_barrier();
-    };
-    stage(lds);
-    int cur = 0, i = from;
-    auto stage_next = [&]() {
-      key += S::kTile;
-      if (++i < to) stage(lds + (cur ^ 1) * S::kStage);
-      else lds_barrier();
-      cur ^= 1;
-    };
-    // Tiles that all query rows see whole, then the ones with a mask.
-    while (i < to && key + S::kTile <= min(seen_by_all, key_end)) {
-      if (r0 < u.rows) {
-        const char* stage = lds + cur * S::kStage;
-#pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          attend_keys<DT, D, false>(stage, at, q, st, 32 * (tb * kN + n), 32, a.scale_log2);
-        }
-      }
-      stage_next();
-    }
-    while (i < to) {
-      if (r0 < u.rows) {
-        const int seen = min(qr.limit, key_end) - key;
-#pragma unroll 1
-        for (int t0 = 32 * tb * kN; t0 < min(32 * (tb + 1) * kN, key_end - key); t0 += 32) {
-          attend_keys<DT, D, true>(lds + cur * S::kStage, at, q, st, t0, seen - t0, a.scale_log2);
-        }
-      }
-      stage_next();
-    }
-  }
   st.l += other_half(st.l);
-
   // The waves that share query rows join in shared memory, each for its part of the dimensions (in
   // groups of four accumulators, as they are stored).
   constexpr int kGroups = 4 * S::kBlocks, kMine = kGroups / kT, kOther = kGroups - kMine;
@@ -807,7 +818,7 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
     static_assert(S::kWaves * (4 * kOther + 2) * 64 * 4 <= 2 * S::kStage, "the waves' results fit the tiles");
     f32x4* area = reinterpret_cast<f32x4*>(lds);
     float* sums = reinterpret_cast<float*>(area + S::kWaves * kOther * 64);
-    __syncthreads();
+    lds_barrier();
     if (r0 < u.rows) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
@@ -817,7 +828,7 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
       sums[2 * wave * 64 + lane] = st.m;
       sums[(2 * wave + 1) * 64 + lane] = st.l;
     }
-    __syncthreads();
+    lds_barrier();
     if (r0 < u.rows) {
       float m = st.m, l = 0.f, weight[kT];
 #pragma unroll
@@ -857,27 +868,128 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
   }
 }
 
-template <int DT, int D, bool WHOLE>
-__global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_attention_kernel(
-    PrefixArgs a) {
+// What a workgroup carries from tile to tile, across units.
+template <int D>
+struct Pipe {
+  Feed<D> feed;
+  Step now, ahead;  // the tile in registers, and the one after it, whose pages are looked up
+  Staged<D> s;
+  int cur;          // the half of shared memory the next tile goes to
+};
+
+template <int D, bool WHOLE>
+__device__ __forceinline__ void load_tile(const PrefixArgs& a, const Step& step, int thread, int wave, int i,
+                                          Staged<D>& s) {
+  if (step.key >= step.key_end) return;
+  if (step.once) load_keys<D, WHOLE, true>(a, step, thread, wave, i, s);
+  else load_keys<D, WHOLE, false>(a, step, thread, wave, i, s);
+}
+
+// The next tile's keys to shared memory; a register is loaded again as soon as its keys are there.
+template <int D, bool WHOLE>
+__device__ __forceinline__ const char* next_tile(const PrefixArgs& a, const Plan& p, const RowTables& t, Pipe<D>& pipe,
+                                                 int wave, char* lds) {
   using S = Shape<D>;
-  __shared__ __attribute__((aligned(16))) char lds[2 * S::kStage];
+  const int thread = fresh_thread();
+  char* stage = lds + pipe.cur * S::kStage;
+#pragma unroll
+  for (int i = 0; i < S::kPasses; ++i) {
+    store_keys<D>(a, stage, pipe.now, thread, wave, i, pipe.s);
+    load_tile<D, WHOLE>(a, pipe.ahead, thread, wave, i, pipe.s);
+  }
+  pipe.now = pipe.ahead;
+  pipe.ahead = pipe.feed.next(a, p, t);
+  find_pages<D, WHOLE>(a, pipe.ahead, wave, pipe.s);
+  pipe.cur ^= 1;
+  lds_barrier();
+  return stage;
+}
+
+// The share's tiles of a unit, from `place` on to `stop`.
+template <int DT, int D, bool WHOLE, bool WIDE>
+__device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, const Unit& u, int place,
+                                         int stop, int group, int wave, Pipe<D>& pipe, char* lds) {
+  using S = Shape<D>;
+  constexpr int kN = Split<D, WIDE>::kN;
+  const int first = 32 * (wave % Split<D, WIDE>::kT) * kN;
+  Queries<D> q;
+  load_queries<D, WIDE>(a, t, u, wave, q);
+  State<D> st;
+#pragma unroll
+  for (int j = 0; j < S::kBlocks; ++j) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) st.acc[j][i] = 0.f;
+  }
+  st.m = -INFINITY;
+  st.l = 0.f;
+  // Tiles that all query rows see whole, then the ones with a mask.
+  for (; place < stop && pipe.now.key + S::kTile <= u.seen_by_all; ++place) {
+    const char* stage = next_tile<D, WHOLE>(a, p, t, pipe, wave, lds);
+    if (q.any) {
+      const Lane at = lane_places<D>();
+#pragma unroll
+      for (int n = 0; n < kN; ++n) attend_keys<DT, D, false>(stage, at, q.q, st, first + 32 * n, 32, a.scale_log2);
+    }
+  }
+  for (; place < stop; ++place) {
+    const int seen = min(q.limit, u.key_end) - pipe.now.key, keys = u.key_end - pipe.now.key;
+    const char* stage = next_tile<D, WHOLE>(a, p, t, pipe, wave, lds);
+    if (q.any) {
+      const Lane at = lane_places<D>();
+#pragma unroll 1
+      for (int t0 = first; t0 < min(first + 32 * kN, keys); t0 += 32) {
+        attend_keys<DT, D, true>(stage, at, q.q, st, t0, seen - t0, a.scale_log2);
+      }
+    }
+  }
+  lds_barrier();
+  finish_unit<D, WIDE>(a, u, u.index + group, st, wave, lds);
+  lds_barrier();
+}
+
+template <int DT, int D, bool WHOLE>
+__global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_attention_kernel(PrefixArgs a) {
+  using S = Shape<D>;
+  __shared__ __attribute__((aligned(512))) char lds[2 * S::kStage];
   __shared__ RowTables tables;
-  const Plan p = make_plan<D, S::kThreads>(a, tables, blockIdx.x == 0);
+  __shared__ Plan p;  // read again at each unit
+  {
+    const Plan made = make_plan<D, S::kThreads>(a, tables, blockIdx.x == 0);
+    if (threadIdx.x == 0) p = made;
+    __syncthreads();
+  }
   // Consecutive shares on one XCD (workgroups are dealt to the eight in turn).
   const int per_xcd = a.groups / 8;
   const int group = a.groups % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + static_cast<int>(blockIdx.x / 8)
                                       : static_cast<int>(blockIdx.x);
-  int w = min(group * p.share, p.work);
-  const int end = min(w + p.share, p.work);
-  while (w < end) {
-    Unit u = unit_at<D>(a, p, tables, w);
-    const int from = w - u.first_work, to = min(u.key_tiles, end - u.first_work);
-    const int slot = u.index + group;
-    if (u.tile_rows != kWideRows) run_unit<DT, D, WHOLE, false, true>(a, p, tables, u, from, to, slot, lds);
-    else if (u.row >= 0 || p.row_tiles == 1) run_unit<DT, D, WHOLE, true, true>(a, p, tables, u, from, to, slot, lds);
-    else run_unit<DT, D, WHOLE, true, false>(a, p, tables, u, from, to, slot, lds);
-    w = u.first_work + to;
+  const int wave = uniform(threadIdx.x >> 6), share = uniform(p.share), work = uniform(p.work);
+  // Four tiles are under way at a time: one is attended to, the keys of the next are in shared memory or
+  // on their way to it, those of the third on their way to registers, the pages of the fourth are looked
+  // up.  The order goes across units, so that the memory does not wait for a unit's end.
+  Pipe<D> pipe;
+  pipe.feed.at = min(group * share, work);
+  pipe.feed.end = min(pipe.feed.at + share, work);
+  if (pipe.feed.at >= pipe.feed.end) return;
+  pipe.feed.start(a, p, tables);
+  int place = pipe.feed.at;
+  const int end = pipe.feed.end;
+  if (place >= end) return;  // the share ends before its unit's first key tile
+  pipe.cur = 0;
+  pipe.s.page = pipe.s.in = pipe.s.bad = 0;
+  pipe.now = pipe.feed.next(a, p, tables);
+  find_pages<D, WHOLE>(a, pipe.now, wave, pipe.s);
+#pragma unroll
+  for (int i = 0; i < S::kPasses; ++i) load_tile<D, WHOLE>(a, pipe.now, threadIdx.x, wave, i, pipe.s);
+  pipe.ahead = pipe.feed.next(a, p, tables);
+  find_pages<D, WHOLE>(a, pipe.ahead, wave, pipe.s);
+  while (place < end) {
+    const Unit u = unit_at<D>(a, p, tables, place);
+    place = max(place, u.first_tile);
+    const int stop = min(end, u.first_tile + u.key_tiles);
+    if (place >= stop) return;  // the share ends before the unit's first key tile
+    if (u.tile_rows == kWideRows) run_unit<DT, D, WHOLE, true>(a, p, tables, u, place, stop, group, wave, pipe, lds);
+    else run_unit<DT, D, WHOLE, false>(a, p, tables, u, place, stop, group, wave, pipe, lds);
+    place = stop;
   }
 }
 
@@ -919,19 +1031,19 @@ __global__ __launch_bounds__(64 * kJoinWaves) void prefix_join_kernel(PrefixArgs
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] = acc[k] * mine + part[k] * other;
   };
-  // A segment is at most a share long: its pieces are of one workgroup or of two.
+  // A segment is about a share long: its pieces are of one workgroup or of two, seldom of more.
   const int tile = 32 * block / p.prefix_tile, in_tile = 32 * block - tile * p.prefix_tile + (lane & 31);
   for (int k = wave; k < 2 * p.segments; k += kJoinWaves) {
     const Unit u = prefix_unit<D>(a, p, h, k >> 1, tile);
-    const int group = u.first_work / p.share + (k & 1);
-    if (group <= (u.first_work + u.key_tiles - 1) / p.share) join(u.index + group, in_tile);
+    const int last = (u.first_tile + u.key_tiles - 1) / p.share;
+    for (int group = u.first_tile / p.share + (k & 1); group <= last; group += 2) join(u.index + group, in_tile);
   }
   if (tables.work[b + 1] > tables.work[b]) {
     const int in_row = i * a.group + (valid ? r : rows - 1) % a.group;
     const int n = tile_rows((tables.token[b + 1] - tables.token[b]) * a.group);
     const Unit u = own_unit<D>(a, p, tables, b, h, in_row / n);
-    const int last = (u.first_work + u.key_tiles - 1) / p.share;
-    for (int group = u.first_work / p.share + wave; group <= last; group += kJoinWaves) join(u.index + group, in_row % n);
+    const int last = (u.first_tile + u.key_tiles - 1) / p.share;
+    for (int group = u.first_tile / p.share + wave; group <= last; group += kJoinWaves) join(u.index + group, in_row % n);
   }
   joined[wave][16][lane] = m;
   joined[wave][17][lane] = l;
