@@ -74,10 +74,10 @@ struct PrefixArgs {
   int64_t o_row, o_head;
   float* lse;
   int64_t l_row, l_head;
-  const uint16_t* k;
-  int64_t k_block, k_token, k_head;
-  const uint16_t* v;
-  int64_t v_block, v_token, v_head;
+  const char* k;
+  uint32_t k_block, k_token, k_head;  // bytes
+  const char* v;
+  uint32_t v_block, v_token, v_head;
   const int32_t* table;
   int64_t bt_stride;
   int capacity;  // keys that a table row can address
@@ -506,13 +506,13 @@ struct Feed {
 
 // A tile's keys and values in flight to shared memory.  One load of a wave takes kPerLoad neighbouring
 // keys (whole 128-byte lines of one head); ranges begin at multiples of 16 keys, so where the page
-// size is a multiple of kPerLoad they lie in one page and the addresses are the wave's, computed on the
-// scalar unit (WHOLE).  Lane i of a wave looks up the page of its load i, a tile ahead.
+// size is a multiple of kPerLoad they lie in one page and the addresses are the wave's (WHOLE).  Lane i
+// of a wave looks up the page of its load i a tile ahead, and computes its place in the caches.
 template <int D>
 struct Staged {
   u32x4 k[Shape<D>::kPasses], v[Shape<D>::kPasses];
   int page, in;  // of the next tile's loads
-  int bad;       // loads of a page out of range
+  int bad;       // loads in flight whose page is out of range
 };
 
 // Loads past the range take its last keys (and are zeroed on their way to shared memory).
@@ -527,49 +527,64 @@ __device__ __forceinline__ void find_pages(const PrefixArgs& a, const Step& step
   s.page = step.pages[j];
 }
 
+// The places of lane i's load in the caches, in bytes.
+struct Places {
+  uint64_t k, v;
+};
+template <int D>
+__device__ __forceinline__ Places load_places(const PrefixArgs& a, const Step& step, Staged<D>& s) {
+  const bool fine = static_cast<unsigned>(s.page) < static_cast<unsigned>(a.num_blocks);
+  s.bad = static_cast<int>(__ballot(!fine)) & ((1 << Shape<D>::kPasses) - 1);
+  const uint32_t page = fine ? s.page : 0, in = s.in;
+  return Places{static_cast<uint64_t>(page) * a.k_block + (in * a.k_token + step.head * a.k_head),
+                static_cast<uint64_t>(page) * a.v_block + (in * a.v_token + step.head * a.v_head)};
+}
+__device__ __forceinline__ uint64_t place_of(uint64_t places, int i) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(places), i))) |
+         static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(places >> 32), i))) << 32;
+}
+
 template <bool ONCE>
-__device__ __forceinline__ u32x4 load_piece(const uint16_t* base, uint32_t bytes) {
-  const u32x4* p = reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(base) + bytes);
+__device__ __forceinline__ u32x4 load_piece(const char* base, uint32_t bytes) {
+  const u32x4* p = reinterpret_cast<const u32x4*>(base + bytes);
   return ONCE ? __builtin_nontemporal_load(p) : *p;
 }
 
 template <int D, bool WHOLE, bool ONCE>
-__device__ __forceinline__ void load_keys(const PrefixArgs& a, const Step& step, int thread, int wave, int i,
-                                          Staged<D>& s) {
+__device__ __forceinline__ void load_keys(const PrefixArgs& a, const Step& step, const Places& at, int thread, int wave,
+                                          int i, Staged<D>& s) {
   using S = Shape<D>;
-  const int lane = thread & 63, piece = lane % S::kLanes, mine = lane / S::kLanes;
-  const uint16_t* keys = a.k + step.head * a.k_head;
-  const uint16_t* values = a.v + step.head * a.v_head;
+  const int lane = thread & 63;
+  const uint32_t piece = 16 * (lane % S::kLanes), mine = lane / S::kLanes;
   if constexpr (WHOLE) {
-    const int found = __builtin_amdgcn_readlane(s.page, i);
-    const int64_t in = __builtin_amdgcn_readlane(s.in, i);
-    const bool fine = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
-    const int64_t page = fine ? found : 0;
-    s.bad = (s.bad & ~(1 << i)) | (fine ? 0 : 1 << i);
-    s.k[i] = load_piece<ONCE>(keys + (page * a.k_block + in * a.k_token),
-                              2 * (mine * static_cast<uint32_t>(a.k_token) + 8 * piece));
-    s.v[i] = load_piece<ONCE>(values + (page * a.v_block + in * a.v_token),
-                              2 * (mine * static_cast<uint32_t>(a.v_token) + 8 * piece));
+    s.k[i] = load_piece<ONCE>(a.k + place_of(at.k, i), mine * a.k_token + piece);
+    s.v[i] = load_piece<ONCE>(a.v + place_of(at.v, i), mine * a.v_token + piece);
   } else {  // a page a lane
-    const int n = step.place + min(i * S::kPerPass + wave * S::kPerLoad + mine, step.key_end - 1 - step.key);
-    const int j = pages_in(a, n);
-    const int found = step.pages[j];
-    const int64_t in = n - j * a.block_size;
+    const int n = step.place + min(i * S::kPerPass + wave * S::kPerLoad + static_cast<int>(mine), step.key_end - 1 - step.key);
+    const int j = pages_in(a, n), found = step.pages[j];
+    const uint32_t in = n - j * a.block_size;
     const bool fine = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
-    const int64_t page = fine ? found : 0;
+    const uint64_t page = fine ? found : 0;
     s.bad = (s.bad & ~(1 << i)) | (fine ? 0 : 1 << i);
-    s.k[i] = load_piece<ONCE>(keys + (page * a.k_block + in * a.k_token), 16 * piece);
-    s.v[i] = load_piece<ONCE>(values + (page * a.v_block + in * a.v_token), 16 * piece);
+    s.k[i] = load_piece<ONCE>(a.k + page * a.k_block, in * a.k_token + step.head * a.k_head + piece);
+    s.v[i] = load_piece<ONCE>(a.v + page * a.v_block, in * a.v_token + step.head * a.v_head + piece);
   }
 }
 
-template <int D>
-__device__ __forceinline__ void store_keys(const PrefixArgs& a, char* stage, const Step& step, int thread, int wave,
-                                           int i, Staged<D>& s) {
+__device__ __forceinline__ bool not_finite2(uint32_t w, uint32_t exponent) {
+  return (w & exponent) == exponent || (w & (exponent << 16)) == (exponent << 16);
+}
+
+// Load i's keys to shared memory, zeros for those past the range or of a page out of it (`tail`: there may
+// be such).  Returns whether a value is not finite (CHECK).
+template <int DT, int D, bool CHECK>
+__device__ __forceinline__ bool store_keys(const PrefixArgs& a, char* stage, const Step& step, bool tail, int thread,
+                                           int wave, int i, Staged<D>& s) {
   using S = Shape<D>;
+  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
   const int lane = thread & 63, piece = lane % S::kLanes;
   const int t = i * S::kPerPass + wave * S::kPerLoad + lane / S::kLanes;
-  if (step.key + S::kTile > step.key_end || __any(s.bad != 0)) {
+  if (tail) {
     if (step.key + t >= step.key_end || (s.bad >> i) & 1) {
       s.k[i] = u32x4{0, 0, 0, 0};
       s.v[i] = u32x4{0, 0, 0, 0};
@@ -580,6 +595,9 @@ __device__ __forceinline__ void store_keys(const PrefixArgs& a, char* stage, con
   }
   *reinterpret_cast<u32x4*>(stage + t * S::kKeyBytes + 16 * piece) = s.k[i];
   reinterpret_cast<u32x4*>(stage + S::kValuesAt)[piece_at<D>(t, piece)] = s.v[i];
+  if constexpr (!CHECK) return false;
+  return not_finite2(s.v[i][0], kExponent) || not_finite2(s.v[i][1], kExponent) || not_finite2(s.v[i][2], kExponent) ||
+         not_finite2(s.v[i][3], kExponent);
 }
 
 // Where a lane reads in a staged tile, in bytes: a key's piece 0 for the score product (key lane % 32
@@ -602,11 +620,7 @@ __device__ __forceinline__ Lane lane_places() {
 
 typedef __attribute__((address_space(3))) char lds_char;
 __device__ __forceinline__ u32x2 read_values(uint32_t at) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_char*)at));
-}
-
-__device__ __forceinline__ bool not_finite2(uint32_t w, uint32_t exponent) {
-  return (w & exponent) == exponent || (w & (exponent << 16)) == (exponent << 16);
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_char*)(uintptr_t)at));
 }
 
 // A wave's softmax state for its 32 query rows (one per lane column): running maximum, the lane's
@@ -643,11 +657,11 @@ __device__ __forceinline__ void add_not_finite(const u32x4* values, State<D>& st
 }
 
 // 32 keys of a staged tile for one wave, from key t0 of the tile on.  `seen` (MASKED): how many of
-// them the lane column's query row sees.  Reads of a step are issued together, ahead of the products
+// them the lane column's query row sees, and `poison` that a value of the tile is not finite.  Reads of a step are issued together, ahead of the products
 // that take them: the keys' before the first product, the values' before the softmax.
 template <int DT, int D, bool MASKED>
 __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, const u32x4 (&q)[Shape<D>::kSteps],
-                                            State<D>& st, int t0, int seen, float scale_log2) {
+                                            State<D>& st, int t0, int seen, bool poison, float scale_log2) {
   using S = Shape<D>;
   constexpr int kBatch = S::kSteps < 8 ? S::kSteps : 8;
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -706,18 +720,6 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, c
     p[i >> 3][(i & 7) >> 1] = pack2<DT>(x, y);
   }
   constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
-  bool poison = false;
-  if constexpr (MASKED) {
-    bool bad = false;
-    const int thread = fresh_thread();
-#pragma unroll 1
-    for (int c = (thread >> 5) & 1; c < D / 8; c += 2) {
-      const u32x4 x = reinterpret_cast<const u32x4*>(stage + S::kValuesAt)[piece_at<D>(t0 + (thread & 31), c)];
-      bad |= not_finite2(x[0], kExponent) || not_finite2(x[1], kExponent) || not_finite2(x[2], kExponent) ||
-             not_finite2(x[3], kExponent);
-    }
-    poison = __any(bad);
-  }
   // The lane's own probabilities are the B operand: k-slot (half, e) of step s is key 16 s + 8 (e /
   // 4) + 4 half + e % 4 of the 32, and the values are read in that order.
   auto output = [&](int j, int s, u32x2 lo, u32x2 hi) {
@@ -878,28 +880,43 @@ struct Pipe {
 };
 
 template <int D, bool WHOLE>
-__device__ __forceinline__ void load_tile(const PrefixArgs& a, const Step& step, int thread, int wave, int i,
-                                          Staged<D>& s) {
+__device__ __forceinline__ void load_tile(const PrefixArgs& a, const Step& step, const Places& at, int thread, int wave,
+                                          int i, Staged<D>& s) {
   if (step.key >= step.key_end) return;
-  if (step.once) load_keys<D, WHOLE, true>(a, step, thread, wave, i, s);
-  else load_keys<D, WHOLE, false>(a, step, thread, wave, i, s);
+  if (step.once) load_keys<D, WHOLE, true>(a, step, at, thread, wave, i, s);
+  else load_keys<D, WHOLE, false>(a, step, at, thread, wave, i, s);
 }
 
 // The next tile's keys to shared memory; a register is loaded again as soon as its keys are there.
-template <int D, bool WHOLE>
+// CHECK: the tile has a mask; `poison` (a word per wave and stage) then says whether one of its values is
+// not finite.
+template <int DT, int D, bool WHOLE, bool CHECK>
 __device__ __forceinline__ const char* next_tile(const PrefixArgs& a, const Plan& p, const RowTables& t, Pipe<D>& pipe,
-                                                 int wave, char* lds) {
+                                                 int wave, char* lds, int* poison) {
   using S = Shape<D>;
   const int thread = fresh_thread();
   char* stage = lds + pipe.cur * S::kStage;
+  const bool tail = pipe.now.key + S::kTile > pipe.now.key_end || __any(pipe.s.bad != 0);
+  Staged<D>& s = pipe.s;
+  const int bad = s.bad;
+  Places at{};
+  if constexpr (WHOLE) at = load_places<D>(a, pipe.ahead, s);
+  const int bad_ahead = s.bad;
+  bool found = false;
 #pragma unroll
   for (int i = 0; i < S::kPasses; ++i) {
-    store_keys<D>(a, stage, pipe.now, thread, wave, i, pipe.s);
-    load_tile<D, WHOLE>(a, pipe.ahead, thread, wave, i, pipe.s);
+    if constexpr (WHOLE) s.bad = bad;
+    found |= store_keys<DT, D, CHECK>(a, stage, pipe.now, tail, thread, wave, i, s);
+    load_tile<D, WHOLE>(a, pipe.ahead, at, thread, wave, i, s);
+  }
+  if constexpr (WHOLE) s.bad = bad_ahead;
+  if constexpr (CHECK) {
+    const int any = __any(found);
+    if ((thread & 63) == 0) poison[pipe.cur * S::kWaves + wave] = any;
   }
   pipe.now = pipe.ahead;
   pipe.ahead = pipe.feed.next(a, p, t);
-  find_pages<D, WHOLE>(a, pipe.ahead, wave, pipe.s);
+  find_pages<D, WHOLE>(a, pipe.ahead, wave, s);
   pipe.cur ^= 1;
   lds_barrier();
   return stage;
@@ -908,7 +925,7 @@ __device__ __forceinline__ const char* next_tile(const PrefixArgs& a, const Plan
 // The share's tiles of a unit, from `place` on to `stop`.
 template <int DT, int D, bool WHOLE, bool WIDE>
 __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, const Unit& u, int place,
-                                         int stop, int group, int wave, Pipe<D>& pipe, char* lds) {
+                                         int stop, int group, int wave, Pipe<D>& pipe, char* lds, int* poison) {
   using S = Shape<D>;
   constexpr int kN = Split<D, WIDE>::kN;
   const int first = 32 * (wave % Split<D, WIDE>::kT) * kN;
@@ -924,21 +941,22 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
   st.l = 0.f;
   // Tiles that all query rows see whole, then the ones with a mask.
   for (; place < stop && pipe.now.key + S::kTile <= u.seen_by_all; ++place) {
-    const char* stage = next_tile<D, WHOLE>(a, p, t, pipe, wave, lds);
+    const char* stage = next_tile<DT, D, WHOLE, false>(a, p, t, pipe, wave, lds, poison);
     if (q.any) {
       const Lane at = lane_places<D>();
 #pragma unroll
-      for (int n = 0; n < kN; ++n) attend_keys<DT, D, false>(stage, at, q.q, st, first + 32 * n, 32, a.scale_log2);
+      for (int n = 0; n < kN; ++n) attend_keys<DT, D, false>(stage, at, q.q, st, first + 32 * n, 32, false, a.scale_log2);
     }
   }
   for (; place < stop; ++place) {
     const int seen = min(q.limit, u.key_end) - pipe.now.key, keys = u.key_end - pipe.now.key;
-    const char* stage = next_tile<D, WHOLE>(a, p, t, pipe, wave, lds);
+    const char* stage = next_tile<DT, D, WHOLE, true>(a, p, t, pipe, wave, lds, poison);
     if (q.any) {
       const Lane at = lane_places<D>();
+      const bool bad = __any(poison[(pipe.cur ^ 1) * S::kWaves + fresh_thread() % S::kWaves] != 0);
 #pragma unroll 1
       for (int t0 = first; t0 < min(first + 32 * kN, keys); t0 += 32) {
-        attend_keys<DT, D, true>(stage, at, q.q, st, t0, seen - t0, a.scale_log2);
+        attend_keys<DT, D, true>(stage, at, q.q, st, t0, seen - t0, bad, a.scale_log2);
       }
     }
   }
@@ -953,6 +971,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_a
   __shared__ __attribute__((aligned(512))) char lds[2 * S::kStage];
   __shared__ RowTables tables;
   __shared__ Plan p;  // read again at each unit
+  __shared__ int poison[2 * S::kWaves];
   {
     const Plan made = make_plan<D, S::kThreads>(a, tables, blockIdx.x == 0);
     if (threadIdx.x == 0) p = made;
@@ -978,8 +997,12 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_a
   pipe.s.page = pipe.s.in = pipe.s.bad = 0;
   pipe.now = pipe.feed.next(a, p, tables);
   find_pages<D, WHOLE>(a, pipe.now, wave, pipe.s);
+  {
+    Places at{};
+    if constexpr (WHOLE) at = load_places<D>(a, pipe.now, pipe.s);
 #pragma unroll
-  for (int i = 0; i < S::kPasses; ++i) load_tile<D, WHOLE>(a, pipe.now, threadIdx.x, wave, i, pipe.s);
+    for (int i = 0; i < S::kPasses; ++i) load_tile<D, WHOLE>(a, pipe.now, at, threadIdx.x, wave, i, pipe.s);
+  }
   pipe.ahead = pipe.feed.next(a, p, tables);
   find_pages<D, WHOLE>(a, pipe.ahead, wave, pipe.s);
   while (place < end) {
@@ -987,8 +1010,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_a
     place = max(place, u.first_tile);
     const int stop = min(end, u.first_tile + u.key_tiles);
     if (place >= stop) return;  // the share ends before the unit's first key tile
-    if (u.tile_rows == kWideRows) run_unit<DT, D, WHOLE, true>(a, p, tables, u, place, stop, group, wave, pipe, lds);
-    else run_unit<DT, D, WHOLE, false>(a, p, tables, u, place, stop, group, wave, pipe, lds);
+    if (u.tile_rows == kWideRows) run_unit<DT, D, WHOLE, true>(a, p, tables, u, place, stop, group, wave, pipe, lds, poison);
+    else run_unit<DT, D, WHOLE, false>(a, p, tables, u, place, stop, group, wave, pipe, lds, poison);
     place = stop;
   }
 }
@@ -1125,7 +1148,13 @@ int prefix_attention_impl(hipStream_t stream, const ds_prefix_attention_desc* d)
   const int64_t strides[] = {d->q_row_stride,   d->q_head_stride,  d->o_row_stride,   d->o_head_stride, d->k_block_stride,
                              d->k_token_stride, d->k_head_stride,  d->v_block_stride, d->v_token_stride, d->v_head_stride};
   for (int64_t s : strides) DS_REQUIRE(s >= 0 && s % 8 == 0, "row, page and head strides must be multiples of 8 elements");
-  DS_SUPPORTED(d->k_token_stride < (1 << 28) && d->v_token_stride < (1 << 28), "token strides of at most 2^28 elements");
+  // Places within a page are 32-bit byte counts.
+  const int64_t in_key = d->k_block_stride + d->block_size * d->k_token_stride + d->num_kv_heads * d->k_head_stride;
+  const int64_t in_value = d->v_block_stride + d->block_size * d->v_token_stride + d->num_kv_heads * d->v_head_stride;
+  DS_SUPPORTED(d->k_block_stride < (1 << 30) && d->v_block_stride < (1 << 30) && d->k_token_stride < (1 << 30) &&
+                   d->v_token_stride < (1 << 30) && d->k_head_stride < (1 << 30) && d->v_head_stride < (1 << 30) &&
+                   in_key < (1 << 30) && in_value < (1 << 30),
+               "pages of at most 2^30 elements");
   DS_REQUIRE(aligned(d->query) && aligned(d->output) && aligned(d->key_cache) && aligned(d->value_cache),
              "query, output and KV caches must be 16-byte aligned");
   const size_t need = workspace_bytes(d->rows, d->tokens, d->num_q_heads, d->num_kv_heads, d->head_dim);
@@ -1146,10 +1175,10 @@ int prefix_attention_impl(hipStream_t stream, const ds_prefix_attention_desc* d)
   a.o_row = d->o_row_stride, a.o_head = d->o_head_stride;
   a.lse = d->lse;
   a.l_row = d->lse_token_stride, a.l_head = d->lse_head_stride;
-  a.k = static_cast<const uint16_t*>(d->key_cache);
-  a.k_block = d->k_block_stride, a.k_token = d->k_token_stride, a.k_head = d->k_head_stride;
-  a.v = static_cast<const uint16_t*>(d->value_cache);
-  a.v_block = d->v_block_stride, a.v_token = d->v_token_stride, a.v_head = d->v_head_stride;
+  a.k = static_cast<const char*>(d->key_cache);
+  a.k_block = 2 * d->k_block_stride, a.k_token = 2 * d->k_token_stride, a.k_head = 2 * d->k_head_stride;
+  a.v = static_cast<const char*>(d->value_cache);
+  a.v_block = 2 * d->v_block_stride, a.v_token = 2 * d->v_token_stride, a.v_head = 2 * d->v_head_stride;
   a.table = d->block_table;
   a.bt_stride = d->bt_stride;
   a.capacity = static_cast<int>(capacity);
