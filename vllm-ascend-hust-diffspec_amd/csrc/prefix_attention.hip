@@ -44,7 +44,7 @@ constexpr float kLn2P = 0.69314718055994530942f;
 constexpr int kWideRows = 128, kNarrowRows = 64;  // query rows of a unit's tile
 // Places that a unit takes in the work beside its key tiles: what its queries' loads, its joins and its
 // piece cost, in tiles.
-constexpr int kUnitCost = 2;
+constexpr int kUnitCost = 3;
 constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range

@@ -54,38 +54,69 @@ struct QkArgs {
   int32_t* status;
 };
 
+// V neighbouring elements as they lie in memory, widened to fp32 and rounded back (to nearest even).
 template <int DT, int V>
-__device__ __forceinline__ void load_vec(const typename Elem<DT>::T* p, float (&x)[V]) {
+struct Raw {
+  typename Elem<DT>::T e[V];
+};
+template <int DT, int V>
+__device__ __forceinline__ Raw<DT, V> load_raw(const typename Elem<DT>::T* p) {
   typedef typename Elem<DT>::T T;
-  typedef T TV __attribute__((ext_vector_type(V)));
+  Raw<DT, V> r;
   if constexpr (V == 1) {
-    x[0] = Elem<DT>::load(*p);
+    r.e[0] = *p;
   } else {
-    const TV v = *reinterpret_cast<const TV*>(p);
+    constexpr int kWords = V * sizeof(T) / 4, kLoad = kWords < 4 ? kWords : 4;
+    typedef uint32_t U __attribute__((ext_vector_type(kLoad)));
+    uint32_t w[kWords];
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = Elem<DT>::load(v[i]);
+    for (int i = 0; i < kWords; i += kLoad) {
+      const U u = *reinterpret_cast<const U*>(reinterpret_cast<const uint32_t*>(p) + i);
+#pragma unroll
+      for (int k = 0; k < kLoad; ++k) w[i + k] = u[k];
+    }
+    __builtin_memcpy(r.e, w, sizeof(w));
   }
+  return r;
+}
+template <int DT, int V>
+__device__ __forceinline__ void store_raw(typename Elem<DT>::T* p, const Raw<DT, V>& r) {
+  typedef typename Elem<DT>::T T;
+  if constexpr (V == 1) {
+    *p = r.e[0];
+  } else {
+    constexpr int kWords = V * sizeof(T) / 4, kLoad = kWords < 4 ? kWords : 4;
+    typedef uint32_t U __attribute__((ext_vector_type(kLoad)));
+    uint32_t w[kWords];
+    __builtin_memcpy(w, r.e, sizeof(w));
+#pragma unroll
+    for (int i = 0; i < kWords; i += kLoad) {
+      U u;
+#pragma unroll
+      for (int k = 0; k < kLoad; ++k) u[k] = w[i + k];
+      *reinterpret_cast<U*>(reinterpret_cast<uint32_t*>(p) + i) = u;
+    }
+  }
+}
+template <int DT, int V>
+__device__ __forceinline__ void widen(const Raw<DT, V>& r, float (&x)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) x[i] = Elem<DT>::load(r.e[i]);
 }
 template <int DT, int V>
 __device__ __forceinline__ void store_vec(typename Elem<DT>::T* p, const float (&x)[V]) {
-  typedef typename Elem<DT>::T T;
-  typedef T TV __attribute__((ext_vector_type(V)));
-  if constexpr (V == 1) {
-    *p = Elem<DT>::store(x[0]);
-  } else {
-    TV v;
+  Raw<DT, V> r;
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = Elem<DT>::store(x[i]);
-    *reinterpret_cast<TV*>(p) = v;
+  for (int i = 0; i < V; ++i) {
+    if constexpr (DT == DS_BF16) r.e[i] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(x[i]));
+    else r.e[i] = Elem<DT>::store(x[i]);
   }
+  store_raw<DT, V>(p, r);
 }
 template <int DT, int V>
-__device__ __forceinline__ void load_any(const void* p, bool f32, int at, float (&x)[V]) {
-  if (f32) {
-    load_vec<DS_FP32, V>(static_cast<const float*>(p) + at, x);
-  } else {
-    load_vec<DT, V>(static_cast<const typename Elem<DT>::T*>(p) + at, x);
-  }
+__device__ __forceinline__ void load_any(const void* p, bool f32, int64_t at, float (&x)[V]) {
+  if (f32) widen<DS_FP32, V>(load_raw<DS_FP32, V>(static_cast<const float*>(p) + at), x);
+  else widen<DT, V>(load_raw<DT, V>(static_cast<const typename Elem<DT>::T*>(p) + at), x);
 }
 
 __device__ __forceinline__ int64_t index_at(const void* p, int is64, int t) {
@@ -98,33 +129,48 @@ struct Item {
   int a, b, pair;  // pair: first cosine, or -1
   bool on;
 };
-template <int V>
+template <int V, bool NEOX>
 __device__ __forceinline__ Item item_at(const QkArgs& g, int i) {
   Item it;
   const int turned = g.rot / (2 * V);
   it.on = i < g.d / (2 * V);
   it.pair = i < turned ? i * V : -1;
-  const bool apart = g.neox && i < turned;
+  const bool apart = NEOX && i < turned;
   it.a = apart ? i * V : 2 * i * V;
   it.b = apart ? g.rot / 2 + i * V : it.a + V;
   if (!it.on) it.a = it.b = 0;
   return it;
 }
 
-template <int DT, int V, int NI>
+template <int DT, int V, int NI, bool NEOX>
 __global__ __launch_bounds__(kThreadsQ) void qk_norm_rope_kernel(QkArgs g) {
   typedef typename Elem<DT>::T T;
   const int lane = threadIdx.x & 63;
-  const int wave = blockIdx.x * (kThreadsQ / 64) + (threadIdx.x >> 6);
+  const int wave = blockIdx.x * (kThreadsQ / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int token = wave / g.chunks, chunk = wave - token * g.chunks;
   if (token >= g.tokens) return;
-  const int64_t position = index_at(g.positions, g.positions64, token);
-  if (position < 0 || position >= g.cs_rows) {
-    if (chunk == 0 && lane == 0 && g.status) {
-      __hip_atomic_fetch_or(g.status, kStatusPosition, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int groups = 64 / g.lanes, group = lane / g.lanes, in_head = lane & (g.lanes - 1);
+  const int heads = g.hq + g.hkv + (g.value_cache ? g.hkv : 0);
+  Item it[NI];
+#pragma unroll
+  for (int n = 0; n < NI; ++n) it[n] = item_at<V, NEOX>(g, in_head + n * g.lanes);
+  // A head's elements as they lie in memory; the next pass's are on their way while one is worked on.
+  Raw<DT, V> ra[NI], rb[NI];
+  auto fetch = [&](int pass) {
+    const int head = (chunk * g.passes + pass) * groups + group;
+    if (pass >= g.passes || head >= heads) return;
+    const bool is_q = head < g.hq, is_v = head >= g.hq + g.hkv;
+    const T* x = static_cast<const T*>(is_q ? g.q.p : is_v ? g.v.p : g.k.p) + token * (is_q ? g.q.token : is_v ? g.v.token : g.k.token) +
+                 (is_q ? head * g.q.head : is_v ? (head - g.hq - g.hkv) * g.v.head : (head - g.hq) * g.k.head);
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+      if (!it[n].on) continue;
+      ra[n] = load_raw<DT, V>(x + it[n].a);
+      rb[n] = load_raw<DT, V>(x + it[n].b);
     }
-    return;
-  }
+  };
+  fetch(0);
+  const int64_t position = index_at(g.positions, g.positions64, token);
   int64_t key_at = -1, value_at = 0;
   if (g.slots) {
     const int64_t slot = index_at(g.slots, g.slots64, token);
@@ -133,67 +179,61 @@ __global__ __launch_bounds__(kThreadsQ) void qk_norm_rope_kernel(QkArgs g) {
         __hip_atomic_fetch_or(g.status, kStatusSlot, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     } else if (slot >= 0) {
-      const int64_t block = slot / g.block_size, in = slot - block * g.block_size;
+      const uint32_t block = static_cast<uint32_t>(slot) / static_cast<uint32_t>(g.block_size);
+      const uint32_t in = static_cast<uint32_t>(slot) - block * static_cast<uint32_t>(g.block_size);
       key_at = block * g.kc_block + in * g.kc_token;
       value_at = block * g.vc_block + in * g.vc_token;
     }
   }
-  const int groups = 64 / g.lanes, group = lane / g.lanes, in_head = lane & (g.lanes - 1);
-  Item it[NI];
+  if (position < 0 || position >= g.cs_rows) {
+    if (chunk == 0 && lane == 0 && g.status) {
+      __hip_atomic_fetch_or(g.status, kStatusPosition, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    return;
+  }
   float c[NI][V], s[NI][V];
 #pragma unroll
   for (int n = 0; n < NI; ++n) {
-    it[n] = item_at<V>(g, in_head + n * g.lanes);
 #pragma unroll
     for (int i = 0; i < V; ++i) c[n][i] = 1.f, s[n][i] = 0.f;
     if (it[n].on && it[n].pair >= 0) {
-      const int64_t row = position * g.cs_stride;
-      if (g.cos_sin_f32) {
-        load_vec<DS_FP32, V>(static_cast<const float*>(g.cos_sin) + row + it[n].pair, c[n]);
-        load_vec<DS_FP32, V>(static_cast<const float*>(g.cos_sin) + row + g.rot / 2 + it[n].pair, s[n]);
-      } else {
-        load_vec<DT, V>(static_cast<const T*>(g.cos_sin) + row + it[n].pair, c[n]);
-        load_vec<DT, V>(static_cast<const T*>(g.cos_sin) + row + g.rot / 2 + it[n].pair, s[n]);
-      }
+      load_any<DT, V>(g.cos_sin, g.cos_sin_f32, position * g.cs_stride + it[n].pair, c[n]);
+      load_any<DT, V>(g.cos_sin, g.cos_sin_f32, position * g.cs_stride + g.rot / 2 + it[n].pair, s[n]);
     }
   }
-  const int heads = g.hq + g.hkv + (g.value_cache ? g.hkv : 0);
+  const float inv_d = 1.f / static_cast<float>(g.d);
   for (int pass = 0; pass < g.passes; ++pass) {
     const int head = (chunk * g.passes + pass) * groups + group;
     const bool on = head < heads;
     const bool is_q = head < g.hq, is_v = head >= g.hq + g.hkv;
     const int h = is_q ? head : is_v ? head - g.hq - g.hkv : head - g.hq;
-    const Heads src = is_q ? g.q : is_v ? g.v : g.k;
-    const T* x = static_cast<const T*>(src.p) + token * src.token + h * src.head;
+    if (on && is_v && key_at >= 0) {
+      T* to = static_cast<T*>(g.value_cache) + value_at + h * g.vc_head;
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        if (!it[n].on) continue;
+        store_raw<DT, V>(to + it[n].a, ra[n]);
+        store_raw<DT, V>(to + it[n].b, rb[n]);
+      }
+    }
     float a[NI][V], b[NI][V], sum = 0.f;
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
 #pragma unroll
       for (int i = 0; i < V; ++i) a[n][i] = b[n][i] = 0.f;
       if (on && it[n].on) {
-        load_vec<DT, V>(x + it[n].a, a[n]);
-        load_vec<DT, V>(x + it[n].b, b[n]);
+        widen<DT, V>(ra[n], a[n]);
+        widen<DT, V>(rb[n], b[n]);
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) sum += a[n][i] * a[n][i] + b[n][i] * b[n][i];
     }
+    fetch(pass + 1);
     for (int off = g.lanes >> 1; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    if (!on) continue;
-    if (is_v) {
-      if (key_at >= 0) {
-        T* to = static_cast<T*>(g.value_cache) + value_at + h * g.vc_head;
-#pragma unroll
-        for (int n = 0; n < NI; ++n) {
-          if (it[n].on) {
-            store_vec<DT, V>(to + it[n].a, a[n]);
-            store_vec<DT, V>(to + it[n].b, b[n]);
-          }
-        }
-      }
-      continue;
-    }
-    const float scale = 1.f / sqrtf(sum / static_cast<float>(g.d) + g.eps);
+    if (!on || is_v) continue;
+    const float scale = 1.f / sqrtf(sum * inv_d + g.eps);
     const void* weight = is_q ? g.q_weight : g.k_weight;
+    const Heads dst = is_q ? g.q_out : g.k_out;
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
       if (!it[n].on) continue;
@@ -211,22 +251,19 @@ __global__ __launch_bounds__(kThreadsQ) void qk_norm_rope_kernel(QkArgs g) {
         store_vec<DT, V>(to + it[n].b, b[n]);
       }
       if (it[n].pair >= 0) {
-        float ra[V], rb[V];
+        float x[2 * V], y[2 * V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = a[n][i], x[V + i] = b[n][i];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          // Neighbouring pairs: the lane's 2 V elements in order are pair i's two in turn.
-          const float p = g.neox ? a[n][i] : (2 * i < V ? a[n][(2 * i) % V] : b[n][(2 * i) % V]);
-          const float q = g.neox ? b[n][i] : (2 * i + 1 < V ? a[n][(2 * i + 1) % V] : b[n][(2 * i + 1) % V]);
-          ra[i] = p * c[n][i] - q * s[n][i];
-          rb[i] = q * c[n][i] + p * s[n][i];
+          // Pair i: the i-th of both halves, or the 2 i-th element and its neighbour.
+          const int p = NEOX ? i : 2 * i, q = NEOX ? V + i : 2 * i + 1;
+          y[p] = x[p] * c[n][i] - x[q] * s[n][i];
+          y[q] = x[q] * c[n][i] + x[p] * s[n][i];
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          a[n][i] = g.neox ? ra[i] : (i % 2 ? rb[i / 2] : ra[i / 2]);
-          b[n][i] = g.neox ? rb[i] : ((V + i) % 2 ? rb[(V + i) / 2] : ra[(V + i) / 2]);
-        }
+        for (int i = 0; i < V; ++i) a[n][i] = y[i], b[n][i] = y[V + i];
       }
-      const Heads dst = is_q ? g.q_out : g.k_out;
       if (dst.p) {
         T* to = static_cast<T*>(dst.p) + token * dst.token + h * dst.head;
         store_vec<DT, V>(to + it[n].a, a[n]);
@@ -255,7 +292,8 @@ int launch(hipStream_t stream, QkArgs& g) {
   const int64_t total = static_cast<int64_t>(g.tokens) * g.chunks;
   const int64_t blocks = (total + kThreadsQ / 64 - 1) / (kThreadsQ / 64);
   DS_SUPPORTED(total < INT_MAX, "too many tokens and heads for one launch");
-  qk_norm_rope_kernel<DT, V, NI><<<static_cast<unsigned>(blocks), kThreadsQ, 0, stream>>>(g);
+  if (g.neox) qk_norm_rope_kernel<DT, V, NI, true><<<static_cast<unsigned>(blocks), kThreadsQ, 0, stream>>>(g);
+  else qk_norm_rope_kernel<DT, V, NI, false><<<static_cast<unsigned>(blocks), kThreadsQ, 0, stream>>>(g);
   return check_launch("ds_qk_norm_rope");
 }
 
@@ -278,6 +316,9 @@ bool covers(const QkArgs& g, int size, int v) {
 template <int DT>
 int launch_type(hipStream_t stream, QkArgs& g) {
   constexpr int kSize = DT == DS_FP32 ? 4 : 2;
+  if constexpr (kSize == 2) {
+    if (covers(g, kSize, 8)) return launch<DT, 8, 1>(stream, g);
+  }
   if (covers(g, kSize, 4)) return launch<DT, 4, 1>(stream, g);
   return launch<DT, 1, 2>(stream, g);
 }
@@ -300,6 +341,7 @@ int qk_impl(hipStream_t stream, const ds_qk_norm_rope_desc* d) {
   DS_REQUIRE(!paged || (d->key_cache && d->value_cache && d->slot_mapping && d->value),
              "the paged write needs key_cache, value_cache, slot_mapping and value together");
   DS_REQUIRE(!paged || (d->block_size > 0 && d->num_blocks > 0), "page sizes and counts must be positive");
+  DS_SUPPORTED(!paged || static_cast<int64_t>(d->num_blocks) * d->block_size <= INT_MAX, "at most 2^31 - 1 cache slots");
   DS_REQUIRE(d->query && d->key && d->q_weight && d->k_weight && d->positions && d->query_out &&
                  (d->cos_sin || d->rotary_dim == 0),
              "null tensor pointer");
