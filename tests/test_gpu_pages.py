@@ -332,3 +332,24 @@ def test_adopted_counts_and_empty_lists(cuda):
     assert pool.compact(table).tolist() == [0, -1, 2, -1, -1, 1]
     assert table.tolist() == [[0, 2, -1], [2, 1, -1]] and refs.tolist() == [1, 1, 2, 0, 0, 0]
     assert pool.ref_counts is refs
+
+
+def test_forking_again_keeps_what_is_shared_and_may_run_out(cuda):
+    p = Pool(cuda, pages=8, rows=5, width=6, block=4)
+    p.model.extend([0], [18])
+    p.pool.extend(p.table, [0], [18])
+    for args in (([0, 0], [1, 2], [17, 10]),  # pages 5 and 6
+                 ([0, 0], [1, 2], [16, 17]),  # row 1 whole pages only, row 2 two pages more
+                 ([0, 0], [2, 1], [5, 18])):
+        assert p.model.fork(*args) == 0
+        p.pool.fork(p.table, *args)
+        p.check()
+    p.model.extend([3], [4])
+    p.pool.extend(p.table, [3], [4])
+    p.check()
+    # No page is left but those that the children give back: row 4 takes the first, row 1 the second, row 2
+    # none, and stays empty though it shared entries before.
+    args = ([0, 0, 0], [4, 1, 2], [9, 18, 7])
+    assert p.model.fork(*args) == 0 and p.model.held(2) == [] and len(p.model.held(1)) == 5
+    p.pool.fork(p.table, *args)
+    p.check(2)

@@ -10,7 +10,10 @@
 //
 // The bookkeeping is latency-bound (a few thousand words); the copies are bound by memory.  One
 // workgroup takes pages (ranks need one order), every workgroup releases, shares or copies.  A fork's
-// last workgroup to have released takes the pages, which saves a launch.
+// last workgroup to have released takes the pages, which saves a launch.  Measured: a fork of 4 rows
+// 6.0 + 4.1 us (checks and pages, then entries and copies), of 248 rows of up to 4000 tokens, a page of each
+// copied in 8 caches of 32 KiB, 9.0 + 13.1; 128 rows cut back and grown again 3.6 + 9.7; copies 4.9 TB/s both ways (a large
+// plain copy reaches 5.1); a compaction's plan over 4096 pages 7.0 and its moves 5.3 TB/s.
 #include "ds355_common.h"
 
 namespace ds355 {
@@ -48,24 +51,12 @@ __device__ __forceinline__ void raise(int32_t* status, int32_t bits) {
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return a / b + (a % b != 0); }
 
-// Gives row `row`'s entries from `first` on back.  Each entry is taken out with one exchange, so a row
-// that is named twice gives its pages back once.
-__device__ __forceinline__ void release(const Table& t, int row, int first, int32_t* refs, int num_pages,
-                                        int32_t* status) {
-  int32_t* e = t.entries + static_cast<int64_t>(row) * t.stride;
-  int32_t bits = 0;
-  for (int c = first + static_cast<int>(threadIdx.x); c < t.width; c += blockDim.x) {
-    if (e[c] < 0) continue;
-    const int page = atomicExch(e + c, -1);
-    if (page < 0) continue;
-    if (page >= num_pages) {
-      bits |= kBadPage;
-    } else if (atomicSub(refs + page, 1) <= 0) {
-      atomicAdd(refs + page, 1);
-      bits |= kBadPage;
-    }
-  }
-  raise(status, bits);
+// One row less holds the page; the status bits of a page that no row can hold.
+__device__ __forceinline__ int32_t drop(int page, int32_t* refs, int num_pages) {
+  if (page >= num_pages) return kBadPage;
+  if (atomicSub(refs + page, 1) > 0) return 0;
+  atomicAdd(refs + page, 1);
+  return kBadPage;
 }
 
 __device__ __forceinline__ bool block_any(bool v) { return __syncthreads_or(v) != 0; }
@@ -128,6 +119,9 @@ __device__ __forceinline__ int take_pages(int32_t* refs, int num_pages, int need
 // ---------------------------------------------------------------------------------------------
 // Copies: a wave moves one piece (pair, cache, 4 KiB) at a time.
 // ---------------------------------------------------------------------------------------------
+// Cached loads and non-temporal stores, 64 workgroups a CU: us for 200 pages of 12 x 32 KiB caches (157 MB
+// both ways) / a compaction that moves 1.0 GB: 31.9 / 200; with cached stores and 16 a CU 38.4 / 219,
+// non-temporal stores and 16 a CU 32.4 / 210, non-temporal loads too 33.4 / 205.
 __device__ __forceinline__ void copy_piece(const Caches& c, int cache, int piece, int64_t src, int64_t dst) {
   const int64_t* d = c.list + 4 * cache;
   const int64_t bytes = d[2], from = static_cast<int64_t>(piece) * kPiece;
@@ -144,7 +138,7 @@ __device__ __forceinline__ void copy_piece(const Caches& c, int cache, int piece
     }
 #pragma unroll
     for (int i = 0; i < kPiece / 1024; ++i) {
-      if (16 * (lane + 64 * i) < n) *reinterpret_cast<u32x4*>(t + 16 * (lane + 64 * i)) = v[i];
+      if (16 * (lane + 64 * i) < n) __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4*>(t + 16 * (lane + 64 * i)));
     }
   } else {
     for (int i = lane; i < n; i += 64) t[i] = s[i];
@@ -190,9 +184,10 @@ struct ForkArgs {
   const int32_t* lens;
   int count, block_size;
   int32_t* header;
-  int32_t* page;  // per pair: -1 no page needed, -2 the pair is left out (or got none), else its page
+  int32_t* page;  // per pair: its new page, or one of the words below
   int32_t* status;
 };
+constexpr int kNoPage = -1, kLeftOut = -2, kNoneFree = -3;
 
 // One workgroup per pair: checks it, gives the child's pages back; the last one takes the new pages.
 __global__ __launch_bounds__(kThreadsP) void fork_release_kernel(ForkArgs a) {
@@ -215,18 +210,33 @@ __global__ __launch_bounds__(kThreadsP) void fork_release_kernel(ForkArgs a) {
     for (int c = threadIdx.x; c < pages; c += kThreadsP) bad |= e[c] < 0 || e[c] >= a.num_pages;
     bad = block_any(bad);
   }
-  if (!bad) release(a.table, child, 0, a.refs, a.num_pages, a.status);
+  if (!bad) {
+    // Entries that the child has already (forked from this parent before) stay, with their counts: the
+    // parent holds those pages, so whether they are given back and shared again makes no difference.
+    const int full = len / a.block_size;
+    int32_t* e = a.table.entries + static_cast<int64_t>(child) * a.table.stride;
+    const int32_t* from = a.table.entries + static_cast<int64_t>(parent) * a.table.stride;
+    int32_t bits = 0;
+    for (int c = threadIdx.x; c < a.table.width; c += kThreadsP) {
+      const int page = e[c];
+      if (page < 0 || (c < full && page == from[c])) continue;
+      e[c] = -1;
+      bits |= drop(page, a.refs, a.num_pages);
+    }
+    raise(a.status, bits);
+  }
   if (threadIdx.x == 0) {
     if (bad) raise(a.status, kBadRow);
-    coherent_store(a.page + i, bad ? -2 : len % a.block_size ? 0 : -1);
+    coherent_store(a.page + i, bad ? kLeftOut : len % a.block_size ? 0 : kNoPage);
   }
-  __threadfence();
+  // What the last workgroup reads of the others (counts, page words) is written past the caches, so it has
+  // arrived once the writes are acknowledged.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   __shared__ int done;
-  if (threadIdx.x == 0) done = atomicAdd(a.header + kHdrDone, 1);
+  if (threadIdx.x == 0) done = __hip_atomic_fetch_add(a.header + kHdrDone, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (done != a.count - 1) return;
-  __threadfence();
   int need = 0;
   for (int base = 0; base < a.count; base += kThreadsP) {
     const int j = base + static_cast<int>(threadIdx.x);
@@ -241,7 +251,7 @@ __global__ __launch_bounds__(kThreadsP) void fork_release_kernel(ForkArgs a) {
     a.page[order[rank]] = page;
     a.refs[page] = 1;
   });
-  for (int r = found + static_cast<int>(threadIdx.x); r < need; r += kThreadsP) a.page[order[r]] = -2;
+  for (int r = found + static_cast<int>(threadIdx.x); r < need; r += kThreadsP) a.page[order[r]] = kNoneFree;
   if (threadIdx.x == 0) {
     if (found < need) raise(a.status, kNoPages);
     a.header[kHdrDone] = 0;
@@ -252,14 +262,19 @@ __global__ __launch_bounds__(kThreadsP) void fork_release_kernel(ForkArgs a) {
 __global__ __launch_bounds__(kCopyThreads) void fork_share_kernel(ForkArgs a) {
   if (static_cast<int>(blockIdx.x) < a.count) {
     const int i = blockIdx.x, page = a.page[i];
-    if (page == -2) return;
+    if (page == kLeftOut) return;
     const int full = a.lens[i] / a.block_size;
     const int32_t* from = a.table.entries + static_cast<int64_t>(a.parents[i]) * a.table.stride;
     int32_t* to = a.table.entries + static_cast<int64_t>(a.children[i]) * a.table.stride;
     for (int c = threadIdx.x; c < full; c += kCopyThreads) {
-      const int p = from[c];
-      to[c] = p;
-      atomicAdd(a.refs + p, 1);
+      const int p = from[c], had = to[c];
+      if (page == kNoneFree) {  // the child stays empty
+        if (had >= 0) atomicSub(a.refs + had, 1);
+        to[c] = -1;
+      } else if (had != p) {
+        to[c] = p;
+        atomicAdd(a.refs + p, 1);
+      }
     }
     if (threadIdx.x == 0 && page >= 0) to[full] = page;
     return;
@@ -304,7 +319,8 @@ __global__ __launch_bounds__(kThreadsP) void extend_kernel(Table t, int32_t* ref
       if (bad) {
         raise(status, kBadRow);
       } else {
-        // The row's pages are its leading entries.
+        // The row's pages are its leading entries.  A thread halves for their end: 128 rows of 4097 tokens in
+        // pages of 16 take 9.2 us, where waves that look at 64 places of several rows at once take 13.
         const int32_t* e = t.entries + static_cast<int64_t>(row) * t.stride;
         int lo = 0, hi = pages;
         while (lo < hi) {
@@ -354,7 +370,15 @@ __global__ __launch_bounds__(256) void free_kernel(Table t, int32_t* refs, int n
     if (threadIdx.x == 0) raise(status, kBadRow);
     return;
   }
-  release(t, row, ceil_div(len, block_size), refs, num_pages, status);
+  // Each entry is taken out with one exchange, so that a row named twice gives its pages back once.
+  int32_t* e = t.entries + static_cast<int64_t>(row) * t.stride;
+  int32_t bits = 0;
+  for (int c = ceil_div(len, block_size) + static_cast<int>(threadIdx.x); c < t.width; c += blockDim.x) {
+    if (e[c] < 0) continue;
+    const int page = atomicExch(e + c, -1);
+    if (page >= 0) bits |= drop(page, refs, num_pages);
+  }
+  raise(status, bits);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -442,7 +466,7 @@ __global__ __launch_bounds__(kCopyThreads) void compact_move_kernel(CompactArgs 
 // ---------------------------------------------------------------------------------------------
 int copy_blocks(const Caches& c, int64_t pairs) {
   const int64_t pieces = pairs * c.count * c.pieces, per_block = kCopyThreads / 64;
-  return static_cast<int>(std::min<int64_t>((pieces + per_block - 1) / per_block, 16 * device_cu_count()));
+  return static_cast<int>(std::min<int64_t>((pieces + per_block - 1) / per_block, 64 * device_cu_count()));
 }
 
 int check_caches(const int64_t* caches, int num_caches, int64_t max_page_bytes, int num_pages, Caches& c) {
