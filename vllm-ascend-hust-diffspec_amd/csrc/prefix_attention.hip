@@ -51,9 +51,14 @@ constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
 template <int D>
 struct Shape {
-  static constexpr int kWaves = D <= 128 ? 8 : 4;
+  // A wave holds its queries and outputs in registers, which 256 dimensions do not fit: there two waves
+  // take half of the dimensions each of 32 query rows, and add up their parts of the scores through shared
+  // memory.  48 rows of two tokens, 32 heads on 8, over 4 k shared keys and 100 to 900 of their own: 102 us;
+  // with four waves of twice the registers, which spilled some between the tiles, 232.
+  static constexpr int kHalves = D <= 128 ? 1 : 2;
+  static constexpr int kWaves = 8;
   static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kTile = 16384 / D;             // keys per tile: 32 KiB of keys and of values
+  static constexpr int kTile = 16384 / D / kHalves;   // keys per tile: 32 KiB of keys and of values (16 of each at 256)
   static constexpr int kLanes = D / 8;                // 16-byte pieces of a key
   static constexpr int kPerPass = kThreads / kLanes;  // keys that one load of all threads covers
   static constexpr int kPerLoad = 64 / kLanes;        // keys that one load of a wave covers
@@ -63,8 +68,9 @@ struct Shape {
   static constexpr int kKeyBytes = 2 * D + 16;
   static constexpr int kValuesAt = kTile * kKeyBytes;
   static constexpr int kStage = kValuesAt + kTile * 2 * D;  // bytes of a staged tile
-  static constexpr int kSteps = D / 16;               // score MFMAs per 32 keys
-  static constexpr int kBlocks = D / 32;              // output blocks of 32 dimensions
+  static constexpr int kSteps = D / 16 / kHalves;     // score MFMAs of a wave per 32 keys
+  static constexpr int kBlocks = D / 32 / kHalves;    // its output blocks of 32 dimensions
+  static constexpr int kScores = kHalves == 1 ? 0 : 4096 * kWaves;  // bytes in which the halves' scores meet
 };
 
 struct PrefixArgs {
@@ -133,9 +139,13 @@ __device__ __forceinline__ Row row_of(const PrefixArgs& a, int b) {
   return r;
 }
 
-__device__ __forceinline__ int tile_rows(int rows) { return rows > kNarrowRows ? kWideRows : kNarrowRows; }
+template <int D>
+__device__ __forceinline__ int tile_rows(int rows) {
+  return rows > kNarrowRows || Shape<D>::kHalves == 2 ? kWideRows : kNarrowRows;
+}
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
-__device__ __forceinline__ int query_tiles(int rows) { return ceil_div(rows, tile_rows(rows)); }
+template <int D>
+__device__ __forceinline__ int query_tiles(int rows) { return ceil_div(rows, tile_rows<D>(rows)); }
 
 // The thread's index, opaque to the compiler: what a part of the loop derives from it is derived there
 // again, instead of being kept in registers that the loop needs (spilled ones would be loaded in order
@@ -229,7 +239,7 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
   p.seen_by_all = uniform(p.seen_by_all);
   p.query_tokens = uniform(cut);
   const int m = p.query_tokens * a.group;
-  p.prefix_tile = tile_rows(m);
+  p.prefix_tile = tile_rows<D>(m);
   p.row_tiles = ceil_div(m, p.prefix_tile);
   p.key_tiles = ceil_div(p.prefix, kTile);
   // Own units.
@@ -248,7 +258,7 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
     }
     int w = 0;
     if (row[i].len > 0 && fits && row[i].keys > p.prefix) {
-      w = query_tiles(row[i].len * a.group) * (kUnitCost + ceil_div(row[i].keys - p.prefix, kTile));
+      w = query_tiles<D>(row[i].len * a.group) * (kUnitCost + ceil_div(row[i].keys - p.prefix, kTile));
     }
     const int work = wave_inclusive_scan(w);
     own_work[i] = work - w;
@@ -328,14 +338,14 @@ __device__ __forceinline__ Unit own_unit(const PrefixArgs& a, const Plan& p, con
   Unit u;
   const int w = t.work[b + 1] - t.work[b];
   u.rows = (t.token[b + 1] - t.token[b]) * a.group;
-  const int n = query_tiles(u.rows);
+  const int n = query_tiles<D>(u.rows);
   // Indexes of a row's units start past those of the rows before: they have at most one tile each
   // more than whole tiles of kNarrowRows query rows.
   u.index = p.prefix_units + a.hkv * (b + t.token[b] * a.group / kNarrowRows) + h * n + tile;
   u.kv_head = h;
   u.row = b;
   u.tile = tile;
-  u.tile_rows = tile_rows(u.rows);
+  u.tile_rows = tile_rows<D>(u.rows);
   u.key_tiles = w / n - kUnitCost;
   u.first_tile = p.prefix_work + a.hkv * t.work[b] + h * w + tile * (w / n) + kUnitCost;
   u.key0 = p.prefix;
@@ -368,7 +378,7 @@ __device__ __forceinline__ Unit unit_at(const PrefixArgs& a, const Plan& plan, c
     }
     const int before = uniform(t.work[lo]), mine = uniform(t.work[lo + 1]) - before;
     const int in_row = rest - a.hkv * before, h = in_row / mine;
-    const int n = query_tiles((uniform(t.token[lo + 1]) - uniform(t.token[lo])) * a.group);
+    const int n = query_tiles<D>((uniform(t.token[lo + 1]) - uniform(t.token[lo])) * a.group);
     u = own_unit<D>(a, p, t, lo, h, (in_row - h * mine) / (mine / n));
   }
   u.index = uniform(u.index), u.kv_head = uniform(u.kv_head), u.row = uniform(u.row), u.tile = uniform(u.tile);
@@ -613,9 +623,10 @@ template <int D>
 __device__ __forceinline__ Lane lane_places() {
   using S = Shape<D>;
   static_assert(S::kValuesAt % 512 == 0 && S::kStage % 512 == 0, "block numbers are address bits of their own");
-  const int lane = fresh_thread() & 63, half = lane >> 5, l = lane & 15;
-  return Lane{(lane & 31) * S::kKeyBytes + 16 * half,
-              S::kValuesAt + 16 * piece_at<D>(4 * half + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) + 8 * (l & 1)};
+  const int thread = fresh_thread(), lane = thread & 63, half = lane >> 5, l = lane & 15;
+  const int dims = S::kHalves == 1 ? 0 : 256 * ((thread >> 6) & 1);  // bytes before the wave's dimensions
+  const int value = 16 * piece_at<D>(4 * half + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1)) + 8 * (l & 1);
+  return Lane{(lane & 31) * S::kKeyBytes + 16 * half + dims, S::kValuesAt + (value ^ dims)};
 }
 
 typedef __attribute__((address_space(3))) char lds_char;
@@ -638,14 +649,15 @@ struct State {
 template <int DT, int D>
 __device__ __forceinline__ void add_not_finite(const u32x4* values, State<D>& st, int t0, int seen) {
   constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
-  const int half = (fresh_thread() >> 5) & 1;
+  const int thread = fresh_thread(), half = (thread >> 5) & 1;
+  const int first = Shape<D>::kHalves == 1 ? 0 : 16 * ((thread >> 6) & 1);
 #pragma unroll 1
   for (int t = 0; t < 32; ++t) {
 #pragma unroll
     for (int j = 0; j < Shape<D>::kBlocks; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const u32x2 v = reinterpret_cast<const u32x2*>(values + piece_at<D>(t0 + t, 4 * j + i))[half];
+        const u32x2 v = reinterpret_cast<const u32x2*>(values + piece_at<D>(t0 + t, first + 4 * j + i))[half];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint16_t x = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
@@ -658,33 +670,44 @@ __device__ __forceinline__ void add_not_finite(const u32x4* values, State<D>& st
 
 // 32 keys of a staged tile for one wave, from key t0 of the tile on.  `seen` (MASKED): how many of
 // them the lane column's query row sees, and `poison` that a value of the tile is not finite.  Reads of a step are issued together, ahead of the products
-// that take them: the keys' before the first product, the values' before the softmax.
+// that take them: the keys' before the first product, the values' before the softmax.  All waves of
+// halves (kHalves) come here together, or to the same barrier.
 template <int DT, int D, bool MASKED>
 __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, const u32x4 (&q)[Shape<D>::kSteps],
-                                            State<D>& st, int t0, int seen, bool poison, float scale_log2) {
+                                            State<D>& st, int t0, int seen, bool poison, float scale_log2,
+                                            char* scores) {
   using S = Shape<D>;
-  constexpr int kBatch = S::kSteps < 8 ? S::kSteps : 8;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const char* keys = stage + at.key + t0 * S::kKeyBytes;
   f32x16 sc;
 #pragma unroll
   for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+  u32x4 k[S::kSteps];
 #pragma unroll
-  for (int s0 = 0; s0 < S::kSteps; s0 += kBatch) {
-    u32x4 k[kBatch];
+  for (int s = 0; s < S::kSteps; ++s) k[s] = *reinterpret_cast<const u32x4*>(keys + 32 * s);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int s = 0; s < kBatch; ++s) k[s] = *reinterpret_cast<const u32x4*>(keys + 32 * (s0 + s));
-    __builtin_amdgcn_sched_barrier(0);
+  for (int s = 0; s < S::kSteps; ++s) sc = mfma32<DT>(k[s], q[s], sc);
+  if constexpr (S::kHalves == 2) {  // the other half's part of the scores
+    const int thread = fresh_thread();
+    f32x4* mine = reinterpret_cast<f32x4*>(scores) + (thread >> 6) * 256 + (thread & 63);
+    const f32x4* other = reinterpret_cast<const f32x4*>(scores) + ((thread >> 6) ^ 1) * 256 + (thread & 63);
 #pragma unroll
-    for (int s = 0; s < kBatch; ++s) sc = mfma32<DT>(k[s], q[s0 + s], sc);
+    for (int i = 0; i < 4; ++i) mine[64 * i] = f32x4{sc[4 * i], sc[4 * i + 1], sc[4 * i + 2], sc[4 * i + 3]};
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 x = other[64 * i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[4 * i + e] += x[e];
+    }
   }
-  constexpr int kAhead = S::kBlocks <= 4 ? S::kBlocks : 4;  // blocks whose values are read before the softmax
-  u32x2 v[2][kAhead][2];
+  u32x2 v[2][S::kBlocks][2];
   const uint32_t values = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)stage)) + at.value;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
+    for (int j = 0; j < S::kBlocks; ++j) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) v[s][j][e] = read_values((values ^ (64 * j)) + (t0 + 16 * s + 8 * e) * 2 * D);
     }
@@ -738,17 +761,7 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, c
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) output(j, s, v[s][j][0], v[s][j][1]);
-  }
-  if constexpr (S::kBlocks > kAhead) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int j = kAhead; j < S::kBlocks; ++j) {
-        const uint32_t from = (values ^ (64 * j)) + (t0 + 16 * s) * 2 * D;
-        output(j, s, read_values(from), read_values(from + 8 * 2 * D));
-      }
-    }
+    for (int j = 0; j < S::kBlocks; ++j) output(j, s, v[s][j][0], v[s][j][1]);
   }
   if constexpr (MASKED) {
     if (poison) add_not_finite<DT, D>(reinterpret_cast<const u32x4*>(stage + S::kValuesAt), st, t0, seen);
@@ -767,7 +780,8 @@ __device__ __forceinline__ float* piece_sums(const PrefixArgs& a, int slot) {
 template <int D, bool WIDE>
 struct Split {
   static constexpr int kQ = WIDE ? 4 : 2;
-  static constexpr int kT = Shape<D>::kWaves / kQ;
+  static constexpr int kT = Shape<D>::kWaves / kQ / Shape<D>::kHalves;
+  static_assert(kT > 0 && Shape<D>::kTile % (32 * kT) == 0);
   static constexpr int kN = Shape<D>::kTile / 32 / kT;
 };
 
@@ -783,11 +797,12 @@ template <int D, bool WIDE>
 __device__ __forceinline__ void load_queries(const PrefixArgs& a, const RowTables& t, const Unit& u, int wave,
                                              Queries<D>& q) {
   using S = Shape<D>;
-  const int lane = fresh_thread() & 63, r0 = u.tile * u.tile_rows + 32 * (wave / Split<D, WIDE>::kT);
+  const int lane = fresh_thread() & 63, r0 = u.tile * u.tile_rows + 32 * (wave / S::kHalves / Split<D, WIDE>::kT);
   const QueryRow row = query_row(a, t, u, r0 + (lane & 31));
   q.any = r0 < u.rows;
   q.limit = row.limit;
-  const uint16_t* src = a.q + row.token * a.q_row + row.head * a.q_head + 8 * (lane >> 5);
+  const uint16_t* src = a.q + row.token * a.q_row + row.head * a.q_head + 8 * (lane >> 5) +
+                        (S::kHalves == 1 ? 0 : 128 * (wave & 1));
 #pragma unroll
   for (int s = 0; s < S::kSteps; ++s) {
     q.q[s] = u32x4{0, 0, 0, 0};
@@ -801,7 +816,8 @@ __device__ __forceinline__ void finish_unit(const PrefixArgs& a, const Unit& u, 
                                             char* lds) {
   using S = Shape<D>;
   constexpr int kT = Split<D, WIDE>::kT;
-  const int lane = fresh_thread() & 63, qb = wave / kT, tb = wave % kT;
+  const int lane = fresh_thread() & 63, qb = wave / S::kHalves / kT, tb = wave % kT;
+  const int dims = S::kHalves == 1 ? 0 : wave & 1;  // which half of them
   const int r0 = u.tile * u.tile_rows + 32 * qb;
   st.l += other_half(st.l);
   // The waves that share query rows join in shared memory, each for its part of the dimensions (in
@@ -860,11 +876,11 @@ __device__ __forceinline__ void finish_unit(const PrefixArgs& a, const Unit& u, 
   }
   if (r0 < u.rows && slot < a.slots) {
     float* sums = piece_sums<D>(a, slot);
-    if (lane < 32 && tb == 0) {
+    if (lane < 32 && tb == 0 && dims == 0) {
       sums[32 * qb + lane] = st.m;
       sums[kWideRows + 32 * qb + lane] = st.l;
     }
-    f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kWideRows) + (qb * kGroups + tb * kMine) * 64 + lane;
+    f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kWideRows) + ((qb * S::kHalves + dims) * kGroups + tb * kMine) * 64 + lane;
 #pragma unroll
     for (int k = 0; k < kMine; ++k) o[k * 64] = sum[k];
   }
@@ -925,7 +941,7 @@ __device__ __forceinline__ const char* next_tile(const PrefixArgs& a, const Plan
 // The share's tiles of a unit, from `place` on to `stop`.
 template <int DT, int D, bool WHOLE, bool WIDE>
 __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, const Unit& u, int place,
-                                         int stop, int group, int wave, Pipe<D>& pipe, char* lds, int* poison) {
+                                         int stop, int group, int wave, Pipe<D>& pipe, char* lds, char* scores, int* poison) {
   using S = Shape<D>;
   constexpr int kN = Split<D, WIDE>::kN;
   const int first = 32 * (wave % Split<D, WIDE>::kT) * kN;
@@ -945,7 +961,11 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
     if (q.any) {
       const Lane at = lane_places<D>();
 #pragma unroll
-      for (int n = 0; n < kN; ++n) attend_keys<DT, D, false>(stage, at, q.q, st, first + 32 * n, 32, false, a.scale_log2);
+      for (int n = 0; n < kN; ++n) {
+        attend_keys<DT, D, false>(stage, at, q.q, st, first + 32 * n, 32, false, a.scale_log2, scores);
+      }
+    } else if constexpr (S::kHalves == 2) {
+      lds_barrier();  // the one in attend_keys
     }
   }
   for (; place < stop; ++place) {
@@ -956,8 +976,10 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
       const bool bad = __any(poison[(pipe.cur ^ 1) * S::kWaves + fresh_thread() % S::kWaves] != 0);
 #pragma unroll 1
       for (int t0 = first; t0 < min(first + 32 * kN, keys); t0 += 32) {
-        attend_keys<DT, D, true>(stage, at, q.q, st, t0, seen - t0, bad, a.scale_log2);
+        attend_keys<DT, D, true>(stage, at, q.q, st, t0, seen - t0, bad, a.scale_log2, scores);
       }
+    } else if constexpr (S::kHalves == 2) {
+      if (keys > 0) lds_barrier();
     }
   }
   lds_barrier();
@@ -966,9 +988,10 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
 }
 
 template <int DT, int D, bool WHOLE>
-__global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_attention_kernel(PrefixArgs a) {
+__global__ __launch_bounds__(Shape<D>::kThreads, 2) void prefix_attention_kernel(PrefixArgs a) {
   using S = Shape<D>;
   __shared__ __attribute__((aligned(512))) char lds[2 * S::kStage];
+  __shared__ __attribute__((aligned(16))) char scores[S::kScores ? S::kScores : 16];
   __shared__ RowTables tables;
   __shared__ Plan p;  // read again at each unit
   __shared__ int poison[2 * S::kWaves];
@@ -1010,8 +1033,13 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_a
     place = max(place, u.first_tile);
     const int stop = min(end, u.first_tile + u.key_tiles);
     if (place >= stop) return;  // the share ends before the unit's first key tile
-    if (u.tile_rows == kWideRows) run_unit<DT, D, WHOLE, true>(a, p, tables, u, place, stop, group, wave, pipe, lds, poison);
-    else run_unit<DT, D, WHOLE, false>(a, p, tables, u, place, stop, group, wave, pipe, lds, poison);
+    if constexpr (S::kHalves == 2) {
+      run_unit<DT, D, WHOLE, true>(a, p, tables, u, place, stop, group, wave, pipe, lds, scores, poison);
+    } else if (u.tile_rows == kWideRows) {
+      run_unit<DT, D, WHOLE, true>(a, p, tables, u, place, stop, group, wave, pipe, lds, scores, poison);
+    } else {
+      run_unit<DT, D, WHOLE, false>(a, p, tables, u, place, stop, group, wave, pipe, lds, scores, poison);
+    }
     place = stop;
   }
 }
@@ -1021,7 +1049,6 @@ __global__ __launch_bounds__(Shape<D>::kThreads, D <= 128 ? 2 : 1) void prefix_a
 constexpr int kJoinWaves = 8;
 template <int DT, int D>
 __global__ __launch_bounds__(64 * kJoinWaves) void prefix_join_kernel(PrefixArgs a) {
-  using S = Shape<D>;
   __shared__ RowTables tables;
   __shared__ float joined[kJoinWaves][18][64];
   const Plan p = make_plan<D, 64 * kJoinWaves>(a, tables, false);
@@ -1042,7 +1069,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void prefix_join_kernel(PrefixArgs
     const float* sums = piece_sums<D>(a, slot);
     const float om = sums[row_in_tile], ol = sums[kWideRows + row_in_tile];
     const f32x4* o = reinterpret_cast<const f32x4*>(sums + 2 * kWideRows) +
-                     ((row_in_tile >> 5) * S::kBlocks + j) * 4 * 64 + (row_in_tile & 31) + (lane & 32);
+                     ((row_in_tile >> 5) * (D / 32) + j) * 4 * 64 + (row_in_tile & 31) + (lane & 32);
     f32x4 part[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) part[k] = o[k * 64];
@@ -1063,7 +1090,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void prefix_join_kernel(PrefixArgs
   }
   if (tables.work[b + 1] > tables.work[b]) {
     const int in_row = i * a.group + (valid ? r : rows - 1) % a.group;
-    const int n = tile_rows((tables.token[b + 1] - tables.token[b]) * a.group);
+    const int n = tile_rows<D>((tables.token[b + 1] - tables.token[b]) * a.group);
     const Unit u = own_unit<D>(a, p, tables, b, h, in_row / n);
     const int last = (u.first_tile + u.key_tiles - 1) / p.share;
     for (int group = u.first_tile / p.share + wave; group <= last; group += kJoinWaves) join(u.index + group, in_row % n);
@@ -1111,7 +1138,7 @@ int launch(hipStream_t stream, const PrefixArgs& a) {
   if (whole) prefix_attention_kernel<DT, D, true><<<a.groups, Shape<D>::kThreads, 0, stream>>>(a);
   else prefix_attention_kernel<DT, D, false><<<a.groups, Shape<D>::kThreads, 0, stream>>>(a);
   const int blocks = static_cast<int>((static_cast<int64_t>(a.tokens) * a.group + 31) / 32);
-  prefix_join_kernel<DT, D><<<dim3(blocks, Shape<D>::kBlocks, a.hkv), 64 * kJoinWaves, 0, stream>>>(a);
+  prefix_join_kernel<DT, D><<<dim3(blocks, D / 32, a.hkv), 64 * kJoinWaves, 0, stream>>>(a);
   return check_launch("ds_prefix_attention");
 }
 
