@@ -41,10 +41,6 @@ def new_prefix_workspace(batch_rows: int, tokens: int, num_q_heads: int, num_kv_
     return torch.empty(size, dtype=torch.uint8, device=device)
 
 
-def _layout(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
-
-
 def shared_prefix_attention(
     query: torch.Tensor,
     key_cache: torch.Tensor,
@@ -87,9 +83,9 @@ def shared_prefix_attention(
     """
     key = None
     if reuse is not None:
-        key = (_layout(query), _layout(key_cache), _layout(value_cache), _layout(output), _layout(lse),
-               _layout(block_table), _layout(query_start), _layout(query_len), _layout(target_len),
-               _layout(prefix_len), _layout(workspace), _layout(status), batch_size)
+        tensors = (query, key_cache, value_cache, output, lse, block_table, query_start, query_len, target_len,
+                   prefix_len, workspace, status)
+        key = (*[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors], batch_size)
         hit = reuse.get(key)
         if hit is not None:
             return _launch(hit[0], hit[1], query, key_cache, value_cache, output, lse, block_table, query_start,
@@ -155,6 +151,8 @@ def shared_prefix_attention(
 
 def _launch(desc, device, query, key_cache, value_cache, output, lse, block_table, query_start, query_len, target_len,
             prefix_len, scale, workspace, status):
+    # Addresses go into a copy: another thread may be launching from the kept descriptor.
+    desc = _lib.PrefixAttentionDesc.from_buffer_copy(desc)
     desc.query, desc.output, desc.lse = query.data_ptr(), output.data_ptr(), _lib.ptr(lse)
     desc.key_cache, desc.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
     desc.block_table, desc.query_start = block_table.data_ptr(), query_start.data_ptr()

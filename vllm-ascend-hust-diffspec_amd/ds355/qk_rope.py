@@ -30,10 +30,6 @@ def _heads(t: torch.Tensor, tokens: int, heads: int | None, head_dim: int | None
         raise ValueError(f"{name} must be contiguous in head_dim")
 
 
-def _layout(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
-
-
 def qk_norm_rope(
     query: torch.Tensor,
     key: torch.Tensor,
@@ -84,7 +80,8 @@ def qk_norm_rope(
                key_cache, value_cache, slot_mapping, status)
     layout = None
     if reuse is not None:
-        layout = (tuple(map(_layout, tensors)), eps, rotary_dim, is_neox_style)
+        layout = (*[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors], eps,
+                  rotary_dim, is_neox_style)
         hit = reuse.get(layout)
         if hit is not None:
             return _launch(hit[0], hit[1], tensors)
@@ -156,6 +153,8 @@ def qk_norm_rope(
 
 
 def _launch(desc, device, tensors):
+    # Addresses go into a copy: another thread may be launching from the kept descriptor.
+    desc = _lib.QkNormRopeDesc.from_buffer_copy(desc)
     (desc.query, desc.key, desc.q_weight, desc.k_weight, desc.positions, desc.cos_sin, desc.query_out, desc.key_out,
      desc.normed_key, desc.value, desc.key_cache, desc.value_cache, desc.slot_mapping, desc.status) = map(_lib.ptr,
                                                                                                          tensors)
