@@ -227,3 +227,17 @@ def test_from_a_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         check(other, args, 128, True)
+
+
+@pytest.mark.parametrize("neox,dtype", ((True, torch.bfloat16), (False, torch.float16)))
+def test_more_than_the_caches_hold(cuda, neox, dtype):
+    # Over 32 MiB of heads: they go past the caches.
+    case = build(47, tokens=3601, hq=36, hkv=2, d=128, rot=64, dtype=dtype)
+    args, _ = run(case, cuda, rot=64, neox=neox)
+    check(case, args, 64, neox)
+    # In place, and no pages.
+    args, _ = run(case, cuda, rot=64, neox=neox, out=False, keys=False, paged=False, normed=False)
+    _, qy, qs = expect(case["query"], case["q_weight"], case, 64, neox)
+    _, ky, ks = expect(case["key"], case["k_weight"], case, 64, neox)
+    assert_close(args["query"], qy, qs, 128)
+    assert_close(args["key"], ky, ks, 128)

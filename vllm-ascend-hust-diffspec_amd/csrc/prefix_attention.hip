@@ -42,9 +42,6 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 constexpr float kLog2eP = 1.44269504088896340736f;
 constexpr float kLn2P = 0.69314718055994530942f;
 constexpr int kWideRows = 128, kNarrowRows = 64;  // query rows of a unit's tile
-// Places that a unit takes in the work beside its key tiles: what its queries' loads, its joins and its
-// piece cost, in tiles.
-constexpr int kUnitCost = 3;
 constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
@@ -59,6 +56,11 @@ struct Shape {
   static constexpr int kWaves = 8;
   static constexpr int kThreads = 64 * kWaves;
   static constexpr int kTile = 16384 / D / kHalves;   // keys per tile: 32 KiB of keys and of values (16 of each at 256)
+  // Places that a unit takes in the work beside its key tiles: what its queries' loads, its joins and its
+  // piece cost, in tiles.  Measured in us: for 128 dimensions, 80 query tokens over 32 k shared keys 99 (1),
+  // 91 (2 to 4), 92 (6); for 64, 57 ragged rows over 5 k 85.5 (1), 75.8 (2), 74.8 (3), 81.5 (4), 87.1 (6);
+  // for 256, 80 tokens over 16 k 75 (2), 70 (3), 64 (5), 62 (8), and 48 rows over 4 k 104, 102, 100, 106.
+  static constexpr int kUnitCost = kHalves == 1 ? 3 : 5;
   static constexpr int kLanes = D / 8;                // 16-byte pieces of a key
   static constexpr int kPerPass = kThreads / kLanes;  // keys that one load of all threads covers
   static constexpr int kPerLoad = 64 / kLanes;        // keys that one load of a wave covers
@@ -258,7 +260,7 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
     }
     int w = 0;
     if (row[i].len > 0 && fits && row[i].keys > p.prefix) {
-      w = query_tiles<D>(row[i].len * a.group) * (kUnitCost + ceil_div(row[i].keys - p.prefix, kTile));
+      w = query_tiles<D>(row[i].len * a.group) * (Shape<D>::kUnitCost + ceil_div(row[i].keys - p.prefix, kTile));
     }
     const int work = wave_inclusive_scan(w);
     own_work[i] = work - w;
@@ -292,7 +294,7 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
   p.segment = max(1, ceil_div(a.hkv * p.row_tiles * p.key_tiles + a.hkv * work, a.groups));
   p.segments = ceil_div(p.key_tiles, p.segment);
   p.prefix_units = a.hkv * p.segments * p.row_tiles;
-  p.prefix_work = a.hkv * p.row_tiles * p.key_tiles + kUnitCost * p.prefix_units;
+  p.prefix_work = a.hkv * p.row_tiles * p.key_tiles + Shape<D>::kUnitCost * p.prefix_units;
   p.work = p.prefix_work + a.hkv * work;
   p.share = max(1, ceil_div(p.work, a.groups));
   return p;
@@ -325,7 +327,7 @@ __device__ __forceinline__ Unit prefix_unit(const PrefixArgs& a, const Plan& p, 
   u.tile = tile;
   u.rows = p.query_tokens * a.group;
   u.tile_rows = p.prefix_tile;
-  u.first_tile = before * a.hkv * p.row_tiles + (h * p.row_tiles + tile) * u.key_tiles + kUnitCost * (u.index + 1);
+  u.first_tile = before * a.hkv * p.row_tiles + (h * p.row_tiles + tile) * u.key_tiles + Shape<D>::kUnitCost * (u.index + 1);
   u.key0 = before * kTile;
   u.key_end = min(p.prefix, u.key0 + u.key_tiles * kTile);
   u.seen_by_all = min(p.seen_by_all, u.key_end);
@@ -346,8 +348,8 @@ __device__ __forceinline__ Unit own_unit(const PrefixArgs& a, const Plan& p, con
   u.row = b;
   u.tile = tile;
   u.tile_rows = tile_rows<D>(u.rows);
-  u.key_tiles = w / n - kUnitCost;
-  u.first_tile = p.prefix_work + a.hkv * t.work[b] + h * w + tile * (w / n) + kUnitCost;
+  u.key_tiles = w / n - Shape<D>::kUnitCost;
+  u.first_tile = p.prefix_work + a.hkv * t.work[b] + h * w + tile * (w / n) + Shape<D>::kUnitCost;
   u.key0 = p.prefix;
   // The tile's last query token sees most.
   u.key_end = t.seen[b] + (min((tile + 1) * u.tile_rows, u.rows) - 1) / a.group + 1;
@@ -365,8 +367,8 @@ __device__ __forceinline__ Unit unit_at(const PrefixArgs& a, const Plan& plan, c
   p.prefix_work = uniform(plan.prefix_work), p.prefix_units = uniform(plan.prefix_units);
   Unit u;
   if (w < p.prefix_work) {
-    const int per_segment = (p.segment + kUnitCost) * a.hkv * p.row_tiles;
-    const int segment = w / per_segment, len = min(p.segment, p.key_tiles - segment * p.segment) + kUnitCost;
+    const int per_segment = (p.segment + Shape<D>::kUnitCost) * a.hkv * p.row_tiles;
+    const int segment = w / per_segment, len = min(p.segment, p.key_tiles - segment * p.segment) + Shape<D>::kUnitCost;
     const int i = (w - segment * per_segment) / len;
     u = prefix_unit<D>(a, p, i / p.row_tiles, segment, i % p.row_tiles);
   } else {
