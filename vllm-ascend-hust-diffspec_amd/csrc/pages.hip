@@ -138,7 +138,8 @@ __device__ __forceinline__ void copy_piece(const Caches& c, int cache, int piece
     }
 #pragma unroll
     for (int i = 0; i < kPiece / 1024; ++i) {
-      if (16 * (lane + 64 * i) < n) __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4*>(t + 16 * (lane + 64 * i)));
+      u32x4* to = reinterpret_cast<u32x4*>(t + 16 * (lane + 64 * i));
+      if (16 * (lane + 64 * i) < n) __builtin_nontemporal_store(v[i], to);
     }
   } else {
     for (int i = lane; i < n; i += 64) t[i] = s[i];

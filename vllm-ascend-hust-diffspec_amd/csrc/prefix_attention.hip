@@ -18,8 +18,9 @@
 //
 // Work: a unit is (KV head, tile of query rows, key range); its key tiles are laid end to end with
 // all other units' and dealt to the workgroups in equal contiguous shares, whatever the rows'
-// lengths (a unit also counts a few places for what it costs beside its tiles).  Every workgroup derives the same layout from the lengths on the device, so a captured
-// launch follows changed lengths.  Prefix ranges are cut into segments of one share with the row
+// lengths (a unit also counts a few places for what it costs beside its tiles).  Every workgroup
+// derives the same layout from the lengths on the device, so a captured launch follows changed
+// lengths.  Prefix ranges are cut into segments of one share with the row
 // tiles inside a segment next to each other, and consecutive shares are given to one XCD, so the
 // row tiles that read the same keys do it at about the same time behind one L2.  A share that ends
 // inside a unit leaves its piece (m, l, O in fp32) in the workspace; prefix_join_kernel joins them.
@@ -46,6 +47,14 @@ constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
+// Keys per tile: 32 KiB of keys and of values, 16 of each for 256 dimensions.
+constexpr int tile_keys(int d) { return d <= 128 ? 16384 / d : 8192 / d; }
+// Places that a unit takes in the work beside its key tiles: what its queries' loads, its joins and its
+// piece cost, in tiles.  Measured in us: for 128 dimensions, 80 query tokens over 32 k shared keys 99 (1),
+// 91 (2 to 4), 92 (6); for 64, 57 ragged rows over 5 k 85.5 (1), 75.8 (2), 74.8 (3), 81.5 (4), 87.1 (6);
+// for 256, 80 tokens over 16 k 75 (2), 70 (3), 64 (5), 62 (8), and 48 rows over 4 k 104, 102, 100, 106.
+constexpr int unit_cost(int d) { return d <= 128 ? 3 : 5; }
+
 template <int D>
 struct Shape {
   // A wave holds its queries and outputs in registers, which 256 dimensions do not fit: there two waves
@@ -55,12 +64,8 @@ struct Shape {
   static constexpr int kHalves = D <= 128 ? 1 : 2;
   static constexpr int kWaves = 8;
   static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kTile = 16384 / D / kHalves;   // keys per tile: 32 KiB of keys and of values (16 of each at 256)
-  // Places that a unit takes in the work beside its key tiles: what its queries' loads, its joins and its
-  // piece cost, in tiles.  Measured in us: for 128 dimensions, 80 query tokens over 32 k shared keys 99 (1),
-  // 91 (2 to 4), 92 (6); for 64, 57 ragged rows over 5 k 85.5 (1), 75.8 (2), 74.8 (3), 81.5 (4), 87.1 (6);
-  // for 256, 80 tokens over 16 k 75 (2), 70 (3), 64 (5), 62 (8), and 48 rows over 4 k 104, 102, 100, 106.
-  static constexpr int kUnitCost = kHalves == 1 ? 3 : 5;
+  static constexpr int kTile = tile_keys(D);
+  static constexpr int kUnitCost = unit_cost(D);
   static constexpr int kLanes = D / 8;                // 16-byte pieces of a key
   static constexpr int kPerPass = kThreads / kLanes;  // keys that one load of all threads covers
   static constexpr int kPerLoad = 64 / kLanes;        // keys that one load of a wave covers
@@ -327,7 +332,8 @@ __device__ __forceinline__ Unit prefix_unit(const PrefixArgs& a, const Plan& p, 
   u.tile = tile;
   u.rows = p.query_tokens * a.group;
   u.tile_rows = p.prefix_tile;
-  u.first_tile = before * a.hkv * p.row_tiles + (h * p.row_tiles + tile) * u.key_tiles + Shape<D>::kUnitCost * (u.index + 1);
+  u.first_tile = before * a.hkv * p.row_tiles + (h * p.row_tiles + tile) * u.key_tiles +
+                 Shape<D>::kUnitCost * (u.index + 1);
   u.key0 = before * kTile;
   u.key_end = min(p.prefix, u.key0 + u.key_tiles * kTile);
   u.seen_by_all = min(p.seen_by_all, u.key_end);
@@ -533,7 +539,8 @@ __device__ __forceinline__ void find_pages(const PrefixArgs& a, const Step& step
   using S = Shape<D>;
   if (step.key >= step.key_end || !WHOLE) return;
   const int i = fresh_thread() % S::kPasses;
-  const int n = step.place + min(i * S::kPerPass + wave * S::kPerLoad, (step.key_end - 1 - step.key) & ~(S::kPerLoad - 1));
+  const int last = (step.key_end - 1 - step.key) & ~(S::kPerLoad - 1);
+  const int n = step.place + min(i * S::kPerPass + wave * S::kPerLoad, last);
   const int j = pages_in(a, n);
   s.in = n - j * a.block_size;
   s.page = step.pages[j];
@@ -552,8 +559,9 @@ __device__ __forceinline__ Places load_places(const PrefixArgs& a, const Step& s
                 static_cast<uint64_t>(page) * a.v_block + (in * a.v_token + step.head * a.v_head)};
 }
 __device__ __forceinline__ uint64_t place_of(uint64_t places, int i) {
-  return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(places), i))) |
-         static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(places >> 32), i))) << 32;
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(places), i);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(places >> 32), i);
+  return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
 template <bool ONCE>
@@ -572,7 +580,8 @@ __device__ __forceinline__ void load_keys(const PrefixArgs& a, const Step& step,
     s.k[i] = load_piece<ONCE>(a.k + place_of(at.k, i), mine * a.k_token + piece);
     s.v[i] = load_piece<ONCE>(a.v + place_of(at.v, i), mine * a.v_token + piece);
   } else {  // a page a lane
-    const int n = step.place + min(i * S::kPerPass + wave * S::kPerLoad + static_cast<int>(mine), step.key_end - 1 - step.key);
+    const int key = i * S::kPerPass + wave * S::kPerLoad + static_cast<int>(mine);
+    const int n = step.place + min(key, step.key_end - 1 - step.key);
     const int j = pages_in(a, n), found = step.pages[j];
     const uint32_t in = n - j * a.block_size;
     const bool fine = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
@@ -671,9 +680,10 @@ __device__ __forceinline__ void add_not_finite(const u32x4* values, State<D>& st
 }
 
 // 32 keys of a staged tile for one wave, from key t0 of the tile on.  `seen` (MASKED): how many of
-// them the lane column's query row sees, and `poison` that a value of the tile is not finite.  Reads of a step are issued together, ahead of the products
-// that take them: the keys' before the first product, the values' before the softmax.  All waves of
-// halves (kHalves) come here together, or to the same barrier.
+// them the lane column's query row sees, and `poison` that a value of the tile is not finite.  Reads
+// of a step are issued together, ahead of the products that take them: the keys' before the first
+// product, the values' before the softmax.  All waves of halves (kHalves) come here together, or to
+// the same barrier.
 template <int DT, int D, bool MASKED>
 __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, const u32x4 (&q)[Shape<D>::kSteps],
                                             State<D>& st, int t0, int seen, bool poison, float scale_log2,
@@ -795,20 +805,25 @@ struct Queries {
   bool any;
 };
 
-template <int D, bool WIDE>
-__device__ __forceinline__ void load_queries(const PrefixArgs& a, const RowTables& t, const Unit& u, int wave,
+// Rows past the unit's end take the tensor's first row, and their results are left out.  Nothing here
+// waits for the queries unless there is a sign to turn: they arrive while the first tile goes to shared
+// memory, behind the keys in flight.
+template <int D>
+__device__ __forceinline__ void load_queries(const PrefixArgs& a, const RowTables& t, const Unit& u, int block,
                                              Queries<D>& q) {
   using S = Shape<D>;
-  const int lane = fresh_thread() & 63, r0 = u.tile * u.tile_rows + 32 * (wave / S::kHalves / Split<D, WIDE>::kT);
+  const int thread = fresh_thread(), lane = thread & 63, r0 = u.tile * u.tile_rows + 32 * block;
   const QueryRow row = query_row(a, t, u, r0 + (lane & 31));
-  q.any = r0 < u.rows;
+  q.any = uniform(r0 < u.rows);
   q.limit = row.limit;
+  if (!q.any) return;
   const uint16_t* src = a.q + row.token * a.q_row + row.head * a.q_head + 8 * (lane >> 5) +
-                        (S::kHalves == 1 ? 0 : 128 * (wave & 1));
+                        (S::kHalves == 1 ? 0 : 2 * (thread & 64));
 #pragma unroll
-  for (int s = 0; s < S::kSteps; ++s) {
-    q.q[s] = u32x4{0, 0, 0, 0};
-    if (row.valid) q.q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s) ^ a.q_sign;
+  for (int s = 0; s < S::kSteps; ++s) q.q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
+  if (a.q_sign) {
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s) q.q[s] ^= a.q_sign;
   }
 }
 
@@ -882,7 +897,8 @@ __device__ __forceinline__ void finish_unit(const PrefixArgs& a, const Unit& u, 
       sums[32 * qb + lane] = st.m;
       sums[kWideRows + 32 * qb + lane] = st.l;
     }
-    f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kWideRows) + ((qb * S::kHalves + dims) * kGroups + tb * kMine) * 64 + lane;
+    f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kWideRows) +
+               ((qb * S::kHalves + dims) * kGroups + tb * kMine) * 64 + lane;
 #pragma unroll
     for (int k = 0; k < kMine; ++k) o[k * 64] = sum[k];
   }
@@ -940,15 +956,19 @@ __device__ __forceinline__ const char* next_tile(const PrefixArgs& a, const Plan
   return stage;
 }
 
-// The share's tiles of a unit, from `place` on to `stop`.
-template <int DT, int D, bool WHOLE, bool WIDE>
-__device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, const Unit& u, int place,
-                                         int stop, int group, int wave, Pipe<D>& pipe, char* lds, char* scores, int* poison) {
+// The share's tiles of a unit, from `place` on to `stop`.  Wide and narrow units share the loops: the keys
+// in flight stay in their registers from one unit to the next, whatever its kind.
+template <int DT, int D, bool WHOLE>
+__device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, const RowTables& t, const Unit& u,
+                                         int place, int stop, int group, int wave, Pipe<D>& pipe, char* lds,
+                                         char* scores, int* poison) {
   using S = Shape<D>;
-  constexpr int kN = Split<D, WIDE>::kN;
-  const int first = 32 * (wave % Split<D, WIDE>::kT) * kN;
+  using Wide = Split<D, true>;
+  using Narrow = Split<D, S::kHalves == 2>;
+  const bool wide = S::kHalves == 2 || u.tile_rows == kWideRows;
+  const int first = wide ? 32 * (wave % Wide::kT) * Wide::kN : 32 * (wave % Narrow::kT) * Narrow::kN;
   Queries<D> q;
-  load_queries<D, WIDE>(a, t, u, wave, q);
+  load_queries<D>(a, t, u, wave / S::kHalves / (wide ? Wide::kT : Narrow::kT), q);
   State<D> st;
 #pragma unroll
   for (int j = 0; j < S::kBlocks; ++j) {
@@ -963,7 +983,8 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
     if (q.any) {
       const Lane at = lane_places<D>();
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
+      for (int n = 0; n < Wide::kN; ++n) {
+        if (n >= Narrow::kN && !wide) break;
         attend_keys<DT, D, false>(stage, at, q.q, st, first + 32 * n, 32, false, a.scale_log2, scores);
       }
     } else if constexpr (S::kHalves == 2) {
@@ -976,8 +997,9 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
     if (q.any) {
       const Lane at = lane_places<D>();
       const bool bad = __any(poison[(pipe.cur ^ 1) * S::kWaves + fresh_thread() % S::kWaves] != 0);
+      const int end = min(first + 32 * (wide ? Wide::kN : Narrow::kN), keys);
 #pragma unroll 1
-      for (int t0 = first; t0 < min(first + 32 * kN, keys); t0 += 32) {
+      for (int t0 = first; t0 < end; t0 += 32) {
         attend_keys<DT, D, true>(stage, at, q.q, st, t0, seen - t0, bad, a.scale_log2, scores);
       }
     } else if constexpr (S::kHalves == 2) {
@@ -985,7 +1007,8 @@ __device__ __forceinline__ void run_unit(const PrefixArgs& a, const Plan& p, con
     }
   }
   lds_barrier();
-  finish_unit<D, WIDE>(a, u, u.index + group, st, wave, lds);
+  if (wide) finish_unit<D, true>(a, u, u.index + group, st, wave, lds);
+  else finish_unit<D, S::kHalves == 2>(a, u, u.index + group, st, wave, lds);
   lds_barrier();
 }
 
@@ -1035,13 +1058,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, 2) void prefix_attention_kernel
     place = max(place, u.first_tile);
     const int stop = min(end, u.first_tile + u.key_tiles);
     if (place >= stop) return;  // the share ends before the unit's first key tile
-    if constexpr (S::kHalves == 2) {
-      run_unit<DT, D, WHOLE, true>(a, p, tables, u, place, stop, group, wave, pipe, lds, scores, poison);
-    } else if (u.tile_rows == kWideRows) {
-      run_unit<DT, D, WHOLE, true>(a, p, tables, u, place, stop, group, wave, pipe, lds, scores, poison);
-    } else {
-      run_unit<DT, D, WHOLE, false>(a, p, tables, u, place, stop, group, wave, pipe, lds, scores, poison);
-    }
+    run_unit<DT, D, WHOLE>(a, p, tables, u, place, stop, group, wave, pipe, lds, scores, poison);
     place = stop;
   }
 }
@@ -1095,7 +1112,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void prefix_join_kernel(PrefixArgs
     const int n = tile_rows<D>((tables.token[b + 1] - tables.token[b]) * a.group);
     const Unit u = own_unit<D>(a, p, tables, b, h, in_row / n);
     const int last = (u.first_tile + u.key_tiles - 1) / p.share;
-    for (int group = u.first_tile / p.share + wave; group <= last; group += kJoinWaves) join(u.index + group, in_row % n);
+    for (int group = u.first_tile / p.share + wave; group <= last; group += kJoinWaves) {
+      join(u.index + group, in_row % n);
+    }
   }
   joined[wave][16][lane] = m;
   joined[wave][17][lane] = l;
@@ -1191,10 +1210,12 @@ int prefix_attention_impl(hipStream_t stream, const ds_prefix_attention_desc* d)
              "workspace must be 256-byte aligned and hold ds_prefix_attention_workspace_bytes()");
   const int group = d->num_q_heads / d->num_kv_heads;
   const int64_t capacity = std::min<int64_t>(static_cast<int64_t>(d->max_blocks) * d->block_size, 1 << 30);
-  const int tile = 16384 / d->head_dim;
+  const int tile = tile_keys(d->head_dim);
   const int64_t tiles = static_cast<int64_t>(d->tokens) * group / kNarrowRows + 1 + d->rows;
   DS_SUPPORTED(d->tokens <= (1 << 20), "at most 2^20 query tokens");
-  DS_SUPPORTED(d->num_kv_heads * tiles * ((capacity + tile - 1) / tile + 1) * 2 < INT_MAX &&
+  // The places of the work (own and prefix tiles, and their costs) are counted in 32 bits.
+  const int64_t places = (capacity + tile - 1) / tile + 2 * unit_cost(d->head_dim) + 2;
+  DS_SUPPORTED(d->num_kv_heads * tiles * places * 2 < INT_MAX &&
                    static_cast<int64_t>(d->tokens) * group < INT_MAX / 2 && d->num_kv_heads <= 65535,
                "too many query tokens, KV heads or keys for one launch");
   PrefixArgs a{};
