@@ -480,7 +480,6 @@ __device__ __forceinline__ int pages_in(const PrefixArgs& a, int n) {
 // places of the others follow by small distances.
 struct Step {
   int key, key_end, head;
-  bool once;             // no other workgroup reads the keys
   const int32_t* pages;  // the table entry of the first key's page
   int place;
 };
@@ -498,7 +497,6 @@ struct Feed {
     step.key = unit.key0 + (at - unit.first_tile) * Shape<D>::kTile;
     step.key_end = unit.key_end;
     step.head = unit.kv_head;
-    step.once = unit.row >= 0 || uniform(p.row_tiles) == 1;
     const int page = uniform(step.key / a.block_size);
     step.place = step.key - page * a.block_size;
     step.pages = a.table + static_cast<int64_t>(unit.row < 0 ? uniform(p.prefix_row) : unit.row) * a.bt_stride + page;
@@ -564,21 +562,20 @@ __device__ __forceinline__ uint64_t place_of(uint64_t places, int i) {
   return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-template <bool ONCE>
 __device__ __forceinline__ u32x4 load_piece(const char* base, uint32_t bytes) {
-  const u32x4* p = reinterpret_cast<const u32x4*>(base + bytes);
-  return ONCE ? __builtin_nontemporal_load(p) : *p;
+  return *reinterpret_cast<const u32x4*>(base + bytes);
 }
 
-template <int D, bool WHOLE, bool ONCE>
+template <int D, bool WHOLE>
 __device__ __forceinline__ void load_keys(const PrefixArgs& a, const Step& step, const Places& at, int thread, int wave,
                                           int i, Staged<D>& s) {
   using S = Shape<D>;
+  if (step.key >= step.key_end) return;
   const int lane = thread & 63;
   const uint32_t piece = 16 * (lane % S::kLanes), mine = lane / S::kLanes;
   if constexpr (WHOLE) {
-    s.k[i] = load_piece<ONCE>(a.k + place_of(at.k, i), mine * a.k_token + piece);
-    s.v[i] = load_piece<ONCE>(a.v + place_of(at.v, i), mine * a.v_token + piece);
+    s.k[i] = load_piece(a.k + place_of(at.k, i), mine * a.k_token + piece);
+    s.v[i] = load_piece(a.v + place_of(at.v, i), mine * a.v_token + piece);
   } else {  // a page a lane
     const int key = i * S::kPerPass + wave * S::kPerLoad + static_cast<int>(mine);
     const int n = step.place + min(key, step.key_end - 1 - step.key);
@@ -587,8 +584,8 @@ __device__ __forceinline__ void load_keys(const PrefixArgs& a, const Step& step,
     const bool fine = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
     const uint64_t page = fine ? found : 0;
     s.bad = (s.bad & ~(1 << i)) | (fine ? 0 : 1 << i);
-    s.k[i] = load_piece<ONCE>(a.k + page * a.k_block, in * a.k_token + step.head * a.k_head + piece);
-    s.v[i] = load_piece<ONCE>(a.v + page * a.v_block, in * a.v_token + step.head * a.v_head + piece);
+    s.k[i] = load_piece(a.k + page * a.k_block, in * a.k_token + step.head * a.k_head + piece);
+    s.v[i] = load_piece(a.v + page * a.v_block, in * a.v_token + step.head * a.v_head + piece);
   }
 }
 
@@ -913,14 +910,6 @@ struct Pipe {
   int cur;          // the half of shared memory the next tile goes to
 };
 
-template <int D, bool WHOLE>
-__device__ __forceinline__ void load_tile(const PrefixArgs& a, const Step& step, const Places& at, int thread, int wave,
-                                          int i, Staged<D>& s) {
-  if (step.key >= step.key_end) return;
-  if (step.once) load_keys<D, WHOLE, true>(a, step, at, thread, wave, i, s);
-  else load_keys<D, WHOLE, false>(a, step, at, thread, wave, i, s);
-}
-
 // The next tile's keys to shared memory; a register is loaded again as soon as its keys are there.
 // CHECK: the tile has a mask; `poison` (a word per wave and stage) then says whether one of its values is
 // not finite.
@@ -941,7 +930,7 @@ __device__ __forceinline__ const char* next_tile(const PrefixArgs& a, const Plan
   for (int i = 0; i < S::kPasses; ++i) {
     if constexpr (WHOLE) s.bad = bad;
     found |= store_keys<DT, D, CHECK>(a, stage, pipe.now, tail, thread, wave, i, s);
-    load_tile<D, WHOLE>(a, pipe.ahead, at, thread, wave, i, s);
+    load_keys<D, WHOLE>(a, pipe.ahead, at, thread, wave, i, s);
   }
   if constexpr (WHOLE) s.bad = bad_ahead;
   if constexpr (CHECK) {
@@ -1049,7 +1038,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, 2) void prefix_attention_kernel
     Places at{};
     if constexpr (WHOLE) at = load_places<D>(a, pipe.now, pipe.s);
 #pragma unroll
-    for (int i = 0; i < S::kPasses; ++i) load_tile<D, WHOLE>(a, pipe.now, at, threadIdx.x, wave, i, pipe.s);
+    for (int i = 0; i < S::kPasses; ++i) load_keys<D, WHOLE>(a, pipe.now, at, threadIdx.x, wave, i, pipe.s);
   }
   pipe.ahead = pipe.feed.next(a, p, tables);
   find_pages<D, WHOLE>(a, pipe.ahead, wave, pipe.s);
