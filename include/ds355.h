@@ -460,7 +460,8 @@ int ds_capture_raw_kv(ds_stream_t stream, int dtype,
  * last key, and keys a query token does not see, have no effect, infinities
  * and NaN included.
  * Output and LSE rows of tokens that belong to no row are left as they were.
- * Rows with query_len <= 0 (graph padding) have no token.  Rows must not share query tokens.
+ * Rows with query_len <= 0 (graph padding) have no token.  Rows must not
+ * share query tokens.
  * *status (optional, the caller clears it) gets bit 0 when a row's query
  * tokens are out of range or more than `tokens` in all (that row and, in the
  * second case, the rows after it are left out), bit 1 when a row is longer
@@ -469,8 +470,9 @@ int ds_capture_raw_kv(ds_stream_t stream, int dtype,
  *
  * query, output: [tokens, Hq, D], strides in the descriptor; key_cache,
  * value_cache: [num_blocks, block_size, Hkv, D].  head_dim 64, 128 or 256
- * contiguous; all other strides multiples of 8 elements, 16-byte aligned
- * pointers; at most 1024 rows.
+ * contiguous; all other strides non-negative multiples of 8 elements, 16-byte
+ * aligned pointers; at most 1024 rows, 2^20 query tokens, 2^20 tokens and 2^30
+ * elements per page.
  * workspace: caller's scratch of ds_prefix_attention_workspace_bytes(),
  * 256-byte aligned, with no state between calls (one launch at a time).
  * Two kernels, launch shape fixed by the sizes (graph-capturable).
@@ -530,9 +532,10 @@ size_t ds_prefix_attention_workspace_bytes(int rows, int tokens, int num_q_heads
  *
  * dtype: DS_BF16, DS_FP16 or DS_FP32 for all heads and caches; the weights
  * ([head_dim] each, contiguous) and the cos/sin cache in it or in DS_FP32.
- * head_dim even and at most 256, contiguous; strides in elements.  Heads,
- * strides and addresses in whole 4-element vectors move as vectors, others
- * element by element.  One launch.
+ * head_dim even and at most 256, contiguous; strides in elements; at most
+ * 2^31 - 1 cache slots.  Heads, strides and addresses in whole 8-element (two
+ * bytes each) or 4-element vectors move as vectors, others element by element.
+ * One launch.
  */
 typedef struct ds_qk_norm_rope_desc {
   int dtype, weight_dtype, cos_sin_dtype;

@@ -835,8 +835,9 @@ __device__ __forceinline__ void finish_unit(const PrefixArgs& a, const Unit& u, 
   const int r0 = u.tile * u.tile_rows + 32 * qb;
   st.l += other_half(st.l);
   // The waves that share query rows join in shared memory, each for its part of the dimensions (in
-  // groups of four accumulators, as they are stored).
-  constexpr int kGroups = 4 * S::kBlocks, kMine = kGroups / kT, kOther = kGroups - kMine;
+  // groups of four accumulators, as they are stored).  Every wave lays down all its groups, its own among
+  // them: which are its own is then a matter of addresses, not of selecting registers.
+  constexpr int kGroups = 4 * S::kBlocks, kMine = kGroups / kT;
   auto group = [&](int g) {
     return f32x4{st.acc[g >> 2][4 * (g & 3)], st.acc[g >> 2][4 * (g & 3) + 1], st.acc[g >> 2][4 * (g & 3) + 2],
                  st.acc[g >> 2][4 * (g & 3) + 3]};
@@ -846,43 +847,35 @@ __device__ __forceinline__ void finish_unit(const PrefixArgs& a, const Unit& u, 
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) sum[g] = group(g);
   } else {
-    // [wave][its groups for the other waves, in their order][lane], then each wave's m and l.
-    static_assert(S::kWaves * (4 * kOther + 2) * 64 * 4 <= 2 * S::kStage, "the waves' results fit the tiles");
+    // [wave][group][lane], then each wave's m and l.
+    static_assert(S::kWaves * (4 * kGroups + 2) * 64 * 4 <= 2 * S::kStage, "the waves' results fit the tiles");
     f32x4* area = reinterpret_cast<f32x4*>(lds);
-    float* sums = reinterpret_cast<float*>(area + S::kWaves * kOther * 64);
+    float* sums = reinterpret_cast<float*>(area + S::kWaves * kGroups * 64);
     lds_barrier();
     if (r0 < u.rows) {
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        const int w = g / kMine;
-        if (w != tb) area[(wave * kOther + (w < tb ? g : g - kMine)) * 64 + lane] = group(g);
-      }
+      for (int g = 0; g < kGroups; ++g) area[(wave * kGroups + g) * 64 + lane] = group(g);
       sums[2 * wave * 64 + lane] = st.m;
       sums[(2 * wave + 1) * 64 + lane] = st.l;
     }
     lds_barrier();
     if (r0 < u.rows) {
-      float m = st.m, l = 0.f, weight[kT];
-#pragma unroll
-      for (int w = 0; w < kT; ++w) m = fmaxf(m, sums[2 * (qb * kT + w) * 64 + lane]);
+      float m = -INFINITY, l = 0.f, weight[kT];
 #pragma unroll
       for (int w = 0; w < kT; ++w) {
-        const float om = sums[2 * (qb * kT + w) * 64 + lane], ol = sums[(2 * (qb * kT + w) + 1) * 64 + lane];
-        weight[w] = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - m);
-        l += ol * weight[w];
-      }
-      const float own = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        if (g / kMine == tb) sum[g % kMine] = group(g) * own;
+        weight[w] = sums[2 * (qb * kT + w) * 64 + lane];
+        m = fmaxf(m, weight[w]);
       }
 #pragma unroll
       for (int w = 0; w < kT; ++w) {
-        if (w == tb) continue;
+        weight[w] = weight[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(weight[w] - m);
+        l += sums[(2 * (qb * kT + w) + 1) * 64 + lane] * weight[w];
+      }
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {  // group tb kMine + k, in wave w's list without its own groups
-          sum[k] += area[((qb * kT + w) * kOther + (tb < w ? tb : tb - 1) * kMine + k) * 64 + lane] * weight[w];
-        }
+      for (int k = 0; k < kMine; ++k) {
+        sum[k] = area[(qb * kT * kGroups + tb * kMine + k) * 64 + lane] * weight[0];
+#pragma unroll
+        for (int w = 1; w < kT; ++w) sum[k] += area[((qb * kT + w) * kGroups + tb * kMine + k) * 64 + lane] * weight[w];
       }
       st.m = m;
       st.l = l;
