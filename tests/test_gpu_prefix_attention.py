@@ -149,6 +149,10 @@ SHAPES = [
     dict(prefix=640, own=[330, 50], qlens=[300, 40], hq=8, hkv=2, d=128, block=64),  # a prompt chunk
     dict(prefix=384, own=[130, 50, 129, 3], qlens=[128, 40, 65, 3], hq=4, hkv=4, d=256, block=64),
     dict(prefix=2048, own=[i + 1 for i in range(40)], qlens=[1] * 40, hq=8, hkv=1, d=64, block=16),
+    # Several tiles of query rows per row in 256 dimensions, most of which see none of the row's last keys;
+    # the last tile has waves without rows.
+    dict(prefix=96, own=[310, 40], qlens=[300, 33], hq=8, hkv=2, d=256, block=17),
+    dict(prefix=0, own=[150, 2], qlens=[150, 1], hq=8, hkv=1, d=256, block=32),
 ]
 
 

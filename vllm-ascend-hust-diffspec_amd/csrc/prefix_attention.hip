@@ -24,6 +24,12 @@
 // tiles inside a segment next to each other, and consecutive shares are given to one XCD, so the
 // row tiles that read the same keys do it at about the same time behind one L2.  A share that ends
 // inside a unit leaves its piece (m, l, O in fp32) in the workspace; prefix_join_kernel joins them.
+//
+// Measured (32 query heads on 4, 128 dimensions, bf16; this kernel + the join, back to back): 16 rows of 5
+// tokens over 32 k shared keys and up to 4 k of their own 89 us (46 GFLOP: 516 TFLOP/s; a large library product
+// reaches 1157), bound by staging and reading the tiles in shared memory, the matrix units busy for a
+// quarter of the time; one token each over 16 k 39 us (2.3 TB/s; a large copy reaches 5.1), bound by
+// loads' latency and the units' ends; two rows over 1 k 16 us, two launches' latency.
 #include <cmath>
 
 #include "ds355_common.h"
@@ -748,7 +754,9 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, c
   for (int i = 0; i < 16; i += 2) {
     const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], scale_log2, -m));
     const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i + 1], scale_log2, -m));
-    st.l += x + y;  // as computed, not as rounded for the product: the LSE is fp32
+    // The product's operands are 16 bits, so the probabilities are rounded for it; the sum is of them as
+    // computed, since the LSE is an fp32 output.
+    st.l += x + y;
     p[i >> 3][(i & 7) >> 1] = pack2<DT>(x, y);
   }
   constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;

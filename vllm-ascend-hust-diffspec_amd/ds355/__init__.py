@@ -9,6 +9,12 @@ Drop-in replacements for the reference plugin's hot path:
 - ``ds355.step.retrieval_step``                    (one launch chain for a whole step)
 - ``ds355.runtime.DiffSpecDraftCache``             (host orchestration, runtime.py:596-1765)
 
+The verifier's side of a step, for targets served through this library:
+
+- ``ds355.prefix_attention.shared_prefix_attention``  (paged attention and LSE, a shared prefix read once)
+- ``ds355.qk_rope.qk_norm_rope``                      (head norm, rotation and paged write in one pass)
+- ``ds355.pages.PagePool``                            (fork, extend, free, copy and compact pages)
+
 All device work runs in the HIP library ``libds355.so`` (C ABI in
 ``include/ds355.h``); there is no CPU fallback.
 """
