@@ -1031,6 +1031,7 @@ __global__ __launch_bounds__(Shape<D>::kThreads, 2) void prefix_attention_kernel
   int place = pipe.feed.at;
   const int end = pipe.feed.end;
   if (place >= end) return;  // the share ends before its unit's first key tile
+  Unit u = pipe.feed.unit;
   pipe.cur = 0;
   pipe.s.page = pipe.s.in = pipe.s.bad = 0;
   pipe.now = pipe.feed.next(a, p, tables);
@@ -1043,13 +1044,14 @@ __global__ __launch_bounds__(Shape<D>::kThreads, 2) void prefix_attention_kernel
   }
   pipe.ahead = pipe.feed.next(a, p, tables);
   find_pages<D, WHOLE>(a, pipe.ahead, wave, pipe.s);
-  while (place < end) {
-    const Unit u = unit_at<D>(a, p, tables, place);
+  for (;;) {
     place = max(place, u.first_tile);
     const int stop = min(end, u.first_tile + u.key_tiles);
     if (place >= stop) return;  // the share ends before the unit's first key tile
     run_unit<DT, D, WHOLE>(a, p, tables, u, place, stop, group, wave, pipe, lds, scores, poison);
     place = stop;
+    if (place >= end) return;
+    u = unit_at<D>(a, p, tables, place);
   }
 }
 
