@@ -29,7 +29,7 @@
 // tokens over 32 k shared keys and up to 4 k of their own 89 us (46 GFLOP: 516 TFLOP/s; a large library product
 // reaches 1157), bound by staging and reading the tiles in shared memory, the matrix units busy for a
 // quarter of the time; one token each over 16 k 39 us (2.3 TB/s; a large copy reaches 5.1), bound by
-// loads' latency and the units' ends; two rows over 1 k 16 us, two launches' latency.
+// loads' latency and the units' ends; two rows over 1 k 15 us, two launches' latency.
 #include <cmath>
 
 #include "ds355_common.h"
