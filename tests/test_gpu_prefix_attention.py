@@ -419,3 +419,49 @@ def test_lse_feeds_the_chunk_scores(cuda):
     own = kernels.paged_chunk_attention_scores(args["query"][rows], args["key_cache"], None, args["block_table"], lens,
                                                **kw)
     assert ((got - own).abs() <= 1e-4 * own.abs() + 1e-12).all()
+
+
+@pytest.mark.parametrize("rows,d", ((1024, 64), (700, 128), (513, 256), (65, 128)))
+def test_many_rows(cuda, rows, d):
+    # Rows in several waves and rounds of the layout: some are padding, some without keys, lengths differ.
+    own = [None if b % 97 == 5 else (b * 37) % 41 + (b % 4) for b in range(rows)]
+    qlens = [0 if b % 11 == 3 else 1 + (b % 29 == 0) * 3 for b in range(rows)]
+    case = build(60, prefix=48, own=own, qlens=qlens, hq=4, hkv=2, d=d, block=16, dtype=torch.bfloat16)
+    args = device_args(case, cuda)
+    run(args)
+    check(case, args)
+
+
+def test_many_rows_that_overlap_are_cut_off(cuda):
+    # As many query tokens as the tensor holds belong to the first rows; the rows after them, of which the
+    # first begins in the last round, are left out.
+    rows, kept = 900, 800
+    case = build(61, prefix=32, own=[b % 23 + 4 for b in range(rows)], qlens=[1] * rows, hq=2, hkv=1, d=128, block=16,
+                 dtype=torch.bfloat16, diverge=False)
+    expected = expect(case)
+    args = device_args(case, cuda)
+    case["tokens"] = kept
+    for name in ("query", "output", "lse"):
+        args[name] = args[name][:kept].contiguous()
+    args["query_start"] = (args["query_start"] - 1) % kept  # row b has token b, those past the end token b - kept
+    args["query"][: kept] = case["query"][1: kept + 1].to(cuda)
+    run(args)
+    out, lse, terms, err, top = (x[1: kept + 1] for x in expected)
+    case.update(query=case["query"][1: kept + 1], starts=list(range(kept)), qlens=[1] * kept, lens=case["lens"][:kept])
+    check(case, args, (out, lse, terms, err, top), status=1)
+
+
+def test_a_long_tail_of_small_probabilities(cuda):
+    # One key outweighs each of the others by e^14, near the smallest normal fp16, and has a value of 0: the
+    # output is the others' sum, which would be percents off were they rounded at fp16's smallest step.
+    n, d, block = 20000, 64, 16
+    keys, values = torch.zeros(n, 1, d, dtype=torch.float16), torch.ones(n, 1, d, dtype=torch.float16)
+    keys[0, 0, 0], values[0] = 1.75, 0
+    query = torch.zeros(1, 1, d, dtype=torch.float16)
+    query[0, 0, 0] = 8
+    cache = [x.view(n // block, block, 1, d) for x in (keys, values)]
+    case = dict(query=query, dense=[[keys, values]], starts=[0], qlens=[1], lens=[n], prefix=0, scale=1.0, hq=1, hkv=1, d=d,
+                tokens=1, cache=cache, table=torch.arange(n // block, dtype=torch.int32)[None])
+    args = device_args(case, cuda)
+    run(args)
+    check(case, args)

@@ -242,3 +242,40 @@ def test_decode_steps_from_one_graph(cuda):
         case = dict(query=query.cpu(), dense=s.dense[0], starts=[0, 1, 2], qlens=[1, 1, 1], lens=[prompt + step + 1] * 3,
                     prefix=prompt, scale=d ** -0.5, hq=hq, hkv=hkv, d=d, tokens=3)
         attention.check(case, dict(output=out, lse=lse, status=s.status))
+
+
+def test_places_past_32_bits(cuda):
+    """Pages a GiB apart: the last one begins past 4 GiB, in elements of a view and in bytes of a copy."""
+    from ds355 import qk_rope
+    from ds355.pages import PagePool
+
+    pages, block, hq, hkv, d, dtype, far = 5, 16, 8, 2, 128, torch.bfloat16, (1 << 29) + 64
+    caches = []
+    for _ in range(2):
+        cache = torch.empty((pages - 1) * far + block * hkv * d, dtype=dtype, device=cuda).as_strided(
+            (pages, block, hkv, d), (far, hkv * d, d, 1))
+        cache.zero_()
+        caches.append(cache)
+    pool = PagePool(caches)
+    g = gen(70)
+    qkv = (randn((block, (hq + 2 * hkv) * d), dtype, g) * 3).to(cuda)
+    part = lambda a, b: qkv[:, a * d: b * d].unflatten(1, (b - a, d))  # noqa: E731
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    phase = torch.arange(block)[:, None] * torch.arange(1, d // 2 + 1)[None] / 37
+    query, keys = torch.empty(block, hq, d, dtype=dtype, device=cuda), torch.empty(block, hkv, d, dtype=dtype, device=cuda)
+    weight = randn((d,), dtype, g).to(cuda)
+    qk_rope.qk_norm_rope(part(0, hq), part(hq, hq + hkv), weight, weight, i32(list(range(block))),
+                         torch.cat((phase.cos(), phase.sin()), -1).to(cuda), eps=1e-6, rotary_dim=d, is_neox_style=True,
+                         query_out=query, key_out=keys, value=part(hq + hkv, hq + 2 * hkv), key_cache=caches[0],
+                         value_cache=caches[1], slot_mapping=i32([4 * block + t for t in range(block)]))
+    values = part(hq + hkv, hq + 2 * hkv)
+    assert torch.equal(caches[0][4], keys) and torch.equal(caches[1][4], values)
+    assert all(int(c[:4].count_nonzero()) == 0 for c in caches)
+    pool.copy([4], [1])
+    assert torch.equal(caches[0][1], keys) and torch.equal(caches[1][1], values)
+    kv = [keys.cpu(), values.cpu()]
+    case = dict(query=query.cpu(), dense=[kv, kv], starts=[0, 8], qlens=[8, 8], lens=[16, 16], prefix=0, scale=d ** -0.5,
+                hq=hq, hkv=hkv, d=d, tokens=block, cache=[c[:1] for c in caches], table=torch.tensor([[4], [1]], dtype=torch.int32))
+    args = attention.device_args(case, cuda, key_cache=caches[0], value_cache=caches[1])
+    attention.run(args)
+    attention.check(case, args)

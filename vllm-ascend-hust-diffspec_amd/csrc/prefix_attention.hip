@@ -734,9 +734,12 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, c
     if constexpr (MASKED) sc[i] = 8 * (i >> 2) + (i & 3) < seen - 4 * half ? sc[i] : -INFINITY;
     top = fmaxf(top, sc[i]);
   }
-  top = fmaxf(top, other_half(top)) * scale_log2;
   // The reference of the exponents follows the maximum only when it is 2^8 behind: weights of up to 2^8
-  // keep their relative precision, and most tiles leave the sums as they are.
+  // keep their relative precision, and most tiles leave the sums as they are.  In fp16 it stays 2^7 below
+  // the maximum, so that weights lie in 2^-24 .. 2^15 of the type: those of a long tail of small
+  // probabilities are then rounded relative to themselves down to 2^-21 of the largest.
+  constexpr float kBelow = DT == DS_FP16 ? 7.f : 0.f;
+  top = __builtin_fmaf(fmaxf(top, other_half(top)), scale_log2, -kBelow);
   if (__any(top > st.m + 8.f)) {
     const float m = fmaxf(st.m, top);
     const float keep = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
