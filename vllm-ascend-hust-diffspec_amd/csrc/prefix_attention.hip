@@ -1060,6 +1060,8 @@ __global__ __launch_bounds__(Shape<D>::kThreads, 2) void prefix_attention_kernel
 
 // Joins the pieces of 32 query rows of one KV head (the batch's order) for 32 dimensions: eight waves
 // take the pieces in turn, and the first four join the waves' sums, four dimensions of a lane each.
+// Latency-bound.  Both kernels in us for two rows over 1 k keys, 16 over 16 k, 80 query tokens over 32 k and 57
+// ragged rows over 5 k: 15.2, 38.8, 86.5, 71.3; with four waves 16.0, 41.1, 86.1, 70.1, with 16 16.0, 38.7, 90.8, 79.4.
 constexpr int kJoinWaves = 8;
 template <int DT, int D>
 __global__ __launch_bounds__(64 * kJoinWaves) void prefix_join_kernel(PrefixArgs a) {
