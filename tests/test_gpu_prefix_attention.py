@@ -465,3 +465,34 @@ def test_a_long_tail_of_small_probabilities(cuda):
     args = device_args(case, cuda)
     run(args)
     check(case, args)
+
+
+def test_a_share_longer_than_the_prefix(cuda):
+    # A prompt batch of 1024 rows of 1024 tokens: 65536 tiles of query rows, whose own keys make a share of
+    # 65536 key tiles, while the shared prefix is one.  (65536 + 3) 65536 places do not fit 32 bits.
+    from ds355 import prefix_attention as pa
+
+    rows, q, hq, d, block, prefix, own, pages = 1024, 1024, 8, 64, 16, 256, 64512, 64
+    g = gen(62)
+    cache = [randn((pages, block, 1, d), torch.bfloat16, g) for _ in range(2)]
+    width = (prefix + own) // block
+    order = torch.arange(width)[None] + torch.where(torch.arange(width) < prefix // block, 0, torch.arange(rows)[:, None])
+    table = (order % pages).int()
+    query = (torch.randn((rows * q, hq, d), generator=torch.Generator(device=cuda).manual_seed(62), device=cuda) * 2).bfloat16()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    output, lse = torch.full_like(query, float("nan")), torch.full((rows * q, hq), float("nan"), device=cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    pa.shared_prefix_attention(
+        query, *(c.to(cuda) for c in cache), output, lse, table.to(cuda), i32([q * b for b in range(rows)]),
+        i32([q] * rows), i32([prefix + own] * rows), i32([prefix]), scale=d ** -0.5,
+        workspace=pa.new_prefix_workspace(rows, rows * q, hq, 1, d, cuda), status=status)
+    torch.cuda.synchronize()
+    assert int(status.item()) == 0 and bool(output.isfinite().all()) and bool(lse.isfinite().all())
+    # A token from the first, a middle and the last row, and each at the other ends of its row.
+    for b, i in ((0, 0), (0, 1023), (511, 300), (1023, 0), (1023, 1023)):
+        dense = [c[table[b].long()].reshape(-1, 1, d)[: prefix + own - q + i + 1] for c in cache]
+        n = dense[0].shape[0]
+        case = dict(query=query[b * q + i][None].cpu(), dense=[dense], starts=[0], qlens=[1], lens=[n], hq=hq, hkv=1, d=d,
+                    scale=d ** -0.5)
+        args = dict(output=output[b * q + i][None], lse=lse[b * q + i][None], status=status)
+        check(case, args)

@@ -301,8 +301,11 @@ __device__ __forceinline__ Plan make_plan(const PrefixArgs& a, RowTables& t, boo
     t.work[a.rows] = work;
   }
   __syncthreads();
-  // A segment of the prefix is a share without the cost of a unit, so that a unit is about a share.
-  p.segment = max(1, ceil_div(a.hkv * p.row_tiles * p.key_tiles + a.hkv * work, a.groups));
+  // A segment of the prefix is a share without the cost of a unit, so that a unit is about a share.  It
+  // ends at the prefix: its places times all row tiles, by which a unit is found, are then no more than
+  // the work, which the host bounds.
+  p.segment = min(ceil_div(a.hkv * p.row_tiles * p.key_tiles + a.hkv * work, a.groups), p.key_tiles);
+  p.segment = max(1, p.segment);
   p.segments = ceil_div(p.key_tiles, p.segment);
   p.prefix_units = a.hkv * p.segments * p.row_tiles;
   p.prefix_work = a.hkv * p.row_tiles * p.key_tiles + Shape<D>::kUnitCost * p.prefix_units;
