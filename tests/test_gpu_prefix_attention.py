@@ -496,3 +496,43 @@ def test_a_share_longer_than_the_prefix(cuda):
                     scale=d ** -0.5)
         args = dict(output=output[b * q + i][None], lse=lse[b * q + i][None], status=status)
         check(case, args)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=("bf16", "fp16"))
+@pytest.mark.parametrize("d,hkv", ((64, 2), (128, 2), (256, 1)))
+@pytest.mark.parametrize("scale", (0.0, -0.0, -1.0, "negative"))
+def test_zero_and_negative_scales(cuda, scale, d, hkv, dtype):
+    # Scale 0 weighs all seen keys alike: the mean of their values, and the logarithm of their number.  The
+    # prefix has tiles that every token sees whole, the rows end inside a tile; one row sees a single key.
+    def run_and_check(case):
+        case["scale"] = -(d ** -0.5) if scale == "negative" else scale
+        args = device_args(case, cuda)
+        run(args)
+        out, lse, terms, err, top = expect(case)
+        # A logit's error is |scale| times that of the product: E has the scale's sign here, a bound has none.
+        check(case, args, (out, lse, terms, err.abs(), top))
+        return args["lse"].cpu()
+
+    case = build(63, prefix=600, own=[17, 300, 1, 64], qlens=[3, 5, 1, 2], hq=8, hkv=hkv, d=d, block=16, dtype=dtype)
+    lse = run_and_check(case)
+    if scale == 0:
+        assert (lse[case["starts"][1] + 4] - torch.tensor(900.0).log()).abs().max() < 1e-5
+    run_and_check(build(64, prefix=0, own=[1, None, 2], qlens=[1, 2, 4], hq=8, hkv=hkv, d=d, block=16, dtype=dtype))
+
+
+def test_scale_zero_and_keys_a_token_does_not_see(cuda):
+    case = build(65, prefix=100, own=[40, 90], qlens=[3, 3], hq=8, hkv=2, d=128, block=16, dtype=torch.bfloat16)
+    case["scale"] = 0.0
+    clean = expect(case)
+    for b, n in enumerate(case["lens"]):
+        page = int(case["table"][b, (n - 1) // 16])
+        case["cache"][0][page, (n - 1) % 16, :, ::2] = float("inf")
+        case["cache"][1][page, (n - 1) % 16, :, ::3] = float("nan")
+    args = device_args(case, cuda)
+    run(args)
+    got, lse = args["output"].cpu().double(), args["lse"].cpu().double()
+    u = 2.0 ** -8
+    for start in case["starts"]:
+        upto = slice(start, start + 2)
+        assert ((got[upto] - clean[0][upto]).abs() <= 1.01 * u * (clean[0][upto].abs() + clean[2][upto])).all()
+        assert (lse[upto] - clean[1][upto]).abs().max() < 1e-5

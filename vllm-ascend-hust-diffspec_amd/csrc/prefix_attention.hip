@@ -732,17 +732,18 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, c
   }
   __builtin_amdgcn_sched_barrier(0);
   float top = -INFINITY;
+  // Masked scores are no part of the maximum, and their weights are 0 as such: -infinity times a scale of 0
+  // is none.
+  auto sees = [&](int i) { return !MASKED || 8 * (i >> 2) + (i & 3) < seen - 4 * half; };
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if constexpr (MASKED) sc[i] = 8 * (i >> 2) + (i & 3) < seen - 4 * half ? sc[i] : -INFINITY;
-    top = fmaxf(top, sc[i]);
-  }
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, sees(i) ? sc[i] : -INFINITY);
   // The reference of the exponents follows the maximum only when it is 2^8 behind: weights of up to 2^8
   // keep their relative precision, and most tiles leave the sums as they are.  In fp16 it stays 2^7 below
   // the maximum, so that weights lie in 2^-24 .. 2^15 of the type: those of a long tail of small
   // probabilities are then rounded relative to themselves down to 2^-21 of the largest.
   constexpr float kBelow = DT == DS_FP16 ? 7.f : 0.f;
-  top = __builtin_fmaf(fmaxf(top, other_half(top)), scale_log2, -kBelow);
+  top = fmaxf(top, other_half(top));
+  if (!MASKED || top != -INFINITY) top = __builtin_fmaf(top, scale_log2, -kBelow);
   if (__any(top > st.m + 8.f)) {
     const float m = fmaxf(st.m, top);
     const float keep = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
@@ -758,8 +759,8 @@ __device__ __forceinline__ void attend_keys(const char* stage, const Lane& at, c
   u32x4 p[2];
 #pragma unroll
   for (int i = 0; i < 16; i += 2) {
-    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], scale_log2, -m));
-    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i + 1], scale_log2, -m));
+    const float x = sees(i) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], scale_log2, -m)) : 0.f;
+    const float y = sees(i + 1) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i + 1], scale_log2, -m)) : 0.f;
     // The product's operands are 16 bits, so the probabilities are rounded for it; the sum is of them as
     // computed, since the LSE is an fp32 output.
     st.l += x + y;
