@@ -528,7 +528,8 @@ size_t ds_prefix_attention_workspace_bytes(int rows, int tokens, int num_q_heads
  * not read).
  * *status (optional, the caller clears it) gets bit 0 for a position outside
  * [0, cs_rows) (nothing of that token is written), bit 1 for a slot past the
- * cache (nothing of it is written there).
+ * cache (nothing of it is written there).  With rotary_dim 0 the table is not
+ * read: it may be NULL, and positions may be anything.
  *
  * dtype: DS_BF16, DS_FP16 or DS_FP32 for all heads and caches; the weights
  * ([head_dim] each, contiguous) and the cos/sin cache in it or in DS_FP32.

@@ -241,3 +241,15 @@ def test_more_than_the_caches_hold(cuda, neox, dtype):
     _, ky, ks = expect(case["key"], case["k_weight"], case, 64, neox)
     assert_close(args["query"], qy, qs, 128)
     assert_close(args["key"], ky, ks, 128)
+
+
+@pytest.mark.parametrize("table", ("none", "short"))
+@pytest.mark.parametrize("d,dtype", ((128, torch.bfloat16), (6, torch.float32)))
+def test_the_norm_alone_needs_no_table(cuda, d, dtype, table):
+    # Nothing is rotated, so no row of the table is read: positions past it are no fault.
+    case = build(48, tokens=9, hq=4, hkv=2, d=d, rot=0, dtype=dtype)
+    given = torch.zeros((0, 0) if table == "none" else (2, 64), device=cuda)
+    positions = torch.tensor([0, 1, 2, 499, -1, 10 ** 6, 3, 4, 5], device=cuda)
+    args, _ = run(case, cuda, rot=0, neox=True, cos_sin_cache=given, positions=positions)
+    check(case, args, 0, True)
+    assert int(args["status"].item()) == 0

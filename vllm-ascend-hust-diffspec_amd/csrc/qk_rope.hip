@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kThreadsQ) void qk_norm_rope_kernel(QkArgs g) {
       value_at = block * g.vc_block + in * g.vc_token;
     }
   }
-  if (position < 0 || position >= g.cs_rows) {
+  if (g.rot > 0 && (position < 0 || position >= g.cs_rows)) {  // without a rotation no row of the table is read
     if (chunk == 0 && lane == 0 && g.status) {
       __hip_atomic_fetch_or(g.status, kStatusPosition, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }

@@ -56,7 +56,8 @@ def qk_norm_rope(
     ``query`` ``[tokens, Hq, D]`` and ``key`` ``[tokens, Hkv, D]`` (views of a
     fused projection are fine), weights ``[D]``, ``positions`` int32 or int64
     ``[tokens]``, ``cos_sin_cache`` ``[positions, >= rotary_dim]`` (cosines,
-    then sines), in the heads' type or fp32 like the weights.
+    then sines), in the heads' type or fp32 like the weights.  A ``rotary_dim``
+    of 0 is the norm alone: the table is not read, whatever the positions.
 
     ``query_out`` is written (None: ``query`` itself, in place), and
     ``key_out`` (None: ``key`` itself when there is no paged cache, else the
