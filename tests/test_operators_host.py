@@ -272,3 +272,21 @@ def test_page_pool_calls_refuse():
             call()
     with pytest.raises(_lib.UnsupportedShapeError, match="4096"):
         pool.compact(torch.zeros((4097, 1), dtype=torch.int32))
+
+
+def test_page_entry_points_refuse_what_32_bits_do_not_count():
+    from ds355 import _lib
+
+    lib = _lib.load()
+    lst, table, work = [None, FAKE, 2, 4096, 100], [FAKE, FAKE, 8, 4, 8], [FAKE, 1 << 62]
+    many = (1 << 30) + 1  # pages: the scans of the counts look ahead of the last one
+    refuses(lambda: lib.ds_pages_copy(None, FAKE, 2, 4096, many, FAKE, FAKE, 3, None), "2^30 pages")
+    refuses(lambda: lib.ds_pages_extend(None, many, *table, FAKE, FAKE, 2, 16, None), "2^30 pages")
+    refuses(lambda: lib.ds_pages_free(None, many, *table, FAKE, None, 2, 16, None), "2^30 pages")
+    refuses(lambda: lib.ds_pages_compact(None, FAKE, 2, 4096, many, *table, FAKE, *work, None), "2^30 pages")
+    # Rows of 2^20 entries: 2048 of them may need 2^31 pages in one call.
+    wide = [FAKE, FAKE, 1 << 20, 2048, 1 << 20]
+    refuses(lambda: lib.ds_pages_extend(None, 100, *wide, FAKE, FAKE, 2, 16, None), "block table entries")
+    refuses(lambda: lib.ds_pages_fork(*lst, *wide, FAKE, FAKE, FAKE, 2, 16, *work, None), "block table entries")
+    # 65536 caches whose largest page has 2^18 pieces.
+    refuses(lambda: lib.ds_pages_copy(None, FAKE, 65536, 1 << 30, 100, FAKE, FAKE, 3, None), "2^43")

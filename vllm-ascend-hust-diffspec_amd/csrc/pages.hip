@@ -23,6 +23,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreadsP = 1024;
 constexpr int kMaxList = 4096;   // rows of a table, and entries of a call's lists
+constexpr int kMaxPages = 1 << 30;  // the scans look a few thousand pages ahead in 32 bits
 constexpr int kCopyThreads = 256;
 constexpr int kPiece = 4096;     // bytes that a wave copies at a time
 constexpr int32_t kBadRow = 1;     // a row (or a list entry) the call leaves out
@@ -474,9 +475,12 @@ int check_caches(const int64_t* caches, int num_caches, int64_t max_page_bytes, 
   DS_REQUIRE(num_pages > 0 && num_caches >= 0 && max_page_bytes >= 0, "page and cache counts must be positive");
   DS_REQUIRE(num_caches == 0 || caches, "null cache list");
   DS_SUPPORTED(max_page_bytes <= (1 << 30) && num_caches <= 65536, "pages of at most 2^30 bytes, at most 65536 caches");
+  DS_SUPPORTED(num_pages <= kMaxPages, "at most 2^30 pages");
   c.list = caches;
   c.count = num_caches;
   c.pieces = static_cast<int>((max_page_bytes + kPiece - 1) / kPiece);
+  // copy_all numbers the pieces of a page over all caches in 32 bits.
+  DS_SUPPORTED(static_cast<int64_t>(c.count) * c.pieces <= INT_MAX, "at most 2^43 bytes per page over all caches");
   return DS_OK;
 }
 
@@ -485,6 +489,9 @@ int check_table(int32_t* table, int64_t stride, int rows, int width, const int32
   DS_REQUIRE(refs && (table || rows == 0 || width == 0), "null tensor pointer");
   DS_REQUIRE(stride >= width || rows <= 1, "block table rows overlap");
   DS_SUPPORTED(rows <= kMaxList, "at most %d block table rows", kMaxList);
+  DS_SUPPORTED(num_pages <= kMaxPages, "at most 2^30 pages");
+  // The pages that an extension needs are counted in 32 bits.
+  DS_SUPPORTED(static_cast<int64_t>(rows) * width <= INT_MAX, "at most 2^31 - 1 block table entries");
   t = {table, stride, rows, width};
   return DS_OK;
 }
