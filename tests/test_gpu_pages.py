@@ -353,3 +353,25 @@ def test_forking_again_keeps_what_is_shared_and_may_run_out(cuda):
     assert p.model.fork(*args) == 0 and p.model.held(2) == [] and len(p.model.held(1)) == 5
     p.pool.fork(p.table, *args)
     p.check(2)
+
+
+def test_a_new_pool_serves_any_stream(cuda):
+    # The pool's own buffers are filled on the stream it is made on; the first call may be on another.
+    from ds355.pages import PagePool
+
+    cache = torch.zeros((200, 4, 8), dtype=torch.float16, device=cuda)
+    table = torch.full((9, 20), -1, dtype=torch.int32, device=cuda)
+    lists = [torch.tensor(x, dtype=torch.int32, device=cuda) for x in ([0], [70], [0] * 8, list(range(1, 9)), [70] * 8)]
+    dirty = [torch.full((1 << 15,), 255, dtype=torch.uint8, device=cuda) for _ in range(16)]
+    torch.cuda.synchronize()
+    del dirty
+    made, used = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(made):
+        pool = PagePool([cache])
+        assert made.query()
+    with torch.cuda.stream(used):
+        pool.extend(table, *lists[:2])
+        pool.fork(table, *lists[2:])
+    used.synchronize()
+    assert int(pool.status.item()) == 0 and pool.ref_counts.tolist() == [9] * 17 + [1] * 9 + [0] * 174
+    assert table[:, :17].tolist() == [list(range(17))] * 9 and table[:, 17].tolist() == list(range(17, 26))

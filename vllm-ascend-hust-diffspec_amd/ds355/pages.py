@@ -40,7 +40,8 @@ class PagePool:
     cannot take are left out and set bits of ``status`` (int32 device word):
     ``STATUS_BAD_ROW``, ``STATUS_NO_PAGES``, ``STATUS_BAD_PAGE``
     (include/ds355.h).  Calls on one pool run in order on the current stream,
-    without host synchronisation when their lists are device tensors.
+    without host synchronisation when their lists are device tensors; a
+    caller that changes streams orders them, from the second call on.
     """
 
     def __init__(self, caches: Sequence[torch.Tensor], ref_counts: torch.Tensor | None = None) -> None:
@@ -75,6 +76,8 @@ class PagePool:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         # Where the last compaction put each page; -1 for pages that were free.
         self.page_map = torch.arange(self.num_pages, dtype=torch.int32, device=self.device)
+        # The first call may be on another stream than the one that fills these.
+        torch.cuda.current_stream(self.device).synchronize()
 
     def _call(self, function: str, *args) -> None:
         with _lib.on_device(self.device):
