@@ -536,3 +536,27 @@ def test_scale_zero_and_keys_a_token_does_not_see(cuda):
         upto = slice(start, start + 2)
         assert ((got[upto] - clean[0][upto]).abs() <= 1.01 * u * (clean[0][upto].abs() + clean[2][upto])).all()
         assert (lse[upto] - clean[1][upto]).abs().max() < 1e-5
+
+
+def test_a_row_longer_than_its_table_ends_there(cuda):
+    # Row 2 fills its table's 11 pages; a length past them counts as 176, for its causal ends as well.
+    case = build(66, prefix=64, own=[20, 30, 112], qlens=[2, 2, 5], hq=8, hkv=2, d=128, block=16, dtype=torch.bfloat16)
+    expected = expect(case)
+    for beyond in (0, 1, 50, 10 ** 9):
+        args = device_args(case, cuda, block_table=case["table"][:, :11].contiguous().to(cuda))
+        args["target_len"][2] = 176 + beyond
+        run(args)
+        check(case, args, expected, status=2 if beyond else 0)
+
+
+def test_rows_in_any_order_of_their_tokens(cuda):
+    # Rows' query tokens need not lie in the rows' order.
+    case = build(67, prefix=300, own=[40, 5, 90, 17], qlens=[3, 1, 5, 2], hq=8, hkv=2, d=64, block=16, dtype=torch.float16)
+    starts = [10, 8, 3, 1]
+    query = case["query"].clone()
+    for old, new, n in zip(case["starts"], starts, case["qlens"]):
+        query[new: new + n] = case["query"][old: old + n]
+    case.update(query=query, starts=starts)
+    args = device_args(case, cuda)
+    run(args)
+    check(case, args)

@@ -279,3 +279,50 @@ def test_places_past_32_bits(cuda):
     args = attention.device_args(case, cuda, key_cache=caches[0], value_cache=caches[1])
     attention.run(args)
     attention.check(case, args)
+
+
+@pytest.mark.parametrize("lse_free", (False, True), ids=("lse", "no_lse"))
+@pytest.mark.parametrize("path", ("chain", "fused"))
+def test_a_retrieval_step_on_a_pools_table(cuda, path, lse_free):
+    """The step takes the pool's table as it is (-1 behind a row's last page, rows without any) and the
+    attention's LSE; pages that no row holds are NaN."""
+    import test_gpu_step as steps
+    from ds355.pages import PagePool
+
+    lens = [900, 333, 64, 65, 1700, 17, 1201, 512]
+    case = steps.build_case(7, real_rows=8, pad_rows=2, target_lens=lens, query_len=4, counts=[1, 3, 0, 4, 2, 1, 4, 3],
+                            hq=16, hkv=4, head_dim=128, chunk=64, token_budget=512, block_size=16, lmax=2048,
+                            slots=[3, 0, 7, 9, 1, 4, 2, 8], num_slots=10)
+    given_k, given_table, given_lse = case["key_cache"], case["table"], case["lse"]
+    caches = [torch.full((400, 16, 4, 128), float("nan"), dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    pool = PagePool(caches)
+    table = torch.full((10, 120), -1, dtype=torch.int32, device=cuda)
+    pool.extend(table, [4, 1, 0, 3], [1700, 1000, 900, 65])
+    pool.extend(table, [7, 5, 2, 6], [512, 17, 64, 1201])
+    pool.free(table, [1], [333])
+    pool.compact(table)
+    held = table.cpu()
+    for b, n in enumerate(lens):
+        pages = -(-n // 16)
+        assert (held[b, :pages] >= 0).all() and (held[b, pages:] == -1).all()
+        caches[0][held[b, :pages].long().to(cuda)] = given_k[given_table[b, :pages].long()].to(cuda)
+        caches[1][held[b, :pages].long().to(cuda)] = randn((pages, 16, 4, 128), torch.bfloat16, gen(b)).to(cuda)
+    assert int(pool.status.item()) == 0 and (held[8:] == -1).all()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    from ds355 import prefix_attention
+
+    query = case["query"].to(cuda)
+    out, lse = torch.zeros_like(query), torch.zeros(query.shape[:2], device=cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    prefix_attention.shared_prefix_attention(
+        query, *caches, out, lse, table, i32(case["starts"]), i32(case["qlens"]), i32(case["tlens"]), i32([0]),
+        scale=case["scale"], workspace=prefix_attention.new_prefix_workspace(10, query.shape[0], 16, 4, 128, cuda),
+        batch_size=8, status=status)
+    assert int(status.item()) == 0 and bool(out.isfinite().all())
+    # The LSE of each scored row's committed query, against the one that the case computed over its own pages.
+    _, q_index, _ = steps.O.retrieval_rows(case["counts"], case["ends"], case["tlens"], 8)
+    assert (lse.cpu()[q_index] - given_lse[q_index]).abs().max() < 1e-4
+    case.update(key_cache=caches[0].cpu(), table=held, lse=lse.cpu())
+    state = steps.run_gpu(case, cuda, path=path, lse_free=lse_free)
+    case["table"] = held.clamp_min(0)  # the oracle's lookup
+    steps.check_step(case, state)
