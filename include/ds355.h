@@ -474,7 +474,9 @@ int ds_capture_raw_kv(ds_stream_t stream, int dtype,
  * aligned pointers; at most 1024 rows, 2^20 query tokens, 2^20 tokens and 2^30
  * elements per page.
  * workspace: caller's scratch of ds_prefix_attention_workspace_bytes(),
- * 256-byte aligned, with no state between calls (one launch at a time).
+ * 256-byte aligned, with no state between calls (one launch at a time).  It
+ * holds two fp32 pieces per 64 query rows of a KV head: 554 MiB for 8192 query
+ * tokens of 32 heads on 8 and 128 dimensions.
  * Two kernels, launch shape fixed by the sizes (graph-capturable).
  */
 typedef struct ds_prefix_attention_desc {

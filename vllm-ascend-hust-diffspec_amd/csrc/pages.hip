@@ -11,9 +11,11 @@
 // The bookkeeping is latency-bound (a few thousand words); the copies are bound by memory.  One
 // workgroup takes pages (ranks need one order), every workgroup releases, shares or copies.  A fork's
 // last workgroup to have released takes the pages, which saves a launch.  Measured: a fork of 4 rows
-// 6.0 + 4.1 us (checks and pages, then entries and copies), of 248 rows of up to 4000 tokens, a page of each
-// copied in 8 caches of 32 KiB, 9.0 + 13.1; 128 rows cut back and grown again 3.6 + 9.7; copies 4.9 TB/s both ways (a large
-// plain copy reaches 5.1); a compaction's plan over 4096 pages 7.0 and its moves 5.3 TB/s.
+// 6.3 + 3.6 us (checks and pages, then entries and copies), of 248 rows of up to 4000 tokens, a page of each
+// copied in 8 caches of 32 KiB, 9.0 + 12.8 to 14.4, both with children that share the parent's entries from the
+// fork before (the two in turn, 153 pages copied: 19.3 us; with another parent for each row every time 24.0); 128
+// rows cut back and grown again 3.5 + 9.6; copies 4.9 TB/s both ways (a large plain copy reaches 5.1); a
+// compaction's plan over 4096 pages 7.0 and its moves 5.3 TB/s.
 #include "ds355_common.h"
 
 namespace ds355 {

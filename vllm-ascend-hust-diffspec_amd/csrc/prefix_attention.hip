@@ -26,10 +26,14 @@
 // inside a unit leaves its piece (m, l, O in fp32) in the workspace; prefix_join_kernel joins them.
 //
 // Measured (32 query heads on 4, 128 dimensions, bf16; this kernel + the join, back to back): 16 rows of 5
-// tokens over 32 k shared keys and up to 4 k of their own 89 us (46 GFLOP: 516 TFLOP/s; a large library product
-// reaches 1157), bound by staging and reading the tiles in shared memory, the matrix units busy for a
-// quarter of the time; one token each over 16 k 39 us (2.3 TB/s; a large copy reaches 5.1), bound by
-// loads' latency and the units' ends; two rows over 1 k 15 us, two launches' latency.
+// tokens over 32 k shared keys and up to 4 k of their own 89 us (46 GFLOP: 517 TFLOP/s; a large library product
+// reaches 1157): no unit is saturated (of the CUs' busy cycles the matrix units take 28%, vector issue 44%,
+// shared memory 32%), waves wait for 37% of theirs, and a SIMD's two waves meet at every tile's barrier, so that
+// products, softmax and staging add up; one token each over 16 k 39 us (2.3 TB/s; a large copy reaches 5.1), bound by
+// loads' latency and the units' ends; two rows over 1 k 15 us, two launches' latency.  A prompt chunk that
+// attends mostly to itself takes about three times its products (4096 tokens, 32 heads on 8: 416 us, floor
+// 119): all query tiles of a row count as many key tiles as the last, and those past a tile's own end are
+// staged as zeros.
 #include <cmath>
 
 #include "ds355_common.h"
