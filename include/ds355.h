@@ -578,7 +578,7 @@ int ds_qk_norm_rope(ds_stream_t stream, const ds_qk_norm_rope_desc* desc);
  * Free pages are taken in ascending order, for the list's entries in turn, so
  * results depend on the state alone.  Lists are int32 device arrays of
  * `count` entries; at most 4096 entries and 4096 table rows, 2^31 - 1 table
- * entries, 2^30 pages, and caches times max_page_bytes of 2^43.
+ * entries, 2^31 - 2^14 - 1 pages, and caches times max_page_bytes of 2^43.
  * workspace: ds_pages_workspace_bytes(), zero-filled once, 16-byte aligned;
  *   one call at a time.
  * *status (optional, the caller clears it): bit 0 an entry was left out (a row

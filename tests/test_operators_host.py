@@ -279,11 +279,11 @@ def test_page_entry_points_refuse_what_32_bits_do_not_count():
 
     lib = _lib.load()
     lst, table, work = [None, FAKE, 2, 4096, 100], [FAKE, FAKE, 8, 4, 8], [FAKE, 1 << 62]
-    many = (1 << 30) + 1  # pages: the scans of the counts look ahead of the last one
-    refuses(lambda: lib.ds_pages_copy(None, FAKE, 2, 4096, many, FAKE, FAKE, 3, None), "2^30 pages")
-    refuses(lambda: lib.ds_pages_extend(None, many, *table, FAKE, FAKE, 2, 16, None), "2^30 pages")
-    refuses(lambda: lib.ds_pages_free(None, many, *table, FAKE, None, 2, 16, None), "2^30 pages")
-    refuses(lambda: lib.ds_pages_compact(None, FAKE, 2, 4096, many, *table, FAKE, *work, None), "2^30 pages")
+    many = (1 << 31) - (1 << 14)  # pages: the scans of the counts look ahead of the last one
+    refuses(lambda: lib.ds_pages_copy(None, FAKE, 2, 4096, many, FAKE, FAKE, 3, None), "2^14 - 1 pages")
+    refuses(lambda: lib.ds_pages_extend(None, many, *table, FAKE, FAKE, 2, 16, None), "2^14 - 1 pages")
+    refuses(lambda: lib.ds_pages_free(None, many, *table, FAKE, None, 2, 16, None), "2^14 - 1 pages")
+    refuses(lambda: lib.ds_pages_compact(None, FAKE, 2, 4096, many, *table, FAKE, *work, None), "2^14 - 1 pages")
     # Rows of 2^20 entries: 2048 of them may need 2^31 pages in one call.
     wide = [FAKE, FAKE, 1 << 20, 2048, 1 << 20]
     refuses(lambda: lib.ds_pages_extend(None, 100, *wide, FAKE, FAKE, 2, 16, None), "block table entries")

@@ -12,9 +12,9 @@
 // workgroup takes pages (ranks need one order), every workgroup releases, shares or copies.  A fork's
 // last workgroup to have released takes the pages, which saves a launch.  Measured: a fork of 4 rows
 // 6.3 + 3.6 us (checks and pages, then entries and copies), of 248 rows of up to 4000 tokens, a page of each
-// copied in 8 caches of 32 KiB, 9.0 + 12.8 to 14.4, both with children that share the parent's entries from the
-// fork before (the two in turn, 153 pages copied: 19.3 us; with another parent for each row every time 24.0); 128
-// rows cut back and grown again 3.5 + 9.6; copies 4.9 TB/s both ways (a large plain copy reaches 5.1); a
+// copied in 8 caches of 32 KiB, 9.0 + 12.8 to 14.4, both with children that share the parent's entries already
+// (248 rows with 153 pages copied: the same fork again 19.3 us, with another parent for each row every time
+// 24.0); 128 rows cut back and grown again 3.5 + 9.6; copies 4.9 TB/s both ways (a large plain copy reaches 5.1); a
 // compaction's plan over 4096 pages 7.0 and its moves 5.3 TB/s.
 #include "ds355_common.h"
 
@@ -25,7 +25,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreadsP = 1024;
 constexpr int kMaxList = 4096;   // rows of a table, and entries of a call's lists
-constexpr int kMaxPages = 1 << 30;  // the scans look a few thousand pages ahead in 32 bits
+constexpr int kMaxPages = INT_MAX - (1 << 14);  // the scans look up to 12288 pages ahead in 32 bits
 constexpr int kCopyThreads = 256;
 constexpr int kPiece = 4096;     // bytes that a wave copies at a time
 constexpr int32_t kBadRow = 1;     // a row (or a list entry) the call leaves out
@@ -477,7 +477,7 @@ int check_caches(const int64_t* caches, int num_caches, int64_t max_page_bytes, 
   DS_REQUIRE(num_pages > 0 && num_caches >= 0 && max_page_bytes >= 0, "page and cache counts must be positive");
   DS_REQUIRE(num_caches == 0 || caches, "null cache list");
   DS_SUPPORTED(max_page_bytes <= (1 << 30) && num_caches <= 65536, "pages of at most 2^30 bytes, at most 65536 caches");
-  DS_SUPPORTED(num_pages <= kMaxPages, "at most 2^30 pages");
+  DS_SUPPORTED(num_pages <= kMaxPages, "at most 2^31 - 2^14 - 1 pages");
   c.list = caches;
   c.count = num_caches;
   c.pieces = static_cast<int>((max_page_bytes + kPiece - 1) / kPiece);
@@ -491,7 +491,7 @@ int check_table(int32_t* table, int64_t stride, int rows, int width, const int32
   DS_REQUIRE(refs && (table || rows == 0 || width == 0), "null tensor pointer");
   DS_REQUIRE(stride >= width || rows <= 1, "block table rows overlap");
   DS_SUPPORTED(rows <= kMaxList, "at most %d block table rows", kMaxList);
-  DS_SUPPORTED(num_pages <= kMaxPages, "at most 2^30 pages");
+  DS_SUPPORTED(num_pages <= kMaxPages, "at most 2^31 - 2^14 - 1 pages");
   // The pages that an extension needs are counted in 32 bits.
   DS_SUPPORTED(static_cast<int64_t>(rows) * width <= INT_MAX, "at most 2^31 - 1 block table entries");
   t = {table, stride, rows, width};
