@@ -458,7 +458,9 @@ int ds_capture_raw_kv(ds_stream_t stream, int dtype,
  * Scores, softmax and sums are fp32; probabilities enter the product with
  * the values rounded to the cache's type.  What pages hold past a row's
  * last key, and keys a query token does not see, have no effect, infinities
- * and NaN included.
+ * and NaN included.  A value that it sees and that is not finite makes that
+ * dimension of its output not finite (an infinity may become NaN where the
+ * weight rounds to 0).
  * Output and LSE rows of tokens that belong to no row are left as they were.
  * Rows with query_len <= 0 (graph padding) have no token.  Rows must not
  * share query tokens.

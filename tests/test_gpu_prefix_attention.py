@@ -560,3 +560,32 @@ def test_rows_in_any_order_of_their_tokens(cuda):
     args = device_args(case, cuda)
     run(args)
     check(case, args)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=("bf16", "fp16"))
+@pytest.mark.parametrize("gap", (1.0, 40.0))
+def test_a_value_that_is_not_finite_in_a_tile_that_all_see(cuda, gap, dtype):
+    # Far from the rows' ends no mask applies: the infinity reaches every token of its row and KV head in its
+    # dimension, whether its weight is an ordinary one or e^-40 of the largest, and nothing else.
+    case = build(68, prefix=0, own=[700, 650], qlens=[2, 3], hq=8, hkv=2, d=64, block=16, dtype=dtype)
+    case["query"][:] = 0
+    case["query"][..., 0] = 8
+    for b in range(2):
+        for t in range(case["lens"][b]):
+            page = int(case["table"][b, t // 16])
+            for x in (case["cache"][0][page, t % 16], case["dense"][b][0][t]):
+                x[:, 0] = 0 if t == 40 else gap
+    case["scale"] = 1 / 8
+    case["cache"][1][int(case["table"][0, 2]), 8, 1, 7] = float("inf")  # key 40
+    args = device_args(case, cuda)
+    run(args)
+    got = args["output"].cpu()
+    start = case["starts"][0]
+    rest = torch.ones(64, dtype=torch.bool)
+    rest[7] = False
+    assert not got[start: start + 2, 4:, 7].isfinite().any()
+    assert got[start: start + 2, 4:][..., rest].isfinite().all() and got[start: start + 2, :4].isfinite().all()
+    start = case["starts"][1]
+    assert got[start: start + 3].isfinite().all()
+    if gap == 1:
+        assert (got[case["starts"][0]: case["starts"][0] + 2, 4:, 7] == float("inf")).all()
