@@ -172,12 +172,14 @@ def _prepare_attend(case, seed):
         state.decay = 0.97
         state.mass = torch.zeros(shape, device="cuda")
     if own:
-        from ds355 import chunk_attention, eviction
-
         if case["kind"] == "chunk":
+            from ds355 import chunk_attention
+
             state.workspace = chunk_attention.new_chunk_workspace(len(qlens), tokens, hq, hkv, d, "cuda:0")
         else:
-            state.workspace = eviction.new_mass_workspace(len(qlens), tokens, hq, hkv, d, "cuda:0")
+            from ds355 import eviction
+
+            state.workspace = eviction.new_mass_workspace("cuda:0")
     return state
 
 
