@@ -512,6 +512,73 @@ int ds_prefix_attention(ds_stream_t stream, const ds_prefix_attention_desc* desc
 size_t ds_prefix_attention_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads, int head_dim);
 
 /*
+ * Attention of a chunk of new tokens over a paged cache, with each query
+ * head's LSE: the verifier's prompt side.  The reference leaves the target's
+ * attention to its platform and captures the query, the LSE and the paged
+ * keys from it (diffspec/ascend_patch.py:191-240, diffspec/runtime.py:841-878).
+ *
+ * Rows, pages and tables as in ds_prefix_attention; rows share nothing.  With
+ * L = target_len[b] - query_len[b] + i + 1, query token i of row b sees the
+ * keys max(0, L - window) <= t < L (window 0: all t < L):
+ *   output[token, h] = sum_t softmax_t(scale * q . k_t) v_t, rounded once;
+ *   lse[token, h]    = ln sum_t exp(scale * q . k_t), fp32 (lse may be NULL);
+ *   nothing seen (L <= 0): output 0, lse -infinity.
+ * Scores, softmax and sums are fp32; probabilities enter the product with
+ * the values rounded to the cache's type.  What pages hold past a row's
+ * last key, and keys a query token does not see, have no effect, infinities
+ * and NaN included.  A value that it sees and that is not finite makes that
+ * dimension of its output not finite (an infinity may become NaN where the
+ * weight rounds to 0).
+ * Output and LSE rows of tokens that belong to no row are left as they were.
+ * Rows with query_len <= 0 (graph padding) have no token.  Rows must not
+ * share query tokens; query_len 1 is a row that decodes.
+ * *status (optional, the caller clears it) gets bit 0 when a row's query
+ * tokens are out of range or more than `tokens` in all (that row and, in the
+ * second case, the rows after it are left out), bit 1 when a row is longer
+ * than max_blocks pages (it ends there), bit 2 when a page id is outside
+ * [0, num_blocks) (its keys and values read as 0).
+ *
+ * query, output: [tokens, Hq, D], strides in the descriptor; key_cache,
+ * value_cache: [num_blocks, block_size, Hkv, D].  head_dim 64, 128 or 256
+ * contiguous; all other strides non-negative multiples of 8 elements, 16-byte
+ * aligned pointers; at most 1024 rows, 2^20 query tokens, 2^20 tokens and 2^30
+ * elements per page.
+ * workspace: caller's scratch of ds_chunk_attention_workspace_bytes(),
+ * 256-byte aligned, with no state between calls (one launch at a time).  Its
+ * size hardly depends on the tokens.
+ * Three kernels, launch shape fixed by the sizes (graph-capturable).
+ */
+typedef struct ds_chunk_attention_desc {
+  int dtype;                         /* DS_BF16 / DS_FP16 */
+  const void* query; int64_t q_row_stride, q_head_stride;
+  void* output; int64_t o_row_stride, o_head_stride;
+  float* lse; int64_t lse_token_stride, lse_head_stride;
+  const void* key_cache; int64_t k_block_stride, k_token_stride, k_head_stride;
+  const void* value_cache; int64_t v_block_stride, v_token_stride, v_head_stride;
+  const int32_t* block_table; int64_t bt_stride;
+  int max_blocks;                    /* entries of a block_table row */
+  int num_blocks, block_size;
+  const int32_t* query_start;        /* [rows] */
+  const int32_t* query_len;          /* [rows] */
+  const int32_t* target_len;         /* [rows] */
+  int rows, tokens;                  /* rows of the batch, rows of query and output */
+  int num_q_heads, num_kv_heads, head_dim;
+  float scale;
+  int window;                        /* keys that a token sees at most; 0: all */
+  void* workspace; size_t workspace_bytes;
+  int32_t* status;                   /* or NULL */
+} ds_chunk_attention_desc;
+
+int ds_chunk_attention(ds_stream_t stream, const ds_chunk_attention_desc* desc);
+
+/*
+ * Workspace bytes of ds_chunk_attention for up to `rows` rows and `tokens`
+ * query tokens on the current device (0 when an argument is not positive, Hq
+ * is not a multiple of Hkv or head_dim is not covered).
+ */
+size_t ds_chunk_attention_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads, int head_dim);
+
+/*
  * RMS norm of each query and key head with the position rotation in the
  * same pass, and the write of the keys and values into a paged cache.
  * The reference's models leave these to their platform; the rotation's two

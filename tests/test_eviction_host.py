@@ -1,0 +1,126 @@
+"""CPU: the refusals and layouts of chunk attention, attention mass and eviction."""
+
+import ctypes
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+ROOT = Path(__file__).resolve().parents[1]
+HEADER = ROOT / "include" / "ds355.h"
+FAKE = 1 << 12  # a 4096-byte aligned address that is never dereferenced: every call fails its checks first
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
+@pytest.mark.parametrize("struct,mirror", (("ds_chunk_attention_desc", "ChunkAttentionDesc"),))
+def test_descriptor_offsets_match_c_compiler(tmp_path, struct, mirror):
+    from ds355 import _lib
+
+    cls = getattr(_lib, mirror)
+    names = [n for n, _ in cls._fields_]
+    src = tmp_path / "layout.c"
+    lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{HEADER}"', "int main(void) {",
+             f'  printf("%zu\\n", sizeof({struct}));']
+    lines += [f'  printf("%zu\\n", offsetof({struct}, {n}));' for n in names]
+    lines += ["  return 0;", "}"]
+    src.write_text("\n".join(lines))
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-O0", "-o", str(exe), str(src)], check=True)
+    values = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert values[0] == ctypes.sizeof(cls)
+    assert values[1:] == [getattr(cls, n).offset for n in names]
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (struct, struct), HEADER.read_text(), flags=re.S).group(1)
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    assert len(re.findall(r"[,;]", body)) == len(names)
+
+
+def refuses(call, message):
+    from ds355 import _lib
+
+    rc = call()
+    assert rc in (_lib.DS_ERR_INVALID, _lib.DS_ERR_UNSUPPORTED)
+    assert message in _lib.load().ds_last_error().decode()
+
+
+def chunk_desc(**over):
+    from ds355 import _lib
+
+    d = _lib.ChunkAttentionDesc()
+    values = dict(dtype=_lib.DS_BF16, query=FAKE, q_row_stride=1024, q_head_stride=128, output=FAKE, o_row_stride=1024,
+                  o_head_stride=128, key_cache=FAKE, k_block_stride=4096, k_token_stride=256, k_head_stride=128,
+                  value_cache=FAKE, v_block_stride=4096, v_token_stride=256, v_head_stride=128, block_table=FAKE,
+                  bt_stride=4, max_blocks=4, num_blocks=8, block_size=16, query_start=FAKE, query_len=FAKE,
+                  target_len=FAKE, rows=2, tokens=3, num_q_heads=8, num_kv_heads=2, head_dim=128, scale=1.0,
+                  workspace=FAKE, workspace_bytes=0)
+    values.update(over)
+    for k, v in values.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("over,message", (
+    (dict(dtype=2), "BF16 or FP16"), (dict(num_q_heads=7), "divisible"), (dict(head_dim=96), "64, 128 or 256"),
+    (dict(rows=1025), "1024 rows"), (dict(rows=-1), "non-negative"), (dict(block_size=0), "positive"),
+    (dict(num_blocks=0), "positive"), (dict(block_size=(1 << 20) + 1), "2^20"), (dict(query=None), "null"),
+    (dict(window=-1), "window"), (dict(q_row_stride=1028), "multiples of 8"), (dict(v_token_stride=12), "multiples of 8"),
+    (dict(k_block_stride=1 << 30), "2^30"), (dict(k_token_stride=1 << 26), "2^30"),
+    (dict(key_cache=FAKE + 8), "16-byte aligned"), (dict(), "ds_chunk_attention_workspace_bytes"),
+    (dict(workspace=FAKE + 16, workspace_bytes=1 << 40), "256-byte aligned"),
+    (dict(tokens=(1 << 20) + 1, workspace_bytes=1 << 60), "2^20 query tokens"),
+    (dict(tokens=1 << 20, num_q_heads=4096, num_kv_heads=2, workspace_bytes=1 << 60), "too many"),
+))
+def test_chunk_attention_refuses(over, message):
+    from ds355 import _lib
+
+    d = chunk_desc(**over)
+    refuses(lambda: _lib.load().ds_chunk_attention(None, ctypes.byref(d)), message)
+    assert _lib.load().ds_chunk_attention(None, None) == _lib.DS_ERR_INVALID
+
+
+def test_chunk_attention_without_work_and_workspace_sizes():
+    from ds355 import _lib, chunk_attention
+
+    lib = _lib.load()
+    assert lib.ds_chunk_attention(None, ctypes.byref(chunk_desc(rows=0))) == 0
+    assert lib.ds_chunk_attention(None, ctypes.byref(chunk_desc(tokens=0, query=None))) == 0
+    size = chunk_attention.chunk_workspace_bytes
+    assert 0 < size(1, 1, 8, 2, 128) < size(64, 5000, 8, 2, 128)
+    assert size(64, 1 << 20, 8, 2, 128) < 100 << 20
+    for bad in ((0, 1, 8, 2, 128), (1, 0, 8, 2, 128), (1, 1, 8, 3, 128), (1, 1, 8, 2, 80)):
+        assert size(*bad) == 0
+    with pytest.raises(ValueError, match="workspace sizes"):
+        chunk_attention.new_chunk_workspace(1, 1, 8, 2, 80, "cpu")
+
+
+def chunk_args(**over):
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    args = dict(query=bf(3, 8, 128), key_cache=bf(4, 16, 2, 128), value_cache=bf(4, 16, 2, 128), output=bf(3, 8, 128),
+                lse=torch.zeros(3, 8), block_table=torch.zeros((2, 2), dtype=torch.int32), query_start=i32(0, 1),
+                query_len=i32(1, 2), target_len=i32(9, 9), scale=1.0, workspace=torch.zeros(16, dtype=torch.uint8))
+    args.update(over)
+    return args
+
+
+@pytest.mark.parametrize("over,message", (
+    (dict(query=torch.zeros(3, 8, 64, dtype=torch.bfloat16)), "query and output"),
+    (dict(value_cache=torch.zeros(4, 8, 2, 128, dtype=torch.bfloat16)), "value caches"),
+    (dict(key_cache=torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16),
+          value_cache=torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)), "head dimensions"),
+    (dict(key_cache=torch.zeros(4, 16, 3, 128, dtype=torch.bfloat16),
+          value_cache=torch.zeros(4, 16, 3, 128, dtype=torch.bfloat16)), "divisible"),
+    (dict(output=torch.zeros(3, 8, 128, dtype=torch.float16)), "share a dtype"),
+    (dict(output=torch.zeros(3, 128, 8, dtype=torch.bfloat16).transpose(1, 2)), "contiguous in head_dim"),
+    (dict(lse=torch.zeros(3, 7)), "lse"), (dict(query_len=torch.zeros(2, dtype=torch.int64)), "int32"),
+    (dict(target_len=torch.zeros(3, dtype=torch.int32)), "one entry per row"), (dict(window=0), "window"),
+    (dict(batch_size=3), "batch_size"), (dict(block_table=torch.zeros((1, 4), dtype=torch.int32)), "block_table"),
+    (dict(workspace=torch.zeros(16)), "workspace"), (dict(status=torch.zeros(1)), "status"), (dict(), "GPU only"),
+))
+def test_chunk_attention_checks_its_arguments(over, message):
+    from ds355.chunk_attention import chunk_attention
+
+    with pytest.raises(ValueError, match=message):
+        chunk_attention(**chunk_args(**over), reuse={})

@@ -1,0 +1,624 @@
+// Attention of a chunk of new tokens over a paged cache.
+//
+// Prompts enter a serving engine in chunks: ragged rows of query tokens (query_start, query_len),
+// the last of their target_len tokens, attend over their pages (block_table); rows that decode a
+// single token ride in the same batch.  With
+//
+//   L(b, i) = target_len[b] - query_len[b] + i + 1     keys before and at query token i of row b
+//
+// query token i sees the keys max(0, L - window) <= t < L, and
+//
+//   out = sum_t softmax_t(scale q . k_t) v_t,  lse = ln sum_t exp(scale q . k_t).
+//
+// The query heads that share a KV head are rows of one matrix (row = token * group + head in the
+// group).  An item is 128 of a row's matrix rows over the keys that they see, for every KV head; items
+// of many key tiles are cut into parts of nearly one size, whose pieces (maximum, sum, output, in fp32)
+// chunk_join_kernel puts together.  chunk_plan_kernel derives items and parts from the lengths on the
+// device, so that a captured launch follows changed lengths, and lists them by size, the largest first.
+#include <cmath>
+
+#include "matrix.h"
+
+namespace ds355 {
+namespace {
+
+constexpr int kItemRows = 128;  // query rows of an item
+constexpr int kMinPart = 4;     // key tiles below which an item is not cut
+constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
+constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
+constexpr uint32_t kStatusPage = 4;    // a page id is out of range
+
+constexpr int chunk_tile(int d) { return d == 64 ? 128 : 64; }       // keys of a staged tile
+constexpr int chunk_waves(int d) { return d <= 128 ? 2 : 1; }        // workgroups of a CU, waves of a SIMD
+int part_slots(int d) { return chunk_waves(d) * device_cu_count(); }  // workgroups that run at a time
+
+template <int D>
+struct Chunk {
+  static constexpr int kWaves = 4;
+  static constexpr int kThreads = 64 * kWaves;
+  static constexpr int kTile = chunk_tile(D);
+  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kPieces = D / 8;  // 16-byte pieces of a key
+  static constexpr int kValuesAt = kTile * kRowBytes;
+  static constexpr int kStage = 2 * kValuesAt;
+  static constexpr int kSteps = D / 16;   // score products of 32 keys
+  static constexpr int kBlocks = D / 32;  // output blocks of 32 dimensions
+};
+
+// An entry of the plan: one part of an item, the same for every KV head.
+struct Part {
+  int start, len, seen;  // the row's first query token, its query tokens, the keys before its first one
+  int row, tile;         // row of the batch, 128 query rows of it
+  int part, parts;       // which of the item's parts
+  int slot;              // its first piece, in units of KV heads
+};
+static_assert(sizeof(Part) == 32);
+
+struct PlanHeader {
+  int parts, joins;
+};
+
+struct ChunkArgs {
+  const uint16_t* q;
+  int64_t q_row, q_head;
+  uint16_t* out;
+  int64_t o_row, o_head;
+  float* lse;
+  int64_t l_row, l_head;
+  const char* k;
+  int64_t k_block, k_token, k_head;  // bytes
+  const char* v;
+  int64_t v_block, v_token, v_head;
+  const int32_t* table;
+  int64_t bt_stride;
+  int capacity;  // keys that a table row can address
+  int num_blocks, block_size;
+  float per_block;  // 1 / block_size
+  const int32_t* q_start;
+  const int32_t* q_len;
+  const int32_t* t_len;
+  int rows, tokens, hkv, group, window;
+  int tile;           // keys of a tile
+  int slots;          // workgroups that run at a time
+  float scale_log2;   // |scale| log2 e
+  uint32_t q_sign;    // sign bits that a negative scale turns in the queries
+  PlanHeader* header;
+  Part* parts;
+  Part* joins;        // items of several parts
+  float* pieces;
+  int32_t* status;
+};
+
+// Keys of one item: [first, end), and its tiles of keys from `first` on.
+struct Keys {
+  int first, end, tiles;
+};
+__device__ __forceinline__ Keys item_keys(const ChunkArgs& a, int len, int seen, int tile) {
+  const int r0 = tile * kItemRows, r1 = min(r0 + kItemRows, len * a.group) - 1;
+  Keys k;
+  k.end = max(seen + r1 / a.group + 1, 0);
+  k.first = max(seen + r0 / a.group + 1 - a.window, 0) & ~31;
+  k.tiles = ceil_div(max(k.end - k.first, 0), a.tile);
+  return k;
+}
+
+// ---------------------------------------------------------------------------------------------
+// The plan: one workgroup.
+// ---------------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+static_assert(kPlanThreads == kMaxRows, "a thread a row");
+
+__device__ __forceinline__ int plan_scan(int v, int* sums, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int inclusive = wave_inclusive_scan(v);
+  if (lane == 63) sums[wave] = inclusive;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
+  }
+  __syncthreads();
+  return before + inclusive - v;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(ChunkArgs a) {
+  __shared__ int sums[kPlanThreads / 64];
+  __shared__ int first_item[kMaxRows + 1], row_start[kMaxRows], row_len[kMaxRows], row_seen[kMaxRows];
+  __shared__ unsigned long long work;
+  constexpr int kSizes = 64;  // classes of part sizes
+  __shared__ int begin[kSizes + 1], slots, joins;
+  const int b = threadIdx.x;
+  int start = 0, len = 0, keys = 0;
+  bool bad = false;
+  if (b < a.rows) {
+    start = a.q_start[b], len = a.q_len[b], keys = a.t_len[b];
+    if (len < 0) len = 0;
+    bad = len > 0 && (start < 0 || len > a.tokens || start > a.tokens - len);
+    if (bad) len = 0;
+    if (keys > a.capacity && a.status) {
+      __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusLength), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    keys = min(max(keys, 0), a.capacity);
+  }
+  // Rows that would bring the sum over the query's own tokens (rows that overlap) are left out, with
+  // the rows behind them, which also bounds the workspace.  Sums are cut short of 32 bits: a row has
+  // at most 2^20 tokens, and 1024 of them reach 2^30.
+  int total = 0;
+  const int at = plan_scan(len, sums, total);
+  if (len > 0 && at + len > a.tokens) {
+    bad = true;
+    len = 0;
+  }
+  if (bad && a.status) {
+    __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusRow), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  int items = 0;
+  const int item = plan_scan(ceil_div(len * a.group, kItemRows), sums, items);
+  first_item[b] = item;
+  row_start[b] = start, row_len[b] = len, row_seen[b] = keys - len;
+  if (b == 0) first_item[kMaxRows] = items, work = 0, slots = 0, joins = 0;
+  if (b <= kSizes) begin[b] = 0;
+  __syncthreads();
+  auto row_of = [&](int i) { return find_row(first_item, kMaxRows, i); };
+  unsigned long long mine = 0;
+  for (int i = b; i < items; i += kPlanThreads) {
+    const int r = row_of(i);
+    mine += max(item_keys(a, row_len[r], row_seen[r], i - first_item[r]).tiles, 1);
+  }
+  if (mine) atomicAdd(&work, mine);
+  __syncthreads();
+  // A part is an equal share of the work at most, so that the last ones to run end together.
+  // (An item has at most 2^24 tiles.)
+  const unsigned long long share = (work * a.hkv + a.slots - 1) / a.slots;
+  const int cap = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart)), 1ull << 25));
+  auto size_class = [&](int size) { return kSizes - 1 - min(static_cast<int>(static_cast<int64_t>(size) * kSizes / (cap + 1)), kSizes - 1); };
+  for (int i = b; i < items; i += kPlanThreads) {
+    const int r = row_of(i);
+    const int n = max(item_keys(a, row_len[r], row_seen[r], i - first_item[r]).tiles, 1), parts = ceil_div(n, cap);
+    atomicAdd(&begin[size_class(n / parts) + 1], parts);
+  }
+  __syncthreads();
+  if (b == 0) {
+    for (int s = 0; s < kSizes; ++s) begin[s + 1] += begin[s];
+    a.header->parts = begin[kSizes];
+  }
+  __syncthreads();
+  for (int i = b; i < items; i += kPlanThreads) {
+    const int r = row_of(i);
+    Part p{row_start[r], row_len[r], row_seen[r], r, i - first_item[r], 0, 0, 0};
+    const int n = max(item_keys(a, p.len, p.seen, p.tile).tiles, 1);
+    p.parts = ceil_div(n, cap);
+    const int place = atomicAdd(&begin[size_class(n / p.parts)], p.parts);
+    if (p.parts > 1) {
+      p.slot = atomicAdd(&slots, p.parts);
+      a.joins[atomicAdd(&joins, 1)] = p;
+    }
+    for (; p.part < p.parts; ++p.part) a.parts[place + p.part] = p;
+  }
+  __syncthreads();
+  if (b == 0) a.header->joins = joins;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention.
+// ---------------------------------------------------------------------------------------------
+// Key t's 16-byte piece c lies at place c ^ turn of its row, so that the reads of 16 neighbouring keys
+// touch different banks.
+template <int D>
+__device__ __forceinline__ int key_turn(int t) {
+  return D == 64 ? (t >> 1) & 7 : t & 15;
+}
+
+// Stages the keys [key, key + kTile) and their values; zeros for those at or past `end` and those of a page
+// out of range.
+template <int D>
+__device__ __forceinline__ void stage_tile(const ChunkArgs& a, const int32_t* pages, int head, int key, int end,
+                                           char* lds) {
+  using C = Chunk<D>;
+  for (int i = threadIdx.x; i < C::kTile * C::kPieces; i += C::kThreads) {
+    const int t = i / C::kPieces, c = i % C::kPieces, n = key + t;
+    u32x4 k{0, 0, 0, 0}, v{0, 0, 0, 0};
+    if (n < end) {
+      const int index = n / a.block_size, page = pages[index], in = n - index * a.block_size;
+      if (static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks)) {
+        k = *reinterpret_cast<const u32x4*>(a.k + page * a.k_block + in * a.k_token + head * a.k_head + 16 * c);
+        v = *reinterpret_cast<const u32x4*>(a.v + page * a.v_block + in * a.v_token + head * a.v_head + 16 * c);
+      } else if (a.status) {
+        __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    }
+    *reinterpret_cast<u32x4*>(lds + t * C::kRowBytes + 16 * (c ^ key_turn<D>(t))) = k;
+    reinterpret_cast<u32x4*>(lds + C::kValuesAt)[piece_at<D>(t, c)] = v;
+  }
+}
+
+// A wave's softmax state for its 32 query rows (one per lane column): running maximum, the lane's
+// part of the sum, and the unnormalised output of the lane's dimensions.
+template <int D>
+struct Softmax {
+  f32x16 acc[Chunk<D>::kBlocks];
+  float m, l;
+};
+
+// A masked key of a tile may hold infinities or NaN, which a probability of 0 does not cancel in the
+// product, while another column sees that key.  The product then takes such values as 0, and they
+// are added to the columns that see them (where the sum is no longer finite whatever the weight): key t0 + t
+// is seen where from <= t < from + count.
+template <int DT, int D>
+__device__ __forceinline__ void add_not_finite(const char* lds, Softmax<D>& st, int t0, int from, unsigned count) {
+  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
+  const u32x4* values = reinterpret_cast<const u32x4*>(lds + Chunk<D>::kValuesAt);
+  const int half = (fresh_thread() >> 5) & 1;
+#pragma unroll 1
+  for (int t = 0; t < 32; ++t) {
+    const bool sees = static_cast<unsigned>(t - from) < count;
+#pragma unroll
+    for (int j = 0; j < Chunk<D>::kBlocks; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x2 v = reinterpret_cast<const u32x2*>(values + piece_at<D>(t0 + t, 4 * j + i))[half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint16_t x = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
+          if (sees && (x & kExponent) == kExponent) st.acc[j][4 * i + e] += Elem<DT>::load(x);
+        }
+      }
+    }
+  }
+}
+
+// 32 keys of a staged tile for one wave, from key t0 of the tile on.  MASKED: the lane column's query row
+// sees those t of them with from <= t < from + count.
+template <int DT, int D, bool MASKED>
+__device__ __forceinline__ void attend(const char* lds, const u32x4 (&q)[Chunk<D>::kSteps], Softmax<D>& st, int t0,
+                                       int from, unsigned count, float scale_log2) {
+  using C = Chunk<D>;
+  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
+  const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 15;
+  const int t = t0 + (lane & 31);
+  f32x16 sc;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+  for (int s = 0; s < C::kSteps; ++s) {
+    const u32x4 k = *reinterpret_cast<const u32x4*>(lds + t * C::kRowBytes + 16 * ((2 * s + half) ^ key_turn<D>(t)));
+    sc = mfma32<DT>(k, q[s], sc);
+  }
+  // Masked scores are no part of the maximum, and their weights are 0 as such: -infinity times a scale of 0
+  // is none.
+  auto sees = [&](int i) { return !MASKED || static_cast<unsigned>(8 * (i >> 2) + (i & 3) + 4 * half - from) < count; };
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, sees(i) ? sc[i] : -INFINITY);
+  // The reference of the exponents follows the maximum only when it is 2^8 behind: weights of up to 2^8
+  // keep their relative precision, and most tiles leave the sums as they are.  In fp16 it stays 2^7 below
+  // the maximum, so that weights lie in 2^-24 .. 2^15 of the type: those of a long tail of small
+  // probabilities are then rounded relative to themselves down to 2^-21 of the largest.
+  constexpr float kBelow = DT == DS_FP16 ? 7.f : 0.f;
+  top = fmaxf(top, other_half(top));
+  if (!MASKED || top != -INFINITY) top = __builtin_fmaf(top, scale_log2, -kBelow);
+  if (__any(top > st.m + 8.f)) {
+    const float m = fmaxf(st.m, top);
+    const float keep = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+    st.m = m;
+    st.l *= keep;
+#pragma unroll
+    for (int j = 0; j < C::kBlocks; ++j) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.acc[j][i] *= keep;
+    }
+  }
+  const float m = st.m == -INFINITY ? 0.f : st.m;
+  u32x4 p[2];
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const float x = sees(i) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], scale_log2, -m)) : 0.f;
+    const float y = sees(i + 1) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i + 1], scale_log2, -m)) : 0.f;
+    // The product's operands are 16 bits, so the probabilities are rounded for it; the sum is of them as
+    // computed, since the LSE is an fp32 output.
+    st.l += x + y;
+    p[i >> 3][(i & 7) >> 1] = pack2<DT>(x, y);
+  }
+  // The lane's own probabilities are the B operand: k-slot (half, e) of step s is key 16 s + 8 (e /
+  // 4) + 4 half + e % 4 of the 32, and the values are read in that order.
+  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)lds)) + C::kValuesAt + 8 * (l & 1) +
+                        16 * piece_at<D>(4 * half + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1));
+  bool poison = false;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+#pragma unroll
+    for (int j = 0; j < C::kBlocks; ++j) {
+      const u32x2 lo = read_values((base ^ (64 * j)) + (t0 + 16 * s) * C::kRowBytes);
+      const u32x2 hi = read_values((base ^ (64 * j)) + (t0 + 16 * s + 8) * C::kRowBytes);
+      u32x4 x{lo[0], lo[1], hi[0], hi[1]};
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool a0 = (x[e] & kExponent) == kExponent, a1 = (x[e] & (kExponent << 16)) == (kExponent << 16);
+          poison |= a0 || a1;
+          x[e] &= (a0 ? 0u : 0xffffu) | (a1 ? 0u : 0xffff0000u);
+        }
+      }
+      st.acc[j] = mfma32<DT>(x, p[s], st.acc[j]);
+    }
+  }
+  if constexpr (MASKED) {
+    if (__any(poison)) add_not_finite<DT, D>(lds, st, t0, from, count);
+  }
+}
+
+// A piece in the workspace: 128 maxima and 128 sums, then the outputs as the waves hold them
+// ([query block][4 x dimension group][lane] of 4 floats).
+template <int D>
+__device__ __forceinline__ float* piece_at_slot(const ChunkArgs& a, int slot) {
+  return a.pieces + static_cast<int64_t>(slot) * (kItemRows * (D + 2));
+}
+
+// Four neighbouring dimensions of one query row's result, and its LSE.
+template <int DT>
+__device__ __forceinline__ void store_out(const ChunkArgs& a, int token, int head, int dim, f32x4 x, float l) {
+  x *= l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // nothing seen: zeros; NaN stays NaN
+  uint16_t* out = a.out + token * a.o_row + head * a.o_head + dim;
+  *reinterpret_cast<u32x2*>(out) = u32x2{pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3])};
+}
+__device__ __forceinline__ void store_lse(const ChunkArgs& a, int token, int head, float m, float l) {
+  if (a.lse) a.lse[token * a.l_row + head * a.l_head] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2P;
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_attention_kernel(ChunkArgs a) {
+  using C = Chunk<D>;
+  __shared__ __attribute__((aligned(512))) char lds[C::kStage + 1024];
+  const int entry = blockIdx.x / a.hkv, h = blockIdx.x - entry * a.hkv;
+  if (entry >= a.header->parts) return;
+  const Part p = a.parts[entry];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
+  const int rows = p.len * a.group;
+  // Items of at most 64 query rows: two waves share a block of 32 rows and take 32 keys in turn.
+  const bool narrow = rows - p.tile * kItemRows <= 64;
+  const int block = narrow ? wave >> 1 : wave;
+  const int r0 = p.tile * kItemRows + 32 * block, r = r0 + (lane & 31);
+  const bool any = r0 < rows;
+  const int token = min(r, rows - 1) / a.group, head = h * a.group + min(r, rows - 1) - token * a.group;
+  const int limit = p.seen + token + 1, lower = max(limit - a.window, 0);
+  u32x4 q[C::kSteps];
+  {
+    const uint16_t* src = a.q + (p.start + token) * a.q_row + head * a.q_head + 8 * half;
+#pragma unroll
+    for (int s = 0; s < C::kSteps; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s) ^ a.q_sign;
+  }
+  Softmax<D> st;
+#pragma unroll
+  for (int j = 0; j < C::kBlocks; ++j) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) st.acc[j][i] = 0.f;
+  }
+  st.m = -INFINITY;
+  st.l = 0.f;
+  const Keys keys = item_keys(a, p.len, p.seen, p.tile);
+  // Keys that all rows of the wave see: [all_from, all_to).
+  const int all_to = p.seen + r0 / a.group + 1;
+  const int all_from = max(p.seen + min(r0 + 31, rows - 1) / a.group + 1 - a.window, 0);
+  const int first = static_cast<int>(static_cast<int64_t>(keys.tiles) * p.part / p.parts);
+  const int last = static_cast<int>(static_cast<int64_t>(keys.tiles) * (p.part + 1) / p.parts);
+  const int32_t* pages = a.table + p.row * a.bt_stride;
+  for (int i = first; i < last; ++i) {
+    const int key = keys.first + i * C::kTile;
+    __syncthreads();
+    stage_tile<D>(a, pages, h, key, keys.end, lds);
+    __syncthreads();
+    if (!any) continue;
+    for (int t0 = narrow ? 32 * (wave & 1) : 0; t0 < C::kTile; t0 += narrow ? 64 : 32) {
+      if (key + t0 >= all_from && key + t0 + 32 <= all_to) {
+        attend<DT, D, false>(lds, q, st, t0, 0, 32, a.scale_log2);
+      } else if (key + t0 < keys.end) {
+        attend<DT, D, true>(lds, q, st, t0, lower - key - t0, max(limit - lower, 0), a.scale_log2);
+      }
+    }
+  }
+  st.l += other_half(st.l);
+  // The two waves of a narrow item's block join in shared memory.
+  constexpr int kGroups = 4 * C::kBlocks;
+  auto group = [&](int g) {
+    return f32x4{st.acc[g >> 2][4 * (g & 3)], st.acc[g >> 2][4 * (g & 3) + 1], st.acc[g >> 2][4 * (g & 3) + 2],
+                 st.acc[g >> 2][4 * (g & 3) + 3]};
+  };
+  if (narrow) {
+    static_assert(2 * (kGroups * 4 + 2) * 64 * 4 <= sizeof(lds), "two waves' results fit the tile");
+    f32x4* area = reinterpret_cast<f32x4*>(lds) + block * kGroups * 64;
+    float* sums = reinterpret_cast<float*>(reinterpret_cast<f32x4*>(lds) + 2 * kGroups * 64) + block * 128;
+    __syncthreads();
+    if (any && (wave & 1)) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) area[g * 64 + lane] = group(g);
+      sums[lane] = st.m;
+      sums[64 + lane] = st.l;
+    }
+    __syncthreads();
+    if (!any || (wave & 1)) return;
+    const float om = sums[lane], m = fmaxf(st.m, om);
+    const float mine = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+    const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - m);
+    st.m = m;
+    st.l = st.l * mine + sums[64 + lane] * other;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const f32x4 x = group(g) * mine + area[g * 64 + lane] * other;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.acc[g >> 2][4 * (g & 3) + e] = x[e];
+    }
+  }
+  if (r >= rows) return;
+  if (p.parts == 1) {
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) store_out<DT>(a, p.start + token, head, 8 * g + 4 * half, group(g), st.l);
+    if (half == 0) store_lse(a, p.start + token, head, st.m, st.l);
+    return;
+  }
+  float* sums = piece_at_slot<D>(a, (p.slot + p.part) * a.hkv + h);
+  if (half == 0) {
+    sums[32 * block + lane] = st.m;
+    sums[kItemRows + 32 * block + lane] = st.l;
+  }
+  f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kItemRows) + block * kGroups * 64 + lane;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) o[g * 64] = group(g);
+}
+
+// Joins the parts of 32 query rows of an item: a wave takes a quarter of the dimensions.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
+  constexpr int kMine = D / 32;  // groups of four dimensions of a wave's lane
+  if (static_cast<int>(blockIdx.x) >= a.header->joins) return;
+  const Part p = a.joins[blockIdx.x];
+  const int h = blockIdx.z, block = blockIdx.y, rows = p.len * a.group;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
+  const int r0 = p.tile * kItemRows + 32 * block, r = r0 + (lane & 31);
+  if (r >= rows) return;
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc[kMine];
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < p.parts; ++i) {
+    const float* sums = piece_at_slot<D>(a, (p.slot + i) * a.hkv + h);
+    const float om = sums[32 * block + (lane & 31)], ol = sums[kItemRows + 32 * block + (lane & 31)];
+    const f32x4* o = reinterpret_cast<const f32x4*>(sums + 2 * kItemRows) + (block * (D / 8) + wave * kMine) * 64 + lane;
+    const float top = fmaxf(m, om);
+    const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - top);
+    m = top;
+    l = l * mine + ol * other;
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) acc[k] = acc[k] * mine + o[k * 64] * other;
+  }
+  const int token = r / a.group, head = h * a.group + r - token * a.group;
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) store_out<DT>(a, p.start + token, head, 8 * (wave * kMine + k) + 4 * half, acc[k], l);
+  if (wave == 0 && half == 0) store_lse(a, p.start + token, head, m, l);
+}
+
+// Bounds of a plan.  Items: whole ones and a last one a row.  A cut item has at most twice the parts that
+// its tiles fill, so all cut items have at most two parts per workgroup that runs at a time, and each
+// part counts once for every KV head.
+struct Bounds {
+  int64_t items, parts, joins, pieces;
+};
+Bounds plan_bounds(int rows, int tokens, int num_q_heads, int num_kv_heads, int d) {
+  const int64_t group = num_q_heads / num_kv_heads;
+  Bounds b;
+  b.items = static_cast<int64_t>(tokens) * group / kItemRows + std::min(rows, tokens);
+  const int64_t cut = 2 * static_cast<int64_t>(part_slots(d)) / num_kv_heads + 1;
+  b.parts = b.items + cut;
+  b.joins = std::min(b.items, cut / 2 + 1);
+  b.pieces = cut * num_kv_heads;
+  return b;
+}
+constexpr size_t kPlanHeader = 256;
+size_t rounded(size_t n) { return (n + 255) & ~size_t{255}; }
+
+size_t chunk_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads, int d) {
+  if (rows <= 0 || tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return 0;
+  if (d != 64 && d != 128 && d != 256) return 0;
+  const Bounds b = plan_bounds(rows, tokens, num_q_heads, num_kv_heads, d);
+  return kPlanHeader + rounded((b.parts + b.joins) * sizeof(Part)) +
+         static_cast<size_t>(b.pieces) * kItemRows * (d + 2) * sizeof(float);
+}
+
+template <int DT, int D>
+int launch(hipStream_t stream, const ChunkArgs& a, const Bounds& b) {
+  chunk_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+  chunk_attention_kernel<DT, D><<<static_cast<int>(b.parts * a.hkv), Chunk<D>::kThreads, 0, stream>>>(a);
+  chunk_join_kernel<DT, D><<<dim3(static_cast<int>(b.joins), kItemRows / 32, a.hkv), 256, 0, stream>>>(a);
+  return check_launch("ds_chunk_attention");
+}
+
+template <int DT>
+int launch_dim(hipStream_t stream, int d, const ChunkArgs& a, const Bounds& b) {
+  if (d == 64) return launch<DT, 64>(stream, a, b);
+  if (d == 128) return launch<DT, 128>(stream, a, b);
+  return launch<DT, 256>(stream, a, b);
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int chunk_attention_impl(hipStream_t stream, const ds_chunk_attention_desc* d) {
+  DS_REQUIRE(d != nullptr, "null descriptor");
+  DS_REQUIRE(d->dtype == DS_BF16 || d->dtype == DS_FP16, "queries and KV caches must use BF16 or FP16");
+  DS_REQUIRE(d->rows >= 0 && d->tokens >= 0, "row and token counts must be non-negative");
+  DS_REQUIRE(d->num_q_heads > 0 && d->num_kv_heads > 0 && d->num_q_heads % d->num_kv_heads == 0,
+             "query heads must be divisible by KV heads");
+  DS_SUPPORTED(d->head_dim == 64 || d->head_dim == 128 || d->head_dim == 256, "head_dim must be 64, 128 or 256");
+  DS_SUPPORTED(d->rows <= kMaxRows, "at most %d rows", kMaxRows);
+  DS_REQUIRE(d->block_size > 0 && d->num_blocks > 0 && d->max_blocks > 0, "block sizes and counts must be positive");
+  DS_REQUIRE(d->window >= 0, "window must not be negative (0: no window)");
+  DS_SUPPORTED(d->block_size <= (1 << 20), "at most 2^20 tokens per page");
+  if (d->rows == 0 || d->tokens == 0) return clear_error();
+  DS_REQUIRE(d->query && d->output && d->key_cache && d->value_cache && d->block_table && d->query_start &&
+                 d->query_len && d->target_len,
+             "null tensor pointer");
+  const int64_t strides[] = {d->q_row_stride,   d->q_head_stride,  d->o_row_stride,   d->o_head_stride, d->k_block_stride,
+                             d->k_token_stride, d->k_head_stride,  d->v_block_stride, d->v_token_stride, d->v_head_stride};
+  for (int64_t s : strides) DS_REQUIRE(s >= 0 && s % 8 == 0, "row, page and head strides must be multiples of 8 elements");
+  // Places within a page are 32-bit byte counts.
+  for (int i = 4; i < 10; ++i) DS_SUPPORTED(strides[i] < (1 << 30), "pages of at most 2^30 elements");
+  DS_SUPPORTED(d->block_size * d->k_token_stride + d->num_kv_heads * d->k_head_stride < (1 << 30) &&
+                   d->block_size * d->v_token_stride + d->num_kv_heads * d->v_head_stride < (1 << 30),
+               "pages of at most 2^30 elements");
+  DS_REQUIRE(aligned(d->query) && aligned(d->output) && aligned(d->key_cache) && aligned(d->value_cache),
+             "query, output and KV caches must be 16-byte aligned");
+  const size_t need = chunk_workspace_bytes(d->rows, d->tokens, d->num_q_heads, d->num_kv_heads, d->head_dim);
+  DS_REQUIRE(d->workspace && d->workspace_bytes >= need && (reinterpret_cast<uintptr_t>(d->workspace) & 255u) == 0,
+             "workspace must be 256-byte aligned and hold ds_chunk_attention_workspace_bytes()");
+  const int group = d->num_q_heads / d->num_kv_heads;
+  const Bounds b = plan_bounds(d->rows, d->tokens, d->num_q_heads, d->num_kv_heads, d->head_dim);
+  DS_SUPPORTED(d->tokens <= (1 << 20), "at most 2^20 query tokens");
+  DS_SUPPORTED(static_cast<int64_t>(d->tokens) * group < (1 << 30) && d->num_kv_heads <= 65535 &&
+                   b.parts * d->num_kv_heads < (1 << 24),
+               "too many query tokens or heads for one launch");
+  ChunkArgs a{};
+  a.q = static_cast<const uint16_t*>(d->query);
+  a.q_row = d->q_row_stride, a.q_head = d->q_head_stride;
+  a.out = static_cast<uint16_t*>(d->output);
+  a.o_row = d->o_row_stride, a.o_head = d->o_head_stride;
+  a.lse = d->lse;
+  a.l_row = d->lse_token_stride, a.l_head = d->lse_head_stride;
+  a.k = static_cast<const char*>(d->key_cache);
+  a.k_block = 2 * d->k_block_stride, a.k_token = 2 * d->k_token_stride, a.k_head = 2 * d->k_head_stride;
+  a.v = static_cast<const char*>(d->value_cache);
+  a.v_block = 2 * d->v_block_stride, a.v_token = 2 * d->v_token_stride, a.v_head = 2 * d->v_head_stride;
+  a.table = d->block_table;
+  a.bt_stride = d->bt_stride;
+  a.capacity = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(d->max_blocks) * d->block_size, 1 << 30));
+  a.num_blocks = d->num_blocks;
+  a.block_size = d->block_size;
+  a.per_block = 1.f / static_cast<float>(d->block_size);
+  a.q_start = d->query_start, a.q_len = d->query_len, a.t_len = d->target_len;
+  a.rows = d->rows, a.tokens = d->tokens, a.hkv = d->num_kv_heads, a.group = group;
+  a.window = d->window ? std::min(d->window, 1 << 30) : 1 << 30;  // rows have at most 2^30 keys
+  a.tile = chunk_tile(d->head_dim);
+  a.slots = part_slots(d->head_dim);
+  a.scale_log2 = std::fabs(d->scale) * kLog2eP;
+  a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
+  char* work = static_cast<char*>(d->workspace);
+  a.header = reinterpret_cast<PlanHeader*>(work);
+  a.parts = reinterpret_cast<Part*>(work + kPlanHeader);
+  a.joins = a.parts + b.parts;
+  a.pieces = reinterpret_cast<float*>(work + kPlanHeader + rounded((b.parts + b.joins) * sizeof(Part)));
+  a.status = d->status;
+  return d->dtype == DS_BF16 ? launch_dim<DS_BF16>(stream, d->head_dim, a, b)
+                             : launch_dim<DS_FP16>(stream, d->head_dim, a, b);
+}
+
+}  // namespace
+}  // namespace ds355
+
+extern "C" size_t ds_chunk_attention_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads,
+                                                     int head_dim) {
+  return ds355::chunk_workspace_bytes(rows, tokens, num_q_heads, num_kv_heads, head_dim);
+}
+
+extern "C" int ds_chunk_attention(ds_stream_t stream, const ds_chunk_attention_desc* desc) {
+  return ds355::chunk_attention_impl(reinterpret_cast<hipStream_t>(stream), desc);
+}

@@ -1,0 +1,89 @@
+// Matrix products and their operands: what the attention kernels over paged caches share.
+#pragma once
+
+#include "ds355_common.h"
+
+namespace ds355 {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr float kLog2eP = 1.44269504088896340736f;
+constexpr float kLn2P = 0.69314718055994530942f;
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// The thread's index, opaque to the compiler: what a part of the loop derives from it is derived there
+// again, instead of being kept in registers that the loop needs (spilled ones would be loaded in order
+// behind the keys in flight).
+__device__ __forceinline__ int fresh_thread() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// A value that is the same in all lanes, to the scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// ---------------------------------------------------------------------------------------------
+// Matrix products: 32x32x16, A rows and B columns of 32, k-slot (lane / 32, e) = 8 (lane / 32) + e;
+// result i of a lane is row 8 (i / 4) + 4 (lane / 32) + i % 4 of column lane % 32.
+// ---------------------------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(u32x4 x, u32x4 y, f32x16 c) {
+  if constexpr (DT == DS_BF16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0,
+                                                   0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0,
+                                                  0);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (DT == DS_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {static_cast<__bf16>(x), static_cast<__bf16>(y)};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 v = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+// Combines a lane's value with lane ^ 32's.
+__device__ __forceinline__ float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+__device__ __forceinline__ bool not_finite2(uint32_t w, uint32_t exponent) {
+  return (w & exponent) == exponent || (w & (exponent << 16)) == (exponent << 16);
+}
+
+// Where 16-byte piece `c` of staged value `t` lies (in pieces): the pieces of eight neighbouring keys
+// are turned against each other by two, so that a transposing read (two pieces of four keys) touches
+// different banks.
+template <int D>
+__device__ __forceinline__ int piece_at(int t, int c) {
+  const int turn = D >= 128 ? 2 * (t & 7) : 2 * ((t >> 1) & 3);
+  return t * (D / 8) + (c ^ turn);
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+// A transposing read: lane l of 16 names key l / 4 and dimensions 4 (l % 4) .. + 3 and gets four keys of dimension l.
+__device__ __forceinline__ u32x2 read_values(uint32_t at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_char*)(uintptr_t)at));
+}
+
+}  // namespace
+}  // namespace ds355
