@@ -579,6 +579,124 @@ int ds_chunk_attention(ds_stream_t stream, const ds_chunk_attention_desc* desc);
 size_t ds_chunk_attention_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads, int head_dim);
 
 /*
+ * The attention weight that each cached key of a row receives from its query
+ * tokens: what ds_evict goes by.  The reference bounds the draft's context
+ * only (diffspec/runtime.py:1650-1681); this is for bounding the target's.
+ *
+ * Rows, pages, tables, L and window as in ds_chunk_attention, and lse as it
+ * wrote it.  For every row b with query tokens, KV head h and t <
+ * target_len[b]:
+ *   mass[b, h, t] = decay * previous[b, h, t]
+ *                 + sum_{i that see t} sum_{query heads g of h} exp(scale * q_ig . k_t - lse_ig)
+ * in fp32, summed in an order that the lengths alone determine.  previous
+ * (may be NULL: all 0, or be mass itself) and mass: fp32 [rows, Hkv,
+ * capacity], contiguous in the last dimension, strides in the descriptor.
+ * Entries at or past target_len[b], and rows with query_len <= 0, are left as
+ * they were.  A query head whose lse is -infinity adds nothing.  A key that
+ * is not finite makes its own entry NaN or any value; others not.
+ * Rows may be a part of the attention's: the last tokens of each, say.
+ * *status (optional, the caller clears it) gets bit 0 when a row's query
+ * tokens are out of range (the row is left out), bit 1 when a row is longer
+ * than max_blocks pages or capacity (it ends there), bit 2 when a page id is
+ * outside [0, num_blocks) (its keys read as 0).
+ *
+ * query, key_cache: as in ds_chunk_attention; lse: fp32, strides in the
+ * descriptor; at most 2^29 keys a row.
+ * workspace: caller's scratch of ds_attention_mass_workspace_bytes(), 256-byte
+ * aligned, with no state between calls (one launch at a time).
+ * One kernel, a second one where a row may have more than 256 / (Hq / Hkv)
+ * query tokens; launch shape fixed by the sizes (graph-capturable).
+ */
+typedef struct ds_attention_mass_desc {
+  int dtype;                         /* DS_BF16 / DS_FP16 */
+  const void* query; int64_t q_row_stride, q_head_stride;
+  const void* key_cache; int64_t k_block_stride, k_token_stride, k_head_stride;
+  const float* lse; int64_t lse_token_stride, lse_head_stride;
+  const float* previous; int64_t previous_row_stride, previous_head_stride;  /* or NULL */
+  float* mass; int64_t mass_row_stride, mass_head_stride;
+  int capacity;                      /* entries of mass and previous for a row and head */
+  const int32_t* block_table; int64_t bt_stride;
+  int max_blocks;                    /* entries of a block_table row */
+  int num_blocks, block_size;
+  const int32_t* query_start;        /* [rows] */
+  const int32_t* query_len;          /* [rows] */
+  const int32_t* target_len;         /* [rows] */
+  int rows, tokens;                  /* rows of the batch, rows of query and lse */
+  int num_q_heads, num_kv_heads, head_dim;
+  float scale;
+  int window;                        /* keys that a token sees at most; 0: all */
+  float decay;
+  void* workspace; size_t workspace_bytes;
+  int32_t* status;                   /* or NULL */
+} ds_attention_mass_desc;
+
+int ds_attention_mass(ds_stream_t stream, const ds_attention_mass_desc* desc);
+
+/* Workspace bytes of ds_attention_mass on the current device, whatever the sizes. */
+size_t ds_attention_mass_workspace_bytes(void);
+
+/*
+ * Eviction from a paged cache by the mass that its keys hold: in place, each
+ * KV head of row b keeps keep_len[b] of its target_len[b] slots (places in
+ * the row's pages).  Rows with target_len <= keep_len are left as they are.
+ *
+ * positions[b, h, t] is the token of the request that slot t of the head
+ * holds, for t < settled[b][0]; slots at or past that hold their tokens in
+ * order, token t + settled[b][1].  A new request starts with settled = {0, 0};
+ * tokens are appended behind the row's last slot.  With n = target_len[b] and
+ * k = keep_len[b] < n, a head keeps
+ *   the tokens < sinks, and those >= n + settled[b][1] - recent;
+ *   then the slots of largest mass, ties to the lowest slot, NaN below all.
+ * Kept slots below k stay.  The j-th kept slot at or past k moves to the j-th
+ * slot below k that is not kept: keys, values, mass and position.  Then
+ * positions holds for all t < k, mass is 0 for k <= t < n, settled[b] = {k,
+ * settled[b][1] + n - k} and kept_len[b] = k; for the other rows kept_len[b] =
+ * max(target_len[b], 0).  Caches and positions at or past k, and mass at or
+ * past n, are left as they were.  What attention over the k slots computes
+ * does not depend on their order; a sliding window over them does.
+ * *status (optional, the caller clears it) gets bit 1 when a row is longer
+ * than max_blocks pages or capacity, bit 2 when one of its page ids is outside
+ * [0, num_blocks), bit 3 when keep_len is negative or below sinks + recent,
+ * bit 4 when ref_counts (int32 [num_blocks], or NULL) says that one of its
+ * first keep_len slots' pages is shared; such a row is left as it is.
+ * Rows must not share the pages of their first keep_len slots.
+ *
+ * key_cache, value_cache: [num_blocks, block_size, Hkv, D], 16-byte aligned,
+ * D contiguous, D and all strides multiples of 16 bytes; mass fp32 and
+ * positions int32 [rows, Hkv, capacity], contiguous in the last dimension;
+ * kept_len is memory of its own.  At most 1024 rows, 65535 heads of all rows
+ * and 2^29 slots a row.
+ * workspace: caller's scratch of ds_evict_workspace_bytes(), 256-byte aligned,
+ * with no state between calls (one launch at a time).
+ * Two kernels, launch shape fixed by the sizes (graph-capturable).
+ */
+typedef struct ds_evict_desc {
+  int dtype;                         /* DS_BF16 / DS_FP16 / DS_FP32 */
+  void* key_cache; int64_t k_block_stride, k_token_stride, k_head_stride;
+  void* value_cache; int64_t v_block_stride, v_token_stride, v_head_stride;
+  float* mass; int64_t mass_row_stride, mass_head_stride;
+  int32_t* positions; int64_t positions_row_stride, positions_head_stride;
+  int capacity;                      /* entries of mass and positions for a row and head */
+  int32_t* settled;                  /* [rows, 2] */
+  const int32_t* block_table; int64_t bt_stride;
+  int max_blocks;                    /* entries of a block_table row */
+  int num_blocks, block_size;
+  const int32_t* ref_counts;         /* [num_blocks], or NULL */
+  const int32_t* target_len;         /* [rows] */
+  const int32_t* keep_len;           /* [rows] */
+  int32_t* kept_len;                 /* [rows] */
+  int rows, num_kv_heads, head_dim;
+  int sinks, recent;
+  void* workspace; size_t workspace_bytes;
+  int32_t* status;                   /* or NULL */
+} ds_evict_desc;
+
+int ds_evict(ds_stream_t stream, const ds_evict_desc* desc);
+
+/* Workspace bytes of ds_evict (0 when an argument is not positive). */
+size_t ds_evict_workspace_bytes(int rows, int num_kv_heads, int capacity);
+
+/*
  * RMS norm of each query and key head with the position rotation in the
  * same pass, and the write of the keys and values into a paged cache.
  * The reference's models leave these to their platform; the rotation's two

@@ -15,7 +15,9 @@ FAKE = 1 << 12  # a 4096-byte aligned address that is never dereferenced: every 
 
 
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc not available")
-@pytest.mark.parametrize("struct,mirror", (("ds_chunk_attention_desc", "ChunkAttentionDesc"),))
+@pytest.mark.parametrize("struct,mirror", (("ds_chunk_attention_desc", "ChunkAttentionDesc"),
+                                           ("ds_attention_mass_desc", "AttentionMassDesc"),
+                                           ("ds_evict_desc", "EvictDesc")))
 def test_descriptor_offsets_match_c_compiler(tmp_path, struct, mirror):
     from ds355 import _lib
 
@@ -124,3 +126,143 @@ def test_chunk_attention_checks_its_arguments(over, message):
 
     with pytest.raises(ValueError, match=message):
         chunk_attention(**chunk_args(**over), reuse={})
+
+
+def mass_desc(**over):
+    from ds355 import _lib
+
+    d = _lib.AttentionMassDesc()
+    values = dict(dtype=_lib.DS_BF16, query=FAKE, q_row_stride=1024, q_head_stride=128, key_cache=FAKE, k_block_stride=4096,
+                  k_token_stride=256, k_head_stride=128, lse=FAKE, lse_token_stride=8, lse_head_stride=1, mass=FAKE,
+                  mass_row_stride=128, mass_head_stride=64, capacity=64, block_table=FAKE, bt_stride=4, max_blocks=4,
+                  num_blocks=8, block_size=16, query_start=FAKE, query_len=FAKE, target_len=FAKE, rows=2, tokens=3,
+                  num_q_heads=8, num_kv_heads=2, head_dim=128, scale=1.0, decay=1.0, workspace=FAKE, workspace_bytes=0)
+    values.update(over)
+    for k, v in values.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("over,message", (
+    (dict(dtype=2), "BF16 or FP16"), (dict(num_q_heads=7), "divisible"), (dict(head_dim=96), "64, 128 or 256"),
+    (dict(rows=1025), "1024 rows"), (dict(tokens=-1), "non-negative"), (dict(block_size=0), "positive"),
+    (dict(capacity=0), "capacity"), (dict(window=-1), "window"), (dict(lse=None), "null"), (dict(mass=None), "null"),
+    (dict(q_head_stride=4), "multiples of 8"), (dict(k_block_stride=1 << 30), "2^30"),
+    (dict(query=FAKE + 2), "16-byte aligned"), (dict(), "ds_attention_mass_workspace_bytes"),
+    (dict(workspace=FAKE + 16, workspace_bytes=1 << 40), "256-byte aligned"),
+    (dict(max_blocks=1 << 30, capacity=1 << 30, workspace_bytes=1 << 60), "2^29"),
+    (dict(tokens=(1 << 20) + 1, workspace_bytes=1 << 60), "2^20 query tokens"),
+    (dict(max_blocks=1 << 25, capacity=1 << 29, rows=1024, workspace_bytes=1 << 60), "too many"),
+))
+def test_attention_mass_refuses(over, message):
+    from ds355 import _lib
+
+    d = mass_desc(**over)
+    refuses(lambda: _lib.load().ds_attention_mass(None, ctypes.byref(d)), message)
+    assert _lib.load().ds_attention_mass(None, None) == _lib.DS_ERR_INVALID
+    assert _lib.load().ds_attention_mass(None, ctypes.byref(mass_desc(rows=0))) == 0
+
+
+def mass_args(**over):
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    args = dict(query=bf(3, 8, 128), key_cache=bf(4, 16, 2, 128), lse=torch.zeros(3, 8), mass=torch.zeros(2, 2, 32),
+                block_table=torch.zeros((2, 2), dtype=torch.int32), query_start=i32(0, 1), query_len=i32(1, 2),
+                target_len=i32(9, 9), scale=1.0, workspace=torch.zeros(16, dtype=torch.uint8))
+    args.update(over)
+    return args
+
+
+@pytest.mark.parametrize("over,message", (
+    (dict(query=torch.zeros(3, 8, 64, dtype=torch.bfloat16)), "head dimensions"),
+    (dict(query=torch.zeros(3, 8, dtype=torch.bfloat16)), "query must be"),
+    (dict(key_cache=torch.zeros(4, 16, 3, 128, dtype=torch.bfloat16)), "divisible"),
+    (dict(key_cache=torch.zeros(4, 16, 2, 128, dtype=torch.float16)), "share a dtype"), (dict(lse=torch.zeros(3, 7)), "lse"),
+    (dict(lse=torch.zeros(3, 8, dtype=torch.float64)), "lse"), (dict(mass=torch.zeros(2, 3, 32)), "mass"),
+    (dict(mass=torch.zeros(1, 2, 32)), "mass"), (dict(mass=torch.zeros(2, 2, 32, dtype=torch.float16)), "mass"),
+    (dict(mass=torch.zeros(2, 1, 32).expand(2, 2, 32)), "overlap"), (dict(previous=torch.zeros(2, 2, 31)), "capacity"),
+    (dict(query_start=torch.zeros(2)), "int32"), (dict(target_len=torch.zeros(3, dtype=torch.int32)), "one entry per row"),
+    (dict(window=0), "window"), (dict(batch_size=-1), "batch_size"), (dict(workspace=torch.zeros(16)), "workspace"),
+    (dict(status=torch.zeros(1)), "status"), (dict(), "GPU only"),
+))
+def test_attention_mass_checks_its_arguments(over, message):
+    from ds355.eviction import attention_mass
+
+    with pytest.raises(ValueError, match=message):
+        attention_mass(**mass_args(**over), reuse={})
+
+
+def evict_desc(**over):
+    from ds355 import _lib
+
+    d = _lib.EvictDesc()
+    values = dict(dtype=_lib.DS_BF16, key_cache=FAKE, k_block_stride=4096, k_token_stride=256, k_head_stride=128,
+                  value_cache=FAKE, v_block_stride=4096, v_token_stride=256, v_head_stride=128, mass=FAKE,
+                  mass_row_stride=128, mass_head_stride=64, positions=FAKE, positions_row_stride=128,
+                  positions_head_stride=64, capacity=64, settled=FAKE, block_table=FAKE, bt_stride=4, max_blocks=4,
+                  num_blocks=8, block_size=16, target_len=FAKE, keep_len=2 * FAKE, kept_len=3 * FAKE, rows=2,
+                  num_kv_heads=2, head_dim=128, workspace=FAKE, workspace_bytes=0)
+    values.update(over)
+    for k, v in values.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("over,message", (
+    (dict(dtype=7), "BF16, FP16 or FP32"), (dict(rows=-1), "non-negative"), (dict(num_kv_heads=0), "positive"),
+    (dict(head_dim=4), "16 bytes"), (dict(rows=1025), "1024 rows"), (dict(block_size=0), "positive"),
+    (dict(capacity=0), "capacity"), (dict(sinks=-1), "sinks"), (dict(recent=-1), "recent"),
+    (dict(sinks=1 << 29, recent=1), "always kept"), (dict(settled=None), "null"), (dict(kept_len=FAKE), "memory of its own"),
+    (dict(kept_len=2 * FAKE), "memory of its own"), (dict(v_head_stride=4), "16 bytes"),
+    (dict(value_cache=FAKE + 8), "16-byte aligned"), (dict(max_blocks=1 << 30, capacity=1 << 30), "2^29"),
+    (dict(rows=1024, num_kv_heads=64), "65535"), (dict(), "ds_evict_workspace_bytes"),
+    (dict(workspace=FAKE + 16, workspace_bytes=1 << 40), "256-byte aligned"),
+))
+def test_evict_refuses(over, message):
+    from ds355 import _lib
+
+    d = evict_desc(**over)
+    refuses(lambda: _lib.load().ds_evict(None, ctypes.byref(d)), message)
+    assert _lib.load().ds_evict(None, None) == _lib.DS_ERR_INVALID
+    assert _lib.load().ds_evict(None, ctypes.byref(evict_desc(rows=0))) == 0
+
+
+def test_eviction_workspace_sizes():
+    from ds355 import eviction
+
+    assert eviction.mass_workspace_bytes() > 0
+    assert 0 < eviction.evict_workspace_bytes(1, 1, 1) < eviction.evict_workspace_bytes(4, 8, 32768)
+    for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 0)):
+        assert eviction.evict_workspace_bytes(*bad) == 0
+    with pytest.raises(ValueError, match="workspace sizes"):
+        eviction.new_evict_workspace(1, 1, 0, "cpu")
+
+
+def evict_args(**over):
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    args = dict(key_cache=bf(4, 16, 2, 128), value_cache=bf(4, 16, 2, 128), mass=torch.zeros(2, 2, 32),
+                positions=torch.zeros((2, 2, 32), dtype=torch.int32), settled=torch.zeros((2, 2), dtype=torch.int32),
+                block_table=torch.zeros((2, 2), dtype=torch.int32), target_len=i32(9, 9), keep_len=i32(5, 5),
+                kept_len=i32(0, 0), workspace=torch.zeros(16, dtype=torch.uint8))
+    args.update(over)
+    return args
+
+
+@pytest.mark.parametrize("over,message", (
+    (dict(value_cache=torch.zeros(4, 8, 2, 128, dtype=torch.bfloat16)), "value caches"),
+    (dict(value_cache=torch.zeros(4, 16, 2, 128, dtype=torch.float16)), "share a dtype"),
+    (dict(key_cache=torch.zeros(4, 16, 128, 2, dtype=torch.bfloat16).transpose(2, 3)), "contiguous in head_dim"),
+    (dict(sinks=-1), "negative"), (dict(recent=-1), "negative"), (dict(mass=torch.zeros(2, 2)), "mass"),
+    (dict(positions=torch.zeros(2, 2, 32)), "positions"), (dict(positions=torch.zeros((2, 2, 31), dtype=torch.int32)), "capacity"),
+    (dict(settled=torch.zeros((2, 1), dtype=torch.int32)), "settled"), (dict(keep_len=torch.zeros(2)), "keep_len"),
+    (dict(kept_len=torch.zeros(1, dtype=torch.int32)), "one entry per row"),
+    (dict(ref_counts=torch.zeros(3, dtype=torch.int32)), "ref_counts"), (dict(batch_size=3), "batch_size"),
+    (dict(block_table=torch.zeros((1, 4), dtype=torch.int32)), "block_table"), (dict(workspace=torch.zeros(16)), "workspace"),
+    (dict(status=torch.zeros(1)), "status"), (dict(), "GPU only"),
+))
+def test_evict_tokens_checks_its_arguments(over, message):
+    from ds355.eviction import evict_tokens
+
+    with pytest.raises(ValueError, match=message):
+        evict_tokens(**evict_args(**over), reuse={})

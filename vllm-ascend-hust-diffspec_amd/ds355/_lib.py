@@ -42,6 +42,10 @@ EXPORTED_SYMBOLS = (
     "ds_prefix_attention_workspace_bytes",
     "ds_chunk_attention",
     "ds_chunk_attention_workspace_bytes",
+    "ds_attention_mass",
+    "ds_attention_mass_workspace_bytes",
+    "ds_evict",
+    "ds_evict_workspace_bytes",
     "ds_qk_norm_rope",
     "ds_pages_workspace_bytes",
     "ds_pages_copy",
@@ -147,6 +151,52 @@ class ChunkAttentionDesc(ctypes.Structure):
     ]
 
 
+class AttentionMassDesc(ctypes.Structure):
+    """Mirror of ``ds_attention_mass_desc`` (include/ds355.h)."""
+
+    _fields_ = [
+        ("dtype", _i32),
+        ("query", _p), ("q_row_stride", _i64), ("q_head_stride", _i64),
+        ("key_cache", _p), ("k_block_stride", _i64), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("lse", _p), ("lse_token_stride", _i64), ("lse_head_stride", _i64),
+        ("previous", _p), ("previous_row_stride", _i64), ("previous_head_stride", _i64),
+        ("mass", _p), ("mass_row_stride", _i64), ("mass_head_stride", _i64),
+        ("capacity", _i32),
+        ("block_table", _p), ("bt_stride", _i64), ("max_blocks", _i32),
+        ("num_blocks", _i32), ("block_size", _i32),
+        ("query_start", _p), ("query_len", _p), ("target_len", _p),
+        ("rows", _i32), ("tokens", _i32),
+        ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("scale", _f32),
+        ("window", _i32),
+        ("decay", _f32),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+        ("status", _p),
+    ]
+
+
+class EvictDesc(ctypes.Structure):
+    """Mirror of ``ds_evict_desc`` (include/ds355.h)."""
+
+    _fields_ = [
+        ("dtype", _i32),
+        ("key_cache", _p), ("k_block_stride", _i64), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("value_cache", _p), ("v_block_stride", _i64), ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("mass", _p), ("mass_row_stride", _i64), ("mass_head_stride", _i64),
+        ("positions", _p), ("positions_row_stride", _i64), ("positions_head_stride", _i64),
+        ("capacity", _i32),
+        ("settled", _p),
+        ("block_table", _p), ("bt_stride", _i64), ("max_blocks", _i32),
+        ("num_blocks", _i32), ("block_size", _i32),
+        ("ref_counts", _p),
+        ("target_len", _p), ("keep_len", _p), ("kept_len", _p),
+        ("rows", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+        ("sinks", _i32), ("recent", _i32),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_size_t),
+        ("status", _p),
+    ]
+
+
 class QkNormRopeDesc(ctypes.Structure):
     """Mirror of ``ds_qk_norm_rope_desc`` (include/ds355.h)."""
 
@@ -201,6 +251,10 @@ _SIGNATURES = {
     "ds_prefix_attention_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32, _i32]),
     "ds_chunk_attention": (_i32, [_p, ctypes.POINTER(ChunkAttentionDesc)]),
     "ds_chunk_attention_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32, _i32]),
+    "ds_attention_mass": (_i32, [_p, ctypes.POINTER(AttentionMassDesc)]),
+    "ds_attention_mass_workspace_bytes": (ctypes.c_size_t, []),
+    "ds_evict": (_i32, [_p, ctypes.POINTER(EvictDesc)]),
+    "ds_evict_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32]),
     "ds_qk_norm_rope": (_i32, [_p, ctypes.POINTER(QkNormRopeDesc)]),
     "ds_pages_workspace_bytes": (ctypes.c_size_t, [_i32]),
     "ds_pages_copy": (_i32, [_p, _p, _i32, _i64, _i32, _p, _p, _i32, _p]),
