@@ -28,21 +28,21 @@ constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
-constexpr int chunk_tile(int d) { return d == 64 ? 128 : 64; }       // keys of a staged tile
-constexpr int chunk_waves(int d) { return d <= 128 ? 2 : 1; }        // workgroups of a CU, waves of a SIMD
+constexpr int kTile = 64;  // keys of a staged tile
+constexpr int chunk_waves(int d) { return d == 64 ? 3 : d == 128 ? 2 : 1; }  // workgroups of a CU, waves of a SIMD
 int part_slots(int d) { return chunk_waves(d) * device_cu_count(); }  // workgroups that run at a time
 
 template <int D>
 struct Chunk {
   static constexpr int kWaves = 4;
   static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kTile = chunk_tile(D);
   static constexpr int kRowBytes = 2 * D;
   static constexpr int kPieces = D / 8;  // 16-byte pieces of a key
-  static constexpr int kValuesAt = kTile * kRowBytes;
-  static constexpr int kStage = 2 * kValuesAt;
+  static constexpr int kStage = kTile * kRowBytes;  // bytes of a tile's keys, or of its values
   static constexpr int kSteps = D / 16;   // score products of 32 keys
   static constexpr int kBlocks = D / 32;  // output blocks of 32 dimensions
+  static constexpr int kPerLoad = 64 / kPieces;               // keys that one load of a wave covers
+  static constexpr int kLoads = kTile / kPerLoad / kWaves;    // such loads of a wave for the keys of a tile
 };
 
 // An entry of the plan: one part of an item, the same for every KV head.
@@ -56,6 +56,8 @@ static_assert(sizeof(Part) == 32);
 
 struct PlanHeader {
   int parts, joins;
+  int unused[62];
+  int zeros[64];  // what keys past an item's end and those of a page out of range are read from
 };
 
 struct ChunkArgs {
@@ -78,7 +80,6 @@ struct ChunkArgs {
   const int32_t* q_len;
   const int32_t* t_len;
   int rows, tokens, hkv, group, window;
-  int tile;           // keys of a tile
   int slots;          // workgroups that run at a time
   float scale_log2;   // |scale| log2 e
   uint32_t q_sign;    // sign bits that a negative scale turns in the queries
@@ -98,7 +99,7 @@ __device__ __forceinline__ Keys item_keys(const ChunkArgs& a, int len, int seen,
   Keys k;
   k.end = max(seen + r1 / a.group + 1, 0);
   k.first = max(seen + r0 / a.group + 1 - a.window, 0) & ~31;
-  k.tiles = ceil_div(max(k.end - k.first, 0), a.tile);
+  k.tiles = ceil_div(max(k.end - k.first, 0), kTile);
   return k;
 }
 
@@ -160,6 +161,7 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(ChunkArgs a) {
   row_start[b] = start, row_len[b] = len, row_seen[b] = keys - len;
   if (b == 0) first_item[kMaxRows] = items, work = 0, slots = 0, joins = 0;
   if (b <= kSizes) begin[b] = 0;
+  if (b < 64) a.header->zeros[b] = 0;
   __syncthreads();
   auto row_of = [&](int i) { return find_row(first_item, kMaxRows, i); };
   unsigned long long mine = 0;
@@ -211,26 +213,86 @@ __device__ __forceinline__ int key_turn(int t) {
   return D == 64 ? (t >> 1) & 7 : t & 15;
 }
 
-// Stages the keys [key, key + kTile) and their values; zeros for those at or past `end` and those of a page
-// out of range.
-template <int D>
-__device__ __forceinline__ void stage_tile(const ChunkArgs& a, const int32_t* pages, int head, int key, int end,
-                                           char* lds) {
+// 64 lanes' 16 bytes each from base + offset to 1 KiB of shared memory from `to` on, a lane after the other.
+// The compiler does not know of the load: what reads that memory waits for it (wait_loads) before a barrier.
+// (It keeps nothing in m0 from one instruction to another.)
+__device__ __forceinline__ void load_lds(uint64_t base, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds(uint64_t from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
+// (n + 0.5) / size in floating point gives the exact quotient for n < 2^22: the half keeps it away from
+// the integers by 0.5 / size, more than the 2^-23 relative error of a product with a rounded reciprocal.
+__device__ __forceinline__ int pages_in(const ChunkArgs& a, int n) {
+  return static_cast<int>((static_cast<float>(n) + 0.5f) * a.per_block);
+}
+
+// A tile of a part's keys: where it begins, and (WHOLE) the places of a wave's loads.  One load of a wave
+// takes kPerLoad neighbouring keys; a part begins at a multiple of 32 keys, so where the page size is a
+// multiple of kPerLoad they lie in one page and the address is the wave's.  Lane i looks up the page of
+// the wave's load i.
+struct Tile {
+  const int32_t* pages;  // the table entry of the first key's page
+  int place;             // the first key in that page
+  int left;              // keys from the first one to the part's end
+  int page, in;          // lane i: of load i
+};
+
+template <int D, bool WHOLE>
+__device__ __forceinline__ void look_up(const ChunkArgs& a, int wave, Tile& x) {
   using C = Chunk<D>;
-  for (int i = threadIdx.x; i < C::kTile * C::kPieces; i += C::kThreads) {
-    const int t = i / C::kPieces, c = i % C::kPieces, n = key + t;
-    u32x4 k{0, 0, 0, 0}, v{0, 0, 0, 0};
-    if (n < end) {
-      const int index = n / a.block_size, page = pages[index], in = n - index * a.block_size;
-      if (static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks)) {
-        k = *reinterpret_cast<const u32x4*>(a.k + page * a.k_block + in * a.k_token + head * a.k_head + 16 * c);
-        v = *reinterpret_cast<const u32x4*>(a.v + page * a.v_block + in * a.v_token + head * a.v_head + 16 * c);
-      } else if (a.status) {
-        __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+  if (!WHOLE || x.left <= 0) return;
+  const int i = (fresh_thread() & 63) % C::kLoads;
+  const int t = min((wave * C::kLoads + i) * C::kPerLoad, (x.left - 1) & ~(C::kPerLoad - 1));
+  const int index = pages_in(a, x.place + t);
+  x.in = x.place + t - index * a.block_size;
+  x.page = x.pages[index];
+}
+
+__device__ __forceinline__ void advance(const ChunkArgs& a, Tile& x) {
+  const int n = uniform(pages_in(a, x.place + kTile));
+  x.left -= kTile;
+  x.pages += n;
+  x.place += kTile - n * a.block_size;
+}
+
+// Sends the wave's part of a tile's keys (or values) to shared memory; zeros for loads past the part's end and
+// for keys of a page out of range.
+template <int D, bool WHOLE, bool VALUES>
+__device__ __forceinline__ void send(const ChunkArgs& a, const Tile& x, int head, int wave, uint32_t to) {
+  using C = Chunk<D>;
+  if (x.left <= 0) return;
+  const int lane = fresh_thread() & 63, piece = lane % C::kPieces, mine = lane / C::kPieces;
+  const uint64_t zeros = reinterpret_cast<uint64_t>(a.header->zeros);
+  const uint64_t cache = reinterpret_cast<uint64_t>(VALUES ? a.v : a.k);
+  const int64_t block_bytes = VALUES ? a.v_block : a.k_block;
+  const uint32_t token_bytes = VALUES ? a.v_token : a.k_token, head_bytes = head * (VALUES ? a.v_head : a.k_head);
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < C::kLoads; ++i) {
+    const int t = (wave * C::kLoads + i) * C::kPerLoad, key = t + mine;
+    const uint32_t turned = 16 * (VALUES ? piece_at<D>(key, piece) - key * C::kPieces : piece ^ key_turn<D>(key));
+    if constexpr (WHOLE) {
+      const int page = __builtin_amdgcn_readlane(x.page, i), in = __builtin_amdgcn_readlane(x.in, i);
+      const bool fine = t < x.left && static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
+      bad |= t < x.left && !fine;
+      const uint64_t base = cache + page * block_bytes + (in * token_bytes + head_bytes);
+      const uint32_t mask = fine ? ~0u : 0u;
+      load_lds(zeros ^ ((base ^ zeros) & (static_cast<uint64_t>(mask) << 32 | mask)), (mine * token_bytes + turned) & mask,
+               to + t * C::kRowBytes);
+    } else {
+      const int n = x.place + min(key, x.left - 1), index = pages_in(a, n), page = x.pages[index];
+      const uint32_t in = n - index * a.block_size;
+      const bool fine = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
+      bad |= !fine;
+      load_lds(fine ? cache + page * block_bytes + (in * token_bytes + head_bytes) + turned : zeros, to + t * C::kRowBytes);
     }
-    *reinterpret_cast<u32x4*>(lds + t * C::kRowBytes + 16 * (c ^ key_turn<D>(t))) = k;
-    reinterpret_cast<u32x4*>(lds + C::kValuesAt)[piece_at<D>(t, c)] = v;
+  }
+  if (bad && a.status) {
+    __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
 
@@ -247,9 +309,9 @@ struct Softmax {
 // are added to the columns that see them (where the sum is no longer finite whatever the weight): key t0 + t
 // is seen where from <= t < from + count.
 template <int DT, int D>
-__device__ __forceinline__ void add_not_finite(const char* lds, Softmax<D>& st, int t0, int from, unsigned count) {
+__device__ __forceinline__ void add_not_finite(const char* values_at, Softmax<D>& st, int t0, int from, unsigned count) {
   constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
-  const u32x4* values = reinterpret_cast<const u32x4*>(lds + Chunk<D>::kValuesAt);
+  const u32x4* values = reinterpret_cast<const u32x4*>(values_at);
   const int half = (fresh_thread() >> 5) & 1;
 #pragma unroll 1
   for (int t = 0; t < 32; ++t) {
@@ -269,29 +331,43 @@ __device__ __forceinline__ void add_not_finite(const char* lds, Softmax<D>& st, 
   }
 }
 
-// 32 keys of a staged tile for one wave, from key t0 of the tile on.  MASKED: the lane column's query row
-// sees those t of them with from <= t < from + count.
-template <int DT, int D, bool MASKED>
-__device__ __forceinline__ void attend(const char* lds, const u32x4 (&q)[Chunk<D>::kSteps], Softmax<D>& st, int t0,
-                                       int from, unsigned count, float scale_log2) {
+// Scores of 32 keys from key t0 of the tile on.
+template <int DT, int D>
+__device__ __forceinline__ f32x16 score(const char* keys, const u32x4 (&q)[Chunk<D>::kSteps], int t0) {
   using C = Chunk<D>;
-  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
-  const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 15;
-  const int t = t0 + (lane & 31);
+  const int lane = threadIdx.x & 63, half = lane >> 5, t = t0 + (lane & 31);
   f32x16 sc;
 #pragma unroll
   for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
   for (int s = 0; s < C::kSteps; ++s) {
-    const u32x4 k = *reinterpret_cast<const u32x4*>(lds + t * C::kRowBytes + 16 * ((2 * s + half) ^ key_turn<D>(t)));
-    sc = mfma32<DT>(k, q[s], sc);
+    sc = mfma32<DT>(*reinterpret_cast<const u32x4*>(keys + t * C::kRowBytes + 16 * ((2 * s + half) ^ key_turn<D>(lane & 31))),
+                    q[s], sc);
   }
+  return sc;
+}
+
+// One tile for one wave: 32 N keys from key t0 of it on, whose scores are in `sc`; `next` gets those of the
+// next tile (unless LAST), whose products run while the weights are computed.  MASKED: the lane column's
+// query row sees those t of the keys with from <= t < from + count.
+template <int DT, int D, int N, bool MASKED, bool LAST>
+__device__ __forceinline__ void attend(const char* next_keys, const char* values, const u32x4 (&q)[Chunk<D>::kSteps],
+                                       Softmax<D>& st, f32x16 (&sc)[N], int t0, int from, unsigned count,
+                                       float scale_log2) {
+  using C = Chunk<D>;
+  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
+  const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 15;
   // Masked scores are no part of the maximum, and their weights are 0 as such: -infinity times a scale of 0
   // is none.
-  auto sees = [&](int i) { return !MASKED || static_cast<unsigned>(8 * (i >> 2) + (i & 3) + 4 * half - from) < count; };
+  auto sees = [&](int n, int i) {
+    return !MASKED || static_cast<unsigned>(32 * n + 8 * (i >> 2) + (i & 3) + 4 * half - from) < count;
+  };
   float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = fmaxf(top, sees(i) ? sc[i] : -INFINITY);
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, sees(n, i) ? sc[n][i] : -INFINITY);
+  }
   // The reference of the exponents follows the maximum only when it is 2^8 behind: weights of up to 2^8
   // keep their relative precision, and most tiles leave the sums as they are.  In fp16 it stays 2^7 below
   // the maximum, so that weights lie in 2^-24 .. 2^15 of the type: those of a long tail of small
@@ -311,33 +387,41 @@ __device__ __forceinline__ void attend(const char* lds, const u32x4 (&q)[Chunk<D
     }
   }
   const float m = st.m == -INFINITY ? 0.f : st.m;
-  u32x4 p[2];
+  f32x16 next[N];
+  if constexpr (!LAST) {
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
-    const float x = sees(i) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], scale_log2, -m)) : 0.f;
-    const float y = sees(i + 1) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i + 1], scale_log2, -m)) : 0.f;
-    // The product's operands are 16 bits, so the probabilities are rounded for it; the sum is of them as
-    // computed, since the LSE is an fp32 output.
-    st.l += x + y;
-    p[i >> 3][(i & 7) >> 1] = pack2<DT>(x, y);
+    for (int n = 0; n < N; ++n) next[n] = score<DT, D>(next_keys, q, t0 + 32 * n);
+  }
+  u32x4 p[2 * N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float x = sees(n, i) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i], scale_log2, -m)) : 0.f;
+      const float y = sees(n, i + 1) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i + 1], scale_log2, -m)) : 0.f;
+      // The product's operands are 16 bits, so the probabilities are rounded for it; the sum is of them as
+      // computed, since the LSE is an fp32 output.
+      st.l += x + y;
+      p[2 * n + (i >> 3)][(i & 7) >> 1] = pack2<DT>(x, y);
+    }
   }
   // The lane's own probabilities are the B operand: k-slot (half, e) of step s is key 16 s + 8 (e /
-  // 4) + 4 half + e % 4 of the 32, and the values are read in that order.
-  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)lds)) + C::kValuesAt + 8 * (l & 1) +
-                        16 * piece_at<D>(4 * half + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1));
-  bool poison = false;
+  // 4) + 4 half + e % 4 of the keys, and the values are read in that order.
+  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)values)) + t0 * C::kRowBytes +
+                        8 * (l & 1) + 16 * piece_at<D>(4 * half + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1));
+  uint32_t poison = 0;  // the 32 keys with a value that is not finite
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
+  for (int s = 0; s < 2 * N; ++s) {
 #pragma unroll
     for (int j = 0; j < C::kBlocks; ++j) {
-      const u32x2 lo = read_values((base ^ (64 * j)) + (t0 + 16 * s) * C::kRowBytes);
-      const u32x2 hi = read_values((base ^ (64 * j)) + (t0 + 16 * s + 8) * C::kRowBytes);
+      const u32x2 lo = read_values((base ^ (64 * j)) + 16 * s * C::kRowBytes);
+      const u32x2 hi = read_values((base ^ (64 * j)) + (16 * s + 8) * C::kRowBytes);
       u32x4 x{lo[0], lo[1], hi[0], hi[1]};
       if constexpr (MASKED) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const bool a0 = (x[e] & kExponent) == kExponent, a1 = (x[e] & (kExponent << 16)) == (kExponent << 16);
-          poison |= a0 || a1;
+          poison |= a0 || a1 ? 1u << (s >> 1) : 0u;
           x[e] &= (a0 ? 0u : 0xffffu) | (a1 ? 0u : 0xffff0000u);
         }
       }
@@ -345,8 +429,93 @@ __device__ __forceinline__ void attend(const char* lds, const u32x4 (&q)[Chunk<D
     }
   }
   if constexpr (MASKED) {
-    if (__any(poison)) add_not_finite<DT, D>(lds, st, t0, from, count);
+    if (__any(poison != 0)) {
+#pragma unroll 1
+      for (int n = 0; n < N; ++n) {
+        if (__any((poison >> n) & 1)) add_not_finite<DT, D>(values, st, t0 + 32 * n, from - 32 * n, count);
+      }
+    }
   }
+  if constexpr (!LAST) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) sc[n] = next[n];
+  }
+}
+
+// A wave's place in its item.
+struct Rows {
+  bool any;              // it has query rows
+  int limit, lower;      // keys that the lane column's row sees: lower <= t < limit
+  int all_from, all_to;  // keys that all its rows see
+};
+
+// The part's tiles of keys, `tiles` from key `key` on, 32 N keys of each for a wave.  In shared memory the keys
+// run a tile ahead of the values: while a tile is weighed, the next one's scores are computed, the keys
+// after that and the next values are on their way, and the pages of the keys behind them are looked up.
+template <int DT, int D, bool WHOLE, int N>
+__device__ __forceinline__ void run_part(const ChunkArgs& a, const int32_t* table, int head, int key, int end, int tiles,
+                                         const Rows& rows, const u32x4 (&q)[Chunk<D>::kSteps], Softmax<D>& st, int t0,
+                                         int wave, char* lds) {
+  using C = Chunk<D>;
+  const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)lds));
+  const int index = uniform(key / a.block_size);
+  Tile x{table + index, key - index * a.block_size, end - key, 0, 0};
+  look_up<D, WHOLE>(a, wave, x);
+  send<D, WHOLE, false>(a, x, head, wave, lds_at);
+  Tile v = x;
+  advance(a, x);
+  look_up<D, WHOLE>(a, wave, x);
+  wait_loads();
+  lds_barrier();
+  send<D, WHOLE, true>(a, v, head, wave, lds_at + 2 * C::kStage);
+  send<D, WHOLE, false>(a, x, head, wave, lds_at + C::kStage);
+  v = x;
+  advance(a, x);
+  look_up<D, WHOLE>(a, wave, x);
+  f32x16 sc[N];
+  if (rows.any) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) sc[n] = score<DT, D>(lds, q, t0 + 32 * n);
+  }
+  int i = 0;  // the tile, and its half of shared memory
+  auto turn = [&]() {
+    wait_loads();
+    lds_barrier();
+    const int here = i & 1;
+    send<D, WHOLE, false>(a, x, head, wave, lds_at + here * C::kStage);
+    send<D, WHOLE, true>(a, v, head, wave, lds_at + (2 + (here ^ 1)) * C::kStage);
+    v = x;
+    advance(a, x);
+    look_up<D, WHOLE>(a, wave, x);
+    return here;
+  };
+  const unsigned count = max(rows.limit - rows.lower, 0);
+  if (!rows.any) {
+    for (; i < tiles; ++i) turn();
+    return;
+  }
+  // Tiles with a mask (of a window), those that all rows see whole, those with a mask; the last one.
+  const int whole_from = min(max(ceil_div(max(rows.all_from - key - t0, 0), kTile), 0), tiles - 1);
+  const int whole_to = max(min(max(rows.all_to - key - t0 + kTile - 32 * N, 0) / kTile, tiles - 1), whole_from);
+  for (;;) {
+    const int stop = i < whole_from ? whole_from : tiles - 1;
+    if (i >= whole_from) {
+      for (; i < whole_to; ++i) {
+        const int here = turn();
+        attend<DT, D, N, false, false>(lds + (here ^ 1) * C::kStage, lds + (2 + here) * C::kStage, q, st, sc, t0, 0, 0,
+                                       a.scale_log2);
+      }
+    }
+    for (; i < stop; ++i) {
+      const int here = turn();
+      attend<DT, D, N, true, false>(lds + (here ^ 1) * C::kStage, lds + (2 + here) * C::kStage, q, st, sc, t0,
+                                    rows.lower - key - i * kTile - t0, count, a.scale_log2);
+    }
+    if (i >= tiles - 1) break;
+  }
+  const int here = turn();
+  attend<DT, D, N, true, true>(nullptr, lds + (2 + here) * C::kStage, q, st, sc, t0, rows.lower - key - i * kTile - t0, count,
+                               a.scale_log2);
 }
 
 // A piece in the workspace: 128 maxima and 128 sums, then the outputs as the waves hold them
@@ -367,22 +536,26 @@ __device__ __forceinline__ void store_lse(const ChunkArgs& a, int token, int hea
   if (a.lse) a.lse[token * a.l_row + head * a.l_head] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2P;
 }
 
-template <int DT, int D>
+template <int DT, int D, bool WHOLE>
 __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_attention_kernel(ChunkArgs a) {
   using C = Chunk<D>;
-  __shared__ __attribute__((aligned(512))) char lds[C::kStage + 1024];
+  __shared__ __attribute__((aligned(512))) char lds[4 * C::kStage];
   const int entry = blockIdx.x / a.hkv, h = blockIdx.x - entry * a.hkv;
   if (entry >= a.header->parts) return;
   const Part p = a.parts[entry];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
   const int rows = p.len * a.group;
-  // Items of at most 64 query rows: two waves share a block of 32 rows and take 32 keys in turn.
+  // Items of at most 64 query rows: two waves share a block of 32 rows and take half of each tile's keys.
   const bool narrow = rows - p.tile * kItemRows <= 64;
   const int block = narrow ? wave >> 1 : wave;
   const int r0 = p.tile * kItemRows + 32 * block, r = r0 + (lane & 31);
-  const bool any = r0 < rows;
   const int token = min(r, rows - 1) / a.group, head = h * a.group + min(r, rows - 1) - token * a.group;
-  const int limit = p.seen + token + 1, lower = max(limit - a.window, 0);
+  Rows w;
+  w.any = r0 < rows;
+  w.limit = p.seen + token + 1;
+  w.lower = max(w.limit - a.window, 0);
+  w.all_to = p.seen + r0 / a.group + 1;
+  w.all_from = max(p.seen + min(r0 + 31, rows - 1) / a.group + 1 - a.window, 0);
   u32x4 q[C::kSteps];
   {
     const uint16_t* src = a.q + (p.start + token) * a.q_row + head * a.q_head + 8 * half;
@@ -398,24 +571,15 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
   st.m = -INFINITY;
   st.l = 0.f;
   const Keys keys = item_keys(a, p.len, p.seen, p.tile);
-  // Keys that all rows of the wave see: [all_from, all_to).
-  const int all_to = p.seen + r0 / a.group + 1;
-  const int all_from = max(p.seen + min(r0 + 31, rows - 1) / a.group + 1 - a.window, 0);
   const int first = static_cast<int>(static_cast<int64_t>(keys.tiles) * p.part / p.parts);
   const int last = static_cast<int>(static_cast<int64_t>(keys.tiles) * (p.part + 1) / p.parts);
-  const int32_t* pages = a.table + p.row * a.bt_stride;
-  for (int i = first; i < last; ++i) {
-    const int key = keys.first + i * C::kTile;
-    __syncthreads();
-    stage_tile<D>(a, pages, h, key, keys.end, lds);
-    __syncthreads();
-    if (!any) continue;
-    for (int t0 = narrow ? 32 * (wave & 1) : 0; t0 < C::kTile; t0 += narrow ? 64 : 32) {
-      if (key + t0 >= all_from && key + t0 + 32 <= all_to) {
-        attend<DT, D, false>(lds, q, st, t0, 0, 32, a.scale_log2);
-      } else if (key + t0 < keys.end) {
-        attend<DT, D, true>(lds, q, st, t0, lower - key - t0, max(limit - lower, 0), a.scale_log2);
-      }
+  if (first < last) {
+    const int key = keys.first + first * kTile, end = min(keys.end, keys.first + last * kTile);
+    const int32_t* table = a.table + p.row * a.bt_stride;
+    if (narrow) {
+      run_part<DT, D, WHOLE, 1>(a, table, h, key, end, last - first, w, q, st, 32 * (wave & 1), wave, lds);
+    } else {
+      run_part<DT, D, WHOLE, 2>(a, table, h, key, end, last - first, w, q, st, 0, wave, lds);
     }
   }
   st.l += other_half(st.l);
@@ -430,14 +594,14 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
     f32x4* area = reinterpret_cast<f32x4*>(lds) + block * kGroups * 64;
     float* sums = reinterpret_cast<float*>(reinterpret_cast<f32x4*>(lds) + 2 * kGroups * 64) + block * 128;
     __syncthreads();
-    if (any && (wave & 1)) {
+    if (w.any && (wave & 1)) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) area[g * 64 + lane] = group(g);
       sums[lane] = st.m;
       sums[64 + lane] = st.l;
     }
     __syncthreads();
-    if (!any || (wave & 1)) return;
+    if (!w.any || (wave & 1)) return;
     const float om = sums[lane], m = fmaxf(st.m, om);
     const float mine = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
     const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - m);
@@ -515,7 +679,7 @@ Bounds plan_bounds(int rows, int tokens, int num_q_heads, int num_kv_heads, int 
   b.pieces = cut * num_kv_heads;
   return b;
 }
-constexpr size_t kPlanHeader = 256;
+constexpr size_t kPlanHeader = sizeof(PlanHeader);
 size_t rounded(size_t n) { return (n + 255) & ~size_t{255}; }
 
 size_t chunk_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_heads, int d) {
@@ -529,7 +693,12 @@ size_t chunk_workspace_bytes(int rows, int tokens, int num_q_heads, int num_kv_h
 template <int DT, int D>
 int launch(hipStream_t stream, const ChunkArgs& a, const Bounds& b) {
   chunk_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
-  chunk_attention_kernel<DT, D><<<static_cast<int>(b.parts * a.hkv), Chunk<D>::kThreads, 0, stream>>>(a);
+  const int groups = static_cast<int>(b.parts * a.hkv);
+  if (a.block_size % Chunk<D>::kPerLoad == 0) {
+    chunk_attention_kernel<DT, D, true><<<groups, Chunk<D>::kThreads, 0, stream>>>(a);
+  } else {
+    chunk_attention_kernel<DT, D, false><<<groups, Chunk<D>::kThreads, 0, stream>>>(a);
+  }
   chunk_join_kernel<DT, D><<<dim3(static_cast<int>(b.joins), kItemRows / 32, a.hkv), 256, 0, stream>>>(a);
   return check_launch("ds_chunk_attention");
 }
@@ -597,7 +766,6 @@ int chunk_attention_impl(hipStream_t stream, const ds_chunk_attention_desc* d) {
   a.q_start = d->query_start, a.q_len = d->query_len, a.t_len = d->target_len;
   a.rows = d->rows, a.tokens = d->tokens, a.hkv = d->num_kv_heads, a.group = group;
   a.window = d->window ? std::min(d->window, 1 << 30) : 1 << 30;  // rows have at most 2^30 keys
-  a.tile = chunk_tile(d->head_dim);
   a.slots = part_slots(d->head_dim);
   a.scale_log2 = std::fabs(d->scale) * kLog2eP;
   a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
