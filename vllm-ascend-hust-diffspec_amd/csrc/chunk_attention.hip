@@ -16,6 +16,7 @@
 // chunk_join_kernel puts together.  chunk_plan_kernel derives items and parts from the lengths on the
 // device, so that a captured launch follows changed lengths, and lists them by size, the largest first.
 #include <cmath>
+#include <type_traits>
 
 #include "matrix.h"
 
@@ -82,7 +83,7 @@ struct ChunkArgs {
   int rows, tokens, hkv, group, window;
   int slots;          // workgroups that run at a time
   float scale_log2;   // |scale| log2 e
-  uint32_t q_sign;    // sign bits that a negative scale turns in the queries
+  uint32_t q_keep, q_sign;  // a scale of 0 clears the queries, the sign bits turn with a negative one
   PlanHeader* header;
   Part* parts;
   Part* joins;        // items of several parts
@@ -213,36 +214,60 @@ __device__ __forceinline__ int key_turn(int t) {
   return D == 64 ? (t >> 1) & 7 : t & 15;
 }
 
-// 64 lanes' 16 bytes each from base + offset to 1 KiB of shared memory from `to` on, a lane after the other.
-// The compiler does not know of the load: what reads that memory waits for it (wait_loads) before a barrier.
-// (It keeps nothing in m0 from one instruction to another.)
+// 64 lanes' 16 bytes each from base + offset to 1 KiB of shared memory from to + PLUS on, a lane after the
+// other.  The compiler does not know of the load: what reads that memory waits for it (wait_loads) before a
+// barrier.  (It keeps nothing in m0 from one instruction to another.)
+template <int PLUS>
 __device__ __forceinline__ void load_lds(uint64_t base, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
+               :
+               : "s"(to), "i"(PLUS), "v"(offset), "s"(base)
+               : "memory", "scc");
 }
+template <int PLUS>
 __device__ __forceinline__ void load_lds(uint64_t from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory");
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off"
+               :
+               : "s"(to), "i"(PLUS), "v"(from)
+               : "memory", "scc");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 
+// What the loop over keys needs of the arguments, for one KV head; the rest is read again behind it, so that
+// scalar registers last.
+struct Cache {
+  uint64_t k, v;  // of the KV head
+  int64_t k_block, v_block;
+  uint32_t k_token, v_token;
+  int num_blocks, block_size;
+  float per_block, scale_log2;
+  int32_t* status;
+  uint64_t zeros;
+};
+
 // (n + 0.5) / size in floating point gives the exact quotient for n < 2^22: the half keeps it away from
 // the integers by 0.5 / size, more than the 2^-23 relative error of a product with a rounded reciprocal.
-__device__ __forceinline__ int pages_in(const ChunkArgs& a, int n) {
+__device__ __forceinline__ int pages_in(const Cache& a, int n) {
   return static_cast<int>((static_cast<float>(n) + 0.5f) * a.per_block);
 }
 
-// A tile of a part's keys: where it begins, and (WHOLE) the places of a wave's loads.  One load of a wave
-// takes kPerLoad neighbouring keys; a part begins at a multiple of 32 keys, so where the page size is a
-// multiple of kPerLoad they lie in one page and the address is the wave's.  Lane i looks up the page of
-// the wave's load i.
+// A tile of a part's keys.  One load of a wave takes kPerLoad neighbouring keys; a part begins at a multiple
+// of 32 keys, so where the page size is a multiple of kPerLoad they lie in one page and the address is the
+// wave's (WHOLE): lane i looks up the page of load i, and computes its places in the caches.
 struct Tile {
   const int32_t* pages;  // the table entry of the first key's page
   int place;             // the first key in that page
   int left;              // keys from the first one to the part's end
   int page, in;          // lane i: of load i
 };
+struct Places {
+  uint64_t k, v;  // lane i: of load i
+  int bad;        // loads of keys past the part's end or of a page out of range
+  Tile tile;
+};
 
 template <int D, bool WHOLE>
-__device__ __forceinline__ void look_up(const ChunkArgs& a, int wave, Tile& x) {
+__device__ __forceinline__ void look_up(const Cache& a, int wave, Tile& x) {
   using C = Chunk<D>;
   if (!WHOLE || x.left <= 0) return;
   const int i = (fresh_thread() & 63) % C::kLoads;
@@ -252,47 +277,82 @@ __device__ __forceinline__ void look_up(const ChunkArgs& a, int wave, Tile& x) {
   x.page = x.pages[index];
 }
 
-__device__ __forceinline__ void advance(const ChunkArgs& a, Tile& x) {
+template <int D, bool WHOLE>
+__device__ __forceinline__ Places find_places(const Cache& a, const Tile& x, int wave) {
+  using C = Chunk<D>;
+  Places p{0, 0, 0, x};
+  if (!WHOLE || x.left <= 0) return p;
+  const int lane = fresh_thread() & 63, t = (wave * C::kLoads + lane) * C::kPerLoad;
+  const bool exists = static_cast<unsigned>(x.page) < static_cast<unsigned>(a.num_blocks);
+  constexpr int kAll = (1 << C::kLoads) - 1;
+  p.bad = static_cast<int>(__ballot(!exists || t >= x.left)) & kAll;
+  const uint32_t page = exists ? x.page : 0, in = x.in;
+  p.k = a.k + page * a.k_block + in * a.k_token;
+  p.v = a.v + page * a.v_block + in * a.v_token;
+  return p;
+}
+
+__device__ __forceinline__ void advance(const Cache& a, Tile& x) {
   const int n = uniform(pages_in(a, x.place + kTile));
   x.left -= kTile;
   x.pages += n;
   x.place += kTile - n * a.block_size;
 }
 
-// Sends the wave's part of a tile's keys (or values) to shared memory; zeros for loads past the part's end and
-// for keys of a page out of range.
-template <int D, bool WHOLE, bool VALUES>
-__device__ __forceinline__ void send(const ChunkArgs& a, const Tile& x, int head, int wave, uint32_t to) {
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int i) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), i);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), i);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// Where a lane's piece of load i lies after the load's first key, in bytes.  (The turns of the pieces repeat
+// every 16 keys, which a wave's loads are a multiple of apart.)
+template <int D, bool VALUES>
+__device__ __forceinline__ uint32_t piece_offset(const Cache& a, int lane, int i) {
   using C = Chunk<D>;
-  if (x.left <= 0) return;
-  const int lane = fresh_thread() & 63, piece = lane % C::kPieces, mine = lane / C::kPieces;
-  const uint64_t zeros = reinterpret_cast<uint64_t>(a.header->zeros);
-  const uint64_t cache = reinterpret_cast<uint64_t>(VALUES ? a.v : a.k);
-  const int64_t block_bytes = VALUES ? a.v_block : a.k_block;
-  const uint32_t token_bytes = VALUES ? a.v_token : a.k_token, head_bytes = head * (VALUES ? a.v_head : a.k_head);
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < C::kLoads; ++i) {
-    const int t = (wave * C::kLoads + i) * C::kPerLoad, key = t + mine;
-    const uint32_t turned = 16 * (VALUES ? piece_at<D>(key, piece) - key * C::kPieces : piece ^ key_turn<D>(key));
-    if constexpr (WHOLE) {
-      const int page = __builtin_amdgcn_readlane(x.page, i), in = __builtin_amdgcn_readlane(x.in, i);
-      const bool fine = t < x.left && static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
-      bad |= t < x.left && !fine;
-      const uint64_t base = cache + page * block_bytes + (in * token_bytes + head_bytes);
-      const uint32_t mask = fine ? ~0u : 0u;
-      load_lds(zeros ^ ((base ^ zeros) & (static_cast<uint64_t>(mask) << 32 | mask)), (mine * token_bytes + turned) & mask,
-               to + t * C::kRowBytes);
-    } else {
-      const int n = x.place + min(key, x.left - 1), index = pages_in(a, n), page = x.pages[index];
-      const uint32_t in = n - index * a.block_size;
-      const bool fine = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
-      bad |= !fine;
-      load_lds(fine ? cache + page * block_bytes + (in * token_bytes + head_bytes) + turned : zeros, to + t * C::kRowBytes);
-    }
+  const int piece = lane % C::kPieces, mine = lane / C::kPieces, key = (i * C::kPerLoad + mine) % 16;
+  return mine * (VALUES ? a.v_token : a.k_token) +
+         16 * (VALUES ? piece_at<D>(key, piece) - key * C::kPieces : piece ^ key_turn<D>(key));
+}
+
+template <int D, bool VALUES, int I = 0>
+__device__ __forceinline__ void send_whole(uint64_t place, const uint32_t (&offset)[Chunk<D>::kLoads], uint32_t to) {
+  using C = Chunk<D>;
+  if constexpr (I < C::kLoads) {
+    load_lds<I * C::kPerLoad * C::kRowBytes>(lane_value(place, I), offset[I], to);
+    send_whole<D, VALUES, I + 1>(place, offset, to);
   }
-  if (bad && a.status) {
-    __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// A page a lane; zeros for loads past the part's end and for keys of a page out of range.
+template <int D, bool VALUES>
+__device__ __forceinline__ void send_lanes(const Cache& a, const Tile& x, int wave, uint32_t to) {
+  using C = Chunk<D>;
+  const int lane = fresh_thread() & 63;
+#pragma unroll 1
+  for (int i = 0; i < C::kLoads; ++i) {
+    const int first = (wave * C::kLoads + i) * C::kPerLoad, key = first + lane / C::kPieces;
+    const int n = x.place + min(key, x.left - 1), index = pages_in(a, n), page = x.pages[index];
+    const uint32_t token_bytes = VALUES ? a.v_token : a.k_token, in = n - index * a.block_size;
+    const bool exists = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
+    if (!exists && a.status) {
+      __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    const uint64_t from = (VALUES ? a.v : a.k) + page * (VALUES ? a.v_block : a.k_block) + in * token_bytes +
+                          (piece_offset<D, VALUES>(a, lane, i) - lane / C::kPieces * token_bytes);
+    load_lds<0>(exists && first < x.left ? from : a.zeros, uniform(to + i * C::kPerLoad * C::kRowBytes));
+  }
+}
+
+// Sends the wave's part of a tile's keys (or values) to shared memory.
+template <int D, bool WHOLE, bool VALUES>
+__device__ __forceinline__ void send(const Cache& a, const Places& p, const uint32_t (&offset)[Chunk<D>::kLoads], int wave,
+                                     uint32_t to) {
+  if (p.tile.left <= 0) return;
+  if (WHOLE && p.bad == 0) {
+    send_whole<D, VALUES>(VALUES ? p.v : p.k, offset, to);
+  } else {
+    send_lanes<D, VALUES>(a, p.tile, wave, to);
   }
 }
 
@@ -305,76 +365,100 @@ struct Softmax {
 };
 
 // A masked key of a tile may hold infinities or NaN, which a probability of 0 does not cancel in the
-// product, while another column sees that key.  The product then takes such values as 0, and they
-// are added to the columns that see them (where the sum is no longer finite whatever the weight): key t0 + t
-// is seen where from <= t < from + count.
+// product, while another column sees that key.  In tiles with a mask such values are replaced by 0 in
+// shared memory, before a barrier, each wave those that it sent; returns whether there was one.
 template <int DT, int D>
-__device__ __forceinline__ void add_not_finite(const char* values_at, Softmax<D>& st, int t0, int from, unsigned count) {
+__device__ __forceinline__ bool clear_not_finite(char* values, int wave) {
+  using C = Chunk<D>;
   constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
-  const u32x4* values = reinterpret_cast<const u32x4*>(values_at);
+  u32x4* mine = reinterpret_cast<u32x4*>(values) + wave * C::kLoads * 64 + (fresh_thread() & 63);
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < C::kLoads; ++i) {
+    u32x4 x = mine[64 * i];
+    bool found = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) found |= not_finite2(x[e], kExponent);
+    if (found) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] &= ((x[e] & kExponent) == kExponent ? 0u : 0xffffu) |
+                ((x[e] & (kExponent << 16)) == (kExponent << 16) ? 0u : 0xffff0000u);
+      }
+      mine[64 * i] = x;
+    }
+    any |= found;
+  }
+  return __any(any);
+}
+
+// The values that were left out, from the cache, added to the columns that see them (where the sum is no
+// longer finite whatever the weight): of `keys` keys from place `place` on, the lane column's query row sees
+// key t where from <= t < from + count.
+template <int DT, int D>
+__device__ __forceinline__ void add_not_finite(const Cache& a, const int32_t* pages, int place, int keys, Softmax<D>& st,
+                                               int from, unsigned count) {
+  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
   const int half = (fresh_thread() >> 5) & 1;
 #pragma unroll 1
-  for (int t = 0; t < 32; ++t) {
+  for (int t = 0; t < keys; ++t) {
+    const int index = pages_in(a, place + t), page = pages[index];
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_blocks)) continue;
+    const uint64_t at = a.v + page * a.v_block + (place + t - index * a.block_size) * a.v_token + 8 * half;
     const bool sees = static_cast<unsigned>(t - from) < count;
 #pragma unroll
     for (int j = 0; j < Chunk<D>::kBlocks; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const u32x2 v = reinterpret_cast<const u32x2*>(values + piece_at<D>(t0 + t, 4 * j + i))[half];
+        const u32x2 v = *reinterpret_cast<const u32x2*>(at + 64 * j + 16 * i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint16_t x = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
           if (sees && (x & kExponent) == kExponent) st.acc[j][4 * i + e] += Elem<DT>::load(x);
         }
+        __builtin_amdgcn_sched_barrier(0);  // or the conditions of all values are held at once
       }
     }
   }
 }
 
-// Scores of 32 keys from key t0 of the tile on.
-template <int DT, int D>
-__device__ __forceinline__ f32x16 score(const char* keys, const u32x4 (&q)[Chunk<D>::kSteps], int t0) {
+// Scores of 32 N keys from key t0 of the tile on.  (Piece 2 s + half of a key is turned as piece `half` is, and 2 s
+// then differs in bits of its own; the turn repeats every 16 keys.)
+template <int DT, int D, int N>
+__device__ __forceinline__ void score(const char* keys, const u32x4 (&q)[Chunk<D>::kSteps], int t0, f32x16 (&sc)[N]) {
   using C = Chunk<D>;
-  const int lane = threadIdx.x & 63, half = lane >> 5, t = t0 + (lane & 31);
-  f32x16 sc;
+  const int lane = fresh_thread() & 63, half = lane >> 5, t = lane & 31;
+  const uint32_t at = (t0 + t) * C::kRowBytes + 16 * (half ^ key_turn<D>(t));
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+  for (int n = 0; n < N; ++n) {
 #pragma unroll
-  for (int s = 0; s < C::kSteps; ++s) {
-    sc = mfma32<DT>(*reinterpret_cast<const u32x4*>(keys + t * C::kRowBytes + 16 * ((2 * s + half) ^ key_turn<D>(lane & 31))),
-                    q[s], sc);
+    for (int i = 0; i < 16; ++i) sc[n][i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < C::kSteps; ++s) {
+      sc[n] = mfma32<DT>(*reinterpret_cast<const u32x4*>(keys + (at ^ (32 * s)) + 32 * n * C::kRowBytes), q[s], sc[n]);
+    }
   }
-  return sc;
 }
 
-// One tile for one wave: 32 N keys from key t0 of it on, whose scores are in `sc`; `next` gets those of the
-// next tile (unless LAST), whose products run while the weights are computed.  MASKED: the lane column's
-// query row sees those t of the keys with from <= t < from + count.
-template <int DT, int D, int N, bool MASKED, bool LAST>
+// One tile for one wave: 32 N keys from key t0 of it on, whose scores are in `sc`; it then gets those of the
+// next tile, whose products run while the weights are computed.
+template <int DT, int D, int N>
 __device__ __forceinline__ void attend(const char* next_keys, const char* values, const u32x4 (&q)[Chunk<D>::kSteps],
-                                       Softmax<D>& st, f32x16 (&sc)[N], int t0, int from, unsigned count,
-                                       float scale_log2) {
+                                       Softmax<D>& st, f32x16 (&sc)[N], int t0, float scale_log2) {
   using C = Chunk<D>;
-  constexpr uint32_t kExponent = DT == DS_BF16 ? 0x7f80u : 0x7c00u;
-  const int lane = threadIdx.x & 63, half = lane >> 5, l = lane & 15;
-  // Masked scores are no part of the maximum, and their weights are 0 as such: -infinity times a scale of 0
-  // is none.
-  auto sees = [&](int n, int i) {
-    return !MASKED || static_cast<unsigned>(32 * n + 8 * (i >> 2) + (i & 3) + 4 * half - from) < count;
-  };
+  const int lane = fresh_thread() & 63, half = lane >> 5, l = lane & 15;
   float top = -INFINITY;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, sees(n, i) ? sc[n][i] : -INFINITY);
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[n][i]);
   }
   // The reference of the exponents follows the maximum only when it is 2^8 behind: weights of up to 2^8
   // keep their relative precision, and most tiles leave the sums as they are.  In fp16 it stays 2^7 below
   // the maximum, so that weights lie in 2^-24 .. 2^15 of the type: those of a long tail of small
   // probabilities are then rounded relative to themselves down to 2^-21 of the largest.
   constexpr float kBelow = DT == DS_FP16 ? 7.f : 0.f;
-  top = fmaxf(top, other_half(top));
-  if (!MASKED || top != -INFINITY) top = __builtin_fmaf(top, scale_log2, -kBelow);
+  top = __builtin_fmaf(fmaxf(top, other_half(top)), scale_log2, -kBelow);
   if (__any(top > st.m + 8.f)) {
     const float m = fmaxf(st.m, top);
     const float keep = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
@@ -388,17 +472,14 @@ __device__ __forceinline__ void attend(const char* next_keys, const char* values
   }
   const float m = st.m == -INFINITY ? 0.f : st.m;
   f32x16 next[N];
-  if constexpr (!LAST) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) next[n] = score<DT, D>(next_keys, q, t0 + 32 * n);
-  }
+  score<DT, D, N>(next_keys, q, t0, next);
   u32x4 p[2 * N];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
-      const float x = sees(n, i) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i], scale_log2, -m)) : 0.f;
-      const float y = sees(n, i + 1) ? __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i + 1], scale_log2, -m)) : 0.f;
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i], scale_log2, -m));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i + 1], scale_log2, -m));
       // The product's operands are 16 bits, so the probabilities are rounded for it; the sum is of them as
       // computed, since the LSE is an fp32 output.
       st.l += x + y;
@@ -409,37 +490,17 @@ __device__ __forceinline__ void attend(const char* next_keys, const char* values
   // 4) + 4 half + e % 4 of the keys, and the values are read in that order.
   const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)values)) + t0 * C::kRowBytes +
                         8 * (l & 1) + 16 * piece_at<D>(4 * half + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1));
-  uint32_t poison = 0;  // the 32 keys with a value that is not finite
 #pragma unroll
   for (int s = 0; s < 2 * N; ++s) {
 #pragma unroll
     for (int j = 0; j < C::kBlocks; ++j) {
       const u32x2 lo = read_values((base ^ (64 * j)) + 16 * s * C::kRowBytes);
       const u32x2 hi = read_values((base ^ (64 * j)) + (16 * s + 8) * C::kRowBytes);
-      u32x4 x{lo[0], lo[1], hi[0], hi[1]};
-      if constexpr (MASKED) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool a0 = (x[e] & kExponent) == kExponent, a1 = (x[e] & (kExponent << 16)) == (kExponent << 16);
-          poison |= a0 || a1 ? 1u << (s >> 1) : 0u;
-          x[e] &= (a0 ? 0u : 0xffffu) | (a1 ? 0u : 0xffff0000u);
-        }
-      }
-      st.acc[j] = mfma32<DT>(x, p[s], st.acc[j]);
+      st.acc[j] = mfma32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, p[s], st.acc[j]);
     }
   }
-  if constexpr (MASKED) {
-    if (__any(poison != 0)) {
-#pragma unroll 1
-      for (int n = 0; n < N; ++n) {
-        if (__any((poison >> n) & 1)) add_not_finite<DT, D>(values, st, t0 + 32 * n, from - 32 * n, count);
-      }
-    }
-  }
-  if constexpr (!LAST) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) sc[n] = next[n];
-  }
+  for (int n = 0; n < N; ++n) sc[n] = next[n];
 }
 
 // A wave's place in its item.
@@ -447,75 +508,88 @@ struct Rows {
   bool any;              // it has query rows
   int limit, lower;      // keys that the lane column's row sees: lower <= t < limit
   int all_from, all_to;  // keys that all its rows see
+  int item_from, item_to;  // keys that all rows of the item see
 };
 
 // The part's tiles of keys, `tiles` from key `key` on, 32 N keys of each for a wave.  In shared memory the keys
 // run a tile ahead of the values: while a tile is weighed, the next one's scores are computed, the keys
 // after that and the next values are on their way, and the pages of the keys behind them are looked up.
 template <int DT, int D, bool WHOLE, int N>
-__device__ __forceinline__ void run_part(const ChunkArgs& a, const int32_t* table, int head, int key, int end, int tiles,
-                                         const Rows& rows, const u32x4 (&q)[Chunk<D>::kSteps], Softmax<D>& st, int t0,
-                                         int wave, char* lds) {
+__device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, int key, int end, int tiles, const Rows& rows,
+                                         const u32x4 (&q)[Chunk<D>::kSteps], Softmax<D>& st, int t0,
+                                         int wave, char* lds, int (&poison)[2][4]) {
   using C = Chunk<D>;
-  const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)lds));
+  const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)lds)) +
+                      wave * C::kLoads * C::kPerLoad * C::kRowBytes;
+  uint32_t k_offset[C::kLoads], v_offset[C::kLoads];
+#pragma unroll
+  for (int i = 0; i < C::kLoads; ++i) {
+    k_offset[i] = piece_offset<D, false>(a, threadIdx.x & 63, i);
+    v_offset[i] = piece_offset<D, true>(a, threadIdx.x & 63, i);
+  }
   const int index = uniform(key / a.block_size);
   Tile x{table + index, key - index * a.block_size, end - key, 0, 0};
-  look_up<D, WHOLE>(a, wave, x);
-  send<D, WHOLE, false>(a, x, head, wave, lds_at);
-  Tile v = x;
-  advance(a, x);
-  look_up<D, WHOLE>(a, wave, x);
-  wait_loads();
-  lds_barrier();
-  send<D, WHOLE, true>(a, v, head, wave, lds_at + 2 * C::kStage);
-  send<D, WHOLE, false>(a, x, head, wave, lds_at + C::kStage);
-  v = x;
-  advance(a, x);
-  look_up<D, WHOLE>(a, wave, x);
-  f32x16 sc[N];
-  if (rows.any) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) sc[n] = score<DT, D>(lds, q, t0 + 32 * n);
-  }
-  int i = 0;  // the tile, and its half of shared memory
-  auto turn = [&]() {
-    wait_loads();
-    lds_barrier();
-    const int here = i & 1;
-    send<D, WHOLE, false>(a, x, head, wave, lds_at + here * C::kStage);
-    send<D, WHOLE, true>(a, v, head, wave, lds_at + (2 + (here ^ 1)) * C::kStage);
-    v = x;
+  Places p;
+  auto send_keys = [&](int half) {
+    p = find_places<D, WHOLE>(a, x, wave);
+    send<D, WHOLE, false>(a, p, k_offset, wave, to + half * C::kStage);
+  };
+  auto send_values = [&](int half) { send<D, WHOLE, true>(a, p, v_offset, wave, to + (2 + half) * C::kStage); };
+  auto ahead = [&]() {
     advance(a, x);
     look_up<D, WHOLE>(a, wave, x);
-    return here;
   };
+  look_up<D, WHOLE>(a, wave, x);
+  send_keys(0);
+  ahead();
+  wait_loads();
+  lds_barrier();
+  send_values(0);
+  send_keys(1);
+  ahead();
+  f32x16 sc[N];
+  if (rows.any) score<DT, D, N>(lds, q, t0, sc);
   const unsigned count = max(rows.limit - rows.lower, 0);
-  if (!rows.any) {
-    for (; i < tiles; ++i) turn();
-    return;
-  }
-  // Tiles with a mask (of a window), those that all rows see whole, those with a mask; the last one.
-  const int whole_from = min(max(ceil_div(max(rows.all_from - key - t0, 0), kTile), 0), tiles - 1);
-  const int whole_to = max(min(max(rows.all_to - key - t0 + kTile - 32 * N, 0) / kTile, tiles - 1), whole_from);
-  for (;;) {
-    const int stop = i < whole_from ? whole_from : tiles - 1;
-    if (i >= whole_from) {
-      for (; i < whole_to; ++i) {
-        const int here = turn();
-        attend<DT, D, N, false, false>(lds + (here ^ 1) * C::kStage, lds + (2 + here) * C::kStage, q, st, sc, t0, 0, 0,
-                                       a.scale_log2);
+  for (int i = 0; i < tiles; ++i, key += kTile) {
+    const int here = i & 1;  // the tile's half of shared memory
+    wait_loads();
+    char* values = lds + (2 + here) * C::kStage;
+    if (key < rows.item_from || key + kTile > rows.item_to) {
+      const bool found = clear_not_finite<DT, D>(values, wave);
+      if ((fresh_thread() & 63) == 0) poison[here][wave] = found;
+    }
+    lds_barrier();
+    send_values(here ^ 1);
+    send_keys(here);
+    ahead();
+    if (!rows.any) continue;
+    const int at = key + t0;
+    if (at < rows.all_from || at + 32 * N > rows.all_to) {
+      const int from = rows.lower - at, half = (fresh_thread() >> 5) & 1;
+      if (__any(poison[here][fresh_thread() & 3])) {
+        const int page = at / a.block_size;
+        add_not_finite<DT, D>(a, table + page, at - page * a.block_size, min(32 * N, end - at), st, from, count);
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (static_cast<unsigned>(32 * n + 8 * (e >> 2) + (e & 3) + 4 * half - from) >= count) sc[n][e] = -INFINITY;
+        }
       }
     }
-    for (; i < stop; ++i) {
-      const int here = turn();
-      attend<DT, D, N, true, false>(lds + (here ^ 1) * C::kStage, lds + (2 + here) * C::kStage, q, st, sc, t0,
-                                    rows.lower - key - i * kTile - t0, count, a.scale_log2);
-    }
-    if (i >= tiles - 1) break;
+    attend<DT, D, N>(lds + (here ^ 1) * C::kStage, values, q, st, sc, t0, a.scale_log2);
   }
-  const int here = turn();
-  attend<DT, D, N, true, true>(nullptr, lds + (2 + here) * C::kStage, q, st, sc, t0, rows.lower - key - i * kTile - t0, count,
-                               a.scale_log2);
+}
+
+// The kernel's arguments, read again.
+__device__ __forceinline__ ChunkArgs arguments() {
+  typedef const __attribute__((address_space(4))) ChunkArgs* pointer;
+  pointer at = (pointer)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  ChunkArgs a;
+  __builtin_memcpy(&a, (const void*)at, sizeof(a));
+  return a;
 }
 
 // A piece in the workspace: 128 maxima and 128 sums, then the outputs as the waves hold them
@@ -540,6 +614,7 @@ template <int DT, int D, bool WHOLE>
 __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_attention_kernel(ChunkArgs a) {
   using C = Chunk<D>;
   __shared__ __attribute__((aligned(512))) char lds[4 * C::kStage];
+  __shared__ int poison[2][4];
   const int entry = blockIdx.x / a.hkv, h = blockIdx.x - entry * a.hkv;
   if (entry >= a.header->parts) return;
   const Part p = a.parts[entry];
@@ -556,11 +631,13 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
   w.lower = max(w.limit - a.window, 0);
   w.all_to = p.seen + r0 / a.group + 1;
   w.all_from = max(p.seen + min(r0 + 31, rows - 1) / a.group + 1 - a.window, 0);
+  w.item_to = p.seen + p.tile * kItemRows / a.group + 1;
+  w.item_from = max(p.seen + (min((p.tile + 1) * kItemRows, rows) - 1) / a.group + 1 - a.window, 0);
   u32x4 q[C::kSteps];
   {
     const uint16_t* src = a.q + (p.start + token) * a.q_row + head * a.q_head + 8 * half;
 #pragma unroll
-    for (int s = 0; s < C::kSteps; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + 16 * s) ^ a.q_sign;
+    for (int s = 0; s < C::kSteps; ++s) q[s] = (*reinterpret_cast<const u32x4*>(src + 16 * s) & a.q_keep) ^ a.q_sign;
   }
   Softmax<D> st;
 #pragma unroll
@@ -576,10 +653,14 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
   if (first < last) {
     const int key = keys.first + first * kTile, end = min(keys.end, keys.first + last * kTile);
     const int32_t* table = a.table + p.row * a.bt_stride;
+    const Cache cache{reinterpret_cast<uint64_t>(a.k) + h * a.k_head, reinterpret_cast<uint64_t>(a.v) + h * a.v_head,
+                      a.k_block, a.v_block, static_cast<uint32_t>(a.k_token), static_cast<uint32_t>(a.v_token),
+                      a.num_blocks, a.block_size, a.per_block, a.scale_log2, a.status,
+                      reinterpret_cast<uint64_t>(a.header->zeros)};
     if (narrow) {
-      run_part<DT, D, WHOLE, 1>(a, table, h, key, end, last - first, w, q, st, 32 * (wave & 1), wave, lds);
+      run_part<DT, D, WHOLE, 1>(cache, table, key, end, last - first, w, q, st, 32 * (wave & 1), wave, lds, poison);
     } else {
-      run_part<DT, D, WHOLE, 2>(a, table, h, key, end, last - first, w, q, st, 0, wave, lds);
+      run_part<DT, D, WHOLE, 2>(cache, table, key, end, last - first, w, q, st, 0, wave, lds, poison);
     }
   }
   st.l += other_half(st.l);
@@ -615,13 +696,14 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
     }
   }
   if (r >= rows) return;
+  const ChunkArgs z = arguments();
   if (p.parts == 1) {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) store_out<DT>(a, p.start + token, head, 8 * g + 4 * half, group(g), st.l);
-    if (half == 0) store_lse(a, p.start + token, head, st.m, st.l);
+    for (int g = 0; g < kGroups; ++g) store_out<DT>(z, p.start + token, head, 8 * g + 4 * half, group(g), st.l);
+    if (half == 0) store_lse(z, p.start + token, head, st.m, st.l);
     return;
   }
-  float* sums = piece_at_slot<D>(a, (p.slot + p.part) * a.hkv + h);
+  float* sums = piece_at_slot<D>(z, (p.slot + p.part) * z.hkv + h);
   if (half == 0) {
     sums[32 * block + lane] = st.m;
     sums[kItemRows + 32 * block + lane] = st.l;
@@ -767,7 +849,9 @@ int chunk_attention_impl(hipStream_t stream, const ds_chunk_attention_desc* d) {
   a.rows = d->rows, a.tokens = d->tokens, a.hkv = d->num_kv_heads, a.group = group;
   a.window = d->window ? std::min(d->window, 1 << 30) : 1 << 30;  // rows have at most 2^30 keys
   a.slots = part_slots(d->head_dim);
-  a.scale_log2 = std::fabs(d->scale) * kLog2eP;
+  // Masked scores are -infinity, which a scale of 0 must not meet.
+  a.scale_log2 = d->scale == 0.f ? 1.f : std::fabs(d->scale) * kLog2eP;
+  a.q_keep = d->scale == 0.f ? 0u : ~0u;
   a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
   char* work = static_cast<char*>(d->workspace);
   a.header = reinterpret_cast<PlanHeader*>(work);
