@@ -7,10 +7,10 @@
 //                   the query heads g of KV head h, of exp(scale q_ig . k_t - lse_ig).
 //
 // The probabilities are those of the attention, so the keys are read once more, and the values not at all.
-// A wave holds 64 keys (32 of 256 dimensions) in registers as the columns of the score product, and the
-// query rows (row = token * group + head in the group) go by in shared memory, 64 at a time.  A lane's
-// results are then 16 query rows of its own key, and the sum over the rows is the lane's own.  Tiles of
-// keys with many query rows are cut into parts of the rows, whose sums mass_join_kernel adds up in order.
+// A wave holds 32 keys in registers as the columns of the score product, and the query rows (row = token *
+// group + head in the group) go by in shared memory, 32 at a time.  A lane's results are then 16 query rows
+// of its own key, and the sum over the rows is the lane's own.  Tiles of keys with many query rows are cut
+// into parts of the rows, whose sums mass_join_kernel adds up in order.
 #include <cmath>
 
 #include "matrix.h"
@@ -18,27 +18,27 @@
 namespace ds355 {
 namespace {
 
-constexpr int kQueryRows = 64;  // staged query rows
-constexpr int kMinPart = 4;     // staged tiles below which the query rows are not cut
+constexpr int kQueryRows = 32;  // staged query rows, a block
+constexpr int kMinPart = 8;     // blocks below which the query rows are not cut
 constexpr int kPartsPerSlot = 4;
 constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table or its mass
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
-constexpr int kWaves = 4;
-constexpr int wave_keys(int d) { return d <= 128 ? 64 : 32; }
-constexpr int mass_tile(int d) { return kWaves * wave_keys(d); }
-constexpr int kMostKeys = 256;  // keys of a tile, at most
-int mass_slots() { return 2 * device_cu_count(); }  // workgroups that run at a time
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kTile = 32 * kWaves;  // keys of a workgroup
+constexpr int mass_groups(int d) { return d == 64 ? 4 : d == 128 ? 3 : 1; }  // workgroups of a CU
+constexpr int kMostGroups = 4;
 
 template <int D>
 struct Mass {
-  static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kTile = mass_tile(D);
-  static constexpr int kColumns = wave_keys(D) / 32;  // blocks of 32 keys of a wave
   static constexpr int kRowBytes = 2 * D;
   static constexpr int kPieces = D / 8;
   static constexpr int kSteps = D / 16;
+  static constexpr int kPerLoad = 64 / kPieces;                      // keys or rows that one load of a wave covers
+  static constexpr int kKeyLoads = 32 / kPerLoad;                    // such loads for a wave's keys
+  static constexpr int kRowLoads = kQueryRows / kPerLoad / kWaves;   // and for its part of the staged query rows
+  static constexpr int kBlockBytes = kQueryRows * kRowBytes;
 };
 
 struct MassArgs {
@@ -60,94 +60,72 @@ struct MassArgs {
   const int32_t* q_len;
   const int32_t* t_len;
   int rows, tokens, hkv, group, window;
-  int tile;  // keys of a tile
-  int slots;
-  float scale_log2;  // |scale| log2 e
-  uint32_t q_sign;   // sign bits that a negative scale turns in the queries
+  int slots;         // workgroups that run at a time
+  float scale_log2;  // scale log2 e
   float decay;
-  float* partial;  // [parts of cut tiles][KV head][kMostKeys]
+  float* partial;  // [parts of cut tiles][KV head][kTile]
   int32_t* status;
 };
 
 // ---------------------------------------------------------------------------------------------
 // The layout of the work, derived by every workgroup from the lengths.
 // ---------------------------------------------------------------------------------------------
-struct Row {
-  int start, len, keys;
-};
-__device__ __forceinline__ Row row_of(const MassArgs& a, int b, bool report) {
-  Row r{a.q_start[b], a.q_len[b], a.t_len[b]};
-  uint32_t bits = 0;
-  if (r.len <= 0) {
-    r.len = 0;
-  } else if (r.start < 0 || r.len > a.tokens || r.start > a.tokens - r.len) {
-    r.len = 0;
-    bits |= kStatusRow;
-  }
-  if (r.keys > a.capacity) bits |= kStatusLength;
-  if (bits && report && a.status) {
-    __hip_atomic_fetch_or(a.status, static_cast<int>(bits), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  r.keys = r.len ? min(max(r.keys, 0), a.capacity) : 0;
-  return r;
-}
-
+// Tables in shared memory, of as many rows as there are.
 struct Layout {
-  int first[kMaxRows + 1];  // parts of the rows before, of one KV head
-  int cut[kMaxRows + 1];    // those of them that are one of several of a tile
-  int cap;                  // staged tiles of a part, at most
+  int *first;  // parts of the rows before, of one KV head
+  int *cut;    // those of them that are one of several of a tile
+  int *start, *len, *keys;
+  int rows, cap;  // cap: blocks of a part, at most
 };
+constexpr int layout_bytes(int rows) { return 4 * (5 * rows + 2); }
 
-// Parts of each tile of the row.
+// Parts of each tile of a row.
 __device__ __forceinline__ int row_parts(const MassArgs& a, int len, int cap) {
   return max(ceil_div(ceil_div(len * a.group, kQueryRows), cap), 1);
 }
 
-__device__ __forceinline__ void make_layout(const MassArgs& a, Layout& y, bool report) {
+__device__ __forceinline__ Layout make_layout(const MassArgs& a, int* memory, bool report) {
   __shared__ int scratch[4];
   __shared__ unsigned long long work;
+  Layout y{memory, memory + a.rows + 1, memory + 2 * a.rows + 2, memory + 3 * a.rows + 2, memory + 4 * a.rows + 2, a.rows, 0};
   if (threadIdx.x == 0) work = 0;
   __syncthreads();
   unsigned long long mine = 0;
-  for (int b = threadIdx.x; b < a.rows; b += blockDim.x) {
-    const Row r = row_of(a, b, report);
-    mine += static_cast<unsigned long long>(ceil_div(r.keys, a.tile)) * ceil_div(r.len * a.group, kQueryRows);
+  for (int b = threadIdx.x; b < a.rows; b += kThreads) {
+    int start = a.q_start[b], len = a.q_len[b], keys = a.t_len[b];
+    uint32_t bits = keys > a.capacity ? kStatusLength : 0;
+    if (len <= 0) {
+      len = 0;
+    } else if (start < 0 || len > a.tokens || start > a.tokens - len) {
+      len = 0;
+      bits |= kStatusRow;
+    }
+    if (bits && report && a.status) {
+      __hip_atomic_fetch_or(a.status, static_cast<int>(bits), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    keys = len ? min(max(keys, 0), a.capacity) : 0;
+    y.start[b] = start, y.len[b] = len, y.keys[b] = keys;
+    mine += static_cast<unsigned long long>(ceil_div(keys, kTile)) * ceil_div(len * a.group, kQueryRows);
   }
   if (mine) atomicAdd(&work, mine);
   __syncthreads();
   const unsigned long long most = static_cast<unsigned long long>(kPartsPerSlot) * a.slots;
   const unsigned long long share = (work * a.hkv + most - 1) / most;
-  const int cap = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart)), 1ull << 25));
-  if (threadIdx.x == 0) y.cap = cap;
-  build_row_prefix(a.rows, y.first, scratch, [&](int b) {
-    const Row r = row_of(a, b, false);
-    return ceil_div(r.keys, a.tile) * row_parts(a, r.len, cap);
-  });
+  y.cap = uniform(static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart)), 1ull << 25)));
+  build_row_prefix(a.rows, y.first, scratch, [&](int b) { return ceil_div(y.keys[b], kTile) * row_parts(a, y.len[b], y.cap); });
   build_row_prefix(a.rows, y.cut, scratch, [&](int b) {
-    const Row r = row_of(a, b, false);
-    const int parts = row_parts(a, r.len, cap);
-    return parts > 1 ? ceil_div(r.keys, a.tile) * parts : 0;
+    const int parts = row_parts(a, y.len[b], y.cap);
+    return parts > 1 ? ceil_div(y.keys[b], kTile) * parts : 0;
   });
+  return y;
 }
 
-// One part: a tile of a row's keys, and which of its query rows.
+// One part: a tile of a row's keys for one KV head, and which of its query rows.
 struct Part {
-  int row, start, len, keys, seen;
+  int head, row, start, len, keys, seen;
   int tile, part, parts, slot;
+  int begin, end;  // blocks of query rows
 };
-__device__ __forceinline__ Part part_at(const MassArgs& a, const Layout& y, int i) {
-  Part p;
-  p.row = uniform(find_row(y.first, a.rows, i));
-  const Row r = row_of(a, p.row, false);
-  p.start = uniform(r.start), p.len = uniform(r.len), p.keys = uniform(r.keys);
-  p.seen = p.keys - p.len;
-  p.parts = row_parts(a, p.len, uniform(y.cap));
-  const int in_row = i - uniform(y.first[p.row]);
-  p.tile = in_row / p.parts;
-  p.part = in_row - p.tile * p.parts;
-  p.slot = uniform(y.cut[p.row]) + in_row;
-  return p;
-}
 
 // Query rows that see key t: [from, to) (rows hold at most 2^29 keys, and windows count as no more).
 __device__ __forceinline__ int first_row(const MassArgs& a, const Part& p, int t) {
@@ -157,147 +135,246 @@ __device__ __forceinline__ int end_row(const MassArgs& a, const Part& p, int t) 
   return min(max(t - p.seen + a.window, 0), p.len) * a.group;
 }
 
-template <int D>
-__device__ __forceinline__ int row_turn(int t) {
-  return D == 64 ? (t >> 1) & 7 : t & 15;
+__device__ __forceinline__ Part part_at(const MassArgs& a, const Layout& y, int entry, int head) {
+  Part p;
+  p.head = head;
+  p.row = uniform(find_row(y.first, y.rows, entry));
+  p.start = uniform(y.start[p.row]), p.len = uniform(y.len[p.row]), p.keys = uniform(y.keys[p.row]);
+  p.seen = p.keys - p.len;
+  p.parts = row_parts(a, p.len, y.cap);
+  const int in_row = entry - uniform(y.first[p.row]);
+  p.tile = in_row / p.parts;
+  p.part = in_row - p.tile * p.parts;
+  p.slot = uniform(y.cut[p.row]) + in_row;
+  // The blocks of query rows that see some key of the tile, and the part's share of them; one block where there
+  // is none, of which no row counts.
+  const int last_key = min((p.tile + 1) * kTile, p.keys) - 1;
+  const int lo = first_row(a, p, p.tile * kTile) / kQueryRows, hi = ceil_div(end_row(a, p, last_key), kQueryRows);
+  const int n = max(hi - lo, 0);
+  p.begin = lo + static_cast<int>(static_cast<int64_t>(n) * p.part / p.parts);
+  p.end = lo + static_cast<int>(static_cast<int64_t>(n) * (p.part + 1) / p.parts);
+  return p;
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(Mass<D>::kThreads, 2) void attention_mass_kernel(MassArgs a) {
+template <int DT, int D, bool WHOLE>
+__global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kernel(MassArgs a) {
   using M = Mass<D>;
-  __shared__ Layout layout;
-  __shared__ __attribute__((aligned(512))) char lds[kQueryRows * M::kRowBytes];
-  __shared__ __attribute__((aligned(16))) float lse[kQueryRows];
-  make_layout(a, layout, blockIdx.x == 0);
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
+  __shared__ __attribute__((aligned(512))) char lds[kTile * M::kRowBytes + 2 * M::kBlockBytes];
+  __shared__ __attribute__((aligned(16))) float lse[2][kQueryRows];
+  extern __shared__ int memory[];
+  const Layout layout = make_layout(a, memory, blockIdx.x == 0);
+  const int wave = uniform(threadIdx.x >> 6);
+  const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)lds));
+  const uint32_t keys_at = lds_at + wave * 32 * M::kRowBytes;
+  const uint32_t rows_at = lds_at + kTile * M::kRowBytes;
   const int total = uniform(layout.first[a.rows]) * a.hkv;
-  for (int i = blockIdx.x; i < total; i += gridDim.x) {
-    const int entry = i / a.hkv, h = i - entry * a.hkv;
-    const Part p = part_at(a, layout, entry);
-    const int t0 = p.tile * M::kTile + wave * 32 * M::kColumns;
-    u32x4 k[M::kColumns][M::kSteps];
-    int from[M::kColumns], to[M::kColumns];
+
+  // Lane i looks up the page of the wave's load i: kPerLoad neighbouring keys, which lie in one page where its
+  // size is a multiple of kPerLoad (WHOLE).
+  int page = 0, in = 0;
+  auto look_up = [&](const Part& p) {
+    const int i = WHOLE ? (fresh_thread() & 63) % M::kKeyLoads : 0;
+    const int t = min(p.tile * kTile + wave * 32 + i * M::kPerLoad, (p.keys - 1) & ~(M::kPerLoad - 1));
+    const int index = t / a.block_size;
+    in = t - index * a.block_size;
+    page = a.table[p.row * a.bt_stride + index];
+  };
+  // Sends the wave's keys to its part of shared memory; returns the loads of a page out of range.
+  auto send_keys = [&](const Part& p) {
+    const int lane = fresh_thread() & 63, piece = lane % M::kPieces, mine = lane / M::kPieces;
+    const uint32_t token_bytes = a.k_token;
+    const uint64_t cache = reinterpret_cast<uint64_t>(a.k) + p.head * a.k_head;
+    uint32_t bad = 0;
+    if constexpr (WHOLE) {
+      const bool exists = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
+      bad = static_cast<uint32_t>(__ballot(!exists)) & static_cast<uint32_t>((1ull << M::kKeyLoads) - 1);
+      const uint64_t place = cache + static_cast<uint32_t>(exists ? page : 0) * a.k_block + static_cast<uint32_t>(in) * token_bytes;
 #pragma unroll
-    for (int c = 0; c < M::kColumns; ++c) {
-      const int t = t0 + 32 * c + (lane & 31);
-      from[c] = first_row(a, p, t), to[c] = t < p.keys ? end_row(a, p, t) : 0;
-      const int n = min(t, p.keys - 1), index = n / a.block_size, in = n - index * a.block_size;
-      const int page = a.table[p.row * a.bt_stride + index];
-      const bool fine = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
-      if (!fine && a.status) {
-        __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int i = 0; i < M::kKeyLoads; ++i) {
+        load_lds<0>(lane_value(place, i), mine * token_bytes + 16 * (piece ^ key_turn<D>(i * M::kPerLoad + mine)),
+                    keys_at + i * M::kPerLoad * M::kRowBytes);
       }
-      const char* src = a.k + (fine ? page : 0) * a.k_block + in * a.k_token + h * a.k_head + 16 * half;
-#pragma unroll
-      for (int s = 0; s < M::kSteps; ++s) {
-        k[c][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
-        if (!fine) k[c][s] = u32x4{0, 0, 0, 0};
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < M::kKeyLoads; ++i) {
+        const int key = i * M::kPerLoad + mine, t = min(p.tile * kTile + wave * 32 + key, p.keys - 1);
+        const int index = t / a.block_size, found = a.table[p.row * a.bt_stride + index];
+        const bool exists = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
+        const uint64_t from = cache + static_cast<uint32_t>(exists ? found : 0) * a.k_block +
+                              static_cast<uint32_t>(t - index * a.block_size) * token_bytes;
+        // A bit a key: there are no more than 32.
+        for (int j = 0; j < M::kPerLoad; ++j) {
+          bad |= (__ballot(!exists) >> (j * M::kPieces)) & 1 ? 1u << (i * M::kPerLoad + j) : 0u;
+        }
+        load_lds<0>(from + 16 * (piece ^ key_turn<D>(key)), uniform(keys_at + i * M::kPerLoad * M::kRowBytes));
       }
     }
-    // The staged tiles of query rows that see some key of the tile, and the part's share of them.
-    const int last_key = min((p.tile + 1) * M::kTile, p.keys) - 1;
-    const int lo = first_row(a, p, p.tile * M::kTile) / kQueryRows, hi = ceil_div(end_row(a, p, last_key), kQueryRows);
-    const int n = max(hi - lo, 0);
-    const int begin = lo + static_cast<int>(static_cast<int64_t>(n) * p.part / p.parts);
-    const int end = lo + static_cast<int>(static_cast<int64_t>(n) * (p.part + 1) / p.parts);
-    const int rows = p.len * a.group;
-    float sum[M::kColumns];
+    if (bad && a.status) {
+      __hip_atomic_fetch_or(a.status, static_cast<int>(kStatusPage), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    return bad;
+  };
+  float next_lse = 0.f;  // lane of wave 0: of a row of the block on its way
+  // Sends a block of query rows to a half of their shared memory; rows past the last one repeat it.
+  auto send_rows = [&](const Part& p, int block, int half) {
+    const int lane = fresh_thread() & 63, piece = lane % M::kPieces, rows = p.len * a.group;
 #pragma unroll
-    for (int c = 0; c < M::kColumns; ++c) sum[c] = 0.f;
+    for (int i = 0; i < M::kRowLoads; ++i) {
+      const int row = (wave * M::kRowLoads + i) * M::kPerLoad + lane / M::kPieces;
+      const int r = min(block * kQueryRows + row, rows - 1), token = r / a.group, head = r - token * a.group;
+      const uint64_t from = reinterpret_cast<uint64_t>(a.q + (p.start + token) * a.q_row + (p.head * a.group + head) * a.q_head);
+      load_lds<0>(from + 16 * (piece ^ key_turn<D>(row)),
+                  uniform(rows_at + half * M::kBlockBytes + (wave * M::kRowLoads + i) * M::kPerLoad * M::kRowBytes));
+    }
+    if (wave == 0) {
+      const int r = min(block * kQueryRows + (lane & 31), rows - 1), token = r / a.group, head = r - token * a.group;
+      next_lse = a.lse[(p.start + token) * a.l_row + (p.head * a.group + head) * a.l_head];
+    }
+  };
+
+  int i = blockIdx.x;
+  if (i >= total) return;
+  // While a part is computed the keys and first query rows of the next one are on their way, and the pages of the
+  // one after it are looked up.
+  Part u = part_at(a, layout, i / a.hkv, i % a.hkv), v = u;
+  look_up(u);
+  uint32_t bad = send_keys(u), bad_ahead = 0;
+  const auto first_block = [&](const Part& p) { return min(p.begin, ceil_div(p.len * a.group, kQueryRows) - 1); };
+  send_rows(u, first_block(u), 0);
+  i += gridDim.x;
+  if (i < total) {
+    v = part_at(a, layout, i / a.hkv, i % a.hkv);
+    look_up(v);
+  }
+  int half = 0;
+  for (;;) {
+    const int lane = threadIdx.x & 63;
+    const int t0 = u.tile * kTile + wave * 32, t = t0 + (lane & 31);
+    // The part's rows that see the lane's key, and those that see all of the wave's.
+    const int part_from = u.begin * kQueryRows, part_to = u.end * kQueryRows;
+    const int from = max(first_row(a, u, t), part_from), to = t < u.keys ? min(end_row(a, u, t), part_to) : 0;
+    const int all_from = max(first_row(a, u, t0 + 31), part_from);
+    const int all_to = t0 + 31 < u.keys ? min(end_row(a, u, t0), part_to) : 0;
+    u32x4 k[M::kSteps];
+    float sum = 0.f;
+    const int begin = first_block(u), end = max(u.end, begin + 1);
     for (int block = begin; block < end; ++block) {
-      __syncthreads();
-      for (int j = threadIdx.x; j < kQueryRows * M::kPieces; j += M::kThreads) {
-        const int row = j / M::kPieces, c = j % M::kPieces, r = min(block * kQueryRows + row, rows - 1);
-        const int token = p.start + r / a.group, head = h * a.group + r % a.group;
-        *reinterpret_cast<u32x4*>(lds + row * M::kRowBytes + 16 * (c ^ row_turn<D>(row))) =
-            *reinterpret_cast<const u32x4*>(a.q + token * a.q_row + head * a.q_head + 8 * c) ^ a.q_sign;
-      }
-      if (threadIdx.x < kQueryRows) {
-        const int r = min(block * kQueryRows + static_cast<int>(threadIdx.x), rows - 1);
-        const float x = a.lse[(p.start + r / a.group) * a.l_row + (h * a.group + r % a.group) * a.l_head];
+      wait_loads();
+      if (wave == 0 && lane < kQueryRows) {
         // A query head that saw nothing adds nothing.
-        lse[threadIdx.x] = x == -INFINITY ? INFINITY : x * kLog2eP;
+        lse[half][lane] = next_lse == -INFINITY ? INFINITY : next_lse * kLog2eP;
       }
-      __syncthreads();
-#pragma unroll
-      for (int b = 0; b < kQueryRows / 32; ++b) {
-        const int r0 = block * kQueryRows + 32 * b;
-        f32x16 sc[M::kColumns];
-#pragma unroll
-        for (int c = 0; c < M::kColumns; ++c) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) sc[c][e] = 0.f;
-        }
-        const int row = 32 * b + (lane & 31);
+      lds_barrier();
+      if (block == begin) {
+        const int key = lane & 31;
+        const char* at = lds + (wave * 32 + key) * M::kRowBytes;
 #pragma unroll
         for (int s = 0; s < M::kSteps; ++s) {
-          const u32x4 q = *reinterpret_cast<const u32x4*>(lds + row * M::kRowBytes + 16 * ((2 * s + half) ^ row_turn<D>(row)));
-#pragma unroll
-          for (int c = 0; c < M::kColumns; ++c) sc[c] = mfma32<DT>(q, k[c][s], sc[c]);
+          k[s] = *reinterpret_cast<const u32x4*>(at + 16 * ((2 * s + (lane >> 5)) ^ key_turn<D>(key)));
         }
-        f32x4 x[4];
+        if (bad) {
+          const bool mine = (bad >> (WHOLE ? key / M::kPerLoad : key)) & 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const f32x4*>(lse + 32 * b + 8 * e + 4 * half);
-#pragma unroll
-        for (int c = 0; c < M::kColumns; ++c) {
-          const bool whole = __all(from[c] <= r0 && r0 + 32 <= to[c]);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[c][e], a.scale_log2, -x[e >> 2][e & 3]));
-            const int r = r0 + 8 * (e >> 2) + 4 * half + (e & 3);
-            if (whole) sum[c] += w;
-            else sum[c] += r >= from[c] && r < to[c] ? w : 0.f;
-          }
+          for (int s = 0; s < M::kSteps; ++s) k[s] = mine ? u32x4{0, 0, 0, 0} : k[s];
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the next keys may come
+      }
+      if (block + 1 < end) {
+        send_rows(u, block + 1, half ^ 1);
+      } else if (i < total) {
+        bad_ahead = send_keys(v);
+        send_rows(v, first_block(v), half ^ 1);
+      }
+      // Scores of 32 query rows with the wave's keys.
+      const int thread = fresh_thread() & 63, row = thread & 31, upper = thread >> 5;
+      const char* rows = lds + kTile * M::kRowBytes + half * M::kBlockBytes;
+      const uint32_t at = row * M::kRowBytes + 16 * (upper ^ key_turn<D>(row));
+      f32x16 sc;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < M::kSteps; ++s) sc = mfma32<DT>(*reinterpret_cast<const u32x4*>(rows + (at ^ (32 * s))), k[s], sc);
+      f32x4 x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const f32x4*>(&lse[half][8 * e + 4 * upper]);
+      const int r0 = block * kQueryRows;
+      if (r0 < all_from || r0 + kQueryRows > all_to) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int r = r0 + 8 * (e >> 2) + 4 * upper + (e & 3);
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], a.scale_log2, -x[e >> 2][e & 3]));
+          sum += r >= from && r < to ? w : 0.f;
+        }
+      } else {
+        float w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], a.scale_log2, -x[e >> 2][e & 3]));
+#pragma unroll
+        for (int n = 8; n >= 1; n >>= 1) {
+#pragma unroll
+          for (int e = 0; e < n; ++e) w[e] += w[e + n];
+        }
+        sum += w[0];
+      }
+      half ^= 1;
+    }
+    sum += other_half(sum);
+    if (lane < 32 && t < u.keys) {
+      if (u.parts > 1) {
+        a.partial[(static_cast<int64_t>(u.slot) * a.hkv + u.head) * kTile + t - u.tile * kTile] = sum;
+      } else {
+        const float old = a.previous ? a.decay * a.previous[u.row * a.p_row + u.head * a.p_head + t] : 0.f;
+        a.mass[u.row * a.m_row + u.head * a.m_head + t] = old + sum;
       }
     }
-#pragma unroll
-    for (int c = 0; c < M::kColumns; ++c) {
-      sum[c] += other_half(sum[c]);
-      const int t = t0 + 32 * c + lane;
-      if (half || t >= p.keys) continue;
-      if (p.parts > 1) {
-        a.partial[(static_cast<int64_t>(p.slot) * a.hkv + h) * kMostKeys + t - p.tile * M::kTile] = sum[c];
-      } else {
-        const float old = a.previous ? a.decay * a.previous[p.row * a.p_row + h * a.p_head + t] : 0.f;
-        a.mass[p.row * a.m_row + h * a.m_head + t] = old + sum[c];
-      }
+    if (i >= total) break;
+    u = v;
+    bad = bad_ahead;
+    i += gridDim.x;
+    if (i < total) {
+      v = part_at(a, layout, i / a.hkv, i % a.hkv);
+      look_up(v);
     }
   }
 }
 
 // Adds up the parts of cut tiles, a thread a key.
-__global__ __launch_bounds__(kMostKeys) void mass_join_kernel(MassArgs a) {
-  __shared__ Layout layout;
-  make_layout(a, layout, false);
+__global__ __launch_bounds__(kThreads) void mass_join_kernel(MassArgs a) {
+  extern __shared__ int memory[];
+  const Layout layout = make_layout(a, memory, false);
   const int total = uniform(layout.cut[a.rows]) * a.hkv;
   for (int i = blockIdx.x; i < total; i += gridDim.x) {
-    const int entry = i / a.hkv, h = i - entry * a.hkv;
+    const int entry = i / a.hkv, head = i - entry * a.hkv;
     // The rows without cut tiles have no entries here.
     const int row = uniform(find_row(layout.cut, a.rows, entry));
-    const int in_row = entry - uniform(layout.cut[row]);
-    const Part p = part_at(a, layout, uniform(layout.first[row]) + in_row);
-    if (p.part) continue;
-    const int t = p.tile * a.tile + threadIdx.x;
-    if (static_cast<int>(threadIdx.x) >= a.tile || t >= p.keys) continue;
-    float sum = a.previous ? a.decay * a.previous[p.row * a.p_row + h * a.p_head + t] : 0.f;
-    for (int j = 0; j < p.parts; ++j) {
-      sum += a.partial[(static_cast<int64_t>(p.slot + j) * a.hkv + h) * kMostKeys + threadIdx.x];
-    }
-    a.mass[p.row * a.m_row + h * a.m_head + t] = sum;
+    const Part p = part_at(a, layout, uniform(layout.first[row]) + entry - uniform(layout.cut[row]), head);
+    const int t = p.tile * kTile + threadIdx.x;
+    if (p.part || threadIdx.x >= kTile || t >= p.keys) continue;
+    float sum = a.previous ? a.decay * a.previous[p.row * a.p_row + head * a.p_head + t] : 0.f;
+    for (int j = 0; j < p.parts; ++j) sum += a.partial[(static_cast<int64_t>(p.slot + j) * a.hkv + head) * kTile + threadIdx.x];
+    a.mass[p.row * a.m_row + head * a.m_head + t] = sum;
   }
 }
 
-// Parts of cut tiles: a row's tiles have at most twice the parts that their staged tiles fill, so at most
-// 2 kPartsPerSlot for each workgroup that runs at a time, all KV heads together.
-int64_t partial_parts() { return 2LL * kPartsPerSlot * mass_slots() + 1; }
-size_t mass_workspace_bytes() { return static_cast<size_t>(partial_parts()) * kMostKeys * sizeof(float); }
+// Parts of cut tiles: a row's tiles have at most twice the parts that their blocks fill, so at most 2
+// kPartsPerSlot for each workgroup that runs at a time, all KV heads together.
+int64_t partial_parts() { return 2LL * kPartsPerSlot * kMostGroups * device_cu_count() + 1; }
+size_t mass_workspace_bytes() { return static_cast<size_t>(partial_parts()) * kTile * sizeof(float); }
+
+template <int DT, int D>
+void launch(hipStream_t stream, const MassArgs& a) {
+  if (a.block_size % Mass<D>::kPerLoad == 0) {
+    attention_mass_kernel<DT, D, true><<<a.slots, kThreads, layout_bytes(a.rows), stream>>>(a);
+  } else {
+    attention_mass_kernel<DT, D, false><<<a.slots, kThreads, layout_bytes(a.rows), stream>>>(a);
+  }
+}
 
 template <int DT>
 void launch_dim(hipStream_t stream, int d, const MassArgs& a) {
-  if (d == 64) attention_mass_kernel<DT, 64><<<a.slots, Mass<64>::kThreads, 0, stream>>>(a);
-  else if (d == 128) attention_mass_kernel<DT, 128><<<a.slots, Mass<128>::kThreads, 0, stream>>>(a);
-  else attention_mass_kernel<DT, 256><<<a.slots, Mass<256>::kThreads, 0, stream>>>(a);
+  if (d == 64) launch<DT, 64>(stream, a);
+  else if (d == 128) launch<DT, 128>(stream, a);
+  else launch<DT, 256>(stream, a);
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -329,11 +406,10 @@ int attention_mass_impl(hipStream_t stream, const ds_attention_mass_desc* d) {
              "workspace must be 256-byte aligned and hold ds_attention_mass_workspace_bytes()");
   const int group = d->num_q_heads / d->num_kv_heads;
   const int64_t capacity = std::min<int64_t>(static_cast<int64_t>(d->max_blocks) * d->block_size, d->capacity);
-  const int tile = mass_tile(d->head_dim);
   DS_SUPPORTED(capacity <= (1 << 29), "rows of at most 2^29 keys");
   DS_SUPPORTED(d->tokens <= (1 << 20), "at most 2^20 query tokens");
   // Parts are counted in 32 bits.
-  const int64_t tiles = static_cast<int64_t>(d->rows) * ((capacity + tile - 1) / tile);
+  const int64_t tiles = static_cast<int64_t>(d->rows) * ((capacity + kTile - 1) / kTile);
   DS_SUPPORTED(static_cast<int64_t>(d->tokens) * group < (1 << 30) && tiles * d->num_kv_heads + partial_parts() < (1 << 30),
                "too many query tokens, KV heads or keys for one launch");
   MassArgs a{};
@@ -355,10 +431,8 @@ int attention_mass_impl(hipStream_t stream, const ds_attention_mass_desc* d) {
   a.q_start = d->query_start, a.q_len = d->query_len, a.t_len = d->target_len;
   a.rows = d->rows, a.tokens = d->tokens, a.hkv = d->num_kv_heads, a.group = group;
   a.window = d->window ? std::min(d->window, 1 << 29) : 1 << 29;
-  a.tile = tile;
-  a.slots = mass_slots();
-  a.scale_log2 = std::fabs(d->scale) * kLog2eP;
-  a.q_sign = d->scale < 0.f ? 0x80008000u : 0u;
+  a.slots = mass_groups(d->head_dim) * device_cu_count();
+  a.scale_log2 = d->scale * kLog2eP;
   a.decay = d->decay;
   a.partial = static_cast<float*>(d->workspace);
   a.status = d->status;
@@ -366,7 +440,7 @@ int attention_mass_impl(hipStream_t stream, const ds_attention_mass_desc* d) {
   else launch_dim<DS_FP16>(stream, d->head_dim, a);
   // Fewer query rows than a part's make no parts.
   if (static_cast<int64_t>(d->tokens) * group > kMinPart * kQueryRows) {
-    mass_join_kernel<<<a.slots, kMostKeys, 0, stream>>>(a);
+    mass_join_kernel<<<a.slots, kThreads, layout_bytes(a.rows), stream>>>(a);
   }
   return check_launch("ds_attention_mass");
 }

@@ -207,32 +207,6 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(ChunkArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Attention.
 // ---------------------------------------------------------------------------------------------
-// Key t's 16-byte piece c lies at place c ^ turn of its row, so that the reads of 16 neighbouring keys
-// touch different banks.
-template <int D>
-__device__ __forceinline__ int key_turn(int t) {
-  return D == 64 ? (t >> 1) & 7 : t & 15;
-}
-
-// 64 lanes' 16 bytes each from base + offset to 1 KiB of shared memory from to + PLUS on, a lane after the
-// other.  The compiler does not know of the load: what reads that memory waits for it (wait_loads) before a
-// barrier.  (It keeps nothing in m0 from one instruction to another.)
-template <int PLUS>
-__device__ __forceinline__ void load_lds(uint64_t base, uint32_t offset, uint32_t to) {
-  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
-               :
-               : "s"(to), "i"(PLUS), "v"(offset), "s"(base)
-               : "memory", "scc");
-}
-template <int PLUS>
-__device__ __forceinline__ void load_lds(uint64_t from, uint32_t to) {
-  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off"
-               :
-               : "s"(to), "i"(PLUS), "v"(from)
-               : "memory", "scc");
-}
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
-
 // What the loop over keys needs of the arguments, for one KV head; the rest is read again behind it, so that
 // scalar registers last.
 struct Cache {
@@ -297,12 +271,6 @@ __device__ __forceinline__ void advance(const Cache& a, Tile& x) {
   x.left -= kTile;
   x.pages += n;
   x.place += kTile - n * a.block_size;
-}
-
-__device__ __forceinline__ uint64_t lane_value(uint64_t v, int i) {
-  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), i);
-  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), i);
-  return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
 // Where a lane's piece of load i lies after the load's first key, in bytes.  (The turns of the pieces repeat

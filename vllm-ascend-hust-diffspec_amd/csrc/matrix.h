@@ -79,6 +79,38 @@ __device__ __forceinline__ int piece_at(int t, int c) {
   return t * (D / 8) + (c ^ turn);
 }
 
+// Key t's 16-byte piece c lies at place c ^ turn of its row, so that the reads of 16 neighbouring keys
+// touch different banks.
+template <int D>
+__device__ __forceinline__ int key_turn(int t) {
+  return D == 64 ? (t >> 1) & 7 : t & 15;
+}
+
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int i) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), i);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), i);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// 64 lanes' 16 bytes each from base + offset to 1 KiB of shared memory from to + PLUS on, a lane after the
+// other.  The compiler does not know of the load: what reads that memory waits for it (wait_loads) before a
+// barrier.  (It keeps nothing in m0 from one instruction to another.)
+template <int PLUS>
+__device__ __forceinline__ void load_lds(uint64_t base, uint32_t offset, uint32_t to) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
+               :
+               : "s"(to), "i"(PLUS), "v"(offset), "s"(base)
+               : "memory", "scc");
+}
+template <int PLUS>
+__device__ __forceinline__ void load_lds(uint64_t from, uint32_t to) {
+  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off"
+               :
+               : "s"(to), "i"(PLUS), "v"(from)
+               : "memory", "scc");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
 typedef __attribute__((address_space(3))) char lds_char;
 // A transposing read: lane l of 16 names key l / 4 and dimensions 4 (l % 4) .. + 3 and gets four keys of dimension l.
 __device__ __forceinline__ u32x2 read_values(uint32_t at) {
