@@ -60,6 +60,7 @@ struct MassArgs {
   const int32_t* q_len;
   const int32_t* t_len;
   int rows, tokens, hkv, group, window;
+  float per_group;   // 1 / group
   int slots;         // workgroups that run at a time
   float scale_log2;  // scale log2 e
   float decay;
@@ -215,21 +216,49 @@ __global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kerne
     return bad;
   };
   float next_lse = 0.f;  // lane of wave 0: of a row of the block on its way
-  // Sends a block of query rows to a half of their shared memory; rows past the last one repeat it.
-  auto send_rows = [&](const Part& p, int block, int half) {
-    const int lane = fresh_thread() & 63, piece = lane % M::kPieces, rows = p.len * a.group;
+  // The block of query rows that is sent next: its first row's token and head in the group.
+  int token = 0, head = 0;
+  const int block_tokens = kQueryRows / a.group, block_heads = kQueryRows - block_tokens * a.group;
+  auto go_to = [&](int block) {
+    token = block * kQueryRows / a.group;
+    head = block * kQueryRows - token * a.group;
+  };
+  // Where the lane's pieces lie after the block's first token, in bytes, and its row's LSE, in elements.  They
+  // depend on the first row's head alone, and on where the last row lies in the last block.
+  uint32_t row_offset[M::kRowLoads], lse_offset = 0;
+  int placed = -1;
+  auto place_rows = [&](int last) {
+    const int lane = fresh_thread() & 63, piece = lane % M::kPieces;
+    // (n + 0.5) / group in floating point gives the exact quotient for n < 2^22.
+    auto split = [&](int row, int& in_group) {
+      const int n = head + min(row, last), t = static_cast<int>((static_cast<float>(n) + 0.5f) * a.per_group);
+      in_group = n - t * a.group;
+      return t;
+    };
+    int in_group;
 #pragma unroll
     for (int i = 0; i < M::kRowLoads; ++i) {
-      const int row = (wave * M::kRowLoads + i) * M::kPerLoad + lane / M::kPieces;
-      const int r = min(block * kQueryRows + row, rows - 1), token = r / a.group, head = r - token * a.group;
-      const uint64_t from = reinterpret_cast<uint64_t>(a.q + (p.start + token) * a.q_row + (p.head * a.group + head) * a.q_head);
-      load_lds<0>(from + 16 * (piece ^ key_turn<D>(row)),
+      const int row = (wave * M::kRowLoads + i) * M::kPerLoad + lane / M::kPieces, t = split(row, in_group);
+      row_offset[i] = 2 * (t * static_cast<uint32_t>(a.q_row) + in_group * static_cast<uint32_t>(a.q_head)) +
+                      16 * (piece ^ key_turn<D>(row));
+    }
+    const int t = split(lane & (kQueryRows - 1), in_group);
+    lse_offset = t * static_cast<uint32_t>(a.l_row) + in_group * static_cast<uint32_t>(a.l_head);
+    placed = last < kQueryRows - 1 ? -1 : head;
+  };
+  // Sends a block of query rows to a half of their shared memory; rows past the last one repeat it.
+  auto send_rows = [&](const Part& p, int block, int half) {
+    const int last = p.len * a.group - 1 - block * kQueryRows;
+    if (placed != head || last < kQueryRows - 1) place_rows(last);
+    const uint64_t base = reinterpret_cast<uint64_t>(a.q + (p.start + token) * a.q_row + p.head * a.group * a.q_head);
+#pragma unroll
+    for (int i = 0; i < M::kRowLoads; ++i) {
+      load_lds<0>(base, row_offset[i],
                   uniform(rows_at + half * M::kBlockBytes + (wave * M::kRowLoads + i) * M::kPerLoad * M::kRowBytes));
     }
-    if (wave == 0) {
-      const int r = min(block * kQueryRows + (lane & 31), rows - 1), token = r / a.group, head = r - token * a.group;
-      next_lse = a.lse[(p.start + token) * a.l_row + (p.head * a.group + head) * a.l_head];
-    }
+    if (wave == 0) next_lse = (a.lse + (p.start + token) * a.l_row + p.head * a.group * a.l_head)[lse_offset];
+    token += block_tokens, head += block_heads;
+    if (head >= a.group) head -= a.group, ++token;
   };
 
   int i = blockIdx.x;
@@ -240,6 +269,7 @@ __global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kerne
   look_up(u);
   uint32_t bad = send_keys(u), bad_ahead = 0;
   const auto first_block = [&](const Part& p) { return min(p.begin, ceil_div(p.len * a.group, kQueryRows) - 1); };
+  go_to(first_block(u));
   send_rows(u, first_block(u), 0);
   i += gridDim.x;
   if (i < total) {
@@ -283,6 +313,7 @@ __global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kerne
         send_rows(u, block + 1, half ^ 1);
       } else if (i < total) {
         bad_ahead = send_keys(v);
+        go_to(first_block(v));
         send_rows(v, first_block(v), half ^ 1);
       }
       // Scores of 32 query rows with the wave's keys.
@@ -408,6 +439,14 @@ int attention_mass_impl(hipStream_t stream, const ds_attention_mass_desc* d) {
   const int64_t capacity = std::min<int64_t>(static_cast<int64_t>(d->max_blocks) * d->block_size, d->capacity);
   DS_SUPPORTED(capacity <= (1 << 29), "rows of at most 2^29 keys");
   DS_SUPPORTED(d->tokens <= (1 << 20), "at most 2^20 query tokens");
+  DS_SUPPORTED(group <= (1 << 16), "at most 2^16 query heads for a KV head");
+  // Places within a block of query rows are 32-bit byte counts, the heads of one more token included.
+  const auto spans = [&](int64_t row, int64_t head) {
+    return std::max<int64_t>(row, -row) * (kQueryRows / group + 2) + std::max<int64_t>(head, -head) * group < (1 << 30);
+  };
+  DS_SUPPORTED(spans(d->q_row_stride, d->q_head_stride) && d->lse_token_stride >= 0 && d->lse_head_stride >= 0 &&
+                   spans(d->lse_token_stride, d->lse_head_stride),
+               "query and LSE strides of at most 2^30 elements a block of rows");
   // Parts are counted in 32 bits.
   const int64_t tiles = static_cast<int64_t>(d->rows) * ((capacity + kTile - 1) / kTile);
   DS_SUPPORTED(static_cast<int64_t>(d->tokens) * group < (1 << 30) && tiles * d->num_kv_heads + partial_parts() < (1 << 30),
@@ -431,6 +470,7 @@ int attention_mass_impl(hipStream_t stream, const ds_attention_mass_desc* d) {
   a.q_start = d->query_start, a.q_len = d->query_len, a.t_len = d->target_len;
   a.rows = d->rows, a.tokens = d->tokens, a.hkv = d->num_kv_heads, a.group = group;
   a.window = d->window ? std::min(d->window, 1 << 29) : 1 << 29;
+  a.per_group = 1.f / static_cast<float>(group);
   a.slots = mass_groups(d->head_dim) * device_cu_count();
   a.scale_log2 = d->scale * kLog2eP;
   a.decay = d->decay;
