@@ -8,7 +8,7 @@
 //
 // The probabilities are those of the attention, so the keys are read once more, and the values not at all.
 // A wave holds 32 keys in registers as the columns of the score product, and the query rows (row = token *
-// group + head in the group) go by in shared memory, 32 at a time.  A lane's results are then 16 query rows
+// group + head in the group) go by in shared memory, 64 at a time.  A lane's results are then 16 query rows
 // of its own key, and the sum over the rows is the lane's own.  Tiles of keys with many query rows are cut
 // into parts of the rows, whose sums mass_join_kernel adds up in order.
 #include <cmath>
@@ -18,20 +18,24 @@
 namespace ds355 {
 namespace {
 
-constexpr int kQueryRows = 32;  // staged query rows, a block
-constexpr int kMinPart = 8;     // blocks below which the query rows are not cut
-constexpr int kPartsPerSlot = 4;
+// Staged query rows, a block: 64, whose two products and weighings overlap, or 32 where the rows have about as
+// many, so that more workgroups fit a CU.
+constexpr int kMostRows = 64;
+constexpr int kMinPart = 256;   // query rows below which they are not cut
+constexpr int kPartsPerSlot = 8;
 constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table or its mass
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTile = 32 * kWaves;  // keys of a workgroup
-constexpr int mass_groups(int d) { return d == 64 ? 4 : d == 128 ? 3 : 1; }  // workgroups of a CU
+// Workgroups of a CU.
+constexpr int mass_groups(int d, int block) { return d == 64 ? 4 : d == 256 ? 1 : block == 64 ? 2 : 3; }
 constexpr int kMostGroups = 4;
 
-template <int D>
+template <int D, int R>
 struct Mass {
+  static constexpr int kQueryRows = R;
   static constexpr int kRowBytes = 2 * D;
   static constexpr int kPieces = D / 8;
   static constexpr int kSteps = D / 16;
@@ -62,6 +66,7 @@ struct MassArgs {
   int rows, tokens, hkv, group, window;
   float per_group;   // 1 / group
   int slots;         // workgroups that run at a time
+  int block;         // query rows of a block
   float scale_log2;  // scale log2 e
   float decay;
   float* partial;  // [parts of cut tiles][KV head][kTile]
@@ -82,7 +87,7 @@ constexpr int layout_bytes(int rows) { return 4 * (5 * rows + 2); }
 
 // Parts of each tile of a row.
 __device__ __forceinline__ int row_parts(const MassArgs& a, int len, int cap) {
-  return max(ceil_div(ceil_div(len * a.group, kQueryRows), cap), 1);
+  return max(ceil_div(ceil_div(len * a.group, a.block), cap), 1);
 }
 
 __device__ __forceinline__ Layout make_layout(const MassArgs& a, int* memory, bool report) {
@@ -106,13 +111,39 @@ __device__ __forceinline__ Layout make_layout(const MassArgs& a, int* memory, bo
     }
     keys = len ? min(max(keys, 0), a.capacity) : 0;
     y.start[b] = start, y.len[b] = len, y.keys[b] = keys;
-    mine += static_cast<unsigned long long>(ceil_div(keys, kTile)) * ceil_div(len * a.group, kQueryRows);
+    mine += static_cast<unsigned long long>(ceil_div(keys, kTile)) * ceil_div(len * a.group, a.block);
   }
   if (mine) atomicAdd(&work, mine);
   __syncthreads();
+  // A part has at least the share of the work at which kPartsPerSlot would fill every workgroup (which bounds the
+  // partial sums).  Among the sizes that cut the longest rows evenly the one that ends first is taken: as
+  // many rounds as all parts take, of a part's blocks and about two for what it costs beside them.
   const unsigned long long most = static_cast<unsigned long long>(kPartsPerSlot) * a.slots;
   const unsigned long long share = (work * a.hkv + most - 1) / most;
-  y.cap = uniform(static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart)), 1ull << 25)));
+  const int least = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart / a.block)), 1ull << 25));
+  __shared__ int longest, cap;
+  if (threadIdx.x == 0) longest = 0, cap = least;
+  __syncthreads();
+  int len = 0;
+  for (int b = threadIdx.x; b < a.rows; b += kThreads) len = max(len, y.len[b]);
+  len = ceil_div(len * a.group, a.block);
+  if (len > least) atomicMax(&longest, len);
+  __syncthreads();
+  if (longest > least && a.rows <= 64 && threadIdx.x < 64) {
+    const int mine = max(ceil_div(longest, static_cast<int>(threadIdx.x) + 1), least);
+    const float per_part = 1.f / static_cast<float>(mine);
+    float parts = 0.f;
+    for (int b = 0; b < a.rows; ++b) {
+      const float blocks = static_cast<float>(ceil_div(y.len[b] * a.group, a.block));
+      parts += static_cast<float>(ceil_div(y.keys[b], kTile)) * fmaxf(ceilf(blocks * per_part - 1e-3f), 1.f);
+    }
+    const float cost = ceilf(parts * static_cast<float>(a.hkv) / static_cast<float>(a.slots)) * static_cast<float>(mine + 2);
+    const uint32_t best = wave_pick<false>(__float_as_uint(cost));
+    const int lane = __builtin_ctzll(__ballot(__float_as_uint(cost) == best));
+    if (static_cast<int>(threadIdx.x) == lane) cap = mine;
+  }
+  __syncthreads();
+  y.cap = uniform(cap);
   build_row_prefix(a.rows, y.first, scratch, [&](int b) { return ceil_div(y.keys[b], kTile) * row_parts(a, y.len[b], y.cap); });
   build_row_prefix(a.rows, y.cut, scratch, [&](int b) {
     const int parts = row_parts(a, y.len[b], y.cap);
@@ -150,38 +181,56 @@ __device__ __forceinline__ Part part_at(const MassArgs& a, const Layout& y, int 
   // The blocks of query rows that see some key of the tile, and the part's share of them; one block where there
   // is none, of which no row counts.
   const int last_key = min((p.tile + 1) * kTile, p.keys) - 1;
-  const int lo = first_row(a, p, p.tile * kTile) / kQueryRows, hi = ceil_div(end_row(a, p, last_key), kQueryRows);
+  const int lo = first_row(a, p, p.tile * kTile) / a.block, hi = ceil_div(end_row(a, p, last_key), a.block);
   const int n = max(hi - lo, 0);
   p.begin = lo + static_cast<int>(static_cast<int64_t>(n) * p.part / p.parts);
   p.end = lo + static_cast<int>(static_cast<int64_t>(n) * (p.part + 1) / p.parts);
   return p;
 }
 
-template <int DT, int D, bool WHOLE>
-__global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kernel(MassArgs a) {
-  using M = Mass<D>;
+// A part's blocks of query rows on their way to shared memory: the next block's first token in the query and
+// the LSE, and its first row's head in the group.
+struct Rows {
+  uint64_t q, lse;
+  int head, block, end;
+};
+
+template <int DT, int D, int R, bool WHOLE>
+__global__ __launch_bounds__(kThreads, mass_groups(D, R)) void attention_mass_kernel(MassArgs args) {
+  using M = Mass<D, R>;
+  constexpr int kQueryRows = R, kHalves = R / 32;
   __shared__ __attribute__((aligned(512))) char lds[kTile * M::kRowBytes + 2 * M::kBlockBytes];
   __shared__ __attribute__((aligned(16))) float lse[2][kQueryRows];
   extern __shared__ int memory[];
-  const Layout layout = make_layout(a, memory, blockIdx.x == 0);
+  const Layout layout = make_layout(args, memory, blockIdx.x == 0);
   const int wave = uniform(threadIdx.x >> 6);
   const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)lds));
   const uint32_t keys_at = lds_at + wave * 32 * M::kRowBytes;
-  const uint32_t rows_at = lds_at + kTile * M::kRowBytes;
-  const int total = uniform(layout.first[a.rows]) * a.hkv;
+  const uint32_t rows_at = lds_at + kTile * M::kRowBytes + wave * M::kRowLoads * M::kPerLoad * M::kRowBytes;
+  const int total = uniform(layout.first[args.rows]) * args.hkv;
+  const float scale_log2 = args.scale_log2;
 
   // Lane i looks up the page of the wave's load i: kPerLoad neighbouring keys, which lie in one page where its
   // size is a multiple of kPerLoad (WHOLE).
   int page = 0, in = 0;
-  auto look_up = [&](const Part& p) {
-    const int i = WHOLE ? (fresh_thread() & 63) % M::kKeyLoads : 0;
-    const int t = min(p.tile * kTile + wave * 32 + i * M::kPerLoad, (p.keys - 1) & ~(M::kPerLoad - 1));
+  // Parts go to the workgroups in turn, every other round backwards: their sizes fall or rise along the list.
+  const int groups = gridDim.x;
+  auto place_of = [&](int round) {
+    return round * groups + (round & 1 ? groups - 1 - static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x));
+  };
+  auto find_part = [&](int i) {
+    const MassArgs a = arguments<MassArgs>();
+    const Part p = part_at(a, layout, i / a.hkv, i % a.hkv);
+    const int load = WHOLE ? (fresh_thread() & 63) % M::kKeyLoads : 0;
+    const int t = min(p.tile * kTile + wave * 32 + load * M::kPerLoad, (p.keys - 1) & ~(M::kPerLoad - 1));
     const int index = t / a.block_size;
     in = t - index * a.block_size;
     page = a.table[p.row * a.bt_stride + index];
+    return p;
   };
   // Sends the wave's keys to its part of shared memory; returns the loads of a page out of range.
   auto send_keys = [&](const Part& p) {
+    const MassArgs a = arguments<MassArgs>();
     const int lane = fresh_thread() & 63, piece = lane % M::kPieces, mine = lane / M::kPieces;
     const uint32_t token_bytes = a.k_token;
     const uint64_t cache = reinterpret_cast<uint64_t>(a.k) + p.head * a.k_head;
@@ -203,8 +252,7 @@ __global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kerne
         const bool exists = static_cast<unsigned>(found) < static_cast<unsigned>(a.num_blocks);
         const uint64_t from = cache + static_cast<uint32_t>(exists ? found : 0) * a.k_block +
                               static_cast<uint32_t>(t - index * a.block_size) * token_bytes;
-        // A bit a key: there are no more than 32.
-        for (int j = 0; j < M::kPerLoad; ++j) {
+        for (int j = 0; j < M::kPerLoad; ++j) {  // a bit a key
           bad |= (__ballot(!exists) >> (j * M::kPieces)) & 1 ? 1u << (i * M::kPerLoad + j) : 0u;
         }
         load_lds<0>(from + 16 * (piece ^ key_turn<D>(key)), uniform(keys_at + i * M::kPerLoad * M::kRowBytes));
@@ -215,19 +263,13 @@ __global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kerne
     }
     return bad;
   };
-  float next_lse = 0.f;  // lane of wave 0: of a row of the block on its way
-  // The block of query rows that is sent next: its first row's token and head in the group.
-  int token = 0, head = 0;
-  const int block_tokens = kQueryRows / a.group, block_heads = kQueryRows - block_tokens * a.group;
-  auto go_to = [&](int block) {
-    token = block * kQueryRows / a.group;
-    head = block * kQueryRows - token * a.group;
-  };
-  // Where the lane's pieces lie after the block's first token, in bytes, and its row's LSE, in elements.  They
+
+  // Where the lane's pieces of a block lie after the block's first token, and its row's LSE, in bytes.  They
   // depend on the first row's head alone, and on where the last row lies in the last block.
   uint32_t row_offset[M::kRowLoads], lse_offset = 0;
   int placed = -1;
-  auto place_rows = [&](int last) {
+  auto place_rows = [&](int head, int last) {
+    const MassArgs a = arguments<MassArgs>();
     const int lane = fresh_thread() & 63, piece = lane % M::kPieces;
     // (n + 0.5) / group in floating point gives the exact quotient for n < 2^22.
     auto split = [&](int row, int& in_group) {
@@ -243,52 +285,72 @@ __global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kerne
                       16 * (piece ^ key_turn<D>(row));
     }
     const int t = split(lane & (kQueryRows - 1), in_group);
-    lse_offset = t * static_cast<uint32_t>(a.l_row) + in_group * static_cast<uint32_t>(a.l_head);
+    lse_offset = 4 * (t * static_cast<uint32_t>(a.l_row) + in_group * static_cast<uint32_t>(a.l_head));
     placed = last < kQueryRows - 1 ? -1 : head;
   };
-  // Sends a block of query rows to a half of their shared memory; rows past the last one repeat it.
-  auto send_rows = [&](const Part& p, int block, int half) {
-    const int last = p.len * a.group - 1 - block * kQueryRows;
-    if (placed != head || last < kQueryRows - 1) place_rows(last);
-    const uint64_t base = reinterpret_cast<uint64_t>(a.q + (p.start + token) * a.q_row + p.head * a.group * a.q_head);
+  const int block_heads = kQueryRows % args.group;
+  const int64_t block_q = 2 * (kQueryRows / args.group) * args.q_row, block_lse = 4 * (kQueryRows / args.group) * args.l_row;
+  auto start_rows = [&](const Part& p) {
+    const MassArgs a = arguments<MassArgs>();
+    Rows r;
+    // One block where there is none, of which no row counts.
+    r.block = min(p.begin, ceil_div(p.len * a.group, kQueryRows) - 1);
+    r.end = max(p.end, r.block + 1);
+    const int token = r.block * kQueryRows / a.group;
+    r.head = r.block * kQueryRows - token * a.group;
+    r.q = reinterpret_cast<uint64_t>(a.q + (p.start + token) * a.q_row + p.head * a.group * a.q_head);
+    r.lse = reinterpret_cast<uint64_t>(a.lse + (p.start + token) * a.l_row + p.head * a.group * a.l_head);
+    return r;
+  };
+  float next_lse = 0.f;  // lane of wave 0: of a row of the block on its way
+  // Sends a block of query rows to a half of their shared memory; rows past the last one (`last`) repeat it.
+  auto send_rows = [&](Rows& r, int last, int half) {
+    if (placed != r.head || last < kQueryRows - 1) place_rows(r.head, last);
 #pragma unroll
     for (int i = 0; i < M::kRowLoads; ++i) {
-      load_lds<0>(base, row_offset[i],
-                  uniform(rows_at + half * M::kBlockBytes + (wave * M::kRowLoads + i) * M::kPerLoad * M::kRowBytes));
+      if ((wave * M::kRowLoads + i) * M::kPerLoad > last) break;
+      load_lds<0>(r.q, row_offset[i], uniform(rows_at + half * M::kBlockBytes + i * M::kPerLoad * M::kRowBytes));
     }
-    if (wave == 0) next_lse = (a.lse + (p.start + token) * a.l_row + p.head * a.group * a.l_head)[lse_offset];
-    token += block_tokens, head += block_heads;
-    if (head >= a.group) head -= a.group, ++token;
+    typedef const __attribute__((address_space(1))) float* global_float;
+    if (wave == 0) next_lse = *(global_float)(r.lse + lse_offset);
+    r.q += block_q, r.lse += block_lse, r.head += block_heads;
+    ++r.block;
+    if (block_heads) {
+      const MassArgs a = arguments<MassArgs>();
+      if (r.head >= a.group) {
+        r.head -= a.group;
+        r.q += 2 * a.q_row, r.lse += 4 * a.l_row;
+      }
+    }
   };
 
-  int i = blockIdx.x;
+  int round = 0, i = place_of(0);
   if (i >= total) return;
   // While a part is computed the keys and first query rows of the next one are on their way, and the pages of the
   // one after it are looked up.
-  Part u = part_at(a, layout, i / a.hkv, i % a.hkv), v = u;
-  look_up(u);
+  Part u = find_part(i), v = u;
   uint32_t bad = send_keys(u), bad_ahead = 0;
-  const auto first_block = [&](const Part& p) { return min(p.begin, ceil_div(p.len * a.group, kQueryRows) - 1); };
-  go_to(first_block(u));
-  send_rows(u, first_block(u), 0);
-  i += gridDim.x;
-  if (i < total) {
-    v = part_at(a, layout, i / a.hkv, i % a.hkv);
-    look_up(v);
-  }
+  Rows rows = start_rows(u);
+  int block = rows.block, last_row = u.len * args.group - 1;
+  send_rows(rows, last_row - block * kQueryRows, 0);
+  i = place_of(++round);
+  if (i < total) v = find_part(i);
   int half = 0;
   for (;;) {
-    const int lane = threadIdx.x & 63;
-    const int t0 = u.tile * kTile + wave * 32, t = t0 + (lane & 31);
-    // The part's rows that see the lane's key, and those that see all of the wave's.
-    const int part_from = u.begin * kQueryRows, part_to = u.end * kQueryRows;
-    const int from = max(first_row(a, u, t), part_from), to = t < u.keys ? min(end_row(a, u, t), part_to) : 0;
-    const int all_from = max(first_row(a, u, t0 + 31), part_from);
-    const int all_to = t0 + 31 < u.keys ? min(end_row(a, u, t0), part_to) : 0;
+    const int lane = threadIdx.x & 63, end_of_rows = last_row + 1;
+    int from, to, all_from, all_to;  // rows that see the lane's key, and that see all of the wave's
+    {
+      const MassArgs a = arguments<MassArgs>();
+      const int t0 = u.tile * kTile + wave * 32, t = t0 + (lane & 31);
+      const int part_from = u.begin * kQueryRows, part_to = u.end * kQueryRows;
+      from = max(first_row(a, u, t), part_from), to = t < u.keys ? min(end_row(a, u, t), part_to) : 0;
+      all_from = max(first_row(a, u, t0 + 31), part_from);
+      all_to = t0 + 31 < u.keys ? min(end_row(a, u, t0), part_to) : 0;
+    }
     u32x4 k[M::kSteps];
     float sum = 0.f;
-    const int begin = first_block(u), end = max(u.end, begin + 1);
-    for (int block = begin; block < end; ++block) {
+    const int begin = block, end = rows.end;
+    for (; block < end; ++block) {
       wait_loads();
       if (wave == 0 && lane < kQueryRows) {
         // A query head that saw nothing adds nothing.
@@ -310,62 +372,118 @@ __global__ __launch_bounds__(kThreads, mass_groups(D)) void attention_mass_kerne
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the next keys may come
       }
       if (block + 1 < end) {
-        send_rows(u, block + 1, half ^ 1);
+        send_rows(rows, last_row - (block + 1) * kQueryRows, half ^ 1);
       } else if (i < total) {
         bad_ahead = send_keys(v);
-        go_to(first_block(v));
-        send_rows(v, first_block(v), half ^ 1);
+        rows = start_rows(v);
+        last_row = v.len * arguments<MassArgs>().group - 1;
+        send_rows(rows, last_row - rows.block * kQueryRows, half ^ 1);
       }
-      // Scores of 32 query rows with the wave's keys.
+      // Scores of the query rows with the wave's keys, 32 rows at a time: the products of the second run while the
+      // first are weighed.
       const int thread = fresh_thread() & 63, row = thread & 31, upper = thread >> 5;
-      const char* rows = lds + kTile * M::kRowBytes + half * M::kBlockBytes;
+      const char* staged = lds + kTile * M::kRowBytes + half * M::kBlockBytes;
       const uint32_t at = row * M::kRowBytes + 16 * (upper ^ key_turn<D>(row));
-      f32x16 sc;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = 0.f;
-#pragma unroll
-      for (int s = 0; s < M::kSteps; ++s) sc = mfma32<DT>(*reinterpret_cast<const u32x4*>(rows + (at ^ (32 * s))), k[s], sc);
-      f32x4 x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const f32x4*>(&lse[half][8 * e + 4 * upper]);
       const int r0 = block * kQueryRows;
-      if (r0 < all_from || r0 + kQueryRows > all_to) {
+      auto score = [&](int b, f32x16& sc) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int r = r0 + 8 * (e >> 2) + 4 * upper + (e & 3);
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], a.scale_log2, -x[e >> 2][e & 3]));
-          sum += r >= from && r < to ? w : 0.f;
+        for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < M::kSteps; ++s) {
+          sc = mfma32<DT>(*reinterpret_cast<const u32x4*>(staged + (at ^ (32 * s)) + 32 * b * M::kRowBytes), k[s], sc);
         }
-      } else {
+      };
+      auto weigh = [&](int b, const f32x16& sc, bool masked) {
         float w[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], a.scale_log2, -x[e >> 2][e & 3]));
+        for (int e = 0; e < 16; ++e) {
+          const float x = lse[half][32 * b + 8 * (e >> 2) + 4 * upper + (e & 3)];
+          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], scale_log2, -x));
+        }
+        if (masked) {
+          const int first = from - r0 - 32 * b - 4 * upper;
+          const unsigned count = max(to - from, 0);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (static_cast<unsigned>(8 * (e >> 2) + (e & 3) - first) >= count) w[e] = 0.f;
+          }
+        }
 #pragma unroll
         for (int n = 8; n >= 1; n >>= 1) {
 #pragma unroll
           for (int e = 0; e < n; ++e) w[e] += w[e + n];
         }
         sum += w[0];
+      };
+      if (kHalves == 2 && r0 >= all_from && r0 + kQueryRows <= all_to) {
+        // The rows are read ahead of the first products, those of the second between them, and the first are weighed
+        // between the second products.  (The compiler orders this otherwise, left to itself.)
+        u32x4 rows0[M::kSteps], rows1[M::kSteps];
+        f32x4 lse0[4], lse1[4];
+        auto read = [&](int b, int s) { return *reinterpret_cast<const u32x4*>(staged + (at ^ (32 * s)) + 32 * b * M::kRowBytes); };
+        auto read_lse = [&](int b, int e) { return *reinterpret_cast<const f32x4*>(&lse[half][32 * b + 8 * e + 4 * upper]); };
+        f32x16 sc0, sc1;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc0[e] = sc1[e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < M::kSteps; ++s) rows0[s] = read(0, s);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < M::kSteps; ++s) {
+          sc0 = mfma32<DT>(rows0[s], k[s], sc0);
+          rows1[s] = read(1, s);
+          if (s < 4) lse0[s] = read_lse(0, s);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        constexpr int kEach = 16 / M::kSteps;
+        float w0 = 0.f, w1 = 0.f;
+        auto weigh = [&](const f32x16& sc, const f32x4(&x)[4], int e) {
+          return __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], scale_log2, -x[e >> 2][e & 3]));
+        };
+#pragma unroll
+        for (int s = 0; s < M::kSteps; ++s) {
+          sc1 = mfma32<DT>(rows1[s], k[s], sc1);
+          if (s < 4) lse1[s] = read_lse(1, s);
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            const float x = weigh(sc0, lse0, s * kEach + e);
+            if (e & 1) w1 += x; else w0 += x;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) w0 += weigh(sc1, lse1, e), w1 += weigh(sc1, lse1, e + 1);
+        sum += w0 + w1;
+      } else {
+#pragma unroll
+        for (int b = 0; b < kHalves; ++b) {
+          if (r0 + 32 * b >= end_of_rows) break;
+          f32x16 sc;
+          score(b, sc);
+          weigh(b, sc, r0 < all_from || r0 + kQueryRows > all_to);
+        }
       }
       half ^= 1;
     }
     sum += other_half(sum);
-    if (lane < 32 && t < u.keys) {
-      if (u.parts > 1) {
-        a.partial[(static_cast<int64_t>(u.slot) * a.hkv + u.head) * kTile + t - u.tile * kTile] = sum;
-      } else {
-        const float old = a.previous ? a.decay * a.previous[u.row * a.p_row + u.head * a.p_head + t] : 0.f;
-        a.mass[u.row * a.m_row + u.head * a.m_head + t] = old + sum;
+    {
+      const MassArgs a = arguments<MassArgs>();
+      const int in_tile = wave * 32 + lane, t = u.tile * kTile + in_tile;
+      if (lane < 32 && t < u.keys) {
+        if (u.parts > 1) {
+          a.partial[(static_cast<int64_t>(u.slot) * a.hkv + u.head) * kTile + in_tile] = sum;
+        } else {
+          const float old = a.previous ? a.decay * a.previous[u.row * a.p_row + u.head * a.p_head + t] : 0.f;
+          a.mass[u.row * a.m_row + u.head * a.m_head + t] = old + sum;
+        }
       }
     }
     if (i >= total) break;
     u = v;
     bad = bad_ahead;
-    i += gridDim.x;
-    if (i < total) {
-      v = part_at(a, layout, i / a.hkv, i % a.hkv);
-      look_up(v);
-    }
+    block = rows.block - 1;
+    i = place_of(++round);
+    if (i < total) v = find_part(i);
   }
 }
 
@@ -392,13 +510,19 @@ __global__ __launch_bounds__(kThreads) void mass_join_kernel(MassArgs a) {
 int64_t partial_parts() { return 2LL * kPartsPerSlot * kMostGroups * device_cu_count() + 1; }
 size_t mass_workspace_bytes() { return static_cast<size_t>(partial_parts()) * kTile * sizeof(float); }
 
+template <int DT, int D, int R>
+void launch_block(hipStream_t stream, const MassArgs& a) {
+  if (a.block_size % Mass<D, R>::kPerLoad == 0) {
+    attention_mass_kernel<DT, D, R, true><<<a.slots, kThreads, layout_bytes(a.rows), stream>>>(a);
+  } else {
+    attention_mass_kernel<DT, D, R, false><<<a.slots, kThreads, layout_bytes(a.rows), stream>>>(a);
+  }
+}
+
 template <int DT, int D>
 void launch(hipStream_t stream, const MassArgs& a) {
-  if (a.block_size % Mass<D>::kPerLoad == 0) {
-    attention_mass_kernel<DT, D, true><<<a.slots, kThreads, layout_bytes(a.rows), stream>>>(a);
-  } else {
-    attention_mass_kernel<DT, D, false><<<a.slots, kThreads, layout_bytes(a.rows), stream>>>(a);
-  }
+  if (a.block == 32) launch_block<DT, D, 32>(stream, a);
+  else launch_block<DT, D, 64>(stream, a);
 }
 
 template <int DT>
@@ -442,7 +566,7 @@ int attention_mass_impl(hipStream_t stream, const ds_attention_mass_desc* d) {
   DS_SUPPORTED(group <= (1 << 16), "at most 2^16 query heads for a KV head");
   // Places within a block of query rows are 32-bit byte counts, the heads of one more token included.
   const auto spans = [&](int64_t row, int64_t head) {
-    return std::max<int64_t>(row, -row) * (kQueryRows / group + 2) + std::max<int64_t>(head, -head) * group < (1 << 30);
+    return std::max<int64_t>(row, -row) * (kMostRows / group + 2) + std::max<int64_t>(head, -head) * group < (1 << 30);
   };
   DS_SUPPORTED(spans(d->q_row_stride, d->q_head_stride) && d->lse_token_stride >= 0 && d->lse_head_stride >= 0 &&
                    spans(d->lse_token_stride, d->lse_head_stride),
@@ -471,7 +595,8 @@ int attention_mass_impl(hipStream_t stream, const ds_attention_mass_desc* d) {
   a.rows = d->rows, a.tokens = d->tokens, a.hkv = d->num_kv_heads, a.group = group;
   a.window = d->window ? std::min(d->window, 1 << 29) : 1 << 29;
   a.per_group = 1.f / static_cast<float>(group);
-  a.slots = mass_groups(d->head_dim) * device_cu_count();
+  a.block = static_cast<int64_t>(d->tokens) * group <= 32LL * d->rows ? 32 : 64;
+  a.slots = mass_groups(d->head_dim, a.block) * device_cu_count();
   a.scale_log2 = d->scale * kLog2eP;
   a.decay = d->decay;
   a.partial = static_cast<float*>(d->workspace);
@@ -479,7 +604,7 @@ int attention_mass_impl(hipStream_t stream, const ds_attention_mass_desc* d) {
   if (d->dtype == DS_BF16) launch_dim<DS_BF16>(stream, d->head_dim, a);
   else launch_dim<DS_FP16>(stream, d->head_dim, a);
   // Fewer query rows than a part's make no parts.
-  if (static_cast<int64_t>(d->tokens) * group > kMinPart * kQueryRows) {
+  if (static_cast<int64_t>(d->tokens) * group > kMinPart) {
     mass_join_kernel<<<a.slots, kThreads, layout_bytes(a.rows), stream>>>(a);
   }
   return check_launch("ds_attention_mass");

@@ -550,16 +550,6 @@ __device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, i
   }
 }
 
-// The kernel's arguments, read again.
-__device__ __forceinline__ ChunkArgs arguments() {
-  typedef const __attribute__((address_space(4))) ChunkArgs* pointer;
-  pointer at = (pointer)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(at));
-  ChunkArgs a;
-  __builtin_memcpy(&a, (const void*)at, sizeof(a));
-  return a;
-}
-
 // A piece in the workspace: 128 maxima and 128 sums, then the outputs as the waves hold them
 // ([query block][4 x dimension group][lane] of 4 floats).
 template <int D>
@@ -664,7 +654,7 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
     }
   }
   if (r >= rows) return;
-  const ChunkArgs z = arguments();
+  const ChunkArgs z = arguments<ChunkArgs>();
   if (p.parts == 1) {
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) store_out<DT>(z, p.start + token, head, 8 * g + 4 * half, group(g), st.l);

@@ -32,6 +32,21 @@ __device__ __forceinline__ int fresh_thread() {
 // A value that is the same in all lanes, to the scalar registers.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// The kernel's one argument, read again, so that what a loop does not need takes no scalar registers in it.
+template <typename Args>
+__device__ __forceinline__ Args arguments() {
+  static_assert(sizeof(Args) % 8 == 0);
+  struct Words {
+    uint64_t w[sizeof(Args) / 8];
+  } words;
+  typedef const __attribute__((address_space(4))) uint64_t* pointer;  // scalar loads
+  pointer at = (pointer)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(Args) / 8; ++i) words.w[i] = at[i];
+  return __builtin_bit_cast(Args, words);
+}
+
 // ---------------------------------------------------------------------------------------------
 // Matrix products: 32x32x16, A rows and B columns of 32, k-slot (lane / 32, e) = 8 (lane / 32) + e;
 // result i of a lane is row 8 (i / 4) + 4 (lane / 32) + i % 4 of column lane % 32.
