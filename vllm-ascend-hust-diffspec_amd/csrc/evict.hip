@@ -12,9 +12,14 @@
 // kept: sources and destinations are apart, so the moves run in any order, in place, and a step that evicts
 // one token moves one token.
 //
-// evict_select_kernel: a workgroup a (row, KV head).  The k-th largest value is found byte by byte from
-// histograms of an order-preserving integer; the moves go to a list, and the masses and positions with
-// them.  evict_move_kernel moves the keys and values.
+// evict_select_kernel: a workgroup a (row, KV head), which holds up to 32 k values in shared memory, as integers
+// of the same order.  The k-th largest is found 11 bits at a time from histograms in shared memory, after the
+// first 11 among the few that share them.  Slots that are always kept and masses of 0, of which there may be many
+// alike, are counted by the lanes instead of by atomics on one word.  It leaves, for every 64 slots, which
+// are kept and how many slots to move to and from lie before them.
+//
+// evict_move_kernel: a workgroup takes 64 of a head's moves at a time, finds their slots from those counts, and
+// moves keys, values, masses and positions.
 #include "matrix.h"
 
 namespace ds355 {
@@ -28,6 +33,16 @@ constexpr uint32_t kStatusShared = 16;  // a page that would be written is share
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / 64;
 constexpr int kMoveThreads = 256;
+
+// What a head leaves for its moves (-1: the row is left alone), and the row's state before them.
+struct Head {
+  int moves, known, gone, groups;
+};
+// 64 slots of a head: which are kept, and how many holes and movers lie before them.
+struct Group {
+  uint64_t kept;
+  int holes, movers;
+};
 
 struct EvictArgs {
   char* k;
@@ -49,56 +64,54 @@ struct EvictArgs {
   int num_blocks, block_size;
   int rows, hkv, pieces;  // pieces: 16-byte pieces of a head's key
   int sinks, recent;
-  int most;           // moves of a head, at most
-  int32_t* counts;    // [rows * hkv], -1: the row is left alone
-  int2* moves;        // [rows * hkv][most]: source, destination
+  int groups;         // of 64 slots, of a head at most
+  Head* heads;    // [rows * hkv]
+  Group* lists;   // [rows * hkv][groups]
   int32_t* status;
 };
 
-// Unsigned integers in the order of floating-point values; NaN below all.
+// Unsigned integers in the order of floating-point values; NaN below all, and 0 for no slot.
 __device__ __forceinline__ uint32_t ordered(float x) {
-  if (x != x) return 0;
+  if (x != x) return 1;
   const uint32_t u = __float_as_uint(x + 0.f);  // -0 as 0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-
-// One head's slots.
-struct Slots {
-  const float* mass;
-  const int32_t* positions;
-  int known, gone, sinks, newest;  // tokens at or past `newest` are always kept
-  __device__ __forceinline__ int position(int t) const { return t < known ? positions[t] : t + gone; }
-  __device__ __forceinline__ uint32_t value(int t) const {
-    const int p = position(t);
-    return p < sinks || p >= newest ? 0xffffffffu : ordered(mass[t]);
-  }
-};
 
 __device__ __forceinline__ void report(const EvictArgs& a, uint32_t bits) {
   if (a.status) __hip_atomic_fetch_or(a.status, static_cast<int>(bits), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Exclusive prefix over the waves of a count that is the same in a wave's lanes; `total` gets the sum.
-__device__ __forceinline__ int wave_prefix(int count, int* scratch, int& total) {
-  const int wave = threadIdx.x >> 6;
+constexpr uint32_t kAlways = 0xffffffffu;  // above every mass
+constexpr uint32_t kZero = 0x80000000u;    // a mass of 0
+constexpr int kBins = 2048;
+
+constexpr int kFew = 4096;  // values that share their first bits, held in shared memory
+
+// Sum over the waves before, and over all (`all`), of a count that is the same in a wave's lanes.
+__device__ __forceinline__ int wave_prefix(int count, int* scratch, int& all) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[wave] = count;
+  if (lane == 0) scratch[wave] = count;
   __syncthreads();
-  int before = 0;
-  total = 0;
-  for (int w = 0; w < kSelectWaves; ++w) {
-    if (w < wave) before += scratch[w];
-    total += scratch[w];
-  }
-  return before;
+  const int mine = lane < kSelectWaves ? scratch[lane] : 0, inclusive = wave_inclusive_scan(mine);
+  all = __builtin_amdgcn_readlane(inclusive, 63);
+  return __builtin_amdgcn_readlane(inclusive - mine, uniform(wave));
 }
 
+// HELD: slots whose values are held in shared memory; those of a longer row are read again for every pass.
+template <int HELD>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs a) {
-  __shared__ int histogram[256];
+  constexpr int kGroups = HELD / 64;  // of 64 slots, a wave's
+  static_assert(kGroups <= kSelectThreads && HELD < 65536, "a thread a group; two counts of a chunk in a word");
+  __shared__ uint32_t values[HELD];
+  __shared__ int histogram[kBins];
+  __shared__ uint32_t few[kFew];
   __shared__ int scratch[kSelectWaves];
-  __shared__ int found, left, refused;
+  __shared__ int group_ties[kGroups];
+  __shared__ uint32_t group_moves[kGroups];  // holes, and movers in the upper half
+  __shared__ int found, left, share, refused, few_held;
   const int b = blockIdx.x / a.hkv, h = blockIdx.x - b * a.hkv;
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63;
   const int n = a.t_len[b], keep = a.keep_len[b];
   uint32_t bits = 0;
   if (n > a.capacity) {
@@ -106,9 +119,37 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
   } else if (n > 0 && (keep < 0 || (keep < n && a.sinks > keep - a.recent))) {
     bits = kStatusBudget;
   }
-  if (tid == 0) refused = 0;
-  __syncthreads();
-  if (!bits && n > keep && n > 0) {
+  const bool asked = !bits && n > keep && n > 0;
+  float* mass = a.mass + b * a.m_row + h * a.m_head;
+  int32_t* positions = a.positions + b * a.p_row + h * a.p_head;
+  const int known = min(max(a.settled[2 * b], 0), n), gone = a.settled[2 * b + 1];
+  const int newest = n + gone - a.recent;  // tokens at or past it are always kept
+  auto position = [&](int t) { return t < known ? positions[t] : t + gone; };
+  auto value_of = [&](int place, float weight) { return place < a.sinks || place >= newest ? kAlways : ordered(weight); };
+  // f(slot, value) for the slots from `first` on, one a thread and 1024 apart, and none (0) past the last one, in
+  // whole waves.
+  auto each = [&](int first, int end, auto f) {
+    int t = first + tid;
+    for (; t - lane < min(end, HELD); t += kSelectThreads) f(t, t < n ? values[t] : 0u);
+    for (; t - lane < end; t += kSelectThreads) f(t, t < n ? value_of(position(t), mass[t]) : 0u);
+  };
+  if (tid == 0) refused = 0, few_held = 0;
+  for (int i = tid; i < kBins; i += kSelectThreads) histogram[i] = 0;
+  if (asked) {
+    // Eight loads of a thread are under way before the first is looked at.
+    const int last = min(n, HELD) - 1;
+    for (int first = tid; first <= last; first += 8 * kSelectThreads) {
+      float weight[8];
+      int place[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) weight[i] = mass[min(first + i * kSelectThreads, last)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) place[i] = position(min(first + i * kSelectThreads, last));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (first + i * kSelectThreads <= last) values[first + i * kSelectThreads] = value_of(place[i], weight[i]);
+      }
+    }
     for (int i = tid; i < ceil_div(n, a.block_size); i += kSelectThreads) {
       const int page = a.table[b * a.bt_stride + i];
       if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_blocks)) {
@@ -119,120 +160,211 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
     }
   }
   __syncthreads();
+  constexpr int kFirst = 21;  // the first histogram is of the bits from it on
+  auto counted = [](uint32_t x) { return x - 1 < kAlways - 1 && x != kZero; };
+  int always = 0, zeros = 0;
+  if (asked) {
+    each(0, n, [&](int, uint32_t x) {
+      always += x == kAlways;
+      zeros += x == kZero;
+      if (counted(x)) atomicAdd(&histogram[x >> kFirst], 1);
+    });
+  }
+  wave_prefix(wave_total(always), scratch, always);
+  wave_prefix(wave_total(zeros), scratch, zeros);
   bits |= refused;
-  const bool work = !bits && n > keep && n > 0;
+  const bool work = asked && !bits;
   if (tid == 0) {
     if (h == 0) a.kept_len[b] = work ? keep : max(n, 0);
-    if (!work) a.counts[blockIdx.x] = -1;
+    if (!work) a.heads[blockIdx.x].moves = -1;
     if (bits && h == 0) report(a, bits);
   }
   if (!work) return;
-  float* mass = a.mass + b * a.m_row + h * a.m_head;
-  int32_t* positions = a.positions + b * a.p_row + h * a.p_head;
-  const int known = min(max(a.settled[2 * b], 0), n), gone = a.settled[2 * b + 1];
-  const Slots slots{mass, positions, known, gone, a.sinks, n + gone - a.recent};
 
-  // The keep-th largest value, byte by byte, and how many of its equals are kept.
-  uint32_t value = 0;
-  int need = keep;  // kept values among those that share the bytes found so far
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelectThreads) histogram[i] = 0;
-    __syncthreads();
-    for (int t = tid; t < n; t += kSelectThreads) {
-      const uint32_t x = slots.value(t);
-      if (shift == 24 || (x >> (shift + 8)) == (value >> (shift + 8))) atomicAdd(&histogram[(x >> shift) & 255], 1);
-    }
-    __syncthreads();
-    if (wave == 0) {  // bins from the largest down, four a lane
-      int own[4], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        own[i] = histogram[255 - 4 * lane - i];
-        sum += own[i];
-      }
-      int above = wave_inclusive_scan(sum) - sum;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (above < need && need <= above + own[i]) {
-          found = 255 - 4 * lane - i;
-          left = need - above;
+  // The least kept value and how many of its equals are kept (all of them where a whole class is).
+  uint32_t value = kAlways;
+  int need = keep == always ? INT_MAX : keep;
+  if (always < keep) {
+    value = 0;
+    need = keep - always;  // kept values among those that share the bits found so far
+    bool in_few = false;
+    for (int high = 32, shift = kFirst; ; high = shift, shift = max(shift - 11, 0)) {
+      auto shares = [&](uint32_t x) { return high == 32 || (x >> high) == (value >> high); };
+      auto bin = [&](uint32_t x) { return (x >> shift) & ((1 << (high - shift)) - 1); };
+      if (high < 32) {
+        for (int i = tid; i < kBins; i += kSelectThreads) histogram[i] = 0;
+        __syncthreads();
+        auto count = [&](uint32_t x) {
+          if (counted(x) && shares(x)) atomicAdd(&histogram[bin(x)], 1);
+        };
+        if (in_few) {
+          for (int i = tid; i < few_held; i += kSelectThreads) count(few[i]);
+        } else {
+          each(0, n, [&](int, uint32_t x) { count(x); });
         }
-        above += own[i];
       }
+      if (tid == 0 && zeros && shares(kZero)) atomicAdd(&histogram[bin(kZero)], zeros);
+      __syncthreads();
+      // Bins from the largest down, two a thread.
+      const int first = histogram[kBins - 1 - 2 * tid], second = histogram[kBins - 2 - 2 * tid];
+      const int inclusive = wave_inclusive_scan(first + second);
+      int all;
+      const int above = wave_prefix(__builtin_amdgcn_readlane(inclusive, 63), scratch, all) + inclusive - first - second;
+      if (above < need && need <= above + first) {
+        found = kBins - 1 - 2 * tid, left = need - above, share = first;
+      } else if (above + first < need && need <= above + first + second) {
+        found = kBins - 2 - 2 * tid, left = need - above - first, share = second;
+      }
+      __syncthreads();
+      value |= static_cast<uint32_t>(found) << shift;
+      need = left;
+      const int sharing = share;
+      if (need == sharing) need = INT_MAX;
+      if (need == INT_MAX || shift == 0) break;
+      if (high == 32 && sharing <= kFew) {  // (masses of 0 among them are counted apart)
+        in_few = true;
+        each(0, n, [&](int, uint32_t x) {
+          if (counted(x) && (x >> kFirst) == (value >> kFirst)) few[atomicAdd(&few_held, 1)] = x;
+        });
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    value |= static_cast<uint32_t>(found) << shift;
-    need = left;
-    __syncthreads();
   }
+  value = max(value, 1u);  // no slots have 0
+  if (keep == 0) value = kAlways, need = 0;
 
-  // Slots in order: a wave takes a range of them, 64 at a time.
-  const int span = ceil_div(ceil_div(n, kSelectWaves), 64) * 64;
-  const int begin = min(wave * span, n), end = min(begin + span, n);
+  // Slots in order, group by group: a scan over the groups' counts says where each begins.
   const uint64_t below = (1ull << lane) - 1;
-  int total;
-  int ties = 0;
-  for (int t = begin + lane; t - lane < end; t += 64) ties += __popcll(__ballot(t < end && slots.value(t) == value));
-  const int ties_before = wave_prefix(ties, scratch, total);
-  auto keeps = [&](int t, int& tie) {  // whether slot t is kept; counts the equals
-    const uint32_t x = t < end ? slots.value(t) : 0;
-    const uint64_t equal = __ballot(t < end && x == value);
-    const bool kept = t < end && keep > 0 && (x > value || (x == value && tie + __popcll(equal & below) < need));
-    tie += __popcll(equal);
-    return kept;
+  auto scan_groups = [&](auto* counts) {  // counts become those of the groups before; returns the sum
+    const int mine = tid < kGroups ? counts[tid] : 0, inclusive = wave_inclusive_scan(mine);
+    int all;
+    const int before = wave_prefix(__builtin_amdgcn_readlane(inclusive, 63), scratch, all);
+    if (tid < kGroups) counts[tid] = before + inclusive - mine;
+    return static_cast<uint32_t>(all);
   };
-  int holes = 0, movers = 0, tie = ties_before;
-  for (int t = begin + lane; t - lane < end; t += 64) {
-    const bool kept = keeps(t, tie);
-    holes += __popcll(__ballot(t < end && t < keep && !kept));
-    movers += __popcll(__ballot(kept && t >= keep));
+  Group* list = a.lists + static_cast<int64_t>(blockIdx.x) * a.groups;
+  int ties = 0, holes = 0, movers = 0;  // of the chunks before
+  constexpr int kChunk = 64 * kGroups;
+  for (int first = 0; first < n; first += kChunk) {
+    const int end = min(first + kChunk, n);
+    auto group_of = [&](int t) { return (t - first) >> 6; };
+    __syncthreads();
+    if (tid < kGroups) group_ties[tid] = 0, group_moves[tid] = 0;
+    __syncthreads();
+    int ties_here = 0;
+    if (need != INT_MAX) {
+      each(first, end, [&](int t, uint32_t x) {
+        const int equal = __popcll(__ballot(x == value));
+        if (lane == 0) group_ties[group_of(t)] = equal;
+      });
+      __syncthreads();
+      ties_here = scan_groups(group_ties);
+      __syncthreads();
+    }
+    each(first, end, [&](int t, uint32_t x) {
+      bool mine = x >= value;
+      if (need != INT_MAX) {
+        const uint64_t equal = __ballot(x == value);
+        mine = x > value || (x == value && ties + group_ties[group_of(t)] + __popcll(equal & below) < need);
+      }
+      const uint64_t kept = __ballot(mine);
+      const int low_slots = keep - (t - lane);  // slots below `keep` exist
+      const uint64_t low = low_slots >= 64 ? ~0ull : low_slots <= 0 ? 0ull : (1ull << low_slots) - 1;
+      if (lane == 0) {
+        group_moves[group_of(t)] = __popcll(low & ~kept) | __popcll(kept & ~low) << 16;
+        list[t >> 6].kept = kept;
+      }
+      if (t >= keep) {
+        if (!mine && t < n) mass[t] = 0.f;
+      } else if (mine && t >= known) {
+        positions[t] = t + gone;
+      }
+    });
+    __syncthreads();
+    const uint32_t moves_here = scan_groups(group_moves);
+    __syncthreads();
+    for (int group = tid; group < ceil_div(end - first, 64); group += kSelectThreads) {
+      Group& g = list[first / 64 + group];
+      g.holes = holes + (group_moves[group] & 0xffff), g.movers = movers + (group_moves[group] >> 16);
+    }
+    ties += ties_here, holes += moves_here & 0xffff, movers += moves_here >> 16;
   }
-  int hole = wave_prefix(holes, scratch, total);
-  const int count = total;  // as many movers as holes
-  int mover = wave_prefix(movers, scratch, total);
-  int2* moves = a.moves + static_cast<int64_t>(blockIdx.x) * a.most;
-  tie = ties_before;
-  for (int t = begin + lane; t - lane < end; t += 64) {
-    const bool kept = keeps(t, tie);
-    const uint64_t to = __ballot(t < end && t < keep && !kept), from = __ballot(kept && t >= keep);
-    if ((to >> lane) & 1) moves[hole + __popcll(to & below)].y = t;
-    if ((from >> lane) & 1) moves[mover + __popcll(from & below)].x = t;
-    if (kept && t < keep && t >= known) positions[t] = t + gone;
-    hole += __popcll(to);
-    mover += __popcll(from);
-  }
-  __syncthreads();
-  for (int i = tid; i < count; i += kSelectThreads) {
-    const int2 move = moves[i];
-    positions[move.y] = slots.position(move.x);
-    mass[move.y] = mass[move.x];
-  }
-  __syncthreads();
-  for (int t = keep + tid; t < n; t += kSelectThreads) mass[t] = 0.f;
-  if (tid == 0) a.counts[blockIdx.x] = count;
+  if (tid == 0) a.heads[blockIdx.x] = Head{holes, known, gone, ceil_div(n, 64)};  // as many movers as holes
 }
 
+// The i-th set bit of `bits`, which has more.
+__device__ __forceinline__ int set_bit(uint64_t bits, int i) {
+  int at = 0;
+#pragma unroll
+  for (int width = 32; width >= 1; width >>= 1) {
+    const int low = __popcll((bits >> at) & ((1ull << width) - 1));
+    if (i >= low) i -= low, at += width;
+  }
+  return at;
+}
+
+constexpr int kMoves = 64;         // moves of a workgroup at a time
+constexpr int kMostSearched = 512;  // groups whose counts are searched in shared memory
+
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
-  const int count = a.counts[blockIdx.y];
-  if (count < 0) return;
-  const int b = blockIdx.y / a.hkv, h = blockIdx.y - b * a.hkv;
-  if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
-    a.settled[2 * b + 1] += a.t_len[b] - a.keep_len[b];
-    a.settled[2 * b] = a.keep_len[b];
+  __shared__ int2 moves[kMoves];
+  __shared__ int2 before[kMostSearched];  // holes and movers before a group
+  const Head head = a.heads[blockIdx.y];
+  if (head.moves < 0) return;
+  const int b = blockIdx.y / a.hkv, h = blockIdx.y - b * a.hkv, keep = a.keep_len[b], tid = threadIdx.x;
+  if (h == 0 && blockIdx.x == 0 && tid == 0) {
+    a.settled[2 * b + 1] = head.gone + a.t_len[b] - keep;
+    a.settled[2 * b] = keep;
+  }
+  if (static_cast<int>(blockIdx.x) * kMoves >= head.moves) return;
+  const Group* list = a.lists + static_cast<int64_t>(blockIdx.y) * a.groups;
+  const bool shared = head.groups <= kMostSearched;
+  if (shared) {
+    for (int g = tid; g < head.groups; g += kMoveThreads) before[g] = int2{list[g].holes, list[g].movers};
   }
   const int32_t* pages = a.table + b * a.bt_stride;
-  const int2* moves = a.moves + static_cast<int64_t>(blockIdx.y) * a.most;
-  const int64_t total = static_cast<int64_t>(count) * a.pieces;
-  for (int64_t i = blockIdx.x * kMoveThreads + threadIdx.x; i < total; i += gridDim.x * kMoveThreads) {
-    const int move = static_cast<int>(i / a.pieces), piece = static_cast<int>(i - static_cast<int64_t>(move) * a.pieces);
-    const int2 m = moves[move];
-    const int from = m.x / a.block_size, to = m.y / a.block_size;
-    const int64_t source = pages[from], target = pages[to];
-    const int in_from = m.x - from * a.block_size, in_to = m.y - to * a.block_size;
-    *reinterpret_cast<u32x4*>(a.k + target * a.k_block + in_to * a.k_token + h * a.k_head + 16 * piece) =
-        *reinterpret_cast<const u32x4*>(a.k + source * a.k_block + in_from * a.k_token + h * a.k_head + 16 * piece);
-    *reinterpret_cast<u32x4*>(a.v + target * a.v_block + in_to * a.v_token + h * a.v_head + 16 * piece) =
-        *reinterpret_cast<const u32x4*>(a.v + source * a.v_block + in_from * a.v_token + h * a.v_head + 16 * piece);
+  float* mass = a.mass + b * a.m_row + h * a.m_head;
+  int32_t* positions = a.positions + b * a.p_row + h * a.p_head;
+  for (int first = blockIdx.x * kMoves; first < head.moves; first += gridDim.x * kMoves) {
+    const int count = min(kMoves, head.moves - first);
+    __syncthreads();
+    // Threads 0 to 63 find the slots that are moved to, 64 to 127 those that are moved from.
+    const int i = tid % kMoves;
+    if (tid < 2 * kMoves && i < count) {
+      const bool from = tid >= kMoves;
+      int lo = 0, hi = head.groups - 1;  // the last group with no more of them before it
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        const int2 x = shared ? before[mid] : int2{list[mid].holes, list[mid].movers};
+        if ((from ? x.y : x.x) <= first + i) lo = mid; else hi = mid - 1;
+      }
+      const Group g = list[lo];
+      const int low_slots = keep - 64 * lo;
+      const uint64_t low = low_slots >= 64 ? ~0ull : low_slots <= 0 ? 0ull : (1ull << low_slots) - 1;
+      const int t = 64 * lo + set_bit(from ? g.kept & ~low : low & ~g.kept, first + i - (from ? g.movers : g.holes));
+      if (from) moves[i].x = t; else moves[i].y = t;
+    }
+    __syncthreads();
+    if (tid < count) {
+      const int2 m = moves[tid];
+      const float weight = mass[m.x];
+      positions[m.y] = m.x < head.known ? positions[m.x] : m.x + head.gone;
+      mass[m.y] = weight;
+      mass[m.x] = 0.f;
+    }
+    for (int j = tid; j < count * a.pieces; j += kMoveThreads) {
+      const int move = j / a.pieces, piece = j - move * a.pieces;
+      const int2 m = moves[move];
+      const int from = m.x / a.block_size, to = m.y / a.block_size;
+      const int64_t source = pages[from], target = pages[to];
+      const int in_from = m.x - from * a.block_size, in_to = m.y - to * a.block_size;
+      const u32x4 key =
+          *reinterpret_cast<const u32x4*>(a.k + source * a.k_block + in_from * a.k_token + h * a.k_head + 16 * piece);
+      const u32x4 value =
+          *reinterpret_cast<const u32x4*>(a.v + source * a.v_block + in_from * a.v_token + h * a.v_head + 16 * piece);
+      *reinterpret_cast<u32x4*>(a.k + target * a.k_block + in_to * a.k_token + h * a.k_head + 16 * piece) = key;
+      *reinterpret_cast<u32x4*>(a.v + target * a.v_block + in_to * a.v_token + h * a.v_head + 16 * piece) = value;
+    }
   }
 }
 
@@ -241,7 +373,7 @@ size_t rounded(size_t n) { return (n + 255) & ~size_t{255}; }
 size_t evict_workspace_bytes(int rows, int num_kv_heads, int capacity) {
   if (rows <= 0 || num_kv_heads <= 0 || capacity <= 0) return 0;
   const size_t heads = static_cast<size_t>(rows) * num_kv_heads;
-  return rounded(heads * sizeof(int32_t)) + heads * (capacity / 2 + 1) * sizeof(int2);
+  return rounded(heads * sizeof(Head)) + heads * ((capacity + 63) / 64) * sizeof(Group);
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -293,15 +425,16 @@ int evict_impl(hipStream_t stream, const ds_evict_desc* d) {
   a.block_size = d->block_size;
   a.rows = d->rows, a.hkv = d->num_kv_heads, a.pieces = d->head_dim * size / 16;
   a.sinks = d->sinks, a.recent = d->recent;
-  a.most = static_cast<int>(capacity / 2 + 1);
+  a.groups = static_cast<int>((capacity + 63) / 64);
   const int heads = d->rows * d->num_kv_heads;
-  a.counts = static_cast<int32_t*>(d->workspace);
-  a.moves = reinterpret_cast<int2*>(static_cast<char*>(d->workspace) + rounded(heads * sizeof(int32_t)));
+  a.heads = static_cast<Head*>(d->workspace);
+  a.lists = reinterpret_cast<Group*>(static_cast<char*>(d->workspace) + rounded(heads * sizeof(Head)));
   a.status = d->status;
-  evict_select_kernel<<<heads, kSelectThreads, 0, stream>>>(a);
+  if (capacity <= 4096) evict_select_kernel<4096><<<heads, kSelectThreads, 0, stream>>>(a);
+  else if (capacity <= 8192) evict_select_kernel<8192><<<heads, kSelectThreads, 0, stream>>>(a);
+  else evict_select_kernel<32768><<<heads, kSelectThreads, 0, stream>>>(a);
   // Workgroups of a head: enough for all its moves at most, and to fill the chip a few times over.
-  const int64_t full = (static_cast<int64_t>(a.most) * a.pieces + kMoveThreads - 1) / kMoveThreads;
-  const int64_t fill = std::max<int64_t>(1, 16LL * device_cu_count() / heads);
+  const int64_t full = (capacity / 2 + kMoves) / kMoves, fill = std::max<int64_t>(1, 16LL * device_cu_count() / heads);
   evict_move_kernel<<<dim3(static_cast<int>(std::min(full, fill)), heads), kMoveThreads, 0, stream>>>(a);
   return check_launch("ds_evict");
 }
