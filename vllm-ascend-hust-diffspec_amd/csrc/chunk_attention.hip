@@ -280,52 +280,45 @@ __device__ __forceinline__ int pages_in(const Cache& a, int n) {
   return static_cast<int>((static_cast<float>(n) + 0.5f) * a.per_block);
 }
 
-// A tile of a part's keys.  One load of a wave takes kPerLoad neighbouring keys; a part begins at a multiple
-// of 32 keys, so where the page size is a multiple of kPerLoad they lie in one page and the address is the
-// wave's (WHOLE): lane i looks up the page of load i, and computes its places in the caches.
+// A part's tiles of keys, one after the other.  One load of a wave takes kPerLoad neighbouring keys; a part
+// begins at a multiple of 32 keys, so where the page size is a multiple of kPerLoad they lie in one page and
+// the address is the wave's (WHOLE).  The lanes then look up the pages of the wave's loads of many tiles
+// together, a run: lane i's load is load i % kLoads of tile i / kLoads of the run.
 struct Tile {
-  const int32_t* pages;  // the table entry of the first key's page
-  int place;             // the first key in that page
-  int left;              // keys from the first one to the part's end
-  int page, in;          // lane i: of load i
+  int key, left;  // its first key, and the keys from it on to the part's end
 };
+struct Run {
+  int page, in;  // the lane's load: its page, and the first key's place in it
+};
+// Places of a run in one of the caches, in the lanes, and which of the loads there is a page and a key for.
 struct Places {
-  uint64_t k, v;  // lane i: of load i
-  int bad;        // loads of keys past the part's end or of a page out of range
-  Tile tile;
+  uint64_t at, fine;
 };
 
 template <int D, bool WHOLE>
-__device__ __forceinline__ void look_up(const Cache& a, int wave, Tile& x) {
+__device__ __forceinline__ Run look_up(const Cache& a, const int32_t* table, int wave, const Tile& x) {
   using C = Chunk<D>;
-  if (!WHOLE || x.left <= 0) return;
-  const int i = (fresh_thread() & 63) % C::kLoads;
-  const int t = min((wave * C::kLoads + i) * C::kPerLoad, (x.left - 1) & ~(C::kPerLoad - 1));
-  const int index = pages_in(a, x.place + t);
-  x.in = x.place + t - index * a.block_size;
-  x.page = x.pages[index];
+  Run r{0, 0};
+  if (!WHOLE || x.left <= 0) return r;
+  const int lane = fresh_thread() & 63, tile = lane / C::kLoads, i = lane % C::kLoads;
+  const int t = x.key + min(tile * kTile + (wave * C::kLoads + i) * C::kPerLoad, (x.left - 1) & ~(C::kPerLoad - 1));
+  const int index = t / a.block_size;
+  r.in = t - index * a.block_size;
+  r.page = table[index];
+  return r;
 }
 
-template <int D, bool WHOLE>
-__device__ __forceinline__ Places find_places(const Cache& a, const Tile& x, int wave) {
+template <int D, bool WHOLE, bool VALUES>
+__device__ __forceinline__ Places find_places(const Cache& a, const Run& r, int wave, const Tile& x) {
   using C = Chunk<D>;
-  Places p{0, 0, 0, x};
+  Places p{0, 0};
   if (!WHOLE || x.left <= 0) return p;
-  const int lane = fresh_thread() & 63, t = (wave * C::kLoads + lane) * C::kPerLoad;
-  const bool exists = static_cast<unsigned>(x.page) < static_cast<unsigned>(a.num_blocks);
-  constexpr int kAll = (1 << C::kLoads) - 1;
-  p.bad = static_cast<int>(__ballot(!exists || t >= x.left)) & kAll;
-  const uint32_t page = exists ? x.page : 0, in = x.in;
-  p.k = a.k + page * a.k_block + in * a.k_token;
-  p.v = a.v + page * a.v_block + in * a.v_token;
+  const int lane = fresh_thread() & 63, t = lane / C::kLoads * kTile + (wave * C::kLoads + lane % C::kLoads) * C::kPerLoad;
+  const bool exists = static_cast<unsigned>(r.page) < static_cast<unsigned>(a.num_blocks);
+  p.fine = __ballot(exists && t < x.left);
+  const uint32_t page = exists ? r.page : 0, in = r.in;
+  p.at = VALUES ? a.v + page * a.v_block + in * a.v_token : a.k + page * a.k_block + in * a.k_token;
   return p;
-}
-
-__device__ __forceinline__ void advance(const Cache& a, Tile& x) {
-  const int n = uniform(pages_in(a, x.place + kTile));
-  x.left -= kTile;
-  x.pages += n;
-  x.place += kTile - n * a.block_size;
 }
 
 // Where a lane's piece of load i lies after the load's first key, in bytes.  (The turns of the pieces repeat
@@ -338,24 +331,24 @@ __device__ __forceinline__ uint32_t piece_offset(const Cache& a, int lane, int i
          16 * (VALUES ? piece_at<D>(key, piece) - key * C::kPieces : piece ^ key_turn<D>(key));
 }
 
-template <int D, bool VALUES, int I = 0>
-__device__ __forceinline__ void send_whole(uint64_t place, const uint32_t (&offset)[Chunk<D>::kLoads], uint32_t to) {
+template <int D, int I = 0>
+__device__ __forceinline__ void send_whole(uint64_t place, int first, const uint32_t (&offset)[Chunk<D>::kLoads], uint32_t to) {
   using C = Chunk<D>;
   if constexpr (I < C::kLoads) {
-    load_lds<I * C::kPerLoad * C::kRowBytes>(lane_value(place, I), offset[I], to);
-    send_whole<D, VALUES, I + 1>(place, offset, to);
+    load_lds<I * C::kPerLoad * C::kRowBytes>(lane_value(place, first + I), offset[I], to);
+    send_whole<D, I + 1>(place, first, offset, to);
   }
 }
 
 // A page a lane; zeros for loads past the part's end and for keys of a page out of range.
 template <int D, bool VALUES>
-__device__ __forceinline__ void send_lanes(const Cache& a, const Tile& x, int wave, uint32_t to) {
+__device__ __forceinline__ void send_lanes(const Cache& a, const int32_t* table, const Tile& x, int wave, uint32_t to) {
   using C = Chunk<D>;
   const int lane = fresh_thread() & 63;
 #pragma unroll 1
   for (int i = 0; i < C::kLoads; ++i) {
     const int first = (wave * C::kLoads + i) * C::kPerLoad, key = first + lane / C::kPieces;
-    const int n = x.place + min(key, x.left - 1), index = pages_in(a, n), page = x.pages[index];
+    const int n = x.key + min(key, x.left - 1), index = n / a.block_size, page = table[index];
     const uint32_t token_bytes = VALUES ? a.v_token : a.k_token, in = n - index * a.block_size;
     const bool exists = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
     if (!exists && a.status) {
@@ -367,15 +360,17 @@ __device__ __forceinline__ void send_lanes(const Cache& a, const Tile& x, int wa
   }
 }
 
-// Sends the wave's part of a tile's keys (or values) to shared memory.
+// Sends the wave's part of a tile's keys (or values), tile `tile` of a run, to shared memory.
 template <int D, bool WHOLE, bool VALUES>
-__device__ __forceinline__ void send(const Cache& a, const Places& p, const uint32_t (&offset)[Chunk<D>::kLoads], int wave,
-                                     uint32_t to) {
-  if (p.tile.left <= 0) return;
-  if (WHOLE && p.bad == 0) {
-    send_whole<D, VALUES>(VALUES ? p.v : p.k, offset, to);
+__device__ __forceinline__ void send(const Cache& a, const int32_t* table, const Tile& x, const Places& p, int tile,
+                                     const uint32_t (&offset)[Chunk<D>::kLoads], int wave, uint32_t to) {
+  using C = Chunk<D>;
+  if (x.left <= 0) return;
+  constexpr uint32_t kAll = (1u << C::kLoads) - 1;
+  if (WHOLE && (static_cast<uint32_t>(p.fine >> (tile * C::kLoads)) & kAll) == kAll) {
+    send_whole<D>(p.at, tile * C::kLoads, offset, to);
   } else {
-    send_lanes<D, VALUES>(a, p.tile, wave, to);
+    send_lanes<D, VALUES>(a, table, x, wave, to);
   }
 }
 
@@ -550,26 +545,35 @@ __device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, i
     k_offset[i] = piece_offset<D, false>(a, threadIdx.x & 63, i);
     v_offset[i] = piece_offset<D, true>(a, threadIdx.x & 63, i);
   }
-  const int index = uniform(key / a.block_size);
-  Tile x{table + index, key - index * a.block_size, end - key, 0, 0};
-  Places p;
+  // The keys' next tile and the run that it belongs to, the values' next tile (one before it) and its run, and the
+  // run that the keys come to next.
+  constexpr int kRun = 64 / C::kLoads;
+  Tile x{key, end - key}, v = x;
+  int x_tile = 0, v_tile = 0;  // of the run
+  Run run = look_up<D, WHOLE>(a, table, wave, x), run_ahead = run;
+  Places k_places = find_places<D, WHOLE, false>(a, run, wave, x), v_places{0, 0};
   auto send_keys = [&](int half) {
-    p = find_places<D, WHOLE>(a, x, wave);
-    send<D, WHOLE, false>(a, p, k_offset, wave, to + half * C::kStage);
+    if (x_tile == kRun) {
+      run = run_ahead, x_tile = 0;
+      k_places = find_places<D, WHOLE, false>(a, run, wave, x);
+    }
+    send<D, WHOLE, false>(a, table, x, k_places, x_tile, k_offset, wave, to + half * C::kStage);
+    // The pages of the next run, half a run ahead.
+    if (x_tile == kRun / 2) run_ahead = look_up<D, WHOLE>(a, table, wave, Tile{x.key + kRun / 2 * kTile, x.left - kRun / 2 * kTile});
+    x.key += kTile, x.left -= kTile, ++x_tile;
   };
-  auto send_values = [&](int half) { send<D, WHOLE, true>(a, p, v_offset, wave, to + (2 + half) * C::kStage); };
-  auto ahead = [&]() {
-    advance(a, x);
-    look_up<D, WHOLE>(a, wave, x);
+  // The values come to a run when the keys are one tile into it.
+  auto send_values = [&](int half) {
+    if (v_tile == kRun) v_tile = 0;
+    if (v_tile == 0) v_places = find_places<D, WHOLE, true>(a, run, wave, v);
+    send<D, WHOLE, true>(a, table, v, v_places, v_tile, v_offset, wave, to + (2 + half) * C::kStage);
+    v.key += kTile, v.left -= kTile, ++v_tile;
   };
-  look_up<D, WHOLE>(a, wave, x);
   send_keys(0);
-  ahead();
   wait_loads();
   lds_barrier();
   send_values(0);
   send_keys(1);
-  ahead();
   f32x16 sc[N];
   if (rows.any) score<DT, D, N>(lds, q, t0, sc);
   const unsigned count = max(rows.limit - rows.lower, 0);
@@ -584,7 +588,6 @@ __device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, i
     lds_barrier();
     send_values(here ^ 1);
     send_keys(here);
-    ahead();
     if (!rows.any) continue;
     const int at = key + t0;
     if (at < rows.all_from || at + 32 * N > rows.all_to) {
