@@ -125,19 +125,12 @@ __device__ __forceinline__ int plan_scan(int v, int* sums, int& total) {
   return before + inclusive - v;
 }
 
-constexpr int kSizes = 64;   // classes of part sizes, the largest first
-constexpr int kHeld = 2048;  // items whose tiles are held
-__device__ __forceinline__ int size_class(int size, int cap) {
-  return kSizes - 1 - min(static_cast<int>(static_cast<int64_t>(size) * kSizes / (cap + 1)), kSizes - 1);
-}
-
 __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(ChunkArgs a) {
   __shared__ int sums[kPlanThreads / 64];
   __shared__ int first_item[kMaxRows + 1], row_start[kMaxRows], row_len[kMaxRows], row_seen[kMaxRows];
   __shared__ unsigned long long work;
-  __shared__ int begin[kSizes + 1], slots, joins, longest;
-  __shared__ int held[kHeld], classes[kPlanThreads / 64][kSizes], caps[kPlanThreads / 64];
-  __shared__ float costs[kPlanThreads / 64];
+  constexpr int kSizes = 64;  // classes of part sizes
+  __shared__ int begin[kSizes + 1], slots, joins;
   const int b = threadIdx.x;
   int start = 0, len = 0, keys = 0;
   bool bad = false;
@@ -167,88 +160,40 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(ChunkArgs a) {
   const int item = plan_scan(ceil_div(len * a.group, kItemRows), sums, items);
   first_item[b] = item;
   row_start[b] = start, row_len[b] = len, row_seen[b] = keys - len;
-  if (b == 0) first_item[kMaxRows] = items, work = 0, slots = 0, joins = 0, longest = 0;
+  if (b == 0) first_item[kMaxRows] = items, work = 0, slots = 0, joins = 0;
   if (b <= kSizes) begin[b] = 0;
   if (b < 64) a.header->zeros[b] = 0;
   __syncthreads();
-  // Key tiles of the items (at least one: an item without keys has an output), held for as many as fit.
-  auto item_tiles = [&](int i) {
-    const int r = find_row(first_item, kMaxRows, i);
-    return max(item_keys(a, row_len[r], row_seen[r], i - first_item[r]).tiles, 1);
-  };
-  auto tiles_of = [&](int i) { return i < kHeld ? held[i] : item_tiles(i); };
+  auto row_of = [&](int i) { return find_row(first_item, kMaxRows, i); };
   unsigned long long mine = 0;
-  int most = 0;
   for (int i = b; i < items; i += kPlanThreads) {
-    const int n = item_tiles(i);
-    if (i < kHeld) held[i] = n;
-    mine += n;
-    most = max(most, n);
+    const int r = row_of(i);
+    mine += max(item_keys(a, row_len[r], row_seen[r], i - first_item[r]).tiles, 1);
   }
   if (mine) atomicAdd(&work, mine);
-  if (most) atomicMax(&longest, most);
   __syncthreads();
-  // Items are cut into parts of at most `cap` tiles.  With an equal share of the work there are no more parts than
-  // the workspace holds; but parts of little more than half of it would then run in two rounds.  So each wave
-  // tries another number of parts for the longest item: in tiles, where `before` parts are at least as long
-  // as one, some workgroup runs ceil(before / slots) of them.  A part costs about two tiles beside its own, and
-  // a piece that is stored and joined about four more, twice.
+  // A part is an equal share of the work at most, so that the last ones to run end together.
   // (An item has at most 2^24 tiles.)
   const unsigned long long share = (work * a.hkv + a.slots - 1) / a.slots;
-  const int equal = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart)), 1ull << 25));
-  const int wave = uniform(b >> 6), lane = b & 63;
-  if (items <= kHeld) {
-    const int cap = max(ceil_div(longest, ceil_div(longest, equal) + wave), kMinPart);
-    int* count = classes[wave];
-    count[lane] = 0;
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront", "local");
-    int pieces = 0, parts_in_all = 0;
-    for (int i = lane; i < items; i += 64) {
-      const int n = held[i], parts = ceil_div(n, cap);
-      atomicAdd(&count[size_class(ceil_div(n, parts), cap)], parts);
-      parts_in_all += parts;
-      if (parts > 1) pieces += parts;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront", "local");
-    pieces = wave_total(pieces), parts_in_all = wave_total(parts_in_all);
-    const int before = wave_inclusive_scan(count[lane]);
-    const float size = static_cast<float>(kSizes - lane) * static_cast<float>(cap) / kSizes;  // of the class, at most
-    const float rounds = ceilf(static_cast<float>(before) * a.hkv / a.slots);
-    const float piece_cost = 4.f * static_cast<float>(pieces) * a.hkv / a.slots;
-    float cost = count[lane] ? rounds * (size + 2.f) : 0.f;
-    cost = __uint_as_float(wave_pick<true>(__float_as_uint(cost)));
-    cost = fmaxf(cost, (static_cast<float>(work) + 2.f * parts_in_all) * a.hkv / a.slots) + 2.f * piece_cost;
-    if (lane == 0) {
-      costs[wave] = static_cast<int64_t>(pieces) * a.hkv <= 2LL * a.slots ? cost : INFINITY;
-      caps[wave] = cap;
-    }
-  }
-  __syncthreads();
-  int cap = equal;
-  if (items <= kHeld) {
-    float best = INFINITY;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-      if (costs[w] < best) best = costs[w], cap = caps[w];
-    }
-  }
+  const int cap = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart)), 1ull << 25));
+  auto size_class = [&](int size) { return kSizes - 1 - min(static_cast<int>(static_cast<int64_t>(size) * kSizes / (cap + 1)), kSizes - 1); };
   for (int i = b; i < items; i += kPlanThreads) {
-    const int n = tiles_of(i), parts = ceil_div(n, cap);
-    atomicAdd(&begin[size_class(n / parts, cap) + 1], parts);
+    const int r = row_of(i);
+    const int n = max(item_keys(a, row_len[r], row_seen[r], i - first_item[r]).tiles, 1), parts = ceil_div(n, cap);
+    atomicAdd(&begin[size_class(n / parts) + 1], parts);
   }
   __syncthreads();
-  if (wave == 0) {
-    static_assert(kSizes == 64, "a lane a class");
-    const int n = begin[lane + 1], inclusive = wave_inclusive_scan(n);
-    begin[lane + 1] = inclusive;
-    if (lane == 63) a.header->parts = inclusive;
+  if (b == 0) {
+    for (int s = 0; s < kSizes; ++s) begin[s + 1] += begin[s];
+    a.header->parts = begin[kSizes];
   }
   __syncthreads();
   for (int i = b; i < items; i += kPlanThreads) {
-    const int r = find_row(first_item, kMaxRows, i);
+    const int r = row_of(i);
     Part p{row_start[r], row_len[r], row_seen[r], r, i - first_item[r], 0, 0, 0};
-    const int n = tiles_of(i);
+    const int n = max(item_keys(a, p.len, p.seen, p.tile).tiles, 1);
     p.parts = ceil_div(n, cap);
-    const int place = atomicAdd(&begin[size_class(n / p.parts, cap)], p.parts);
+    const int place = atomicAdd(&begin[size_class(n / p.parts)], p.parts);
     if (p.parts > 1) {
       p.slot = atomicAdd(&slots, p.parts);
       a.joins[atomicAdd(&joins, 1)] = p;
@@ -762,8 +707,8 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a) {
 }
 
 // Bounds of a plan.  Items: whole ones and a last one a row.  A cut item has at most twice the parts that
-// its tiles fill, so with equal shares all cut items have at most two parts per workgroup that runs at a
-// time, each part counted once for every KV head; plans of more are not taken.
+// its tiles fill, so all cut items have at most two parts per workgroup that runs at a time, and each
+// part counts once for every KV head.
 struct Bounds {
   int64_t items, parts, joins, pieces;
 };
