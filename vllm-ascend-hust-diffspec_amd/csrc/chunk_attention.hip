@@ -164,34 +164,42 @@ __global__ __launch_bounds__(kPlanThreads) void chunk_plan_kernel(ChunkArgs a) {
   if (b <= kSizes) begin[b] = 0;
   if (b < 64) a.header->zeros[b] = 0;
   __syncthreads();
-  auto row_of = [&](int i) { return find_row(first_item, kMaxRows, i); };
+  // An item's row and its key tiles (at least one: an item without keys has an output).  A thread's first
+  // item, for most calls its only one, is looked up once.
+  struct Found {
+    int row, tiles;
+  };
+  auto find = [&](int i) {
+    const int r = find_row(first_item, kMaxRows, i);
+    return Found{r, max(item_keys(a, row_len[r], row_seen[r], i - first_item[r]).tiles, 1)};
+  };
+  const Found first = b < items ? find(b) : Found{0, 0};
+  auto found = [&](int i) { return i == b ? first : find(i); };
   unsigned long long mine = 0;
-  for (int i = b; i < items; i += kPlanThreads) {
-    const int r = row_of(i);
-    mine += max(item_keys(a, row_len[r], row_seen[r], i - first_item[r]).tiles, 1);
-  }
+  for (int i = b; i < items; i += kPlanThreads) mine += found(i).tiles;
   if (mine) atomicAdd(&work, mine);
   __syncthreads();
-  // A part is an equal share of the work at most, so that the last ones to run end together.
-  // (An item has at most 2^24 tiles.)
-  const unsigned long long share = (work * a.hkv + a.slots - 1) / a.slots;
-  const int cap = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart)), 1ull << 25));
-  auto size_class = [&](int size) { return kSizes - 1 - min(static_cast<int>(static_cast<int64_t>(size) * kSizes / (cap + 1)), kSizes - 1); };
+  // A part is an equal share of the work at most, so that the last ones to run end together.  (An item has at
+  // most 2^24 tiles.  The share's four roundings, of 2^-24 each, may not make it less than equal.)
+  const float share = static_cast<float>(work) * static_cast<float>(a.hkv) / static_cast<float>(a.slots);
+  const int cap = max(static_cast<int>(fminf(ceilf(share * (1.f + 0x1p-20f)), 0x1p25f)), kMinPart);
+  const float classes = static_cast<float>(kSizes) / static_cast<float>(cap + 1);
+  auto size_class = [&](int size) { return kSizes - 1 - min(static_cast<int>(static_cast<float>(size) * classes), kSizes - 1); };
   for (int i = b; i < items; i += kPlanThreads) {
-    const int r = row_of(i);
-    const int n = max(item_keys(a, row_len[r], row_seen[r], i - first_item[r]).tiles, 1), parts = ceil_div(n, cap);
+    const int n = found(i).tiles, parts = ceil_div(n, cap);
     atomicAdd(&begin[size_class(n / parts) + 1], parts);
   }
   __syncthreads();
-  if (b == 0) {
-    for (int s = 0; s < kSizes; ++s) begin[s + 1] += begin[s];
-    a.header->parts = begin[kSizes];
+  if (b < 64) {
+    static_assert(kSizes == 64, "a lane a class");
+    const int inclusive = wave_inclusive_scan(begin[b + 1]);
+    begin[b + 1] = inclusive;
+    if (b == 63) a.header->parts = inclusive;
   }
   __syncthreads();
   for (int i = b; i < items; i += kPlanThreads) {
-    const int r = row_of(i);
+    const auto [r, n] = found(i);
     Part p{row_start[r], row_len[r], row_seen[r], r, i - first_item[r], 0, 0, 0};
-    const int n = max(item_keys(a, p.len, p.seen, p.tile).tiles, 1);
     p.parts = ceil_div(n, cap);
     const int place = atomicAdd(&begin[size_class(n / p.parts)], p.parts);
     if (p.parts > 1) {
