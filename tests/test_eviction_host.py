@@ -266,3 +266,26 @@ def test_evict_tokens_checks_its_arguments(over, message):
 
     with pytest.raises(ValueError, match=message):
         evict_tokens(**evict_args(**over), reuse={})
+
+
+@pytest.mark.parametrize("name", ("target_len", "keep_len"))
+@pytest.mark.parametrize("words", (-1, 1))
+def test_evict_refuses_a_new_length_that_overlaps_an_old_one(name, words):
+    from ds355 import _lib
+
+    d = evict_desc(**{name: 3 * FAKE + 4 * words})
+    refuses(lambda: _lib.load().ds_evict(None, ctypes.byref(d)), "memory of its own")
+    d = evict_desc(**{name: 3 * FAKE + 8 * words})  # the two rows' words are apart
+    refuses(lambda: _lib.load().ds_evict(None, ctypes.byref(d)), "ds_evict_workspace_bytes")
+
+
+@pytest.mark.parametrize("over,message", (
+    (dict(num_q_heads=1 << 17, num_kv_heads=1), "query heads for a KV head"),
+    (dict(q_row_stride=1 << 29), "strides"), (dict(lse_token_stride=-8), "strides"), (dict(lse_head_stride=1 << 29), "strides"),
+    (dict(num_q_heads=1 << 16, num_kv_heads=1, tokens=1 << 14, q_head_stride=8, q_row_stride=8), "too many"),
+))
+def test_attention_mass_refuses_places_past_32_bits(over, message):
+    from ds355 import _lib
+
+    d = mass_desc(workspace_bytes=1 << 60, **over)
+    refuses(lambda: _lib.load().ds_attention_mass(None, ctypes.byref(d)), message)

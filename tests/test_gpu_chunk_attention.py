@@ -489,3 +489,54 @@ def test_shared_prefix_attention_gives_the_same(cuda):
     pa.shared_prefix_attention(**other)
     torch.cuda.synchronize()
     check(case, other, expected)
+
+
+def test_two_calls_at_once_on_two_streams(cuda):
+    from ds355 import chunk_attention as ca
+
+    cases = [build(70 + i, lens=[900, 120], qlens=[300, 1], hq=8, hkv=2, d=128, block=16, dtype=torch.bfloat16)
+             for i in range(2)]
+    args = [device_args(c, cuda) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for s, a in zip(streams, args):
+        with torch.cuda.stream(s):
+            ca.chunk_attention(**a)
+    torch.cuda.synchronize()
+    for c, a in zip(cases, args):
+        check(c, a)
+
+
+def test_output_in_place_of_the_query(cuda):
+    case = build(72, lens=[3000, 200, 64], qlens=[3, 200, 64], hq=8, hkv=2, d=128, block=16, dtype=torch.bfloat16)
+    args = device_args(case, cuda)
+    run(args)
+    again = dict(args, output=args["query"].clone())
+    run(dict(again, query=again["output"]))
+    # Tokens that no row has keep what was there, here the query.
+    check(case, dict(again, output=torch.where((args["output"] == 7).all(-1, keepdim=True), args["output"], again["output"])))
+    for start, q in zip(case["starts"], case["qlens"]):
+        assert torch.equal(again["output"][start: start + q], args["output"][start: start + q])
+    assert torch.equal(again["output"][:1], args["query"][:1])
+
+
+@pytest.mark.parametrize("d,hkv,block", ((64, 1, 8), (64, 2, 24), (128, 1, 4), (128, 2, 20), (256, 1, 2), (256, 1, 6), (128, 1, 2)))
+def test_runs_of_pages(cuda, d, hkv, block):
+    # Long rows of small pages: their places are looked up for many tiles at a time.
+    case = build(73, lens=[5003, 4096, 1033], qlens=[1, 200, 33], hq=4 * hkv, hkv=hkv, d=d, block=block, dtype=torch.bfloat16,
+                 window=None)
+    args = device_args(case, cuda)
+    run(args)
+    check(case, args)
+    # A page that is not there, in the middle of a run, reads as zeros.
+    page = 2500 // block
+    for b, n in enumerate(case["lens"]):
+        if page * block < n:
+            args["block_table"][b, page] = 10 ** 6
+            for kv in case["dense"][b][:2]:
+                kv[page * block: (page + 1) * block] = 0
+    args["output"].fill_(7)
+    args["lse"].fill_(7)
+    run(args)
+    check(case, args, status=4)

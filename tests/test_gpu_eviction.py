@@ -609,3 +609,184 @@ def test_a_request_kept_at_its_budget(cuda):
                     held = set(positions[b, h, :n].tolist())
                     assert len(held) == n and set(range(4)) <= held and set(range(done[b] - 16, done[b])) <= held
     assert int(pool.status.item()) == 0
+
+
+# ---- sizes, graphs and streams -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("d,hq,hkv,most", ((256, 16, 1, 2), (128, 32, 2, 3), (128, 4, 4, 5), (64, 8, 1, 4)))
+def test_mass_of_as_many_rows_as_there_may_be(cuda, d, hq, hkv, most):
+    lens = [1 + (b * 37) % 90 for b in range(1024)]
+    case = mass_case(400, lens=lens, qlens=[min(n, 1 + b % most) for b, n in enumerate(lens)], hq=hq, hkv=hkv, d=d, block=16,
+                     dtype=torch.bfloat16)
+    args = mass_args(case, cuda)
+    run_mass(args)
+    check_mass(case, args)
+
+
+def test_mass_of_one_long_row_beside_short_ones(cuda):
+    lens = [3000, 1, 17, 64, 65, 2] + [5] * 20
+    case = mass_case(401, lens=lens, qlens=[700, 1, 17, 1, 65, 2] + [1] * 20, hq=8, hkv=2, d=64, block=16,
+                     dtype=torch.float16, window=900)
+    args = mass_args(case, cuda)
+    run_mass(args)
+    check_mass(case, args)
+
+
+def test_mass_graphs_share_a_workspace(cuda):
+    from ds355 import eviction
+
+    shape = dict(hq=8, hkv=2, d=128, block=16, dtype=torch.bfloat16, capacity=640)
+    cases = [mass_case(410 + i, lens=n, qlens=q, **shape)
+             for i, (n, q) in enumerate((([600, 31, 80], [100, 1, 19]), ([44, 620, 300], [1, 118, 1])))]
+    args = [mass_args(c, cuda) for c in cases]
+    for a in args:
+        a["workspace"] = args[0]["workspace"]
+        run_mass(a)
+    stream, graphs = torch.cuda.Stream(), []
+    for a in args:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            eviction.attention_mass(**a)
+        graphs.append(graph)
+    expected = [expect_mass(c) for c in cases]
+    for i in (0, 1, 1, 0, 1):
+        args[i]["mass"].fill_(7)
+        args[i]["workspace"].fill_(255)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        check_mass(cases[i], args[i], expected[i])
+        replayed = args[i]["mass"].clone()
+        run_mass(args[i])
+        assert torch.equal(replayed, args[i]["mass"])
+    # Other lengths at the same addresses.
+    a = args[0]
+    for n, q in (([300, 0, 79], [100, 0, 19]), ([1, 31, 5], [1, 1, 0])):
+        case = dict(cases[0], lens=n, qlens=q)
+        a["target_len"].copy_(i32(n, "cpu"))
+        a["query_len"].copy_(i32(q, "cpu"))
+        a["mass"].fill_(7)
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        case["dense"] = [tuple(x[:m] for x in kv) for kv, m in zip(cases[0]["dense"], n)]
+        check_mass(case, a)
+
+
+def test_mass_on_two_streams_and_with_reuse(cuda):
+    cases = [mass_case(420 + i, lens=[500, 90], qlens=[60, 1], hq=8, hkv=2, d=128, block=16, dtype=torch.bfloat16)
+             for i in range(2)]
+    reuse = {}
+    args = [mass_args(c, cuda, reuse=reuse) for c in cases]
+    from ds355 import eviction
+
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for s, a in zip(streams, args):
+        with torch.cuda.stream(s):
+            eviction.attention_mass(**a)
+    torch.cuda.synchronize()
+    for c, a in zip(cases, args):
+        check_mass(c, a)
+    assert len(reuse) == 1
+
+
+def test_mass_places_past_32_bits(cuda):
+    # A cache of 5 GiB: the row's pages lie at both of its ends.
+    block, hkv, d = 128, 8, 128
+    pages = 20500
+    keys = torch.zeros((pages, block, hkv, d), dtype=torch.bfloat16, device=cuda)
+    case = mass_case(430, lens=[500], qlens=[90], hq=16, hkv=hkv, d=d, block=block, dtype=torch.bfloat16)
+    spots = [pages - 1, 3, pages - 700, 16400]
+    for i, page in enumerate(case["table"][0, :4].tolist()):
+        keys[spots[i]] = case["cache"][0][page].to(cuda)
+    args = mass_args(case, cuda, key_cache=keys)
+    args["block_table"][0, :4] = torch.tensor(spots, dtype=torch.int32)
+    run_mass(args)
+    check_mass(case, args)
+
+
+def test_eviction_places_past_32_bits(cuda):
+    block, hkv, d = 128, 8, 128
+    pages = 20500
+    case = evict_case(431, lens=[500], keep=[300], hkv=hkv, d=d, block=block, sinks=2, recent=9)
+    expected = expect_evict(case)
+    spots = [16400, pages - 1, 3, pages - 700]
+    args = evict_args(case, cuda)
+    mine = case["table"][0, :4].tolist()
+    for i, name in enumerate(("key_cache", "value_cache")):
+        big = torch.zeros((pages, block, hkv, d), dtype=torch.bfloat16, device=cuda)
+        big[spots] = case["caches"][i][mine].to(cuda)
+        args[name] = big
+    args["block_table"][0, :4] = torch.tensor(spots, dtype=torch.int32)
+    run_evict(args)
+    for name in ("key_cache", "value_cache"):
+        assert same(args[name][spots], expected.pop(name)[mine])
+        assert int((args[name].flatten(1) != 0).any(1).sum()) == 4
+    check_evict(case, args, expected)
+
+
+@pytest.mark.parametrize("shape", (
+    dict(lens=[70000], keep=[66000], spread=50),  # more slots than are held, ties on both sides of that many
+    dict(lens=[32769, 32768], keep=[32768, 1], settled=[(32768, 5), (100, 3)], recent=0),
+    dict(lens=[40000], keep=[33000], settled=[(39000, 12)], sinks=70, recent=500, spread=3),
+    dict(lens=[8192, 8193, 4096, 4097], keep=[8000, 8192, 64, 4032], sinks=1, recent=2),
+))
+def test_eviction_of_long_rows(cuda, shape):
+    case = evict_case(440, hkv=1, d=8, block=128, **shape)
+    args = evict_args(case, cuda)
+    run_evict(args)
+    check_evict(case, args)
+
+
+def test_evictions_graphs_share_a_workspace(cuda):
+    from ds355 import eviction
+
+    cases = [evict_case(450 + i, lens=n, keep=k, hkv=2, d=64, block=16, recent=5)
+             for i, (n, k) in enumerate((([500, 300], [100, 299]), ([77, 400], [76, 33])))]
+    args = [evict_args(c, cuda) for c in cases]
+    work = eviction.new_evict_workspace(2, 2, max(c["capacity"] for c in cases), cuda)
+    starts = []
+    stream, graphs = torch.cuda.Stream(), []
+    for a in args:
+        a["workspace"] = work
+        starts.append({k: v.clone() for k, v in a.items() if isinstance(v, torch.Tensor) and k != "workspace"})
+        run_evict(a)
+    for a in args:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            eviction.evict_tokens(**a)
+        graphs.append(graph)
+    for order in ((0, 1), (1, 0), (1, 1, 0, 0)):
+        for i in order:
+            for k, v in starts[i].items():
+                args[i][k].copy_(v)
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            check_evict(cases[i], args[i])
+
+
+def test_eviction_without_rows_and_of_padding_rows(cuda):
+    case = evict_case(460, lens=[200, 300, 100], keep=[100, 100, 50], hkv=2, d=64, block=16)
+    args = evict_args(case, cuda)
+    before = {k: args[k].clone() for k in ("key_cache", "value_cache", "mass", "positions", "settled", "kept_len")}
+    run_evict(dict(args, batch_size=0))
+    for k, v in before.items():
+        assert same(args[k], v), k
+    # Rows of no length and of fewer slots than they may keep.
+    case["lens"] = [0, 99, -3]
+    args["target_len"].copy_(i32(case["lens"], "cpu"))
+    run_evict(args)
+    check_evict(case, args)
+
+
+def test_the_same_eviction_twice_changes_nothing(cuda):
+    case = evict_case(461, lens=[700, 90], keep=[128, 64], hkv=2, d=128, block=16, sinks=4, recent=32)
+    args = evict_args(case, cuda)
+    run_evict(args)
+    check_evict(case, args)
+    after = {k: args[k].clone() for k in ("key_cache", "value_cache", "mass", "positions", "settled", "kept_len")}
+    args["target_len"].copy_(args["kept_len"])
+    run_evict(args)
+    for k, v in after.items():
+        assert same(args[k], v), k

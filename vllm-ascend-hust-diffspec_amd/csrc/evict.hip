@@ -395,7 +395,12 @@ int evict_impl(hipStream_t stream, const ds_evict_desc* d) {
                  d->keep_len && d->kept_len,
              "null tensor pointer");
   // Heads of a row read its lengths while one of them writes its new one.
-  DS_REQUIRE(d->kept_len != d->target_len && d->kept_len != d->keep_len, "kept_len must be memory of its own");
+  const auto apart = [&](const int32_t* x) {
+    const uintptr_t one = reinterpret_cast<uintptr_t>(d->kept_len), other = reinterpret_cast<uintptr_t>(x);
+    const uintptr_t bytes = sizeof(int32_t) * static_cast<uintptr_t>(d->rows);
+    return one + bytes <= other || other + bytes <= one;
+  };
+  DS_REQUIRE(apart(d->target_len) && apart(d->keep_len), "kept_len must be memory of its own");
   const int64_t strides[] = {d->k_block_stride, d->k_token_stride, d->k_head_stride,
                              d->v_block_stride, d->v_token_stride, d->v_head_stride};
   for (int64_t s : strides) DS_REQUIRE(s >= 0 && s * size % 16 == 0, "page and head strides must be multiples of 16 bytes");
