@@ -19,7 +19,8 @@
 // are kept and how many slots to move to and from lie before them.
 //
 // evict_move_kernel: a workgroup takes 64 of a head's moves at a time, finds their slots from those counts, and
-// moves keys, values, masses and positions.
+// moves keys, values, masses and positions.  Slots that do not move get their masses and positions here as well,
+// where there are many workgroups.
 #include "matrix.h"
 
 namespace ds355 {
@@ -98,17 +99,31 @@ __device__ __forceinline__ int wave_prefix(int count, int* scratch, int& all) {
   return __builtin_amdgcn_readlane(inclusive - mine, uniform(wave));
 }
 
+// The i-th set bit of `bits`, which has more.
+__device__ __forceinline__ int set_bit(uint64_t bits, int i) {
+  int at = 0;
+#pragma unroll
+  for (int width = 32; width >= 1; width >>= 1) {
+    const int low = __popcll((bits >> at) & ((1ull << width) - 1));
+    if (i >= low) i -= low, at += width;
+  }
+  return at;
+}
+
 // HELD: slots whose values are held in shared memory; those of a longer row are read again for every pass.
 template <int HELD>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs a) {
   constexpr int kGroups = HELD / 64;  // of 64 slots, a wave's
   static_assert(kGroups <= kSelectThreads && HELD < 65536, "a thread a group; two counts of a chunk in a word");
   __shared__ uint32_t values[HELD];
-  __shared__ int histogram[kBins];
+  __shared__ __attribute__((aligned(16))) int histogram[kBins];
   __shared__ uint32_t few[kFew];
   __shared__ int scratch[kSelectWaves];
-  __shared__ int group_ties[kGroups];
-  __shared__ uint32_t group_moves[kGroups];  // holes, and movers in the upper half
+  struct Masks {
+    uint64_t more, equal;  // of a group's slots: values above the least kept one, and like it
+  };
+  static_assert(kGroups * sizeof(Masks) <= sizeof(histogram), "where the histogram was");
+  Masks* masks = reinterpret_cast<Masks*>(histogram);
   __shared__ int found, left, share, refused, few_held;
   const int b = blockIdx.x / a.hkv, h = blockIdx.x - b * a.hkv;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -135,6 +150,15 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
   };
   if (tid == 0) refused = 0, few_held = 0;
   for (int i = tid; i < kBins; i += kSelectThreads) histogram[i] = 0;
+  constexpr int kFirst = 21;  // the first histogram is of the bits from it on
+  auto counted = [](uint32_t x) { return x - 1 < kAlways - 1 && x != kZero; };
+  int always = 0, zeros = 0;
+  auto count_first = [&](uint32_t x) {
+    always += x == kAlways;
+    zeros += x == kZero;
+    if (counted(x)) atomicAdd(&histogram[x >> kFirst], 1);
+  };
+  __syncthreads();
   if (asked) {
     // Eight loads of a thread are under way before the first is looked at.
     const int last = min(n, HELD) - 1;
@@ -147,7 +171,11 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
       for (int i = 0; i < 8; ++i) place[i] = position(min(first + i * kSelectThreads, last));
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (first + i * kSelectThreads <= last) values[first + i * kSelectThreads] = value_of(place[i], weight[i]);
+        if (first + i * kSelectThreads <= last) {
+          const uint32_t x = value_of(place[i], weight[i]);
+          values[first + i * kSelectThreads] = x;
+          count_first(x);
+        }
       }
     }
     for (int i = tid; i < ceil_div(n, a.block_size); i += kSelectThreads) {
@@ -159,17 +187,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
       }
     }
   }
-  __syncthreads();
-  constexpr int kFirst = 21;  // the first histogram is of the bits from it on
-  auto counted = [](uint32_t x) { return x - 1 < kAlways - 1 && x != kZero; };
-  int always = 0, zeros = 0;
-  if (asked) {
-    each(0, n, [&](int, uint32_t x) {
-      always += x == kAlways;
-      zeros += x == kZero;
-      if (counted(x)) atomicAdd(&histogram[x >> kFirst], 1);
-    });
-  }
+  if (asked) each(HELD, n, [&](int, uint32_t x) { count_first(x); });
   wave_prefix(wave_total(always), scratch, always);
   wave_prefix(wave_total(zeros), scratch, zeros);
   bits |= refused;
@@ -233,74 +251,41 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs 
   value = max(value, 1u);  // no slots have 0
   if (keep == 0) value = kAlways, need = 0;
 
-  // Slots in order, group by group: a scan over the groups' counts says where each begins.
-  const uint64_t below = (1ull << lane) - 1;
-  auto scan_groups = [&](auto* counts) {  // counts become those of the groups before; returns the sum
-    const int mine = tid < kGroups ? counts[tid] : 0, inclusive = wave_inclusive_scan(mine);
-    int all;
-    const int before = wave_prefix(__builtin_amdgcn_readlane(inclusive, 63), scratch, all);
-    if (tid < kGroups) counts[tid] = before + inclusive - mine;
-    return static_cast<uint32_t>(all);
-  };
+  // Slots in order, group by group: a scan over the groups' counts says what lies before each.
   Group* list = a.lists + static_cast<int64_t>(blockIdx.x) * a.groups;
   int ties = 0, holes = 0, movers = 0;  // of the chunks before
   constexpr int kChunk = 64 * kGroups;
   for (int first = 0; first < n; first += kChunk) {
     const int end = min(first + kChunk, n);
-    auto group_of = [&](int t) { return (t - first) >> 6; };
     __syncthreads();
-    if (tid < kGroups) group_ties[tid] = 0, group_moves[tid] = 0;
-    __syncthreads();
-    int ties_here = 0;
-    if (need != INT_MAX) {
-      each(first, end, [&](int t, uint32_t x) {
-        const int equal = __popcll(__ballot(x == value));
-        if (lane == 0) group_ties[group_of(t)] = equal;
-      });
-      __syncthreads();
-      ties_here = scan_groups(group_ties);
-      __syncthreads();
-    }
     each(first, end, [&](int t, uint32_t x) {
-      bool mine = x >= value;
-      if (need != INT_MAX) {
-        const uint64_t equal = __ballot(x == value);
-        mine = x > value || (x == value && ties + group_ties[group_of(t)] + __popcll(equal & below) < need);
-      }
-      const uint64_t kept = __ballot(mine);
-      const int low_slots = keep - (t - lane);  // slots below `keep` exist
-      const uint64_t low = low_slots >= 64 ? ~0ull : low_slots <= 0 ? 0ull : (1ull << low_slots) - 1;
-      if (lane == 0) {
-        group_moves[group_of(t)] = __popcll(low & ~kept) | __popcll(kept & ~low) << 16;
-        list[t >> 6].kept = kept;
-      }
-      if (t >= keep) {
-        if (!mine && t < n) mass[t] = 0.f;
-      } else if (mine && t >= known) {
-        positions[t] = t + gone;
-      }
+      const uint64_t more = __ballot(x > value), equal = __ballot(x == value);
+      if (lane == 0) masks[(t - first) >> 6] = Masks{more, equal};
     });
     __syncthreads();
-    const uint32_t moves_here = scan_groups(group_moves);
-    __syncthreads();
-    for (int group = tid; group < ceil_div(end - first, 64); group += kSelectThreads) {
-      Group& g = list[first / 64 + group];
-      g.holes = holes + (group_moves[group] & 0xffff), g.movers = movers + (group_moves[group] >> 16);
+    const bool mine = tid < ceil_div(end - first, 64);  // a thread a group
+    const Masks m = mine ? masks[tid] : Masks{0, 0};
+    const int equal = __popcll(m.equal), inclusive = wave_inclusive_scan(equal);
+    int ties_here;
+    const int before = ties + wave_prefix(__builtin_amdgcn_readlane(inclusive, 63), scratch, ties_here) + inclusive - equal;
+    const int take = need - before;  // of the values like the least kept one
+    const uint64_t kept =
+        m.more | (take >= equal ? m.equal : take <= 0 ? 0 : m.equal & ((1ull << set_bit(m.equal, take)) - 1));
+    const int low_slots = keep - (first + 64 * tid);  // slots below `keep` exist
+    const uint64_t low = low_slots >= 64 ? ~0ull : low_slots <= 0 ? 0ull : (1ull << low_slots) - 1;
+    // Holes, and movers in the upper half.
+    const int moves = mine ? __popcll(low & ~kept) | __popcll(kept & ~low) << 16 : 0;
+    const int moves_inclusive = wave_inclusive_scan(moves);
+    int moves_here;
+    const uint32_t moves_before =
+        wave_prefix(__builtin_amdgcn_readlane(moves_inclusive, 63), scratch, moves_here) + moves_inclusive - moves;
+    if (mine) {
+      list[first / 64 + tid] =
+          Group{kept, holes + static_cast<int>(moves_before & 0xffff), movers + static_cast<int>(moves_before >> 16)};
     }
-    ties += ties_here, holes += moves_here & 0xffff, movers += moves_here >> 16;
+    ties += ties_here, holes += moves_here & 0xffff, movers += static_cast<uint32_t>(moves_here) >> 16;
   }
   if (tid == 0) a.heads[blockIdx.x] = Head{holes, known, gone, ceil_div(n, 64)};  // as many movers as holes
-}
-
-// The i-th set bit of `bits`, which has more.
-__device__ __forceinline__ int set_bit(uint64_t bits, int i) {
-  int at = 0;
-#pragma unroll
-  for (int width = 32; width >= 1; width >>= 1) {
-    const int low = __popcll((bits >> at) & ((1ull << width) - 1));
-    if (i >= low) i -= low, at += width;
-  }
-  return at;
 }
 
 constexpr int kMoves = 64;         // moves of a workgroup at a time
@@ -316,15 +301,27 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
     a.settled[2 * b + 1] = head.gone + a.t_len[b] - keep;
     a.settled[2 * b] = keep;
   }
-  if (static_cast<int>(blockIdx.x) * kMoves >= head.moves) return;
   const Group* list = a.lists + static_cast<int64_t>(blockIdx.y) * a.groups;
+  float* mass = a.mass + b * a.m_row + h * a.m_head;
+  int32_t* positions = a.positions + b * a.p_row + h * a.p_head;
+  // Slots that do not move: those given up lose their mass, and kept ones get their positions.
+  constexpr int kWaves = kMoveThreads / 64;
+  const int n = a.t_len[b], lane = tid & 63;
+  for (int g = min(head.known, keep) / 64 + blockIdx.x * kWaves + (tid >> 6); g < head.groups; g += gridDim.x * kWaves) {
+    const int t = 64 * g + lane;
+    const bool kept = list[g].kept >> lane & 1;
+    if (t >= keep) {
+      if (!kept && t < n) mass[t] = 0.f;
+    } else if (kept && t >= head.known) {
+      positions[t] = t + head.gone;
+    }
+  }
+  if (static_cast<int>(blockIdx.x) * kMoves >= head.moves) return;
   const bool shared = head.groups <= kMostSearched;
   if (shared) {
     for (int g = tid; g < head.groups; g += kMoveThreads) before[g] = int2{list[g].holes, list[g].movers};
   }
   const int32_t* pages = a.table + b * a.bt_stride;
-  float* mass = a.mass + b * a.m_row + h * a.m_head;
-  int32_t* positions = a.positions + b * a.p_row + h * a.p_head;
   for (int first = blockIdx.x * kMoves; first < head.moves; first += gridDim.x * kMoves) {
     const int count = min(kMoves, head.moves - first);
     __syncthreads();
