@@ -531,7 +531,8 @@ size_t ds_prefix_attention_workspace_bytes(int rows, int tokens, int num_q_heads
  * weight rounds to 0).
  * Output and LSE rows of tokens that belong to no row are left as they were.
  * Rows with query_len <= 0 (graph padding) have no token.  Rows must not
- * share query tokens; query_len 1 is a row that decodes.
+ * share query tokens; query_len 1 is a row that decodes.  output may be query
+ * itself, and else must be memory apart.
  * *status (optional, the caller clears it) gets bit 0 when a row's query
  * tokens are out of range or more than `tokens` in all (that row and, in the
  * second case, the rows after it are left out), bit 1 when a row is longer
@@ -589,7 +590,8 @@ size_t ds_chunk_attention_workspace_bytes(int rows, int tokens, int num_q_heads,
  *   mass[b, h, t] = decay * previous[b, h, t]
  *                 + sum_{i that see t} sum_{query heads g of h} exp(scale * q_ig . k_t - lse_ig)
  * in fp32, summed in an order that the lengths alone determine.  previous
- * (may be NULL: all 0, or be mass itself) and mass: fp32 [rows, Hkv,
+ * (may be NULL: all 0, or be mass itself with its strides, or memory apart
+ * from it) and mass: fp32 [rows, Hkv,
  * capacity], contiguous in the last dimension, strides in the descriptor.
  * Entries at or past target_len[b], and rows with query_len <= 0, are left as
  * they were.  A query head whose lse is -infinity adds nothing.  A key that
@@ -601,11 +603,13 @@ size_t ds_chunk_attention_workspace_bytes(int rows, int tokens, int num_q_heads,
  * outside [0, num_blocks) (its keys read as 0).
  *
  * query, key_cache: as in ds_chunk_attention; lse: fp32, strides in the
- * descriptor; at most 2^29 keys a row.
+ * descriptor; at most 2^29 keys a row, 2^16 query heads for a KV head, and
+ * query and LSE strides that are not negative and of at most 2^30 elements
+ * over 64 query rows (row = token * (Hq / Hkv) + head).
  * workspace: caller's scratch of ds_attention_mass_workspace_bytes(), 256-byte
  * aligned, with no state between calls (one launch at a time).
- * One kernel, a second one where a row may have more than 256 / (Hq / Hkv)
- * query tokens; launch shape fixed by the sizes (graph-capturable).
+ * One kernel, a second one where tokens * Hq / Hkv > 256; launch shape fixed by
+ * the sizes (graph-capturable).
  */
 typedef struct ds_attention_mass_desc {
   int dtype;                         /* DS_BF16 / DS_FP16 */
@@ -664,7 +668,7 @@ size_t ds_attention_mass_workspace_bytes(void);
  * key_cache, value_cache: [num_blocks, block_size, Hkv, D], 16-byte aligned,
  * D contiguous, D and all strides multiples of 16 bytes; mass fp32 and
  * positions int32 [rows, Hkv, capacity], contiguous in the last dimension;
- * kept_len is memory of its own.  At most 1024 rows, 65535 heads of all rows
+ * kept_len overlaps neither target_len nor keep_len.  At most 1024 rows, 65535 heads of all rows
  * and 2^29 slots a row.
  * workspace: caller's scratch of ds_evict_workspace_bytes(), 256-byte aligned,
  * with no state between calls (one launch at a time).

@@ -12,6 +12,8 @@ Drop-in replacements for the reference plugin's hot path:
 The verifier's side of a step, for targets served through this library:
 
 - ``ds355.prefix_attention.shared_prefix_attention``  (paged attention and LSE, a shared prefix read once)
+- ``ds355.chunk_attention.chunk_attention``           (chunks of new tokens over the paged cache, causal, windowed)
+- ``ds355.eviction.attention_mass``, ``evict_tokens`` (a bounded target cache: received attention weight, kept slots)
 - ``ds355.qk_rope.qk_norm_rope``                      (head norm, rotation and paged write in one pass)
 - ``ds355.pages.PagePool``                            (fork, extend, free, copy and compact pages)
 

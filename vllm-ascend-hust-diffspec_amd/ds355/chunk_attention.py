@@ -70,7 +70,8 @@ def chunk_attention(
     ``window``: each query token sees itself and the ``window - 1`` keys
     before it (None: all).  A query token that sees no key gets a zero
     output and an LSE of -infinity; output and LSE rows of tokens that no
-    row has (graph padding) are left as they were.  Rows at or beyond
+    row has (graph padding) are left as they were.  ``output`` may be
+    ``query`` itself.  Rows at or beyond
     ``batch_size`` are padding.  Rows must not share query tokens.
 
     ``status`` (an int32 device word the caller clears) receives

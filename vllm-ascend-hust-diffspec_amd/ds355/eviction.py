@@ -125,7 +125,7 @@ def attention_mass(
     whose rows, table, ``window`` and ``lse`` these are) and the query heads
     of KV head h, for t < ``target_len[b]``.  ``mass`` and ``previous`` are
     fp32 ``[rows, Hkv, capacity]``; ``previous`` may be ``mass`` itself (it
-    is then added to in place) or None for zeros.  Entries at or past a
+    is then added to in place), memory apart from it, or None for zeros.  Entries at or past a
     row's length, and rows without query tokens, are left as they were.
     Rows may name only the last tokens of each request.
 
@@ -231,8 +231,8 @@ def evict_tokens(
     ``recent`` ones, then the slots of largest ``mass`` (ties to the lowest
     slot, NaN below all numbers).  Kept slots below ``keep_len[b]`` stay; the
     others move, in order, to the slots that are given up there, with their
-    keys, values, mass and positions.  ``kept_len`` (int32 ``[rows]``, memory
-    of its own) gets each row's new length.
+    keys, values, mass and positions.  ``kept_len`` (int32 ``[rows]``, apart
+    from the other lengths) gets each row's new length.
 
     ``key_cache`` / ``value_cache`` ``[blocks, block_size, Hkv, D]`` (bf16,
     fp16 or fp32); ``mass`` fp32 and ``positions`` int32 ``[rows, Hkv,
