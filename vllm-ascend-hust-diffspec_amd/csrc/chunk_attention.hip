@@ -30,6 +30,7 @@ constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
 constexpr int kTile = 64;  // keys of a staged tile
+constexpr int kScores = kTile / 32;  // score products of a wave's tile
 constexpr int chunk_waves(int d) { return d == 64 ? 3 : d == 128 ? 2 : 1; }  // workgroups of a CU, waves of a SIMD
 int part_slots(int d) { return chunk_waves(d) * device_cu_count(); }  // workgroups that run at a time
 
@@ -393,15 +394,15 @@ __device__ __forceinline__ void add_not_finite(const Cache& a, const int32_t* pa
   }
 }
 
-// Scores of 32 N keys from key t0 of the tile on.  (Piece 2 s + half of a key is turned as piece `half` is, and 2 s
+// Scores of a tile's keys.  (Piece 2 s + half of a key is turned as piece `half` is, and 2 s
 // then differs in bits of its own; the turn repeats every 16 keys.)
-template <int DT, int D, int N>
-__device__ __forceinline__ void score(const char* keys, const u32x4 (&q)[Chunk<D>::kSteps], int t0, f32x16 (&sc)[N]) {
+template <int DT, int D>
+__device__ __forceinline__ void score(const char* keys, const u32x4 (&q)[Chunk<D>::kSteps], f32x16 (&sc)[kScores]) {
   using C = Chunk<D>;
   const int lane = fresh_thread() & 63, half = lane >> 5, t = lane & 31;
-  const uint32_t at = (t0 + t) * C::kRowBytes + 16 * (half ^ key_turn<D>(t));
+  const uint32_t at = t * C::kRowBytes + 16 * (half ^ key_turn<D>(t));
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
+  for (int n = 0; n < kScores; ++n) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[n][i] = 0.f;
 #pragma unroll
@@ -411,16 +412,16 @@ __device__ __forceinline__ void score(const char* keys, const u32x4 (&q)[Chunk<D
   }
 }
 
-// One tile for one wave: 32 N keys from key t0 of it on, whose scores are in `sc`; it then gets those of the
+// One tile for one wave, whose scores are in `sc`; it then gets those of the
 // next tile, whose products run while the weights are computed.
-template <int DT, int D, int N>
+template <int DT, int D>
 __device__ __forceinline__ void attend(const char* next_keys, const char* values, const u32x4 (&q)[Chunk<D>::kSteps],
-                                       Softmax<D>& st, f32x16 (&sc)[N], int t0, float scale_log2) {
+                                       Softmax<D>& st, f32x16 (&sc)[kScores], float scale_log2) {
   using C = Chunk<D>;
   const int lane = fresh_thread() & 63, half = lane >> 5, l = lane & 15;
   float top = -INFINITY;
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
+  for (int n = 0; n < kScores; ++n) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[n][i]);
   }
@@ -442,11 +443,11 @@ __device__ __forceinline__ void attend(const char* next_keys, const char* values
     }
   }
   const float m = st.m == -INFINITY ? 0.f : st.m;
-  f32x16 next[N];
-  score<DT, D, N>(next_keys, q, t0, next);
-  u32x4 p[2 * N];
+  f32x16 next[kScores];
+  score<DT, D>(next_keys, q, next);
+  u32x4 p[2 * kScores];
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
+  for (int n = 0; n < kScores; ++n) {
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
       const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i], scale_log2, -m));
@@ -459,10 +460,10 @@ __device__ __forceinline__ void attend(const char* next_keys, const char* values
   }
   // The lane's own probabilities are the B operand: k-slot (half, e) of step s is key 16 s + 8 (e /
   // 4) + 4 half + e % 4 of the keys, and the values are read in that order.
-  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)values)) + t0 * C::kRowBytes +
+  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)values)) +
                         8 * (l & 1) + 16 * piece_at<D>(4 * half + (l >> 2), 2 * ((lane >> 4) & 1) + ((l & 3) >> 1));
 #pragma unroll
-  for (int s = 0; s < 2 * N; ++s) {
+  for (int s = 0; s < 2 * kScores; ++s) {
 #pragma unroll
     for (int j = 0; j < C::kBlocks; ++j) {
       const u32x2 lo = read_values((base ^ (64 * j)) + 16 * s * C::kRowBytes);
@@ -471,7 +472,7 @@ __device__ __forceinline__ void attend(const char* next_keys, const char* values
     }
   }
 #pragma unroll
-  for (int n = 0; n < N; ++n) sc[n] = next[n];
+  for (int n = 0; n < kScores; ++n) sc[n] = next[n];
 }
 
 // A wave's place in its item.
@@ -482,12 +483,11 @@ struct Rows {
   int item_from, item_to;  // keys that all rows of the item see
 };
 
-// The part's tiles of keys, `tiles` from key `key` on, 32 N keys of each for a wave.  In shared memory the keys
-// run a tile ahead of the values: while a tile is weighed, the next one's scores are computed, the keys
-// after that and the next values are on their way, and the pages of the keys behind them are looked up.
-template <int DT, int D, bool WHOLE, int N>
+// The part's tiles of keys, `tiles` from key `key` on.  In shared memory the keys run a tile ahead of the values: while a tile is weighed, the next one's scores are computed, and the keys
+// after that and the next values are on their way.
+template <int DT, int D, bool WHOLE>
 __device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, int key, int end, int tiles, const Rows& rows,
-                                         const u32x4 (&q)[Chunk<D>::kSteps], Softmax<D>& st, int t0,
+                                         const u32x4 (&q)[Chunk<D>::kSteps], Softmax<D>& st,
                                          int wave, char* lds, int (&poison)[2][4]) {
   using C = Chunk<D>;
   const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_char*)lds)) +
@@ -527,8 +527,8 @@ __device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, i
   lds_barrier();
   send_values(0);
   send_keys(1);
-  f32x16 sc[N];
-  if (rows.any) score<DT, D, N>(lds, q, t0, sc);
+  f32x16 sc[kScores];
+  if (rows.any) score<DT, D>(lds, q, sc);
   const unsigned count = max(rows.limit - rows.lower, 0);
   for (int i = 0; i < tiles; ++i, key += kTile) {
     const int here = i & 1;  // the tile's half of shared memory
@@ -542,22 +542,21 @@ __device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, i
     send_values(here ^ 1);
     send_keys(here);
     if (!rows.any) continue;
-    const int at = key + t0;
-    if (at < rows.all_from || at + 32 * N > rows.all_to) {
-      const int from = rows.lower - at, half = (fresh_thread() >> 5) & 1;
+    if (key < rows.all_from || key + kTile > rows.all_to) {
+      const int from = rows.lower - key, half = (fresh_thread() >> 5) & 1;
       if (__any(poison[here][fresh_thread() & 3])) {
-        const int page = at / a.block_size;
-        add_not_finite<DT, D>(a, table + page, at - page * a.block_size, min(32 * N, end - at), st, from, count);
+        const int page = key / a.block_size;
+        add_not_finite<DT, D>(a, table + page, key - page * a.block_size, min(kTile, end - key), st, from, count);
       }
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
+      for (int n = 0; n < kScores; ++n) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           if (static_cast<unsigned>(32 * n + 8 * (e >> 2) + (e & 3) + 4 * half - from) >= count) sc[n][e] = -INFINITY;
         }
       }
     }
-    attend<DT, D, N>(lds + (here ^ 1) * C::kStage, values, q, st, sc, t0, a.scale_log2);
+    attend<DT, D>(lds + (here ^ 1) * C::kStage, values, q, st, sc, a.scale_log2);
   }
 }
 
@@ -589,10 +588,7 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
   const Part p = a.parts[entry];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), half = lane >> 5;
   const int rows = p.len * a.group;
-  // Items of at most 64 query rows: two waves share a block of 32 rows and take half of each tile's keys.
-  const bool narrow = rows - p.tile * kItemRows <= 64;
-  const int block = narrow ? wave >> 1 : wave;
-  const int r0 = p.tile * kItemRows + 32 * block, r = r0 + (lane & 31);
+  const int r0 = p.tile * kItemRows + 32 * wave, r = r0 + (lane & 31);
   const int token = min(r, rows - 1) / a.group, head = h * a.group + min(r, rows - 1) - token * a.group;
   Rows w;
   w.any = r0 < rows;
@@ -626,44 +622,14 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
                       a.k_block, a.v_block, static_cast<uint32_t>(a.k_token), static_cast<uint32_t>(a.v_token),
                       a.num_blocks, a.block_size, a.per_block, a.scale_log2, a.status,
                       reinterpret_cast<uint64_t>(a.header->zeros)};
-    if (narrow) {
-      run_part<DT, D, WHOLE, 1>(cache, table, key, end, last - first, w, q, st, 32 * (wave & 1), wave, lds, poison);
-    } else {
-      run_part<DT, D, WHOLE, 2>(cache, table, key, end, last - first, w, q, st, 0, wave, lds, poison);
-    }
+    run_part<DT, D, WHOLE>(cache, table, key, end, last - first, w, q, st, wave, lds, poison);
   }
   st.l += other_half(st.l);
-  // The two waves of a narrow item's block join in shared memory.
   constexpr int kGroups = 4 * C::kBlocks;
   auto group = [&](int g) {
     return f32x4{st.acc[g >> 2][4 * (g & 3)], st.acc[g >> 2][4 * (g & 3) + 1], st.acc[g >> 2][4 * (g & 3) + 2],
                  st.acc[g >> 2][4 * (g & 3) + 3]};
   };
-  if (narrow) {
-    static_assert(2 * (kGroups * 4 + 2) * 64 * 4 <= sizeof(lds), "two waves' results fit the tile");
-    f32x4* area = reinterpret_cast<f32x4*>(lds) + block * kGroups * 64;
-    float* sums = reinterpret_cast<float*>(reinterpret_cast<f32x4*>(lds) + 2 * kGroups * 64) + block * 128;
-    __syncthreads();
-    if (w.any && (wave & 1)) {
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) area[g * 64 + lane] = group(g);
-      sums[lane] = st.m;
-      sums[64 + lane] = st.l;
-    }
-    __syncthreads();
-    if (!w.any || (wave & 1)) return;
-    const float om = sums[lane], m = fmaxf(st.m, om);
-    const float mine = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
-    const float other = om == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(om - m);
-    st.m = m;
-    st.l = st.l * mine + sums[64 + lane] * other;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const f32x4 x = group(g) * mine + area[g * 64 + lane] * other;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) st.acc[g >> 2][4 * (g & 3) + e] = x[e];
-    }
-  }
   if (r >= rows) return;
   const ChunkArgs z = arguments<ChunkArgs>();
   if (p.parts == 1) {
@@ -674,10 +640,10 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
   }
   float* sums = piece_at_slot<D>(z, (p.slot + p.part) * z.hkv + h);
   if (half == 0) {
-    sums[32 * block + lane] = st.m;
-    sums[kItemRows + 32 * block + lane] = st.l;
+    sums[32 * wave + lane] = st.m;
+    sums[kItemRows + 32 * wave + lane] = st.l;
   }
-  f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kItemRows) + block * kGroups * 64 + lane;
+  f32x4* o = reinterpret_cast<f32x4*>(sums + 2 * kItemRows) + wave * kGroups * 64 + lane;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) o[g * 64] = group(g);
 }
