@@ -15,6 +15,14 @@
 // of many key tiles are cut into parts of nearly one size, whose pieces (maximum, sum, output, in fp32)
 // chunk_join_kernel puts together.  chunk_plan_kernel derives items and parts from the lengths on the
 // device, so that a captured launch follows changed lengths, and lists them by size, the largest first.
+//
+// Each of four waves has 32 query rows as columns of the score product, so that a lane's scores are of one row and the
+// weights are in the layout that the second product takes; tiles of 64 keys go by in shared memory for all
+// four.  What bounds it: vector instructions beside the matrix units (about 210 a wave and tile against 32 products
+// of 32 cycles at 128 dimensions), and at 256 dimensions that a SIMD has registers for one wave only.  Measured,
+// 32 query heads on 8 of 128 dimensions: 4096 tokens on themselves 167 us (823 TFLOP/s), of which plan and join take 8;
+// 32 on 4, 512 tokens on 32 k keys 292 us (935); 11 mixed requests, 64 heads on 8 of 64 dimensions, 102 us (518); 3 chunks
+// of 16 heads on 2 of 256 dimensions, window 1024, 181 us (530); 37 tokens 19.8 us.  A large library product reaches 1273.
 #include <cmath>
 #include <type_traits>
 
@@ -31,6 +39,8 @@ constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
 constexpr int kTile = 64;  // keys of a staged tile
 constexpr int kScores = kTile / 32;  // score products of a wave's tile
+// As many as fit: a wave's outputs and queries take 48, 96 or 192 registers (162, 230 and 256 in all), and the tiles 32,
+// 64 or 128 KiB of shared memory.
 constexpr int chunk_waves(int d) { return d == 64 ? 3 : d == 128 ? 2 : 1; }  // workgroups of a CU, waves of a SIMD
 int part_slots(int d) { return chunk_waves(d) * device_cu_count(); }  // workgroups that run at a time
 
@@ -236,7 +246,7 @@ __device__ __forceinline__ int pages_in(const Cache& a, int n) {
 
 // A part's tiles of keys, one after the other.  One load of a wave takes kPerLoad neighbouring keys; a part
 // begins at a multiple of 32 keys, so where the page size is a multiple of kPerLoad they lie in one page and
-// the address is the wave's (WHOLE).  The lanes then look up the pages of the wave's loads of many tiles
+// the address is the wave's (WHOLE; 4096 tokens on themselves 165 us, and 304 with an address a lane).  The lanes then look up the pages of the wave's loads of many tiles
 // together, a run: lane i's load is load i % kLoads of tile i / kLoads of the run.
 struct Tile {
   int key, left;  // its first key, and the keys from it on to the part's end

@@ -21,6 +21,10 @@
 // evict_move_kernel: a workgroup takes 64 of a head's moves at a time, finds their slots from those counts, and
 // moves keys, values, masses and positions.  Slots that do not move get their masses and positions here as well,
 // where there are many workgroups.
+//
+// What bounds it: the selection is one CU's work for a head, in a handful of dependent passes (10 us for 2049
+// slots, 27 for 28 k, of which the search takes 9); moves run at the rate of a large copy.  4 rows of 20 k to 32 k
+// slots, 8 heads of 128 dimensions, cut to 4096: 67 us; one token too many in 16 rows of 2049: 16.5 us.
 #include "matrix.h"
 
 namespace ds355 {
@@ -110,7 +114,9 @@ __device__ __forceinline__ int set_bit(uint64_t bits, int i) {
   return at;
 }
 
-// HELD: slots whose values are held in shared memory; those of a longer row are read again for every pass.
+// HELD: slots whose values are held in shared memory; those of a longer row are read again for every pass.  The least
+// that holds the longest row is taken, so that more workgroups fit a CU: 57 rows of up to 6000 slots, 8 heads, take
+// 68 us with 8192 and 73 with 32768, 16 rows of 2049, 4 heads, 16.5 with 4096 and 16.8.
 template <int HELD>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs a) {
   constexpr int kGroups = HELD / 64;  // of 64 slots, a wave's
