@@ -540,3 +540,46 @@ def test_runs_of_pages(cuda, d, hkv, block):
     args["lse"].fill_(7)
     run(args)
     check(case, args, status=4)
+
+
+# Tiles that a mask hides from some query rows of an item and that others, in another wave, see whole; where a row's or
+# a window's first tile has the mask; parts that begin in one; pages that no load lies in.
+NOT_FINITE = [
+    dict(lens=[128], qlens=[128], hq=1, hkv=1, d=128, block=16),
+    dict(lens=[84, 300], qlens=[40, 256], hq=8, hkv=2, d=128, block=16),
+    dict(lens=[50, 63, 64, 65], qlens=[50, 63, 64, 65], hq=4, hkv=4, d=64, block=16),
+    dict(lens=[300], qlens=[300], hq=8, hkv=2, d=128, block=16, window=200),
+    dict(lens=[300, 90], qlens=[280, 90], hq=4, hkv=4, d=64, block=48, window=70),
+    dict(lens=[200, 130], qlens=[150, 130], hq=2, hkv=1, d=256, block=16),
+    dict(lens=[2000, 1500], qlens=[128, 70], hq=8, hkv=8, d=128, block=16),
+    dict(lens=[190], qlens=[128], hq=4, hkv=2, d=128, block=7, window=100),
+]
+
+
+def not_finite_values(i, value, dtype, cuda):
+    """(got, seen, rows): some values of head 0 are `value`, each in a dimension of its own; seen[token, head, dimension]
+    says whether a query row sees the one of that dimension."""
+    case = build(80 + i, dtype=dtype, **NOT_FINITE[i])
+    block, hkv, d = NOT_FINITE[i]["block"], case["hkv"], case["d"]
+    t, hq, _ = case["query"].shape
+    seen, rows = torch.zeros((t, hq, d), dtype=torch.bool), torch.zeros(t, dtype=torch.bool)
+    for b, (start, q, n) in enumerate(zip(case["starts"], case["qlens"], case["lens"])):
+        rows[start: start + q] = True
+        ends = torch.arange(n - q + 1, n + 1)
+        at = sorted({0, 10, 31, 32, 63, 64, 70, n // 3, n // 2, n - q, n - 65, n - 64, n - 33, n - 10, n - 1})
+        for dim, key in enumerate(k for k in at if 0 <= k < n):
+            page = int(case["table"][b, key // block])
+            case["cache"][1][page, key % block, 0, 3 * dim] = value
+            sees = (key < ends) & (key >= ends - case["window"] if case["window"] else True)
+            seen[start: start + q, : hq // hkv, 3 * dim] = sees[:, None]
+    args = device_args(case, cuda)
+    run(args)
+    return args["output"].cpu(), seen, rows
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=("bf16", "fp16"))
+@pytest.mark.parametrize("value", (float("nan"), INF, -INF))
+@pytest.mark.parametrize("i", range(len(NOT_FINITE)))
+def test_every_row_gets_the_values_that_are_not_finite_and_seen(cuda, i, value, dtype):
+    got, seen, rows = not_finite_values(i, value, dtype, cuda)
+    assert torch.equal(got[rows].isfinite(), ~seen[rows])

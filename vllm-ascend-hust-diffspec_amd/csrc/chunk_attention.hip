@@ -489,7 +489,6 @@ __device__ __forceinline__ void attend(const char* next_keys, const char* values
 struct Rows {
   bool any;              // it has query rows
   int limit, lower;      // keys that the lane column's row sees: lower <= t < limit
-  int all_from, all_to;  // keys that all its rows see
   int item_from, item_to;  // keys that all rows of the item see
 };
 
@@ -544,7 +543,8 @@ __device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, i
     const int here = i & 1;  // the tile's half of shared memory
     wait_loads();
     char* values = lds + (2 + here) * C::kStage;
-    if (key < rows.item_from || key + kTile > rows.item_to) {
+    const bool item_masked = key < rows.item_from || key + kTile > rows.item_to;
+    if (item_masked) {
       const bool found = clear_not_finite<DT, D>(values, wave);
       if ((fresh_thread() & 63) == 0) poison[here][wave] = found;
     }
@@ -552,7 +552,8 @@ __device__ __forceinline__ void run_part(const Cache& a, const int32_t* table, i
     send_values(here ^ 1);
     send_keys(here);
     if (!rows.any) continue;
-    if (key < rows.all_from || key + kTile > rows.all_to) {
+    if (item_masked) {
+      // Also for a wave whose rows see the whole tile: the values were cleared for all waves.
       const int from = rows.lower - key, half = (fresh_thread() >> 5) & 1;
       if (__any(poison[here][fresh_thread() & 3])) {
         const int page = key / a.block_size;
@@ -604,8 +605,6 @@ __global__ __launch_bounds__(Chunk<D>::kThreads, chunk_waves(D)) void chunk_atte
   w.any = r0 < rows;
   w.limit = p.seen + token + 1;
   w.lower = max(w.limit - a.window, 0);
-  w.all_to = p.seen + r0 / a.group + 1;
-  w.all_from = max(p.seen + min(r0 + 31, rows - 1) / a.group + 1 - a.window, 0);
   w.item_to = p.seen + p.tile * kItemRows / a.group + 1;
   w.item_from = max(p.seen + (min((p.tile + 1) * kItemRows, rows) - 1) / a.group + 1 - a.window, 0);
   u32x4 q[C::kSteps];
