@@ -583,3 +583,36 @@ def not_finite_values(i, value, dtype, cuda):
 def test_every_row_gets_the_values_that_are_not_finite_and_seen(cuda, i, value, dtype):
     got, seen, rows = not_finite_values(i, value, dtype, cuda)
     assert torch.equal(got[rows].isfinite(), ~seen[rows])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=("bf16", "fp16"))
+@pytest.mark.parametrize("value", (INF, -INF))
+@pytest.mark.parametrize("i", range(len(NOT_FINITE)))
+def test_a_seen_infinity_stays_one(cuda, i, value, dtype):
+    # No weight here is below 2^-25 of its row's largest (2^-24.9 in 64 bits), and fp16 holds weights down to 2^-31 of it: none
+    # rounds to 0.
+    got, seen, _ = not_finite_values(i, value, dtype, cuda)
+    assert (got[seen] == value).all()
+
+
+@pytest.mark.parametrize("d", (64, 128, 256))
+def test_an_infinity_behind_keys_of_no_weight_stays_one(cuda, d):
+    # The keys of the first tile lie 2^-288 below those of the second, where the infinity is.
+    case = build(95, lens=[100], qlens=[40], hq=1, hkv=1, d=d, block=16, dtype=torch.bfloat16, scale=1.0)
+    case["query"].zero_()[..., 0] = 1
+    k, v = case["dense"][0]
+    k.zero_()[:64, :, 0] = -200
+    exact = torch.stack([v[64: n].double().mean(0) if n > 64 else v[:n].double().mean(0) for n in range(61, 101)])
+    terms = torch.stack([v[64: n].double().abs().mean(0) if n > 64 else v[:n].double().abs().mean(0) for n in range(61, 101)])
+    v[70, 0, 5] = INF
+    for t in range(100):
+        for c, x in zip(case["cache"], (k, v)):
+            c[int(case["table"][0, t // 16]), t % 16] = x[t]
+    args = device_args(case, cuda)
+    run(args)
+    got = args["output"].cpu().double()[case["starts"][0]:][:40]
+    assert (got[10:, 0, 5] == INF).all()  # query token 10 is the first that sees key 70
+    rest = torch.ones((40, 1, d), dtype=torch.bool)
+    rest[10:, 0, 5] = False
+    # Weights are 1 each: the output rounds (2^-8), and fp32 sums.
+    assert ((got - exact).abs()[rest] <= (2.0 ** -8 * exact.abs() + 2.0 ** -18 * terms)[rest]).all()

@@ -443,7 +443,9 @@ __device__ __forceinline__ void attend(const char* next_keys, const char* values
   top = __builtin_fmaf(fmaxf(top, other_half(top)), scale_log2, -kBelow);
   if (__any(top > st.m + 8.f)) {
     const float m = fmaxf(st.m, top);
-    const float keep = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m);
+    // A factor that underflows, or is of sums of nothing yet, is taken as 2^-126 instead of 0, which is as near: an
+    // infinity that is in the output already (the tile's own are, see add_not_finite) stays one.
+    const float keep = fmaxf(__builtin_amdgcn_exp2f(st.m - m), 0x1p-126f);
     st.m = m;
     st.l *= keep;
 #pragma unroll
