@@ -289,3 +289,34 @@ def test_attention_mass_refuses_places_past_32_bits(over, message):
 
     d = mass_desc(workspace_bytes=1 << 60, **over)
     refuses(lambda: _lib.load().ds_attention_mass(None, ctypes.byref(d)), message)
+
+
+OVERLAPPING = (((2, 2), (32, 32)), ((2, 3), (32, 63)), ((3, 2), (63, 32)), ((2, 4), (64, 32)), ((4, 2), (32, 96)),
+               ((3, 3), (40, 70)))
+APART = (((2, 2), (64, 32)), ((2, 2), (32, 64)), ((2, 3), (32, 70)), ((1, 3), (0, 32)), ((3, 1), (40, 7)), ((2, 2), (96, 64)))
+
+
+@pytest.mark.parametrize("name", ("mass", "positions"))
+@pytest.mark.parametrize("shape,strides", OVERLAPPING + APART)
+def test_rows_and_heads_that_overlap_are_refused(name, shape, strides):
+    # 32 slots each: rows and heads nested either way, equal strides, or the last of one inside the first of another.
+    from ds355.eviction import attention_mass, evict_tokens
+
+    rows, heads = shape
+    places = sorted(strides[0] * b + strides[1] * h for b in range(rows) for h in range(heads))
+    assert all(y - x >= 32 for x, y in zip(places, places[1:])) == ((shape, strides) in APART)
+    lens = {k: torch.zeros(rows, dtype=torch.int32) for k in ("target_len", "keep_len", "kept_len")}
+    tensors = dict(mass=torch.zeros(rows, heads, 32), positions=torch.zeros((rows, heads, 32), dtype=torch.int32))
+    tensors[name] = torch.zeros(1000, dtype=tensors[name].dtype).as_strided((rows, heads, 32), (*strides, 1))
+    cache = torch.zeros(4, 16, heads, 128, dtype=torch.bfloat16)
+    table = torch.zeros((rows, 2), dtype=torch.int32)
+    message = "GPU only" if (shape, strides) in APART else f"{name}'s rows and heads overlap"
+    with pytest.raises(ValueError, match=message):
+        evict_tokens(**evict_args(key_cache=cache, value_cache=cache, settled=torch.zeros((rows, 2), dtype=torch.int32),
+                                  block_table=table, **lens, **tensors))
+    if name == "mass":
+        with pytest.raises(ValueError, match=message):
+            attention_mass(**mass_args(query=torch.zeros(3, heads, 128, dtype=torch.bfloat16), key_cache=cache,
+                                       lse=torch.zeros(3, heads), mass=tensors["mass"], block_table=table,
+                                       query_start=lens["target_len"], query_len=lens["target_len"],
+                                       target_len=lens["target_len"]))

@@ -88,7 +88,12 @@ def _per_slot(t, name, dtype, rows, heads):
     if t.dtype != dtype or t.ndim != 3 or t.shape[0] < rows or t.shape[1] != heads or t.shape[2] < 1 or t.stride(2) != 1:
         kind = "fp32" if dtype == torch.float32 else "int32"
         raise ValueError(f"{name} must be {kind} [rows, kv_heads, capacity] with unit last stride")
-    if (t.shape[1] > 1 and t.stride(1) < t.shape[2]) or (t.shape[0] > 1 and t.stride(0) < t.shape[2]):
+    # Rows of heads or heads of rows, as a rule; places of other layouts are looked at one by one.
+    (inner, count), (outer, others) = sorted(((t.stride(0), t.shape[0]), (t.stride(1), t.shape[1])))
+    if (count == 1 or inner >= t.shape[2]) and (others == 1 or outer >= (count - 1) * inner + t.shape[2]):
+        return
+    places = sorted(i * inner + j * outer for i in range(count) for j in range(others))
+    if any(y - x < t.shape[2] for x, y in zip(places, places[1:])):
         raise ValueError(f"{name}'s rows and heads overlap")
 
 
