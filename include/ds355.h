@@ -668,8 +668,8 @@ size_t ds_attention_mass_workspace_bytes(void);
  * key_cache, value_cache: [num_blocks, block_size, Hkv, D], 16-byte aligned,
  * D contiguous, D and all strides multiples of 16 bytes; mass fp32 and
  * positions int32 [rows, Hkv, capacity], contiguous in the last dimension;
- * kept_len overlaps neither target_len nor keep_len.  At most 1024 rows, 65535 heads of all rows
- * and 2^29 slots a row.
+ * kept_len overlaps neither target_len nor keep_len.  At most 1024 rows, 65535 heads of all rows,
+ * 2^29 slots a row and 2^30 tokens per page.
  * workspace: caller's scratch of ds_evict_workspace_bytes(), 256-byte aligned,
  * with no state between calls (one launch at a time).
  * Two kernels, launch shape fixed by the sizes (graph-capturable).

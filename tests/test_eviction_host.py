@@ -320,3 +320,13 @@ def test_rows_and_heads_that_overlap_are_refused(name, shape, strides):
                                        lse=torch.zeros(3, heads), mass=tensors["mass"], block_table=table,
                                        query_start=lens["target_len"], query_len=lens["target_len"],
                                        target_len=lens["target_len"]))
+
+
+@pytest.mark.parametrize("block_size", ((1 << 30) + 1, (1 << 31) - 1))
+def test_evict_refuses_pages_whose_count_passes_32_bits(block_size):
+    # A row's slots plus a page size past 2^31 made no pages of the row, and none of its page ids was checked.
+    from ds355 import _lib
+
+    d = evict_desc(block_size=block_size, max_blocks=1, workspace_bytes=1 << 40)
+    d.workspace = FAKE + 16  # refused before a launch in any case
+    refuses(lambda: _lib.load().ds_evict(None, ctypes.byref(d)), "2^30 tokens per page")

@@ -390,6 +390,7 @@ int evict_impl(hipStream_t stream, const ds_evict_desc* d) {
   DS_SUPPORTED(static_cast<int64_t>(d->head_dim) * size % 16 == 0, "heads must be multiples of 16 bytes");
   DS_SUPPORTED(d->rows <= kMaxRows, "at most %d rows", kMaxRows);
   DS_REQUIRE(d->block_size > 0 && d->num_blocks > 0 && d->max_blocks > 0, "block sizes and counts must be positive");
+  DS_SUPPORTED(d->block_size <= (1 << 30), "at most 2^30 tokens per page");  // a row's pages are counted in 32 bits
   DS_REQUIRE(d->capacity > 0, "capacity must be positive");
   DS_REQUIRE(d->sinks >= 0 && d->recent >= 0, "sinks and recent must not be negative");
   DS_SUPPORTED(static_cast<int64_t>(d->sinks) + d->recent <= (1 << 29), "at most 2^29 tokens that are always kept");
