@@ -330,3 +330,25 @@ def test_evict_refuses_pages_whose_count_passes_32_bits(block_size):
     d = evict_desc(block_size=block_size, max_blocks=1, workspace_bytes=1 << 40)
     d.workspace = FAKE + 16  # refused before a launch in any case
     refuses(lambda: _lib.load().ds_evict(None, ctypes.byref(d)), "2^30 tokens per page")
+
+
+def test_sizes_past_32_bits_reach_the_library_as_its_largest(monkeypatch):
+    # The descriptors' fields are 32-bit; 2^32 + 5 used to become 5.
+    from ds355 import chunk_attention, eviction
+
+    much, most = (1 << 32) + 5, (1 << 31) - 1
+    meta = dict(device="meta")
+    descs = []
+    for module, name in ((chunk_attention, "_launch"), (eviction, "_launch_mass"), (eviction, "_launch_evict")):
+        monkeypatch.setattr(module, name, lambda desc, *_: descs.append(desc))
+    monkeypatch.setattr(chunk_attention._lib, "require_gpu", lambda *_: torch.device("cpu"))
+    cache = torch.zeros((1, 16, 2, 128), dtype=torch.bfloat16, **meta).expand(much, 16, 2, 128)
+    table = torch.zeros((2, much), dtype=torch.int32, **meta)
+    chunk_attention.chunk_attention(**chunk_args(key_cache=cache, value_cache=cache, block_table=table))
+    mass, positions = (torch.zeros((2, 2, much), dtype=t, **meta) for t in (torch.float32, torch.int32))
+    eviction.attention_mass(**mass_args(key_cache=cache, block_table=table, mass=mass))
+    eviction.evict_tokens(**evict_args(key_cache=cache, value_cache=cache, block_table=table, mass=mass, positions=positions),
+                          sinks=much, recent=much)
+    for desc in descs:
+        assert (desc.num_blocks, desc.max_blocks) == (most, most)
+    assert len(descs) == 3 and descs[1].capacity == descs[2].capacity == descs[2].sinks == descs[2].recent == most

@@ -311,6 +311,11 @@ def dtype_code(dtype: torch.dtype) -> int:
         raise ValueError(f"unsupported dtype {dtype}") from None
 
 
+def count(n: int) -> int:
+    """A size for a descriptor's 32-bit field, which would take one past 2^31 for another: its largest then."""
+    return min(int(n), (1 << 31) - 1)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

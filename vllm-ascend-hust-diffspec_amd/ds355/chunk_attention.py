@@ -136,10 +136,10 @@ def chunk_attention(
         desc.lse_token_stride, desc.lse_head_stride = lse.stride(0), lse.stride(1)
     desc.k_block_stride, desc.k_token_stride, desc.k_head_stride = key_cache.stride()[:3]
     desc.v_block_stride, desc.v_token_stride, desc.v_head_stride = value_cache.stride()[:3]
-    desc.bt_stride, desc.max_blocks = block_table.stride(0), block_table.shape[1]
-    desc.num_blocks, desc.block_size = blocks, block_size
-    desc.rows, desc.tokens = rows, tokens
-    desc.num_q_heads, desc.num_kv_heads, desc.head_dim = hq, hkv, head_dim
+    desc.bt_stride, desc.max_blocks = block_table.stride(0), _lib.count(block_table.shape[1])
+    desc.num_blocks, desc.block_size = _lib.count(blocks), _lib.count(block_size)
+    desc.rows, desc.tokens = _lib.count(rows), _lib.count(tokens)
+    desc.num_q_heads, desc.num_kv_heads, desc.head_dim = (_lib.count(n) for n in (hq, hkv, head_dim))
     desc.window = 0 if window is None else min(int(window), 1 << 30)
     desc.workspace_bytes = workspace.numel()
     _launch(desc, device, query, key_cache, value_cache, output, lse, block_table, query_start, query_len, target_len,

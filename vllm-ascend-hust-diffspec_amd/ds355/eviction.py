@@ -183,11 +183,11 @@ def attention_mass(
     desc.lse_token_stride, desc.lse_head_stride = lse.stride(0), lse.stride(1)
     if previous is not None:
         desc.previous_row_stride, desc.previous_head_stride = previous.stride(0), previous.stride(1)
-    desc.mass_row_stride, desc.mass_head_stride, desc.capacity = mass.stride(0), mass.stride(1), mass.shape[2]
-    desc.bt_stride, desc.max_blocks = block_table.stride(0), block_table.shape[1]
-    desc.num_blocks, desc.block_size = blocks, block_size
-    desc.rows, desc.tokens = rows, tokens
-    desc.num_q_heads, desc.num_kv_heads, desc.head_dim = hq, hkv, head_dim
+    desc.mass_row_stride, desc.mass_head_stride, desc.capacity = mass.stride(0), mass.stride(1), _lib.count(mass.shape[2])
+    desc.bt_stride, desc.max_blocks = block_table.stride(0), _lib.count(block_table.shape[1])
+    desc.num_blocks, desc.block_size = _lib.count(blocks), _lib.count(block_size)
+    desc.rows, desc.tokens = _lib.count(rows), _lib.count(tokens)
+    desc.num_q_heads, desc.num_kv_heads, desc.head_dim = (_lib.count(n) for n in (hq, hkv, head_dim))
     desc.window = 0 if window is None else min(int(window), 1 << 30)
     desc.workspace_bytes = workspace.numel()
     _launch_mass(desc, device, query, key_cache, lse, mass, block_table, query_start, query_len, target_len, scale,
@@ -293,12 +293,12 @@ def evict_tokens(
     desc.dtype = _lib.dtype_code(key_cache.dtype)
     desc.k_block_stride, desc.k_token_stride, desc.k_head_stride = key_cache.stride()[:3]
     desc.v_block_stride, desc.v_token_stride, desc.v_head_stride = value_cache.stride()[:3]
-    desc.mass_row_stride, desc.mass_head_stride, desc.capacity = mass.stride(0), mass.stride(1), mass.shape[2]
+    desc.mass_row_stride, desc.mass_head_stride, desc.capacity = mass.stride(0), mass.stride(1), _lib.count(mass.shape[2])
     desc.positions_row_stride, desc.positions_head_stride = positions.stride(0), positions.stride(1)
-    desc.bt_stride, desc.max_blocks = block_table.stride(0), block_table.shape[1]
-    desc.num_blocks, desc.block_size = blocks, block_size
-    desc.rows, desc.num_kv_heads, desc.head_dim = rows, hkv, head_dim
-    desc.sinks, desc.recent = int(sinks), int(recent)
+    desc.bt_stride, desc.max_blocks = block_table.stride(0), _lib.count(block_table.shape[1])
+    desc.num_blocks, desc.block_size = _lib.count(blocks), _lib.count(block_size)
+    desc.rows, desc.num_kv_heads, desc.head_dim = _lib.count(rows), _lib.count(hkv), _lib.count(head_dim)
+    desc.sinks, desc.recent = _lib.count(sinks), _lib.count(recent)
     desc.workspace_bytes = workspace.numel()
     _launch_evict(desc, device, key_cache, value_cache, mass, positions, settled, block_table, target_len, keep_len,
                   kept_len, workspace, ref_counts, status)
