@@ -352,3 +352,25 @@ def test_sizes_past_32_bits_reach_the_library_as_its_largest(monkeypatch):
     for desc in descs:
         assert (desc.num_blocks, desc.max_blocks) == (most, most)
     assert len(descs) == 3 and descs[1].capacity == descs[2].capacity == descs[2].sinks == descs[2].recent == most
+
+
+def test_workspaces_are_sized_for_the_device_they_are_on(monkeypatch):
+    # Both sizes follow the compute units of the device that is current while they are worked out.
+    import contextlib
+
+    from ds355 import chunk_attention, eviction
+
+    current, asked = [None], []
+
+    @contextlib.contextmanager
+    def on_device(device):
+        current.append(device)
+        yield
+        current.pop()
+
+    monkeypatch.setattr(chunk_attention._lib, "on_device", on_device)
+    monkeypatch.setattr(chunk_attention, "chunk_workspace_bytes", lambda *_: asked.append(current[-1]) or 256)
+    monkeypatch.setattr(eviction, "mass_workspace_bytes", lambda: asked.append(current[-1]) or 256)
+    assert chunk_attention.new_chunk_workspace(1, 1, 8, 2, 128, "cpu").numel() == 256
+    assert eviction.new_mass_workspace("cpu").numel() == 256
+    assert asked == [torch.device("cpu")] * 2

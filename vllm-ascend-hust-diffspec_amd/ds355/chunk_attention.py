@@ -27,14 +27,15 @@ STATUS_BAD_PAGE = 4
 
 
 def chunk_workspace_bytes(batch_rows: int, tokens: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
-    """Bytes of the workspace for up to ``batch_rows`` rows and ``tokens`` query tokens."""
+    """Bytes of the workspace on the current device for up to ``batch_rows`` rows and ``tokens`` query tokens."""
     return int(_lib.load().ds_chunk_attention_workspace_bytes(batch_rows, tokens, num_q_heads, num_kv_heads, head_dim))
 
 
 def new_chunk_workspace(batch_rows: int, tokens: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
                         device: torch.device | str) -> torch.Tensor:
     """A workspace (uint8); it keeps nothing between calls, and serves one launch at a time."""
-    size = chunk_workspace_bytes(batch_rows, tokens, num_q_heads, num_kv_heads, head_dim)
+    with _lib.on_device(torch.device(device)):
+        size = chunk_workspace_bytes(batch_rows, tokens, num_q_heads, num_kv_heads, head_dim)
     if size <= 0:
         raise ValueError("workspace sizes must be positive, num_q_heads a multiple of num_kv_heads and head_dim "
                          "64, 128 or 256")
