@@ -596,7 +596,11 @@ size_t ds_chunk_attention_workspace_bytes(int rows, int tokens, int num_q_heads,
  * Entries at or past target_len[b], and rows with query_len <= 0, are left as
  * they were.  A query head whose lse is -infinity adds nothing.  A key that
  * is not finite makes its own entry NaN or any value; others not.
- * Rows may be a part of the attention's: the last tokens of each, say.
+ * Rows may be a part of the attention's: the last tokens of each, say, or of a
+ * verified draft the accepted ones, which are the first (query_len their number,
+ * target_len the accepted length).  Entries that previous holds for slots of
+ * tokens that were then cut back count for the tokens that come there next:
+ * where cut-back tokens were among the rows, they are the caller's to clear.
  * *status (optional, the caller clears it) gets bit 0 when a row's query
  * tokens are out of range (the row is left out), bit 1 when a row is longer
  * than max_blocks pages or capacity (it ends there), bit 2 when a page id is

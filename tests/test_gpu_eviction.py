@@ -790,3 +790,98 @@ def test_the_same_eviction_twice_changes_nothing(cuda):
     run_evict(args)
     for k, v in after.items():
         assert same(args[k], v), k
+
+
+def _weights(query, lse, keys, ends, scale):
+    """(weights [rows, keys], the errors of their logits) in 64 bits: row i sees the keys below ends[i]."""
+    d = query.shape[1]
+    x = query @ keys.t() * scale
+    hidden = torch.arange(keys.shape[0]) >= ends[:, None]
+    exact = torch.logsumexp(x.masked_fill(hidden, -INF), -1, keepdim=True)
+    e = (d + 4) * 2.0 ** -24 * scale * (query.abs() @ keys.abs().t())
+    own = (e + 2.0 ** -22 * (1 + x.abs())).masked_fill(hidden, 0).amax(-1, keepdim=True)
+    # The LSE's own error, as the attention's tests have it, and that of the weight.
+    error = own + (keys.shape[0] / 16 + 64) * 2.0 ** -24 + e + 2.0 ** -22 * (2 + x.abs() + 2 * exact.abs())
+    assert ((lse[:, None].double() - exact).abs() <= error.amax(-1, keepdim=True)).all()
+    return torch.exp(x - exact).masked_fill(hidden, 0.0), error
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=("bf16", "fp16"))
+def test_rejected_drafts_leave_no_mass(cuda, dtype):
+    """Prompts in chunks, then verified drafts of which some are rejected: mass and eviction of what was accepted, pages cut
+    back, other tokens in the slots.  Masses are those of the accepted tokens alone, in 64 bits, and the kept slots
+    those that the rule picks from the masses."""
+    from ds355 import chunk_attention, eviction, pages, prefix_attention
+
+    hq, hkv, d, block, rows, budget, capacity, decay = 8, 2, 128, 16, 2, 96, 320, 0.9
+    group, scale, g = hq // hkv, d ** -0.5, gen(365)
+    caches = [torch.zeros((64, block, hkv, d), dtype=dtype, device=cuda) for _ in range(2)]
+    pool = pages.PagePool(caches)
+    table = torch.full((rows, capacity // block), -1, dtype=torch.int32, device=cuda)
+    mass = torch.zeros((rows, hkv, capacity), device=cuda)
+    positions = torch.zeros((rows, hkv, capacity), dtype=torch.int32, device=cuda)
+    settled, row_ids = torch.zeros((rows, 2), dtype=torch.int32, device=cuda), i32([0, 1], cuda)
+    length, kept, keep = i32([0, 0], cuda), i32([0, 0], cuda), i32([budget] * rows, cuda)
+    work = chunk_attention.new_chunk_workspace(rows, 256, hq, hkv, d, cuda)
+    prefix_work = prefix_attention.new_prefix_workspace(rows, 256, hq, hkv, d, cuda)
+    mass_work, evict_work = eviction.new_mass_workspace(cuda), eviction.new_evict_workspace(rows, hkv, capacity, cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    held = [[[] for _ in range(hkv)] for _ in range(rows)]  # by slot: [key, mass, its error] of a head
+    for new, taken in [([100, 64], [100, 64]), ([37, 20], [37, 20])] + [([5, 5], t) for t in ([2, 5], [1, 1], [4, 3], [5, 1], [1, 2])]:
+        total, committed = length + i32(new, cuda), length + i32(taken, cuda)
+        pool.extend(table, row_ids, total)
+        host_table, lens = table.cpu(), length.cpu().tolist()
+        tokens = [randn((n, 2, hkv, d), dtype, g) for n in new]
+        for b, n in enumerate(new):
+            for i in range(n):
+                slot = lens[b] + i
+                for c in range(2):
+                    caches[c][int(host_table[b, slot // block]), slot % block] = tokens[b][i, c].to(cuda)
+        query = (randn((sum(new), hq, d), dtype, g) * 2).to(cuda)
+        out, lse = torch.zeros_like(query), torch.zeros((sum(new), hq), device=cuda)
+        starts = i32([0, new[0]], cuda)
+        if new[0] > 5:
+            chunk_attention.chunk_attention(query, *caches, out, lse, table, starts, i32(new, cuda), total, scale=scale,
+                                            workspace=work, status=status)
+        else:
+            prefix_attention.shared_prefix_attention(query, *caches, out, lse, table, starts, i32(new, cuda), total,
+                                                     i32([0], cuda), scale=scale, workspace=prefix_work, status=status)
+        # The accepted tokens are the first ones of each row.
+        eviction.attention_mass(query, caches[0], lse, mass, table, starts, i32(taken, cuda), committed, scale=scale,
+                                previous=mass, decay=decay, workspace=mass_work, status=status)
+        torch.cuda.synchronize()
+        got, host_q, host_lse = mass.cpu().double(), query.cpu().double(), lse.cpu()
+        at = 0
+        for b, n in enumerate(new):
+            for h in range(hkv):
+                slots = held[b][h]
+                slots += [[tokens[b][i, 0, h].double(), 0.0, 0.0] for i in range(taken[b])]
+                keys, ends = torch.stack([s[0] for s in slots]), lens[b] + 1 + torch.arange(taken[b])
+                sums, errors = torch.zeros(len(slots), dtype=torch.float64), torch.zeros(len(slots), dtype=torch.float64)
+                for j in range(h * group, (h + 1) * group):
+                    w, e = _weights(host_q[at: at + taken[b], j], host_lse[at: at + taken[b], j], keys, ends, scale)
+                    sums, errors = sums + w.sum(0), errors + (w * torch.expm1(e)).sum(0)
+                for t, slot in enumerate(slots):
+                    slot[1] = slot[1] * decay + float(sums[t])
+                    slot[2] = slot[2] + float(errors[t]) + (taken[b] * group / 8 + 64) * 2.0 ** -24 * slot[1] + 2.0 ** -23
+                    assert abs(float(got[b, h, t]) - slot[1]) <= slot[2], (b, h, t)
+                assert (got[b, h, len(slots):] == 0).all()  # of rejected tokens, and of none
+            at += n
+        case = dict(lens=committed.cpu().tolist(), keep=[budget] * rows, table=host_table, caches=[c.cpu() for c in caches],
+                    mass=mass.cpu(), positions=positions.cpu(), settled=settled.cpu(), sinks=4, recent=16, block=block, hkv=hkv)
+        expected = expect_evict(case)
+        args = dict(key_cache=caches[0], value_cache=caches[1], mass=mass, positions=positions, settled=settled,
+                    block_table=table, target_len=committed, keep_len=keep, kept_len=kept, sinks=4, recent=16,
+                    ref_counts=pool.ref_counts, workspace=evict_work, status=status)
+        run_evict(args)
+        check_evict(case, args, expected)
+        for b, n in enumerate(case["lens"]):
+            if n > budget:  # which slots the rule kept, and where
+                for h in range(hkv):
+                    page = lambda t: (int(host_table[b, t // block]), t % block, h)  # noqa: E731
+                    slot_of = {tuple(case["caches"][0][page(t)].tolist()): t for t in range(n)}
+                    held[b][h] = [held[b][h][slot_of[tuple(expected["key_cache"][page(t)].tolist())]] for t in range(budget)]
+        pool.free(table, row_ids, kept)
+        length = kept.clone()
+    # 150 tokens were accepted in the first row, and 96, which is its budget, in the second.
+    assert int(pool.status.item()) == 0 and settled[:, 1].tolist() == [54, 0]

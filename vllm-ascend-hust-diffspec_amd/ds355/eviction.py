@@ -132,7 +132,10 @@ def attention_mass(
     fp32 ``[rows, Hkv, capacity]``; ``previous`` may be ``mass`` itself (it
     is then added to in place), memory apart from it, or None for zeros.  Entries at or past a
     row's length, and rows without query tokens, are left as they were.
-    Rows may name only the last tokens of each request.
+    Rows may name only the last tokens of each request, or only the accepted
+    ones of a verified draft: ``query_len`` their number and ``target_len``
+    the accepted length.  Rejected tokens then add nothing, and their slots
+    hold no mass that the next tokens there would inherit.
 
     ``status`` receives ``STATUS_BAD_ROW``, ``STATUS_LENGTH`` and
     ``STATUS_BAD_PAGE`` (include/ds355.h); ``reuse`` as in
