@@ -662,6 +662,8 @@ size_t ds_attention_mass_workspace_bytes(void);
  * max(target_len[b], 0).  Caches and positions at or past k, and mass at or
  * past n, are left as they were.  What attention over the k slots computes
  * does not depend on their order; a sliding window over them does.
+ * So does drafting by retrieval: ds_chunk_scores and ds_retrieval_step take slot t
+ * of the pages for token t, which a row that was cut no longer has.
  * *status (optional, the caller clears it) gets bit 1 when a row is longer
  * than max_blocks pages or capacity, bit 2 when one of its page ids is outside
  * [0, num_blocks), bit 3 when keep_len is negative or below sinks + recent,

@@ -6,7 +6,8 @@ up, from the LSE that ``chunk_attention`` or ``prefix_attention`` wrote, how
 much weight each cached key got, and ``evict_tokens`` keeps the heaviest keys
 of each KV head, in place.  The pages behind the kept slots go back with
 ``pages.PagePool.free``, and the attention of the next step reads the shorter
-rows like any others.
+rows like any others.  Drafting by retrieval (``step.retrieval_step``) takes
+slots for tokens: rows that draft so must be kept out of the eviction.
 """
 
 from __future__ import annotations
