@@ -616,3 +616,21 @@ def test_an_infinity_behind_keys_of_no_weight_stays_one(cuda, d):
     rest[10:, 0, 5] = False
     # Weights are 1 each: the output rounds (2^-8), and fp32 sums.
     assert ((got - exact).abs()[rest] <= (2.0 ** -8 * exact.abs() + 2.0 ** -18 * terms)[rest]).all()
+
+
+@pytest.mark.parametrize("shape", (
+    dict(lens=[3000, 900], qlens=[5, 1], hq=8, hkv=1, d=128, block=16, window=2000),  # long rows in parts
+    dict(lens=[2500], qlens=[200], hq=4, hkv=4, d=64, block=7, window=333),
+    dict(lens=[1800, 300], qlens=[70, 300], hq=2, hkv=1, d=256, block=48, window=129),
+))
+def test_what_lies_before_every_window_has_no_effect(cuda, shape):
+    case = build(96, dtype=torch.bfloat16, **shape)
+    expected = expect(case)
+    for b, (n, q) in enumerate(zip(case["lens"], case["qlens"])):
+        for t in range(max(n - q + 1 - shape["window"], 0)):
+            page = int(case["table"][b, t // shape["block"]])
+            case["cache"][0][page, t % shape["block"]] = (float("nan"), INF, -INF)[t % 3]
+            case["cache"][1][page, t % shape["block"]] = (INF, float("nan"))[t % 2]
+    args = device_args(case, cuda)
+    run(args)
+    check(case, args, expected)
