@@ -13,8 +13,9 @@
 // into parts of the rows, whose sums mass_join_kernel adds up in order.
 //
 // What bounds it: with few query rows the keys' bytes (16 tokens, 32 heads on 4 of 128 dimensions, over 4 k to 16 k keys:
-// 43 us, 3.9 TB/s); with many the exponential and the sum of each score beside its product (2048 tokens on 8 k keys,
-// 32 heads on 8: 170 us, 711 TFLOP/s; 6 times 32 tokens, 64 heads on 8 of 64 dimensions, 50 us).
+// 43 us, 3.9 TB/s); with many vector issue (52% of the cycles at 128 dimensions, 62% at 64, the exponentials 30% of that)
+// and what a part costs beside its blocks (2048 tokens on 8 k keys, 32 heads on 8: 169 us, 711 TFLOP/s; 6 times 32 tokens,
+// 64 heads on 8 of 64 dimensions, whose parts are of four blocks, 50 us).
 #include <cmath>
 
 #include "matrix.h"
@@ -26,8 +27,15 @@ namespace {
 // many, so that more workgroups fit a CU.  16 rows of 8 query rows each over 4 k to 16 k keys take 43 us with 32
 // and 53 with 64, 6 rows of 256 take 64 and 50, one of 8192 takes 176 and 170.
 constexpr int kMostRows = 64;
-constexpr int kMinPart = 256;   // query rows below which they are not cut
+// Query rows below which they are not cut: 128 tokens on 1 k keys, 32 heads on 4 of 128 dimensions, take 17.7 us with 256, 15.7
+// with 128 and 23.5 with 512, 100 rows of 8 tokens beside one of 1500 147, 157 and 147.
+constexpr int kMinPart = 256;
+// What a slot's workgroup gets of the least parts.  More are dealt more evenly and cost more: 40 rows of 64 tokens on 2 k keys take
+// 95 us with 8, 88 with 4 and 95 with 16, 65 such rows 135, 134 and 188, 16 rows on 4 k 79, 77 and 78.
 constexpr int kPartsPerSlot = 8;
+// Rows up to which the sizes of parts are compared, since a lane goes over all rows: 16 rows of 64 tokens on 4 k keys take
+// 79 us, and 100 uncompared; 65 rows of 64 on 2 k 135 either way, 100 rows of 8 beside one of 1500 147, and 169 compared.
+constexpr int kComparedRows = 64;
 constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table or its mass
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
@@ -122,7 +130,8 @@ __device__ __forceinline__ Layout make_layout(const MassArgs& a, int* memory, bo
   __syncthreads();
   // A part has at least the share of the work at which kPartsPerSlot would fill every workgroup (which bounds the
   // partial sums).  Among the sizes that cut the longest rows evenly the one that ends first is taken: as
-  // many rounds as all parts take, of a part's blocks and about two for what it costs beside them.
+  // many rounds as all parts take, of a part's blocks and about two for what it costs beside them.  Of many rows it is the
+  // least one.
   const unsigned long long most = static_cast<unsigned long long>(kPartsPerSlot) * a.slots;
   const unsigned long long share = (work * a.hkv + most - 1) / most;
   const int least = static_cast<int>(min(max(share, static_cast<unsigned long long>(kMinPart / a.block)), 1ull << 25));
@@ -134,7 +143,7 @@ __device__ __forceinline__ Layout make_layout(const MassArgs& a, int* memory, bo
   len = ceil_div(len * a.group, a.block);
   if (len > least) atomicMax(&longest, len);
   __syncthreads();
-  if (longest > least && a.rows <= 64 && threadIdx.x < 64) {
+  if (longest > least && a.rows <= kComparedRows && threadIdx.x < 64) {
     const int mine = max(ceil_div(longest, static_cast<int>(threadIdx.x) + 1), least);
     const float per_part = 1.f / static_cast<float>(mine);
     float parts = 0.f;

@@ -18,9 +18,11 @@
 //
 // Each of four waves has 32 query rows as columns of the score product, so that a lane's scores are of one row and the
 // weights are in the layout that the second product takes; tiles of 64 keys go by in shared memory for all
-// four.  What bounds it: vector instructions beside the matrix units (about 210 a wave and tile against 32 products
-// of 32 cycles at 128 dimensions), and at 256 dimensions that a SIMD has registers for one wave only.  Measured,
-// 32 query heads on 8 of 128 dimensions: 4096 tokens on themselves 167 us (823 TFLOP/s), of which plan and join take 8;
+// four.  What bounds it: vector instructions beside the matrix units (about 240 a wave and tile, 32 of them exponentials,
+// against 32 products of 32 cycles at 128 dimensions: 58% and 46% of the cycles), and at 256 dimensions that a SIMD has
+// registers for one wave only, which waits for a third of its cycles.  Measured,
+// 32 query heads on 8 of 128 dimensions: 4096 tokens on themselves 167 us (823 TFLOP/s), of which the plan and a join
+// with nothing to join take 8 to 10;
 // 32 on 4, 512 tokens on 32 k keys 292 us (935); 11 mixed requests, 64 heads on 8 of 64 dimensions, 102 us (518); 3 chunks
 // of 16 heads on 2 of 256 dimensions, window 1024, 181 us (530); 37 tokens 19.8 us.  A large library product reaches 1273.
 #include <cmath>
@@ -32,15 +34,18 @@ namespace ds355 {
 namespace {
 
 constexpr int kItemRows = 128;  // query rows of an item
-constexpr int kMinPart = 4;     // key tiles below which an item is not cut
+// Key tiles below which an item is not cut.  A part waits for its first tile, and pieces have to be joined: 37 tokens on
+// 248 keys take 19.3 us with 4 and 18.2 with 1 or 2, 128 on 1 k 25.3 and 34.8 with 1, 27.1 with 2, 28.1 with 8, eight single
+// tokens on 500 keys 19.6 and 18.7 with 2, 23.2 with 8; a single token on 32 k 81 and 61 with 8, whose pieces are fewer.
+constexpr int kMinPart = 4;
 constexpr uint32_t kStatusRow = 1;     // a row's query tokens are out of range
 constexpr uint32_t kStatusLength = 2;  // a row is longer than its block table
 constexpr uint32_t kStatusPage = 4;    // a page id is out of range
 
 constexpr int kTile = 64;  // keys of a staged tile
 constexpr int kScores = kTile / 32;  // score products of a wave's tile
-// As many as fit: a wave's outputs and queries take 48, 96 or 192 registers (162, 230 and 256 in all), and the tiles 32,
-// 64 or 128 KiB of shared memory.
+// As many as fit: a wave's outputs and queries take 48, 96 or 192 registers (162, 229 and, with accumulation registers, 432 in
+// all), and the tiles 32, 64 or 128 KiB of shared memory.
 constexpr int chunk_waves(int d) { return d == 64 ? 3 : d == 128 ? 2 : 1; }  // workgroups of a CU, waves of a SIMD
 int part_slots(int d) { return chunk_waves(d) * device_cu_count(); }  // workgroups that run at a time
 

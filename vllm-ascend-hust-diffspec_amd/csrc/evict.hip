@@ -22,9 +22,9 @@
 // moves keys, values, masses and positions.  Slots that do not move get their masses and positions here as well,
 // where there are many workgroups.
 //
-// What bounds it: the selection is one CU's work for a head, in a handful of dependent passes (10 us for 2049
-// slots, 27 for 28 k, of which the search takes 9); moves run at the rate of a large copy.  4 rows of 20 k to 32 k
-// slots, 8 heads of 128 dimensions, cut to 4096: 67 us; one token too many in 16 rows of 2049: 16.5 us.
+// What bounds it: the selection is one CU's work for a head, in a handful of dependent passes before any move (10 us
+// for 2049 slots, 27 for 28 k, of which the search takes 9); long heads' moves run at the rate of a large copy.  4 rows of
+// 20 k to 32 k slots, 8 heads of 128 dimensions, cut to 4096: 67 us; one token too many in 16 rows of 2049: 16.5 us.
 #include "matrix.h"
 
 namespace ds355 {

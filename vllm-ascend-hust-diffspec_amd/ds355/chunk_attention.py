@@ -6,7 +6,8 @@ captures query, softmax LSE and paged keys from it
 attention for prompts that enter in chunks: ragged rows of many query tokens,
 each causal at its end and over a sliding window where the layer has one,
 with rows that decode a single token beside them.  For a verified batch that
-shares a long prefix there is ``prefix_attention``.  The LSE it writes is
+shares a long prefix there is ``prefix_attention``, which is also the faster
+one for steps of single tokens only.  The LSE it writes is
 what ``step.VerifierSnapshot``, ``kernels.paged_chunk_attention_scores`` and
 ``eviction.attention_mass`` take.
 """
