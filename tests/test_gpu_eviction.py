@@ -885,3 +885,99 @@ def test_rejected_drafts_leave_no_mass(cuda, dtype):
         length = kept.clone()
     # 150 tokens were accepted in the first row, and 96, which is its budget, in the second.
     assert int(pool.status.item()) == 0 and settled[:, 1].tolist() == [54, 0]
+
+
+def test_a_captured_step_of_all_calls(cuda):
+    """Two layers, one set of workspaces and one `reuse` for all calls: attention, mass of what is accepted, eviction and pages
+    given back, replayed with changed lengths, and the same calls eagerly on a state of their own."""
+    from ds355 import chunk_attention, eviction, pages, prefix_attention
+
+    hq, hkv, d, block, rows, budget, capacity, most = 8, 2, 64, 16, 3, 64, 160, 40
+    g = gen(370)
+
+    class State:
+        def __init__(self):
+            zeros = lambda *s, dtype=torch.int32: torch.zeros(s, dtype=dtype, device=cuda)  # noqa: E731
+            self.caches = [[zeros(40, block, hkv, d, dtype=torch.float16) for _ in range(2)] for _ in range(2)]
+            self.pool = pages.PagePool([c for layer in self.caches for c in layer])
+            self.table = torch.full((rows, capacity // block), -1, dtype=torch.int32, device=cuda)
+            self.mass = [zeros(rows, hkv, capacity, dtype=torch.float32) for _ in range(2)]
+            self.positions = [zeros(rows, hkv, capacity) for _ in range(2)]
+            self.settled = [zeros(rows, 2) for _ in range(2)]
+            self.length, self.kept, self.total, self.committed = (zeros(rows) for _ in range(4))
+            self.start, self.new, self.taken, self.row_ids = zeros(rows), zeros(rows), zeros(rows), i32([0, 1, 2], cuda)
+            self.keep, self.status, self.prefix = i32([budget] * rows, cuda), zeros(1), zeros(1)
+            self.query = [zeros(most, hq, d, dtype=torch.float16) for _ in range(2)]
+            self.out = [[torch.zeros_like(q) for _ in range(2)] for q in self.query]
+            self.lse = [[zeros(most, hq, dtype=torch.float32) for _ in range(2)] for _ in range(2)]
+            self.work = chunk_attention.new_chunk_workspace(rows, most, hq, hkv, d, cuda)
+            self.prefix_work = prefix_attention.new_prefix_workspace(rows, most, hq, hkv, d, cuda)
+            self.mass_work = eviction.new_mass_workspace(cuda)
+            self.evict_work = eviction.new_evict_workspace(rows, hkv, capacity, cuda)
+            self.reuse = {}
+
+        def step(self):
+            for i, cache in enumerate(self.caches):
+                rest = dict(scale=d ** -0.5, status=self.status, reuse=self.reuse)
+                chunk_attention.chunk_attention(self.query[i], *cache, self.out[i][0], self.lse[i][0], self.table, self.start,
+                                                self.new, self.total, workspace=self.work, **rest)
+                prefix_attention.shared_prefix_attention(self.query[i], *cache, self.out[i][1], self.lse[i][1], self.table,
+                                                         self.start, self.new, self.total, self.prefix,
+                                                         workspace=self.prefix_work, **rest)
+            for i, cache in enumerate(self.caches):
+                eviction.attention_mass(self.query[i], cache[0], self.lse[i][0], self.mass[i], self.table, self.start, self.taken,
+                                        self.committed, scale=d ** -0.5, previous=self.mass[i], decay=0.9,
+                                        workspace=self.mass_work, status=self.status, reuse=self.reuse)
+                eviction.evict_tokens(*cache, self.mass[i], self.positions[i], self.settled[i], self.table, self.committed,
+                                      self.keep, self.kept, sinks=2, recent=8, ref_counts=self.pool.ref_counts,
+                                      workspace=self.evict_work, status=self.status, reuse=self.reuse)
+            self.pool.free(self.table, self.row_ids, self.kept)
+
+        def prepare(self, new, taken, queries, tokens):
+            self.new.copy_(i32(new, "cpu"))
+            self.taken.copy_(i32(taken, "cpu"))
+            self.start.copy_(i32([sum(new[:b]) for b in range(rows)], "cpu"))
+            self.length.copy_(self.kept)
+            torch.add(self.length, self.new, out=self.total)
+            torch.add(self.length, self.taken, out=self.committed)
+            self.pool.extend(self.table, self.row_ids, self.total)
+            table, length = self.table.cpu(), self.length.cpu().tolist()
+            for i, layer in enumerate(self.caches):
+                self.query[i][: sum(new)].copy_(queries[i])
+                at = 0
+                for b, n in enumerate(new):
+                    for slot in range(length[b], length[b] + n):
+                        for c in range(2):
+                            layer[c][int(table[b, slot // block]), slot % block] = tokens[i, at, c].to(cuda)
+                        at += 1
+            torch.cuda.synchronize()
+
+        def tensors(self):
+            return [*sum(self.caches, []), *self.mass, *self.positions, *self.settled, self.kept, self.table, *sum(self.out, []),
+                    *sum(self.lse, []), self.pool.ref_counts, self.status]
+
+    replayed, eager = State(), State()
+    warm = State()  # the calls are captured from their second time on, on a state that is thrown away
+    warm.step()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    replayed.reuse = warm.reuse
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        replayed.step()
+    steps = [([30, 7, 1], [30, 7, 1]), ([4, 33, 3], [4, 33, 3]), ([30, 5, 5], [30, 2, 5]), ([1, 30, 5], [1, 30, 1]),
+             ([5, 5, 30], [3, 1, 30]), ([5, 1, 5], [5, 1, 2]), ([2, 5, 33], [1, 5, 33]), ([0, 4, 5], [0, 2, 5])]
+    for new, taken in steps:
+        n = sum(new)
+        queries = [randn((n, hq, d), torch.float16, g) * 2 for _ in range(2)]
+        tokens = randn((2, n, 2, hkv, d), torch.float16, g)
+        for state in (replayed, eager):
+            state.prepare(new, taken, queries, tokens)
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        for x, y in zip(replayed.tensors(), eager.tensors()):
+            assert same(x, y)
+        for i in range(2):  # the two attentions: both roundings of the output and of the weights, terms of at most 5 each
+            assert (eager.out[i][0][:n].float() - eager.out[i][1][:n].float()).abs().max() < 4 * 2.0 ** -11 * 5
+    assert int(eager.status.item()) == 0 and int(eager.pool.status.item()) == 0 and int(replayed.pool.status.item()) == 0
+    assert int(eager.settled[0][:, 1].min()) > 0 and len(eager.reuse) >= 4
